@@ -13,11 +13,13 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libgranulelayer_amd.so"
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 GL_ACT = {"identity": 0, "relu": 1, "gelu": 2}
 GL_POOL = {"mean": 0, "sum": 1, "max": 2, "topk_mean": 3, "logmeanexp": 4, "power_mean": 5, "softmax_weighted": 6}
 GL_DTYPE_F32, GL_DTYPE_BF16 = 0, 1
+GL_KEEP = {"none": 0, "sign": 1, "z": 2, "z8": 3}
+DENSE_MAX_FEATURES = 1 << 20  # GL_DENSE_MAX_FEATURES
 GL_ERR_SCRATCH = -8
 FWD_STATIC_SCRATCH_BYTES = 64 << 20  # GL_FWD_STATIC_SCRATCH_BYTES
 
@@ -60,19 +62,41 @@ class GlCoverArgs(ctypes.Structure):
                 ("swaps", _P), ("loss", _P), ("status", _P)]
 
 
-STRUCTS = (GlFwdArgs, GlBwdArgs, GlEdgeArgs, GlAdamArgs, GlCoverArgs)  # gl_struct_layout ids 0..4
+class GlPack8Args(ctypes.Structure):
+    _fields_ = [("x", _P), ("sx", _I64), ("rows", _I64), ("cols", _I32), ("x_dtype", _I32), ("q", _P), ("e", _P)]
+
+
+class GlDenseArgs(ctypes.Structure):
+    _fields_ = [("X", _P), ("sx", _I64), ("W", _P), ("sw", _I64), ("bias", _P), ("res", _P), ("sr", _I64), ("Y", _P),
+                ("sy", _I64), ("M", _I64), ("N", _I32), ("K", _I32), ("dtype", _I32), ("res_dtype", _I32),
+                ("y_dtype", _I32), ("act", _I32), ("keep", _I32), ("z", _P), ("z_exp", _P), ("ws", _P),
+                ("ws_bytes", _SZ)]
+
+
+class GlDenseBwdArgs(ctypes.Structure):
+    _fields_ = [("dY", _P), ("sdy", _I64), ("z", _P), ("z_exp", _P), ("X", _P), ("sx", _I64), ("xq", _P), ("xe", _P),
+                ("W", _P), ("sw", _I64), ("M", _I64), ("N", _I32), ("K", _I32), ("dtype", _I32), ("dy_dtype", _I32),
+                ("act", _I32), ("keep", _I32), ("dX", _P), ("dW", _P), ("db", _P), ("g_dtype", _I32),
+                ("accumulate", _I32), ("ws", _P), ("ws_bytes", _SZ)]
+
+
+# gl_struct_layout ids 0..7
+STRUCTS = (GlFwdArgs, GlBwdArgs, GlEdgeArgs, GlAdamArgs, GlCoverArgs, GlPack8Args, GlDenseArgs, GlDenseBwdArgs)
 # every symbol include/granulelayer_amd.h declares
 EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_workspace", "gl_fwd", "gl_fwd_static",
            "gl_fwd_mask_bytes",
            "gl_edges_size",
            "gl_edges_build", "gl_bwd_workspace", "gl_bwd", "gl_adam", "gl_sched_size", "gl_sched_build_host",
            "gl_sched_build", "gl_window_build_host", "gl_window_build", "gl_cover_select", "gl_trace_begin",
-           "gl_trace_end")
+           "gl_trace_end", "gl_pack8", "gl_unpack8", "gl_dense_fwd_workspace", "gl_dense_fwd", "gl_dense_bwd_workspace",
+           "gl_dense_bwd")
 KERNEL_NAMES = {1: "tile_x_kernel", 2: "fwd_kernel", 3: "fwd_finalize_kernel", 4: "c1t_kernel", 5: "bwd_w_kernel",
                 6: "dx_kernel", 7: "dx_reduce_kernel", 8: "adam_kernel", 9: "edges_build", 10: "fwd_kernel_win",
                 11: "bwd_w_kernel_win", 12: "max_events_dw_kernel", 13: "max_events_dx_kernel",
                 14: "cover_select_kernel", 15: "sched_build_kernel", 16: "dx_dense_kernel",
-                17: "dx_dma_kernel"}
+                17: "dx_dma_kernel", 18: "pack8_kernel", 19: "unpack8_kernel", 20: "dense_tile_kernel",
+                21: "dense_few_kernel", 22: "dense_join_kernel", 23: "dense_dz_kernel", 24: "dense_db_kernel",
+                25: "dense_align_kernel"}
 
 
 class NativeError(RuntimeError):
@@ -99,10 +123,12 @@ class Library:
         L.gl_error_string.restype = ctypes.c_char_p
         L.gl_error_string.argtypes = [ctypes.c_int]
         for name, st in (("gl_fwd", GlFwdArgs), ("gl_fwd_static", GlFwdArgs), ("gl_bwd", GlBwdArgs),
-                         ("gl_edges_build", GlEdgeArgs), ("gl_adam", GlAdamArgs), ("gl_cover_select", GlCoverArgs)):
+                         ("gl_edges_build", GlEdgeArgs), ("gl_adam", GlAdamArgs), ("gl_cover_select", GlCoverArgs), ("gl_pack8", GlPack8Args), ("gl_unpack8", GlPack8Args),
+                         ("gl_dense_fwd", GlDenseArgs), ("gl_dense_bwd", GlDenseBwdArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), _P]
-        for name, st in (("gl_fwd_workspace", GlFwdArgs), ("gl_bwd_workspace", GlBwdArgs)):
+        for name, st in (("gl_fwd_workspace", GlFwdArgs), ("gl_bwd_workspace", GlBwdArgs),
+                         ("gl_dense_fwd_workspace", GlDenseArgs), ("gl_dense_bwd_workspace", GlDenseBwdArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), ctypes.POINTER(_SZ)]
         L.gl_trace_begin.restype = ctypes.c_int

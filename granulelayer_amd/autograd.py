@@ -163,6 +163,7 @@ class Level1Runtime:
         self.last_info: Dict = {}
         self.det = False
         self.grad_call = True  # set per call by the layer: grad mode was on (a backward can follow)
+        self.activation_checkpoint = "exact"  # set per call by the layer: how the input is kept for the backward
 
     def check_devices(self, *tensors):
         dev = self.idx.device
@@ -259,6 +260,31 @@ def _saved_stats(level: LevelSpec, out: Dict[str, torch.Tensor], policy: str) ->
     return keep
 
 
+def _keep_input(ctx, rt: Level1Runtime, x, xc) -> list:
+    """Tensors that stand for the input in ctx's saved ones: x itself, or with
+    activation_checkpoint="int8" the 8-bit form of the kernels' operand xc when a backward can run.
+    The gradients are then those at the values that were kept: dW sums over them, and neurons whose
+    z the backward recomputes are recomputed from them."""
+    ctx.x_kept = None
+    if (rt.activation_checkpoint == "int8" and getattr(rt, "grad_call", True) and any(ctx.needs_input_grad)
+            and rt.backend is not None):
+        ctx.x_kept = (xc.shape, xc.dtype, x.dtype)
+        kept = list(rt.backend.pack8(xc))
+    else:
+        kept = [x]
+    rt.last_info["input_checkpoint_bytes"] = sum(t.numel() * t.element_size() for t in kept)
+    ctx.n_x = len(kept)
+    return kept
+
+
+def _kept_input(ctx, kept):
+    """(the input as the kernels' operands take it, the dtype of its gradient) from _keep_input's tensors."""
+    if ctx.x_kept is None:
+        return kept[0], kept[0].dtype
+    shape, dtype, grad_dtype = ctx.x_kept
+    return ctx.rt.backend.unpack8(*kept, shape[-1], dtype), grad_dtype
+
+
 def _level1_backward(rt: Level1Runtime, xc, wc, bc, dy, saved: Dict[str, torch.Tensor], policy: str, dw_buf,
                      db_buf, recomputed: bool = False) -> torch.Tensor:
     """dX of the level-1 kernels for dy [B, U], the gradient of out_act(pre); dW / db accumulate
@@ -315,21 +341,22 @@ class SparsePoolFunction(torch.autograd.Function):
         saved = _saved_stats(lv, out, policy)
         ctx.rt, ctx.policy, ctx.compute_dtype = rt, policy, compute_dtype
         ctx.saved_keys = list(saved.keys())
-        ctx.save_for_backward(x, w, b, *saved.values())
+        ctx.save_for_backward(*_keep_input(ctx, rt, x, xc), w, b, *saved.values())
         rt.last_info["checkpoint_bytes"] = sum(t.numel() * t.element_size() for t in saved.values())
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, w, b, *svals = ctx.saved_tensors
+        kept, (w, b, *svals) = ctx.saved_tensors[:ctx.n_x], ctx.saved_tensors[ctx.n_x:]
         saved = dict(zip(ctx.saved_keys, svals))
         rt: Level1Runtime = ctx.rt
+        x, x_dtype = _kept_input(ctx, kept)
         xc, wc, bc = _compute_operands(x, w, b, ctx.compute_dtype)
         dw_buf, db_buf, use_main = _grad_buffers(w, b)
         dx = _level1_backward(rt, xc, wc, bc, dy, saved, ctx.policy, dw_buf, db_buf)
         gw = None if use_main else dw_buf.to(w.dtype)
         gb = None if use_main else db_buf.to(b.dtype)
-        return dx.to(x.dtype, memory_format=torch.contiguous_format), gw, gb, None, None, None
+        return dx.to(x_dtype, memory_format=torch.contiguous_format), gw, gb, None, None, None
 
 
 # the two-level function lives beside its level-2 code; exported here as the reference's module does

@@ -403,6 +403,108 @@ class HipBackend:
         with _on(p.device):
             self.lib.call("gl_adam", ctypes.byref(a), ctypes.c_void_p(_stream(p.device)))
 
+    # ------------------------------------------------------------------ activations in 8 bits
+    def pack8(self, x):
+        """x [rows, features] in 8 bits: (codes [rows, round_up(features, 32)] int8, exponents
+        [rows, ceil(features / 32)] uint8), the format of activations8.py."""
+        x, code, sx = _x_operand(x.resolve_neg())
+        rows, cols = x.shape
+        if cols > N.DENSE_MAX_FEATURES:
+            raise ValueError(f"{cols} features (at most {N.DENSE_MAX_FEATURES})")
+        nb = -(-cols // 32)
+        q = torch.empty((rows, nb * 32), device=x.device, dtype=torch.int8)
+        e = torch.empty((rows, nb), device=x.device, dtype=torch.uint8)
+        a = N.GlPack8Args(_ptr(x), sx, rows, cols, code, _ptr(q), _ptr(e))
+        with _on(x.device):
+            self.lib.call("gl_pack8", ctypes.byref(a), _stream(x.device))
+        return q, e
+
+    def unpack8(self, q, e, cols, dtype):
+        """The values [rows, cols] of ``pack8``'s codes and exponents, of ``dtype``."""
+        if dtype not in _DENSE_DTYPES:
+            raise TypeError(f"unpacks to float32 or bfloat16 (got {dtype})")
+        rows, nb = q.shape[0], -(-cols // 32)
+        if (q.dtype != torch.int8 or e.dtype != torch.uint8 or tuple(q.shape) != (rows, nb * 32)
+                or tuple(e.shape) != (rows, nb) or not q.is_contiguous() or not e.is_contiguous()
+                or e.device != q.device or q.data_ptr() % 8):
+            raise ValueError(f"codes must be a contiguous int8 [rows, {nb * 32}] and exponents a contiguous uint8 "
+                             f"[rows, {nb}] tensor on one device, the codes 8-byte aligned")
+        x = torch.empty((rows, cols), device=q.device, dtype=dtype)
+        a = N.GlPack8Args(_ptr(x), cols, rows, cols, _DENSE_DTYPES[dtype], _ptr(q), _ptr(e))
+        with _on(q.device):
+            self.lib.call("gl_unpack8", ctypes.byref(a), _stream(q.device))
+        return x
+
+    # ------------------------------------------------------------------ dense projection
+    def dense_forward(self, x, w, b, res, activation, keep):
+        """y = act(x W^T + b) + res of x [M, K], w [N, K], b [N] or None (all of one dtype), res [M, N]
+        or None, and what ``keep`` (N.GL_KEEP) says of z for ``dense_backward``: (y, z, z_exp)."""
+        x, code, sx = _x_operand(x.resolve_neg())
+        w, _, sw = _x_operand(w.resolve_neg())
+        M, K = x.shape
+        F = w.shape[0]
+        if max(F, K) > N.DENSE_MAX_FEATURES:
+            raise ValueError(f"{max(F, K)} features (at most {N.DENSE_MAX_FEATURES})")
+        dev = x.device
+        sr, rcode, ycode, ytype = 0, 0, code, x.dtype
+        if b is not None:
+            b = b.resolve_neg().contiguous()
+        if res is not None:
+            res = res.resolve_neg()
+            if res.stride(1) != 1 or 0 < res.stride(0) < F:
+                res = res.contiguous()
+            sr, rcode = res.stride(0), _DENSE_DTYPES[res.dtype]
+            if res.dtype == torch.float32:
+                ycode, ytype = N.GL_DTYPE_F32, torch.float32
+        y = torch.empty((M, F), device=dev, dtype=ytype)
+        z = z_exp = None
+        if keep == "sign":
+            z = torch.empty((M, -(-F // 32)), device=dev, dtype=torch.int32)
+        elif keep == "z":
+            z = torch.empty((M, -(-F // 8) * 8), device=dev, dtype=x.dtype)
+        elif keep == "z8":
+            z = torch.empty((M, -(-F // 32) * 32), device=dev, dtype=torch.int8)
+            z_exp = torch.empty((M, -(-F // 32)), device=dev, dtype=torch.uint8)
+        a = N.GlDenseArgs(_ptr(x), sx, _ptr(w), sw, _ptr(b), _ptr(res), sr, _ptr(y), F, M, F, K, code, rcode, ycode,
+                          N.GL_ACT[activation], N.GL_KEEP[keep], _ptr(z), _ptr(z_exp), 0, 0)
+        with _on(dev):
+            need = self.lib.size_query("gl_dense_fwd_workspace", a)
+            if need:
+                ws = torch.empty(need, device=dev, dtype=torch.uint8)
+                a.ws, a.ws_bytes = _ptr(ws), need
+            self.lib.call("gl_dense_fwd", ctypes.byref(a), _stream(dev))
+        return y, z, z_exp
+
+    def dense_backward(self, dy, activation, keep, z, z_exp, x, xq, xe, w, dx, dw, db, accumulate):
+        """Gradients of ``dense_forward`` into dx [M, K] (x's dtype), dw [N, K] and db [N] (w's dtype, or fp32
+        and added to with ``accumulate``); None for what is not needed.  x as it was, or in 8 bits (xq, xe)."""
+        dy, ycode, sdy = _x_operand(dy)
+        w, code, sw = _x_operand(w.resolve_neg())
+        sx = 0
+        if x is not None:
+            x, _, sx = _x_operand(x.resolve_neg())
+        M, F = dy.shape
+        K = w.shape[1]
+        dev = dy.device
+        if M == 0:  # sums over no rows
+            for t in (dw, db):
+                if t is not None and not accumulate:
+                    t.zero_()
+            return
+        gcode = N.GL_DTYPE_F32 if accumulate else code
+        a = N.GlDenseBwdArgs(_ptr(dy), sdy, _ptr(z), _ptr(z_exp), _ptr(x), sx, _ptr(xq), _ptr(xe), _ptr(w), sw, M, F, K,
+                             code, ycode, N.GL_ACT[activation], N.GL_KEEP[keep], _ptr(dx), _ptr(dw), _ptr(db), gcode,
+                             int(accumulate), 0, 0)
+        with _on(dev):
+            need = self.lib.size_query("gl_dense_bwd_workspace", a)
+            if need:
+                ws = torch.empty(need, device=dev, dtype=torch.uint8)
+                a.ws, a.ws_bytes = _ptr(ws), need
+            self.lib.call("gl_dense_bwd", ctypes.byref(a), _stream(dev))
+
+
+_DENSE_DTYPES = {torch.float32: N.GL_DTYPE_F32, torch.bfloat16: N.GL_DTYPE_BF16}
+
 
 def backend_for(device) -> HipBackend:
     """Backend of a device (the reference's backends.cuda.runtime.backend_for, runtime.py:188-197)."""

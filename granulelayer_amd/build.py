@@ -25,7 +25,8 @@ PROBE_LIB = OUT_DIR / "libgl_lds_probe.so"
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 SOURCES = ["gl_abi.hip", "gl_forward.hip", "gl_backward.hip", "gl_record.hip", "gl_max_bwd.hip", "gl_edges.hip", "gl_adam.hip",
-           "gl_sched.hip", "gl_cover.hip"]
+           "gl_sched.hip", "gl_cover.hip", "gl_pack8.hip", "gl_dense.hip", "gl_dense_bf16.hip", "gl_dense_f32.hip",
+           "gl_dense_few.hip"]
 FLAGS = [
     "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
     # keep the compiler from emitting packed fp32 (v_pk_*_f32) instructions

@@ -41,6 +41,7 @@ import torch
 from torch import nn
 
 from . import _native as N
+from .activations8 import check_activation_checkpoint
 from .autograd import Level1Runtime, SparsePoolFunction, resolve_policy
 from .config import PhysicalPlan, PoolingConfig, check_workspace_budget
 
@@ -261,7 +262,8 @@ class CoverTopK16Layer(nn.Module):
 
     def __init__(self, input_dim: int, hidden_dim: int, output_dim: int, slots_per_group: int, *,
                  pooling: Union[str, dict, PoolingConfig] = "mean", checkpoint_policy: str = "auto",
-                 plan: Optional[PhysicalPlan] = None, workspace_budget: Optional[int] = None, device=None):
+                 plan: Optional[PhysicalPlan] = None, workspace_budget: Optional[int] = None, device=None,
+                 activation_checkpoint: str = "exact"):
         super().__init__()
         if slots_per_group % 16:
             raise ValueError("slots_per_group must be a multiple of 16")
@@ -276,6 +278,7 @@ class CoverTopK16Layer(nn.Module):
         reason = self.cfg.levels[0].hip_reason()
         if reason:
             raise NotImplementedError(reason)
+        self.activation_checkpoint = check_activation_checkpoint(activation_checkpoint)
         self.plan = plan or PhysicalPlan()
         self.workspace_budget = check_workspace_budget(workspace_budget)
         self.compute_dtype = torch.float32
@@ -294,7 +297,8 @@ class CoverTopK16Layer(nn.Module):
     @torch.no_grad()
     def from_envelope(cls, weight: torch.Tensor, bias: torch.Tensor, env_indices: torch.Tensor, *, input_dim: int,
                       hidden_dim: int, output_dim: int, envelope_C: int = 256, normalization: str = "none",
-                      pooling="mean", plan: Optional[PhysicalPlan] = None, device=None) -> "CoverTopK16Layer":
+                      pooling="mean", plan: Optional[PhysicalPlan] = None, device=None,
+                      activation_checkpoint: str = "exact") -> "CoverTopK16Layer":
         """Select the Cover-TopK/16 support from K64 envelope values and build the compact layer.
 
         ``weight`` [G, NB, envelope_C, 64] / ``bias`` [G, NB, envelope_C]: the pre-pruning envelope
@@ -333,7 +337,8 @@ class CoverTopK16Layer(nn.Module):
             nrec = dict(treatment="energy", applied=True, s_max=S_MAX, eps_rel=EPS_REL,
                         clipped=int((s == S_MAX).sum()), scale_mean=float(s[valid].mean()))
         S = L.slots_per_group
-        lay = cls(input_dim, hidden_dim, output_dim, S, pooling=pooling, plan=plan, device=dev)
+        lay = cls(input_dim, hidden_dim, output_dim, S, pooling=pooling, plan=plan, device=dev,
+                  activation_checkpoint=activation_checkpoint)
         lay.indices.copy_(sel["rec_idx"].view(lay.layout.index_shape))
         lay.env.copy_(sel["env"].view(lay.layout.index_shape))
         lay.weight.copy_(W_kept.view(lay.layout.weight_shape))
@@ -371,8 +376,8 @@ class CoverTopK16Layer(nn.Module):
         return dict(path=str(path), fingerprints=blob["fingerprints"])
 
     @classmethod
-    def load_packed(cls, path, *, device=None, pooling="mean", plan: Optional[PhysicalPlan] = None
-                    ) -> "CoverTopK16Layer":
+    def load_packed(cls, path, *, device=None, pooling="mean", plan: Optional[PhysicalPlan] = None,
+                    activation_checkpoint: str = "exact") -> "CoverTopK16Layer":
         """Restore a ``save_packed`` file (no selection, no envelope needed), refusing files whose
         immutable buffers differ from their recorded fingerprints (cover_topk16.py:214-236)."""
         blob = torch.load(Path(path), map_location="cpu", weights_only=True)
@@ -380,7 +385,7 @@ class CoverTopK16Layer(nn.Module):
             raise ValueError(f"{path}: schema {blob.get('schema')!r}, expected {PACKED_SCHEMA!r}")
         lo = blob["layout"]
         lay = cls(lo["input_dim"], lo["hidden_dim"], lo["output_dim"], lo["slots_per_group"], pooling=pooling,
-                  plan=plan, device=device)
+                  plan=plan, device=device, activation_checkpoint=activation_checkpoint)
         lay.load_state_dict(blob["state"])
         lay.cover_meta = blob["meta"]
         if lay.immutable_fingerprints() != blob["fingerprints"]:
@@ -430,7 +435,7 @@ class CoverTopK16Layer(nn.Module):
         lead = x.shape[:-1]
         x2 = x.reshape(-1, x.shape[-1])
         rt = self._runtime()
-        rt.grad_call = torch.is_grad_enabled()
+        rt.grad_call, rt.activation_checkpoint = torch.is_grad_enabled(), self.activation_checkpoint
         y = SparsePoolFunction.apply(x2, self.weight, self.bias, rt, self.effective_policy,
                                      self.compute_dtype)
         return y.reshape(*lead, y.shape[-1])

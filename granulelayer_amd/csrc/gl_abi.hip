@@ -137,6 +137,31 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       for (long long x : t) v[c++] = x;
       break;
     }
+    case 5: {
+      typedef GlPack8Args S;
+      long long t[] = {(long long)sizeof(S), OFF(S, x), OFF(S, sx), OFF(S, rows), OFF(S, cols), OFF(S, x_dtype), OFF(S, q),
+                       OFF(S, e)};
+      for (long long x : t) v[c++] = x;
+      break;
+    }
+    case 6: {
+      typedef GlDenseArgs S;
+      long long t[] = {(long long)sizeof(S), OFF(S, X), OFF(S, sx), OFF(S, W), OFF(S, sw), OFF(S, bias), OFF(S, res),
+                       OFF(S, sr), OFF(S, Y), OFF(S, sy), OFF(S, M), OFF(S, N), OFF(S, K), OFF(S, dtype),
+                       OFF(S, res_dtype), OFF(S, y_dtype), OFF(S, act), OFF(S, keep), OFF(S, z), OFF(S, z_exp),
+                       OFF(S, ws), OFF(S, ws_bytes)};
+      for (long long x : t) v[c++] = x;
+      break;
+    }
+    case 7: {
+      typedef GlDenseBwdArgs S;
+      long long t[] = {(long long)sizeof(S), OFF(S, dY), OFF(S, sdy), OFF(S, z), OFF(S, z_exp), OFF(S, X), OFF(S, sx),
+                       OFF(S, xq), OFF(S, xe), OFF(S, W), OFF(S, sw), OFF(S, M), OFF(S, N), OFF(S, K), OFF(S, dtype),
+                       OFF(S, dy_dtype), OFF(S, act), OFF(S, keep), OFF(S, dX), OFF(S, dW), OFF(S, db), OFF(S, g_dtype),
+                       OFF(S, accumulate), OFF(S, ws), OFF(S, ws_bytes)};
+      for (long long x : t) v[c++] = x;
+      break;
+    }
     default:
       return GL_ERR_ARG;
   }

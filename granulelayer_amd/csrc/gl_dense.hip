@@ -1,0 +1,442 @@
+// The dense projection's entry points: plans, the kernels around the products, launches.
+#include "gl_dense.h"
+
+namespace gl {
+
+namespace {
+
+constexpr int es_of(int dtype) { return dtype == GL_DTYPE_BF16 ? 2 : 4; }
+inline long long padded(long long n) { return round_up(n, 8); }  // row of a copied or computed operand
+
+// ---- rows at 16-byte addresses --------------------------------------------------------------------
+// The tile kernel loads 16 bytes at a time straight into LDS.  An operand whose rows do not start at
+// 16-byte addresses, or (reduction along the row) end inside 16 bytes, is copied to rows of padded(cols)
+// elements first, zeros behind the last: one pass over an operand that the product reads many times.
+template <typename T>
+__global__ __launch_bounds__(256) void dense_align_kernel(const T* __restrict__ src, long long ld, long long rows, int cols,
+                                                          T* __restrict__ dst) {
+  const int ldd = (cols + 7) / 8 * 8;
+  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int c0 = (blockIdx.y * 64 + (threadIdx.x & 63)) * 8;
+  if (r >= rows || c0 >= ldd) return;
+  T v[8];
+  if (c0 + 8 <= cols) {
+    struct __attribute__((packed, aligned(2))) U { T x[8]; };
+    const U u = *reinterpret_cast<const U*>(src + r * ld + c0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = u.x[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c0 + j < cols ? src[r * ld + c0 + j] : T(0);
+  }
+  T* d = dst + r * ldd + c0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) d[j] = v[j];
+}
+
+struct Operand {
+  const void* p;
+  long long ld;  // elements
+  long long rows;
+  int cols;
+  bool rc;       // reduction along the row
+  bool copied;   // through workspace
+};
+// Whether the tile kernel takes the operand as it is.  Its 32-bit offsets span 256 rows.
+inline bool in_place(const Operand& o, int es) {
+  const long long ldb = o.ld * es;
+  return ((uintptr_t)o.p & 15) == 0 && (o.rows == 1 || ldb % 16 == 0) && (!o.rc || (long long)o.cols * es % 16 == 0) &&
+         ldb * 256 < (1LL << 31);
+}
+inline Operand operand(const void* p, long long ld, long long rows, int cols, bool rc, int es) {
+  Operand o{p, rows == 1 ? cols : ld, rows, cols, rc, false};
+  if (!in_place(o, es)) o.copied = true;
+  if (rows == 1) o.ld = padded(cols);  // never stepped along; keeps the buffer's size whole
+  return o;
+}
+inline size_t copy_bytes(const Operand& o, int es) {
+  return o.copied ? (size_t)round_up(o.rows * padded(o.cols) * es, 256) : 0;
+}
+
+int launch_align(Operand& o, int es, void* dst, hipStream_t s) {
+  const dim3 grid((unsigned)((o.rows + 3) / 4), (unsigned)ceil_div(padded(o.cols), 512));
+  if (es == 2)
+    GL_LAUNCH(GL_KERNEL_DENSE_ALIGN, dense_align_kernel<unsigned short>, grid, dim3(256), 0, s, (const unsigned short*)o.p,
+              o.ld, o.rows, o.cols, (unsigned short*)dst);
+  else
+    GL_LAUNCH(GL_KERNEL_DENSE_ALIGN, dense_align_kernel<unsigned>, grid, dim3(256), 0, s, (const unsigned*)o.p, o.ld, o.rows,
+              o.cols, (unsigned*)dst);
+  GL_CHECK_LAUNCH();
+  o.p = dst;
+  o.ld = padded(o.cols);
+  return 0;
+}
+
+// ---- the sums of a split product --------------------------------------------------------------------
+// A lane holds 4 neighbouring columns and adds the splits in their order, then the epilogue.
+__global__ __launch_bounds__(256) void dense_join_kernel(const float* __restrict__ part, int splits, DenseEpi e) {
+  const long long m = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int l = threadIdx.x & 63, n = blockIdx.y * 256 + l * 4;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (m < e.M && n < e.N) {
+    for (int s = 0; s < splits; ++s) {
+      float t[4];
+      load4(part, false, ((long long)s * e.M + m) * e.N + n, e.N - n, t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += t[j];
+    }
+  }
+  dense_epilogue(e, m, n, v);
+}
+
+// ---- plan of a product --------------------------------------------------------------------------------
+struct Product {
+  int tile, splits, steps_per_split, steps, tiles_m, tiles_n;
+  size_t part_bytes;
+};
+Product plan_product(int dtype, long long M, int N, long long R) {
+  const int es = es_of(dtype);
+  Product best{};
+  double best_t = 0;
+  const int steps = (int)((R * es + DENSE_BK - 1) / DENSE_BK);
+  for (int t = dtype == GL_DTYPE_BF16 ? DENSE_256 : DENSE_128; t < DENSE_TILES; ++t) {
+    const long long tm = (M + DENSE_BM[t] - 1) / DENSE_BM[t], tn = (N + DENSE_BN[t] - 1) / DENSE_BN[t];
+    if (tm * tn > (1LL << 30)) continue;
+    // workgroups that run at once, and microseconds of a stage of each then
+    const double slots = t == DENSE_256 ? 256 : (t == DENSE_128 ? 512 : 768);
+    const double us = (t == DENSE_256 ? 2.1 : (t == DENSE_128 ? 1.4 : 1.2)) * (dtype == GL_DTYPE_BF16 ? 1.0 : 5.6);
+    for (int s = 1; s <= 32 && s <= steps; s = s < 4 ? s + 1 : s * 2) {
+      const int per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
+      if (splits != s || tm * tn * s > (1LL << 30)) continue;
+      const double rounds = (double)((tm * tn * s + (long long)slots - 1) / (long long)slots);
+      // a partly filled chip runs its workgroups a little faster each
+      double time = rounds * (per * us + 3.0);
+      if (s > 1) time += 4.0 + (double)s * M * N * 8 / 4.0e6;
+      if (best_t == 0 || time < best_t) {
+        best_t = time;
+        best = Product{t, s, per, steps, (int)tm, (int)tn, s > 1 ? (size_t)round_up((long long)s * M * N * 4, 256) : 0};
+      }
+    }
+  }
+  return best;
+}
+
+int run_product(int dtype, int form, const Operand& p, const Operand& q, long long R, const Product& pl, void* part,
+                const DenseEpi& e, hipStream_t s) {
+  const int es = es_of(dtype);
+  DenseK k{};
+  k.P = p.p;
+  k.Q = q.p;
+  k.ldp = p.ld * es;
+  k.ldq = q.ld * es;
+  k.R = R;
+  k.tiles_m = pl.tiles_m;
+  k.tiles_n = pl.tiles_n;
+  k.steps = pl.steps;
+  k.steps_per_split = pl.steps_per_split;
+  k.part = pl.splits > 1 ? (float*)part : nullptr;
+  k.e = e;
+  GL_TRY(dtype == GL_DTYPE_BF16 ? launch_dense_tile_bf16(form, pl.tile, k, pl.splits, s)
+                                : launch_dense_tile_f32(form, pl.tile, k, pl.splits, s));
+  if (pl.splits > 1) {
+    const dim3 grid((unsigned)((e.M + 3) / 4), (unsigned)ceil_div(e.N, 256));
+    GL_LAUNCH(GL_KERNEL_DENSE_JOIN, dense_join_kernel, grid, dim3(256), 0, s, (const float*)part, pl.splits, e);
+    GL_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+// ---- dz = dY act'(z) and the sums of its columns -------------------------------------------------------
+__device__ __forceinline__ float dgelu_f(float z) {
+  const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+  return __builtin_fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), cdf);
+}
+
+constexpr int DZ_ROWS = 64, DZ_COLS = 256;  // of a workgroup; 32 lanes of 8 columns by 8 rows at a time
+
+// dz may be null (only the sums), part too (only dz).  Rows of dz are padded(N) apart, zeros behind N.
+template <bool YBF, bool OBF>
+__global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ dY, long long sdy, const void* __restrict__ z,
+                                                       const uint8_t* __restrict__ ze, int keep, long long M, int N,
+                                                       void* __restrict__ dz, float* __restrict__ part) {
+  __shared__ float sums[8][DZ_COLS];
+  const int ct = threadIdx.x & 31, rt = threadIdx.x >> 5;
+  const int n = blockIdx.y * DZ_COLS + ct * 8;
+  const long long ldz = (N + 7) / 8 * 8;
+  const int nblk = (N + 31) / 32;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (n < N) {
+    for (int i = 0; i < DZ_ROWS / 8; ++i) {
+      const long long m = (long long)blockIdx.x * DZ_ROWS + i * 8 + rt;
+      if (m >= M) break;
+      float g[8];
+      load8<YBF>(dY, m * sdy + n, N - n, g);
+      if (keep == GL_KEEP_SIGN) {
+        const unsigned w = ((const unsigned*)z)[m * nblk + (n >> 5)] >> (n & 31);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = (w >> j) & 1u ? g[j] : 0.f;
+      } else if (keep != GL_KEEP_NONE) {
+        float t[8];
+        if (keep == GL_KEEP_Z) {
+          load8<OBF>(z, m * ldz + n, N - n, t);
+        } else {
+          const uv2 w = *reinterpret_cast<const uv2*>((const uint8_t*)z + (m * nblk * 32 + n));
+          const float st = p8_step(ze[m * nblk + (n >> 5)]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) t[j] = p8_value(w[j >> 2], j & 3, st);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] *= n + j < N ? dgelu_f(t[j]) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += g[j];
+      if (dz) store8<OBF>(dz, m * ldz + n, 8, g);
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sums[rt][ct * 8 + j] = s[j];
+  __syncthreads();
+  const int c = blockIdx.y * DZ_COLS + threadIdx.x;
+  if (c >= N) return;
+  float t = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) t += sums[r][threadIdx.x];
+  part[(long long)blockIdx.x * N + c] = t;
+}
+
+// db from the sums of `chunks` row blocks: 32 columns a workgroup, 32 rows of lanes, then LDS
+__global__ __launch_bounds__(1024) void dense_db_kernel(const float* __restrict__ part, long long chunks, int N,
+                                                        void* __restrict__ db, int g_bf, int accumulate) {
+  __shared__ float sums[32][33];
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
+  float s = 0.f;
+  if (n < N)
+    for (long long i = r; i < chunks; i += 32) s += part[i * N + n];
+  sums[r][c] = s;
+  __syncthreads();
+  if (r != 0 || n >= N) return;
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) t += sums[i][c];
+  if (g_bf) ((unsigned short*)db)[n] = to_bf16(t);
+  else ((float*)db)[n] = accumulate ? ((float*)db)[n] + t : t;
+}
+
+bool dtype_ok(int d) { return d == GL_DTYPE_F32 || d == GL_DTYPE_BF16; }
+bool on_element(const void* p, int dtype) { return ((uintptr_t)p & (uintptr_t)(es_of(dtype) - 1)) == 0; }
+bool row_ok(long long stride, long long rows, long long cols) { return rows <= 1 || stride >= cols; }
+
+// ---- forward --------------------------------------------------------------------------------------------
+int check_fwd(const GlDenseArgs* a) {
+  if (!a || a->M < 0 || a->N < 1 || a->K < 1) return GL_ERR_ARG;
+  if (a->N > GL_DENSE_MAX_FEATURES || a->K > GL_DENSE_MAX_FEATURES || a->M >= GL_DENSE_MAX_ROWS) return GL_ERR_UNSUPPORTED;
+  if (!dtype_ok(a->dtype) || !dtype_ok(a->y_dtype) || (a->res && !dtype_ok(a->res_dtype))) return GL_ERR_UNSUPPORTED;
+  if (a->act < GL_ACT_IDENTITY || a->act > GL_ACT_GELU || a->keep < GL_KEEP_NONE || a->keep > GL_KEEP_Z8) return GL_ERR_ARG;
+  if (a->M == 0) return 0;
+  if (!a->X || !a->W || !a->Y || (a->keep != GL_KEEP_NONE && !a->z) || (a->keep == GL_KEEP_Z8 && !a->z_exp)) return GL_ERR_ARG;
+  if (!row_ok(a->sx, a->M, a->K) || !row_ok(a->sw, a->N, a->K) || !row_ok(a->sy, a->M, a->N)) return GL_ERR_ARG;
+  if (a->res && a->sr != 0 && !row_ok(a->sr, a->M, a->N)) return GL_ERR_ARG;
+  if (!on_element(a->X, a->dtype) || !on_element(a->W, a->dtype) || !on_element(a->bias, a->dtype) ||
+      !on_element(a->Y, a->y_dtype) || (a->res && !on_element(a->res, a->res_dtype)) || ((uintptr_t)a->z & 15))
+    return GL_ERR_ARG;
+  return 0;
+}
+struct FwdPlan {
+  bool few;
+  Operand x, w;
+  Product pr;
+  size_t off_w, off_part, bytes;
+};
+FwdPlan plan_fwd(const GlDenseArgs* a) {
+  FwdPlan p{};
+  p.few = a->M <= DENSE_FEW_ROWS && a->keep == GL_KEEP_NONE;
+  if (p.few) return p;
+  const int es = es_of(a->dtype);
+  p.x = operand(a->X, a->sx, a->M, a->K, true, es);
+  p.w = operand(a->W, a->sw, a->N, a->K, true, es);
+  p.pr = plan_product(a->dtype, a->M, a->N, a->K);
+  p.off_w = copy_bytes(p.x, es);
+  p.off_part = p.off_w + copy_bytes(p.w, es);
+  p.bytes = p.off_part + p.pr.part_bytes;
+  return p;
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------
+int check_bwd(const GlDenseBwdArgs* a) {
+  if (!a || a->M < 0 || a->N < 1 || a->K < 1) return GL_ERR_ARG;
+  if (a->N > GL_DENSE_MAX_FEATURES || a->K > GL_DENSE_MAX_FEATURES || a->M >= GL_DENSE_MAX_ROWS) return GL_ERR_UNSUPPORTED;
+  if (!dtype_ok(a->dtype) || !dtype_ok(a->dy_dtype) || !dtype_ok(a->g_dtype)) return GL_ERR_UNSUPPORTED;
+  if (a->act < GL_ACT_IDENTITY || a->act > GL_ACT_GELU) return GL_ERR_ARG;
+  const bool fits = a->act == GL_ACT_IDENTITY ? a->keep == GL_KEEP_NONE
+                    : a->act == GL_ACT_RELU   ? a->keep == GL_KEEP_SIGN
+                                              : (a->keep == GL_KEEP_Z || a->keep == GL_KEEP_Z8);
+  if (!fits || (a->accumulate && a->g_dtype != GL_DTYPE_F32)) return GL_ERR_ARG;
+  if (a->M == 0) return 0;
+  if (!a->dY || (a->keep != GL_KEEP_NONE && !a->z) || (a->keep == GL_KEEP_Z8 && !a->z_exp)) return GL_ERR_ARG;
+  if (a->dX && !a->W) return GL_ERR_ARG;
+  if (a->dW && !a->X && (!a->xq || !a->xe)) return GL_ERR_ARG;
+  if (!row_ok(a->sdy, a->M, a->N) || (a->X && !row_ok(a->sx, a->M, a->K)) || (a->W && !row_ok(a->sw, a->N, a->K)))
+    return GL_ERR_ARG;
+  if (!on_element(a->dY, a->dy_dtype) || !on_element(a->X, a->dtype) || !on_element(a->W, a->dtype) ||
+      !on_element(a->dX, a->dtype) || !on_element(a->dW, a->g_dtype) || !on_element(a->db, a->g_dtype) ||
+      ((uintptr_t)a->z & 15) || ((uintptr_t)a->xq & 7))
+    return GL_ERR_ARG;
+  return 0;
+}
+struct BwdPlan {
+  bool own_dz;  // dz is written to workspace (else dY is dz as it stands)
+  Operand dz_nn, dz_tn, w, x;
+  Product px, pw;
+  long long chunks;
+  size_t off_x, off_w, off_part, off_db, bytes;
+};
+BwdPlan plan_bwd(const GlDenseBwdArgs* a) {
+  BwdPlan p{};
+  const int es = es_of(a->dtype);
+  const long long ldz = padded(a->N);
+  const bool products = a->dX || a->dW;
+  p.dz_nn = Operand{a->dY, a->sdy, a->M, a->N, true, false};
+  p.dz_tn = Operand{a->dY, a->sdy, a->M, a->N, false, false};
+  if (a->M == 1) p.dz_nn.ld = p.dz_tn.ld = ldz;
+  p.own_dz = products && (a->keep != GL_KEEP_NONE || a->dy_dtype != a->dtype || !in_place(p.dz_nn, es));
+  size_t at = 0;
+  if (p.own_dz) {
+    p.dz_nn.ld = p.dz_tn.ld = ldz;
+    at += (size_t)round_up(a->M * ldz * es, 256);
+  }
+  p.off_x = at;
+  size_t part = 0;
+  if (a->dW) {
+    if (a->X) {
+      p.x = operand(a->X, a->sx, a->M, a->K, false, es);
+      at += copy_bytes(p.x, es);
+    } else {
+      p.x = Operand{nullptr, padded(a->K), a->M, a->K, false, false};
+      at += (size_t)round_up(a->M * padded(a->K) * es, 256);
+    }
+    p.pw = plan_product(a->dtype, a->N, a->K, a->M);
+    part = p.pw.part_bytes;
+  }
+  p.off_w = at;
+  if (a->dX) {
+    p.w = operand(a->W, a->sw, a->N, a->K, false, es);
+    at += copy_bytes(p.w, es);
+    p.px = plan_product(a->dtype, a->M, a->K, a->N);
+    part = part > p.px.part_bytes ? part : p.px.part_bytes;
+  }
+  p.off_part = at;
+  at += part;
+  p.off_db = at;
+  p.chunks = (a->M + DZ_ROWS - 1) / DZ_ROWS;
+  if (a->db) at += (size_t)round_up(p.chunks * a->N * 4, 256);
+  p.bytes = at;
+  return p;
+}
+
+template <bool YBF>
+int launch_dz(const GlDenseBwdArgs* a, void* dz, float* part, hipStream_t s) {
+  const dim3 grid((unsigned)((a->M + DZ_ROWS - 1) / DZ_ROWS), (unsigned)ceil_div(a->N, DZ_COLS));
+  if (a->dtype == GL_DTYPE_BF16)
+    GL_LAUNCH(GL_KERNEL_DENSE_DZ, (dense_dz_kernel<YBF, true>), grid, dim3(256), 0, s, a->dY, a->sdy, a->z, a->z_exp, a->keep,
+              (long long)a->M, a->N, dz, part);
+  else
+    GL_LAUNCH(GL_KERNEL_DENSE_DZ, (dense_dz_kernel<YBF, false>), grid, dim3(256), 0, s, a->dY, a->sdy, a->z, a->z_exp,
+              a->keep, (long long)a->M, a->N, dz, part);
+  GL_CHECK_LAUNCH();
+  return 0;
+}
+
+DenseEpi store_epi(void* C, long long sc, int c_dtype, long long M, int N, int op_dtype, int accumulate) {
+  DenseEpi e{};
+  e.C = C;
+  e.sc = sc;
+  e.M = M;
+  e.N = N;
+  e.act = GL_ACT_IDENTITY;
+  e.keep = GL_KEEP_NONE;
+  e.op_bf = op_dtype == GL_DTYPE_BF16;
+  e.c_bf = c_dtype == GL_DTYPE_BF16;
+  e.accumulate = accumulate;
+  return e;
+}
+
+}  // namespace
+
+}  // namespace gl
+
+using namespace gl;
+
+extern "C" int gl_dense_fwd_workspace(const GlDenseArgs* a, size_t* bytes) {
+  GL_TRY(check_fwd(a));
+  if (!bytes) return GL_ERR_ARG;
+  *bytes = a->M == 0 ? 0 : plan_fwd(a).bytes;
+  return 0;
+}
+
+extern "C" int gl_dense_fwd(const GlDenseArgs* a, void* stream) {
+  GL_TRY(check_fwd(a));
+  if (a->M == 0) return 0;
+  FwdPlan p = plan_fwd(a);
+  if (p.bytes && (!a->ws || ((uintptr_t)a->ws & 255))) return GL_ERR_ARG;
+  if (a->ws_bytes < p.bytes) return GL_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  DenseEpi e = store_epi(a->Y, a->sy, a->y_dtype, a->M, a->N, a->dtype, 0);
+  e.bias = a->bias;
+  e.res = a->res;
+  e.sr = a->sr;
+  e.res_bf = a->res_dtype == GL_DTYPE_BF16;
+  e.z = a->z;
+  e.ze = a->z_exp;
+  e.act = a->act;
+  e.keep = a->keep;
+  if (p.few) return launch_dense_few(a, e, s);
+  const int es = es_of(a->dtype);
+  char* ws = (char*)a->ws;
+  if (p.x.copied) GL_TRY(launch_align(p.x, es, ws, s));
+  if (p.w.copied) GL_TRY(launch_align(p.w, es, ws + p.off_w, s));
+  return run_product(a->dtype, DENSE_NT, p.x, p.w, a->K, p.pr, ws + p.off_part, e, s);
+}
+
+extern "C" int gl_dense_bwd_workspace(const GlDenseBwdArgs* a, size_t* bytes) {
+  GL_TRY(check_bwd(a));
+  if (!bytes) return GL_ERR_ARG;
+  *bytes = a->M == 0 ? 0 : plan_bwd(a).bytes;
+  return 0;
+}
+
+extern "C" int gl_dense_bwd(const GlDenseBwdArgs* a, void* stream) {
+  GL_TRY(check_bwd(a));
+  if (a->M == 0) return 0;
+  BwdPlan p = plan_bwd(a);
+  if (p.bytes && (!a->ws || ((uintptr_t)a->ws & 255))) return GL_ERR_ARG;
+  if (a->ws_bytes < p.bytes) return GL_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  const int es = es_of(a->dtype);
+  char* ws = (char*)a->ws;
+  void* dz = p.own_dz ? ws : nullptr;
+  float* db_part = a->db ? (float*)(ws + p.off_db) : nullptr;
+  if (dz || db_part) GL_TRY(a->dy_dtype == GL_DTYPE_BF16 ? launch_dz<true>(a, dz, db_part, s) : launch_dz<false>(a, dz, db_part, s));
+  if (a->db) {
+    GL_LAUNCH(GL_KERNEL_DENSE_DB, dense_db_kernel, dim3((unsigned)ceil_div(a->N, 32)), dim3(1024), 0, s, (const float*)db_part,
+              p.chunks, a->N, a->db, (int)(a->g_dtype == GL_DTYPE_BF16), a->accumulate);
+    GL_CHECK_LAUNCH();
+  }
+  if (dz) p.dz_nn.p = p.dz_tn.p = dz;
+  if (a->dX) {
+    if (p.w.copied) GL_TRY(launch_align(p.w, es, ws + p.off_w, s));
+    GL_TRY(run_product(a->dtype, DENSE_NN, p.dz_nn, p.w, a->N, p.px, ws + p.off_part,
+                       store_epi(a->dX, a->K, a->dtype, a->M, a->K, a->dtype, 0), s));
+  }
+  if (a->dW) {
+    if (!a->X) {
+      GL_TRY(launch_unpack8(a->xq, a->xe, a->M, a->K, ws + p.off_x, p.x.ld, a->dtype, s));
+      p.x.p = ws + p.off_x;
+    } else if (p.x.copied) {
+      GL_TRY(launch_align(p.x, es, ws + p.off_x, s));
+    }
+    GL_TRY(run_product(a->dtype, DENSE_TN, p.dz_tn, p.x, a->M, p.pw, ws + p.off_part,
+                       store_epi(a->dW, a->K, a->g_dtype, a->N, a->K, a->dtype, a->accumulate), s));
+  }
+  return 0;
+}

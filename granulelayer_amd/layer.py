@@ -16,6 +16,7 @@ from typing import Optional, Union
 import torch
 from torch import nn
 
+from .activations8 import check_activation_checkpoint
 from .autograd import Level1Runtime, SparsePoolFunction, resolve_policy
 from .semantic import SemanticPoolFunction
 from .config import PhysicalPlan, PoolingConfig, check_workspace_budget
@@ -44,6 +45,7 @@ class SparsePoolingLayer(nn.Module):
         backend: str = "auto",
         weight_layout: str = "auto",
         connectivity=None,
+        activation_checkpoint: str = "exact",
     ):
         super().__init__()
         if shared_neurons is not None:
@@ -55,6 +57,8 @@ class SparsePoolingLayer(nn.Module):
             raise ValueError("weight_layout must be 'auto' or 'canonical' (packed storage is Mode B only)")
         if backend not in ("auto", "cuda", "hip"):
             raise ValueError("backend must be 'auto', 'cuda' or 'hip' (there is no Triton path)")
+        # "int8": between forward and backward the input is kept in 8 bits (activations8.py)
+        self.activation_checkpoint = check_activation_checkpoint(activation_checkpoint)
         self.cfg = PoolingConfig.parse(pooling, checkpoint_policy)
         if isinstance(pooling, (str, PoolingConfig)) or "checkpoint_policy" not in (pooling or {}):
             self.cfg.checkpoint_policy = checkpoint_policy
@@ -149,12 +153,12 @@ class SparsePoolingLayer(nn.Module):
         lead = x.shape[:-1]
         x2 = x.reshape(-1, x.shape[-1])
         rt = self._runtime()
+        rt.grad_call, rt.activation_checkpoint = torch.is_grad_enabled(), self.activation_checkpoint
         if self.cfg.is_semantic_hierarchy:
             tparams = [getattr(self, "t_" + n) for n in self._tnames]
             y = SemanticPoolFunction.apply(x2, self.weight, self.bias, rt, self.cfg, self.effective_policy,
                                            self.compute_dtype, self._tnames, *tparams)
         else:
-            rt.grad_call = torch.is_grad_enabled()
             y = SparsePoolFunction.apply(x2, self.weight, self.bias, rt, self.effective_policy, self.compute_dtype)
         return y.reshape(*lead, y.shape[-1])
 

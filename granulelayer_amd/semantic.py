@@ -22,7 +22,7 @@ from typing import Dict, List
 import torch
 
 from .autograd import (CHECKPOINT_BUDGET, Level1Runtime, _compute_operands, _grad_buffers, _ids_per_token,
-                       _level1_backward, _saved_stats, act_torch, fit_policy)
+                       _keep_input, _kept_input, _level1_backward, _saved_stats, act_torch, fit_policy)
 from .config import LevelSpec, PoolingConfig
 
 
@@ -121,17 +121,18 @@ class SemanticPoolFunction(torch.autograd.Function):
         ctx.rt, ctx.cfg, ctx.policy, ctx.compute_dtype, ctx.tnames = rt, cfg, policy, compute_dtype, tnames
         ctx.saved_keys = list(saved.keys())
         ctx.n_t = len(tparams)
-        ctx.save_for_backward(x, w, b, *tparams, *saved.values())
+        ctx.save_for_backward(*_keep_input(ctx, rt, x, xc), w, b, *tparams, *saved.values())
         rt.last_info["checkpoint_bytes"] = sum(t.numel() * t.element_size() for t in saved.values())
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, w, b, *rest = ctx.saved_tensors
+        kept, (w, b, *rest) = ctx.saved_tensors[:ctx.n_x], ctx.saved_tensors[ctx.n_x:]
         tparams = rest[: ctx.n_t]
         saved = dict(zip(ctx.saved_keys, rest[ctx.n_t:]))
         rt: Level1Runtime = ctx.rt
         l1 = rt.level
+        x, x_dtype = _kept_input(ctx, kept)
         xc, wc, bc = _compute_operands(x, w, b, ctx.compute_dtype)
         rebuilt = "pre" not in saved
         B = x.shape[0]
@@ -154,5 +155,5 @@ class SemanticPoolFunction(torch.autograd.Function):
         dx = _level1_backward(rt, xc, wc, bc, dF, saved, policy, dw_buf, db_buf, rebuilt)
         gw = None if use_main else dw_buf.to(w.dtype)
         gb = None if use_main else db_buf.to(b.dtype)
-        return (dx.to(x.dtype, memory_format=torch.contiguous_format), gw, gb, None, None, None, None, None,
+        return (dx.to(x_dtype, memory_format=torch.contiguous_format), gw, gb, None, None, None, None, None,
                 *grads[1:])

@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define GL_ABI_VERSION 13
+#define GL_ABI_VERSION 14
 
 enum {
   GL_OK = 0,
@@ -295,6 +295,88 @@ int gl_window_build_host(const int32_t* idx, const int32_t* counts, int32_t D, i
 int gl_window_build(const int32_t* idx, const int32_t* counts, int32_t D, int32_t G, int32_t S, int32_t sps,
                     int32_t gs, int32_t K, int32_t rec_shift, uint32_t* lo, int32_t* width, void* stream);
 
+/* ---- the dense projection beside the sparse one, and activations kept in 8 bits ----------------
+ *
+ *   z[m,n] = sum_k X[m,k] W[n,k] + bias[n]        Y[m,n] = act(z[m,n]) + res[m,n]
+ *
+ * with the layer's activations.  Operands are fp32, or bf16 with products and sums in fp32.  Rows of
+ * every tensor are a stride apart (in elements, any stride of at least the width), features are
+ * neighbours, and no address needs more than its element's alignment. */
+#define GL_DENSE_MAX_FEATURES 1048576 /* largest K, N and packed row */
+#define GL_DENSE_MAX_ROWS (1LL << 31) /* rows are fewer than this */
+/* What the forward keeps of z for the backward, [M, *] in `z`: nothing; z > 0 as bits (word n / 32
+ * of a row's ceil(N / 32) words, bit n % 32); z in the operands' type, rows round_up(N, 8) apart; z in
+ * 8 bits (gl_pack8's codes in z and exponents in z_exp). */
+enum { GL_KEEP_NONE = 0, GL_KEEP_SIGN = 1, GL_KEEP_Z = 2, GL_KEEP_Z8 = 3 };
+
+/* x [rows, cols] <-> its 8-bit form: blocks of 32 columns share a power of two step = 2^(e - 127),
+ * the smallest from 2^-126 to 2^121 that keeps every |rint(x / step)| <= 127, and every value is such a
+ * quotient (cut to 127 where a value is within 1/256 of the largest fp32 number).  q: rows of round_up(cols, 32) int8 codes, contiguous, 8-byte aligned; e: rows of
+ * ceil(cols / 32) bytes.  A block with an infinity or a NaN has e = 255 and reads back as NaN. */
+typedef struct GlPack8Args {
+  void* x;          /* read by gl_pack8, written by gl_unpack8 */
+  int64_t sx;       /* elements between rows */
+  int64_t rows;
+  int32_t cols;
+  int32_t x_dtype;  /* GL_DTYPE_* */
+  uint8_t* q;
+  uint8_t* e;
+} GlPack8Args;
+int gl_pack8(const GlPack8Args* a, void* stream);
+int gl_unpack8(const GlPack8Args* a, void* stream);
+
+typedef struct GlDenseArgs {
+  const void* X;    /* [M, K] of `dtype` */
+  int64_t sx;
+  const void* W;    /* [N, K] of `dtype` */
+  int64_t sw;
+  const void* bias; /* [N] of `dtype`, or NULL */
+  const void* res;  /* [M, N] of res_dtype, or NULL */
+  int64_t sr;       /* 0: every row adds the same */
+  void* Y;          /* [M, N] of y_dtype */
+  int64_t sy;
+  int64_t M;
+  int32_t N, K;
+  int32_t dtype, res_dtype, y_dtype;
+  int32_t act;      /* GL_ACT_* */
+  int32_t keep;     /* GL_KEEP_* */
+  void* z;
+  uint8_t* z_exp;
+  void* ws;         /* 256-byte aligned */
+  size_t ws_bytes;
+} GlDenseArgs;
+int gl_dense_fwd_workspace(const GlDenseArgs* a, size_t* bytes);
+int gl_dense_fwd(const GlDenseArgs* a, void* stream);
+
+/* The backward, from dY and what the forward kept:
+ *   dz = dY act'(z)     dX = dz W     dW (+)= dz^T X     db (+)= sum over the rows of dz
+ * Gradients that are NULL are not computed.  X comes as it was or in 8 bits (xq, xe). */
+typedef struct GlDenseBwdArgs {
+  const void* dY;   /* [M, N] of dy_dtype */
+  int64_t sdy;
+  const void* z;    /* what `keep` says (GL_KEEP_NONE: identity) */
+  const uint8_t* z_exp;
+  const void* X;    /* [M, K] of `dtype`, or NULL */
+  int64_t sx;
+  const uint8_t* xq; /* 8-bit codes and exponents of X where X is NULL */
+  const uint8_t* xe;
+  const void* W;    /* [N, K] of `dtype` (for dX) */
+  int64_t sw;
+  int64_t M;
+  int32_t N, K;
+  int32_t dtype, dy_dtype;
+  int32_t act, keep;
+  void* dX;         /* [M, K] of `dtype`, contiguous */
+  void* dW;         /* [N, K] of g_dtype, contiguous */
+  void* db;         /* [N] of g_dtype */
+  int32_t g_dtype;
+  int32_t accumulate; /* dW and db (fp32) are added to */
+  void* ws;         /* 256-byte aligned */
+  size_t ws_bytes;
+} GlDenseBwdArgs;
+int gl_dense_bwd_workspace(const GlDenseBwdArgs* a, size_t* bytes);
+int gl_dense_bwd(const GlDenseBwdArgs* a, void* stream);
+
 /* Kernel ids reported by the trace below. */
 enum {
   GL_KERNEL_TILE_X = 1, GL_KERNEL_FWD = 2, GL_KERNEL_FWD_FINALIZE = 3, GL_KERNEL_C1T = 4, GL_KERNEL_BWD_W = 5,
@@ -304,7 +386,12 @@ enum {
   GL_KERNEL_COVER = 14,                                /* Cover-TopK support selection */
   GL_KERNEL_SCHED = 15,                                /* gather schedule / pool windows on the GPU */
   GL_KERNEL_DX_DENSE = 16,                             /* dX of the smooth pools from per-neuron dz */
-  GL_KERNEL_DX_DMA = 17                                /* dX of 256-token slices, short segments */
+  GL_KERNEL_DX_DMA = 17,                               /* dX of 256-token slices, short segments */
+  GL_KERNEL_PACK8 = 18, GL_KERNEL_UNPACK8 = 19,        /* activations to 8 bits and back */
+  GL_KERNEL_DENSE = 20, GL_KERNEL_DENSE_FEW = 21,      /* dense products: tiled; few rows */
+  GL_KERNEL_DENSE_JOIN = 22,                           /* sums of a split product, with its epilogue */
+  GL_KERNEL_DENSE_DZ = 23, GL_KERNEL_DENSE_DB = 24,    /* dz and the partial sums of db; their sum */
+  GL_KERNEL_DENSE_ALIGN = 25                           /* operands copied to 16-byte rows */
 };
 
 /* Launch trace for benchmarks and tests (process-wide, not for concurrent callers): after

@@ -1,0 +1,119 @@
+"""Refusals and host logic of the dense projection and of activations in 8 bits (no GPU)."""
+import ctypes
+
+import pytest
+import torch
+
+from granulelayer_amd import (CoverTopK16Layer, DenseProjection, SparsePoolingLayer, dense_projection,
+                              pack_activation)
+from granulelayer_amd import _native as N
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def test_refused_arguments():
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    for bad in (dict(activation="tanh"), dict(activation_checkpoint="fp8"), dict(bias=torch.zeros(8)),
+                dict(residual=torch.zeros(4, 8)), dict(residual=torch.zeros(1, 6)), dict(residual=torch.zeros(6))):
+        with pytest.raises(ValueError):
+            dense_projection(x, w, **bad)
+    for bad in ((x, w[:, :7]), (x, w[0]), (x, w[:0]), (torch.zeros(4, 7), w), (torch.tensor(1.0), w)):
+        with pytest.raises(ValueError):
+            dense_projection(*bad)
+    for bad in (dict(x=x.half(), weight=w.half()), dict(x=x.bfloat16(), weight=w), dict(x=x, weight=w, bias=torch.zeros(6).bfloat16()),
+                dict(x=x, weight=w, residual=torch.zeros(4, 6).half()), dict(x=x.double(), weight=w.double())):
+        with pytest.raises(TypeError):
+            dense_projection(**bad)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        dense_projection(x, w)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        dense_projection(x, w.requires_grad_(True))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        pack_activation(x)
+    for bad in (torch.tensor(1.0), torch.zeros(3, 0)):
+        with pytest.raises(ValueError):
+            pack_activation(bad)
+
+
+def test_module():
+    lay = DenseProjection(64, 48, "relu", dtype=F32, seed=3, bias_std=0.1)
+    again = DenseProjection(64, 48, "relu", dtype=F32, seed=3, bias_std=0.1)
+    assert torch.equal(lay.weight, again.weight) and torch.equal(lay.bias, again.bias)
+    assert sorted(lay.state_dict()) == ["bias", "weight"] and lay.weight.shape == (48, 64)
+    assert abs(float(lay.weight.detach().std()) * 8 - 1) < 0.1  # 3072 values: the deviation is good to 1.3%
+    assert DenseProjection(64, 48, bias=False).bias is None
+    lay.enable_main_grad()
+    assert lay.weight.main_grad.dtype == F32 and lay.bias.main_grad.shape == (48,)
+    assert "activation_checkpoint=exact" in repr(lay)
+    for bad in (dict(activation="swish"), dict(activation_checkpoint="int4")):
+        with pytest.raises(ValueError):
+            DenseProjection(8, 8, **bad)
+    with pytest.raises(ValueError):
+        DenseProjection(0, 8)
+    with pytest.raises(NotImplementedError):
+        DenseProjection(8, 8, dtype=torch.float16)
+
+
+def test_library_refuses_before_the_device():
+    L = N.library().lib
+    out = ctypes.c_size_t()
+
+    def pack(**kw):
+        base = dict(x=4096, sx=40, rows=4, cols=40, x_dtype=0, q=4096, e=4096)
+        return L.gl_pack8(ctypes.byref(N.GlPack8Args(**dict(base, **kw))), None)
+
+    for bad in (dict(rows=-1), dict(cols=0), dict(cols=N.DENSE_MAX_FEATURES + 1), dict(x=0), dict(q=0), dict(e=0), dict(sx=39),
+                dict(x=4098), dict(q=4100)):
+        assert pack(**bad) == -1, bad
+    for bad in (dict(x_dtype=2), dict(rows=1 << 31)):
+        assert pack(**bad) == -2, bad
+    assert pack(rows=0, x=0, q=0, e=0) == 0
+    assert L.gl_pack8(None, None) == -1 and L.gl_unpack8(None, None) == -1
+
+    def fwd(query=True, **kw):
+        base = dict(X=4096, sx=64, W=8192, sw=64, Y=16384, sy=48, M=100, N=48, K=64, dtype=1, y_dtype=1)
+        a = N.GlDenseArgs(**dict(base, **kw))
+        return L.gl_dense_fwd_workspace(ctypes.byref(a), ctypes.byref(out)) if query else L.gl_dense_fwd(ctypes.byref(a), None)
+
+    assert fwd() == 0
+    for bad in (dict(X=0), dict(W=0), dict(Y=0), dict(sx=63), dict(sw=63), dict(sy=47), dict(M=-1), dict(N=0), dict(K=0),
+                dict(act=3), dict(keep=4), dict(keep=2), dict(keep=3, z=4096), dict(X=4097), dict(bias=4097),
+                dict(res=4096, sr=47, res_dtype=1), dict(res=4098, sr=48, res_dtype=0), dict(keep=1, z=4100)):
+        assert fwd(**bad) == -1 and fwd(False, **bad) == -1, bad
+    for bad in (dict(dtype=2), dict(y_dtype=7), dict(res=4096, sr=48, res_dtype=9), dict(N=N.DENSE_MAX_FEATURES + 1),
+                dict(M=1 << 31)):
+        assert fwd(**bad) == -2, bad
+    # odd rows are copied through workspace, which has to be there, aligned and large enough
+    assert fwd(sx=65) == 0 and out.value >= 100 * 64 * 2
+    assert fwd(False, sx=65) == -1 and fwd(False, sx=65, ws=4096 + 16, ws_bytes=1 << 20) == -1
+    assert fwd(False, sx=65, ws=4096, ws_bytes=100) == -3
+    assert fwd(False, M=0, X=0, W=0, Y=0) == 0
+
+    def bwd(query=True, **kw):
+        base = dict(dY=4096, sdy=48, X=4096, sx=64, W=8192, sw=64, M=100, N=48, K=64, dtype=1, dy_dtype=1, dX=4096, dW=4096,
+                    db=4096, g_dtype=1)
+        a = N.GlDenseBwdArgs(**dict(base, **kw))
+        return L.gl_dense_bwd_workspace(ctypes.byref(a), ctypes.byref(out)) if query else L.gl_dense_bwd(ctypes.byref(a), None)
+
+    assert bwd() == 0 and bwd(act=1, keep=1, z=4096) == 0 and bwd(act=2, keep=3, z=4096, z_exp=4096) == 0
+    for bad in (dict(dY=0), dict(sdy=47), dict(act=1), dict(act=2, keep=1, z=4096), dict(act=0, keep=2, z=4096),
+                dict(act=2, keep=2), dict(act=2, keep=3, z=4096), dict(W=0), dict(X=0), dict(X=0, xq=4096), dict(sx=3),
+                dict(accumulate=1), dict(dX=4097), dict(X=0, xq=4100, xe=4096)):
+        assert bwd(**bad) == -1 and bwd(False, **bad) == -1, bad
+    for bad in (dict(dtype=3), dict(dy_dtype=3), dict(g_dtype=3), dict(K=N.DENSE_MAX_FEATURES + 1)):
+        assert bwd(**bad) == -2, bad
+    assert bwd(False, ws=4096, ws_bytes=8) == -3
+    assert bwd(False, M=0, dY=0) == 0
+
+
+@pytest.mark.parametrize("form", ["sparse", "cover"])
+def test_sparse_layers_take_the_option(form):
+    def make(**kw):
+        if form == "sparse":
+            return SparsePoolingLayer(64, 2048, 8, shared_neurons=None, pooling="mean", dtype=F32, **kw)
+        return CoverTopK16Layer(64, 2048, 8, 256, **kw)
+
+    assert make().activation_checkpoint == "exact"
+    assert make(activation_checkpoint="int8").activation_checkpoint == "int8"
+    with pytest.raises(ValueError, match="activation_checkpoint"):
+        make(activation_checkpoint="int2")
