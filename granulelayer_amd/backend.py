@@ -42,7 +42,8 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 
 
 def _stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    # the handle itself: a Stream object around it costs the smallest calls several microseconds
+    return torch._C._cuda_getCurrentRawStream(dev.index if dev.index is not None else torch.cuda.current_device())
 
 
 _NO_SWITCH = contextlib.nullcontext()
@@ -468,11 +469,12 @@ class HipBackend:
         a = N.GlDenseArgs(_ptr(x), sx, _ptr(w), sw, _ptr(b), _ptr(res), sr, _ptr(y), F, M, F, K, code, rcode, ycode,
                           N.GL_ACT[activation], N.GL_KEEP[keep], _ptr(z), _ptr(z_exp), 0, 0)
         with _on(dev):
-            need = self.lib.size_query("gl_dense_fwd_workspace", a)
-            if need:
+            # few rows and whole tiles need no workspace: the call says so faster than a query before it
+            if self.lib.lib.gl_dense_fwd(ctypes.byref(a), _stream(dev)) != 0:
+                need = self.lib.size_query("gl_dense_fwd_workspace", a)
                 ws = torch.empty(need, device=dev, dtype=torch.uint8)
                 a.ws, a.ws_bytes = _ptr(ws), need
-            self.lib.call("gl_dense_fwd", ctypes.byref(a), _stream(dev))
+                self.lib.call("gl_dense_fwd", ctypes.byref(a), _stream(dev))
         return y, z, z_exp
 
     def dense_backward(self, dy, activation, keep, z, z_exp, x, xq, xe, w, dx, dw, db, accumulate):

@@ -20,9 +20,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-// Bytes of the reduction a stage holds per row: 64 bf16 or 32 fp32.
-constexpr int DENSE_BK = 128;
-
 // What becomes of a product's sums.
 struct DenseEpi {
   const void* bias;  // operands' type, or null
@@ -45,17 +42,49 @@ struct DenseK {
   long long ldp, ldq;  // bytes between rows
   long long R;         // reduction; behind it an RC operand's rows have zeros up to 16 bytes
   int tiles_m, tiles_n;
-  int steps, steps_per_split;  // stages of DENSE_BK bytes
+  int steps, steps_per_split;  // stages of the tile's dense_bk() bytes
   float* part;                 // split products: sums [split][M][N], joined by dense_join_kernel
   DenseEpi e;
 };
 
-// ---- epilogue ------------------------------------------------------------------------------------
-__device__ __forceinline__ float gelu_f(float z) { return 0.5f * z * (1.f + erff(z * 0.70710678118654752f)); }
+// ---- activations -----------------------------------------------------------------------------------
+// GELU from the normal distribution's upper tail: with a = |z| and Q(a) = 1 - Phi(a),
+//     gelu(z) = max(z, 0) - a Q(a)        gelu'(z) = Phi(z) + z phi(z)
+// and Q(a) = exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.305 a): P of degree 7 fitted to exp(a^2 / 2) Q(a) on
+// [0, 14] by weighted least squares, 1e-7 relative.  The form keeps its relative accuracy in the negative
+// tail, where 1 + erf cancels, and takes one exponential for Q and phi together: evaluated in fp32 gelu and
+// gelu' are within 2.4e-7 of the exact ones over [-13, 13].  Past 40, Q and phi are zero in fp32.
+// max(z, 0) by comparison: NaN stays NaN.
+__device__ __forceinline__ float tail_arg(float z) {
+  return __builtin_fabsf(z) > 40.f ? __builtin_copysignf(40.f, z) : z;
+}
+__device__ __forceinline__ float gauss(float z) { return __builtin_amdgcn_exp2f(z * z * -0.72134752f); }
+__device__ __forceinline__ float upper_tail(float a, float ex) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.305f, a, 1.f));
+  float p = 0.0366991945f;
+  p = __builtin_fmaf(p, t, -0.152988315f);
+  p = __builtin_fmaf(p, t, 0.185716912f);
+  p = __builtin_fmaf(p, t, -0.0379768424f);
+  p = __builtin_fmaf(p, t, 0.121021688f);
+  p = __builtin_fmaf(p, t, 0.103420861f);
+  p = __builtin_fmaf(p, t, 0.122466817f);
+  p = __builtin_fmaf(p, t, 0.121639736f);
+  return p * t * ex;
+}
+__device__ __forceinline__ float relu_f(float z) { return z < 0.f ? 0.f : z; }
+__device__ __forceinline__ float gelu_f(float z) {
+  const float a = __builtin_fminf(__builtin_fabsf(z), 40.f);  // NaN goes through relu_f
+  return __builtin_fmaf(-a, upper_tail(a, gauss(a)), relu_f(z));
+}
+__device__ __forceinline__ float dgelu_f(float z) {
+  const float c = tail_arg(z), ex = gauss(c), q = upper_tail(__builtin_fabsf(c), ex);
+  return __builtin_fmaf(c * 0.39894228f, ex, c < 0.f ? q : 1.f - q);
+}
 __device__ __forceinline__ float act_rt(int act, float z) {
-  return act == GL_ACT_RELU ? __builtin_fmaxf(z, 0.f) : (act == GL_ACT_GELU ? gelu_f(z) : z);
+  return act == GL_ACT_RELU ? relu_f(z) : (act == GL_ACT_GELU ? gelu_f(z) : z);
 }
 
+// ---- epilogue ------------------------------------------------------------------------------------
 // four neighbours of a row, of which the first n are there
 __device__ __forceinline__ void load4(const void* p, bool bf, long long i, int n, float (&v)[4]) {
   if (n >= 4) {
@@ -98,62 +127,115 @@ __device__ __forceinline__ void store4(void* p, bool bf, long long i, int n, con
   }
 }
 
-// The sums v of columns n..n + 3 of row m (n a multiple of 4).  Eight neighbouring lanes hold the 32
-// columns of a block, and all of them call this, whatever m and n.
-__device__ __forceinline__ void dense_epilogue(const DenseEpi& e, long long m, int n, float (&v)[4]) {
-  const bool in = m < e.M && n < e.N;
-  if (e.bias) {
-    float b[4];
-    load4(e.bias, e.op_bf, n, e.N - n, b);
+// Over the eight lanes that share 32 columns: neighbours, pairs, then the halves of the eight.
+template <typename OP>
+__device__ __forceinline__ unsigned over8(unsigned v, OP op) {
+  v = op(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));   // lane ^ 1
+  v = op(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));   // lane ^ 2
+  v = op(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));  // 7 - lane: the other four
+  return v;
+}
+
+// What is kept of z and the activation, for the sums v of columns n..n + 3 (n a multiple of 4) of the G rows m,
+// m + dm, ..., to which the bias b is added.  Eight neighbouring lanes hold the 32 columns of a block, and all of
+// them call this, whatever m and n.  Choices are made for all rows at once.
+template <int G>
+__device__ __forceinline__ void dense_forward(const DenseEpi& e, long long m, int dm, int n, float (&v)[G][4],
+                                              const float (&b)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += b[j];
-  }
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[g][j] += b[j];
+  const int there = e.N - n, nblk = (e.N + 31) / 32;
   if (e.keep == GL_KEEP_SIGN) {
-    unsigned w = 0;
+    unsigned* z = (unsigned*)e.z + m * nblk + n / 32;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (n + j < e.N && v[j] > 0.f) w |= 1u << ((n & 31) + j);
-    w |= (unsigned)__shfl_xor((int)w, 1);
-    w |= (unsigned)__shfl_xor((int)w, 2);
-    w |= (unsigned)__shfl_xor((int)w, 4);
-    if (in && (n & 31) == 0) ((unsigned*)e.z)[m * ((e.N + 31) / 32) + n / 32] = w;
+    for (int g = 0; g < G; ++g) {
+      unsigned w = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < there && v[g][j] > 0.f) w |= 1u << j;
+      w = over8(w << (n & 31), [](unsigned x, unsigned y) { return x | y; });
+      if (m + g * dm < e.M && there > 0 && (n & 31) == 0) z[(long long)g * dm * nblk] = w;
+    }
   } else if (e.keep == GL_KEEP_Z) {
-    if (in) store4(e.z, e.op_bf, m * ((e.N + 7) / 8 * 8) + n, e.N - n, v);
+    const long long ldz = (e.N + 7) / 8 * 8;  // rows have room to 8
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (m + g * dm < e.M && there > 0) store4(e.z, e.op_bf, (m + g * dm) * ldz + n, 4, v[g]);
   } else if (e.keep == GL_KEEP_Z8) {
-    const int nblk = (e.N + 31) / 32;
-    unsigned a = 0;
-    float t[4];
+    uint8_t* z = (uint8_t*)e.z + (m * nblk * 32 + n);
+    uint8_t* ze = e.ze + (m * nblk + n / 32);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      t[j] = n + j < e.N ? v[j] : 0.f;
-      a = umax(a, abs_bits(t[j]));
+    for (int g = 0; g < G; ++g) {
+      float t[4];
+      unsigned a = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t[j] = j < there ? v[g][j] : 0.f;
+        a = umax(a, abs_bits(t[j]));
+      }
+      a = over8(a, [](unsigned x, unsigned y) { return umax(x, y); });
+      const int ex = p8_exp(a);
+      const unsigned q = p8_codes4(t[0], t[1], t[2], t[3], p8_inv_step(ex));
+      if (m + g * dm < e.M && n < nblk * 32) {
+        *(unsigned*)(z + (long long)g * dm * nblk * 32) = q;
+        if ((n & 31) == 0) ze[(long long)g * dm * nblk] = (uint8_t)ex;
+      }
     }
-    a = umax(a, (unsigned)__shfl_xor((int)a, 1));
-    a = umax(a, (unsigned)__shfl_xor((int)a, 2));
-    a = umax(a, (unsigned)__shfl_xor((int)a, 4));
-    const int ex = p8_exp(a);
-    if (m < e.M && n < nblk * 32) {
-      *(unsigned*)((uint8_t*)e.z + (m * nblk * 32 + n)) = p8_codes4(t[0], t[1], t[2], t[3], p8_inv_step(ex));
-      if ((n & 31) == 0) e.ze[m * nblk + n / 32] = (uint8_t)ex;
+  }
+  if (e.act == GL_ACT_GELU) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[g][j] = gelu_f(v[g][j]);
+  } else if (e.act == GL_ACT_RELU) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[g][j] = relu_f(v[g][j]);
+  }
+}
+__device__ __forceinline__ void dense_bias(const DenseEpi& e, int n, float (&b)[4]) {
+  if (e.bias) load4(e.bias, e.op_bf, n, e.N - n, b);
+  else b[0] = b[1] = b[2] = b[3] = 0.f;
+}
+// What is added last, as it is stored: the residual, or the gradient that C accumulates.
+struct Added {
+  const char* p;
+  long long step;  // bytes of a row
+  bool bf;
+};
+__device__ __forceinline__ Added dense_added(const DenseEpi& e) {
+  if (e.res) return {(const char*)e.res, e.sr * (e.res_bf ? 2 : 4), e.res_bf != 0};
+  if (e.accumulate) return {(const char*)e.C, e.sc * 4, false};
+  return {nullptr, 0, false};
+}
+__device__ __forceinline__ uv4 load_added(const char* p, bool bf, int n) {
+  uv4 v = {0u, 0u, 0u, 0u};
+  if (n >= 4) {
+    if (bf) {
+      const uv2 w = reinterpret_cast<const bytes8*>(p)->v;
+      v[0] = w[0];
+      v[1] = w[1];
+    } else {
+      v = reinterpret_cast<const bytes16*>(p)->v;
     }
-  }
-  if (!in) return;
-  if (e.act != GL_ACT_IDENTITY) {
+  } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = act_rt(e.act, v[j]);
+    for (int j = 0; j < 3; ++j)
+      if (j < n) {
+        if (bf) v[j >> 1] |= (unsigned)((const unsigned short*)p)[j] << (16 * (j & 1));
+        else v[j] = ((const unsigned*)p)[j];
+      }
   }
-  float r[4];
-  if (e.res) {
-    load4(e.res, e.res_bf, m * e.sr + n, e.N - n, r);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += r[j];
-  }
-  if (e.accumulate) {
-    load4(e.C, false, m * e.sc + n, e.N - n, r);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += r[j];
-  }
-  store4(e.C, e.c_bf, m * e.sc + n, e.N - n, v);
+  return v;
+}
+__device__ __forceinline__ void add_added(float (&v)[4], uv4 r, bool bf) {
+  v[0] += __uint_as_float(bf ? r[0] << 16 : r[0]);
+  v[1] += __uint_as_float(bf ? r[0] & 0xffff0000u : r[1]);
+  v[2] += __uint_as_float(bf ? r[1] << 16 : r[2]);
+  v[3] += __uint_as_float(bf ? r[1] & 0xffff0000u : r[3]);
 }
 
 // ---- the tile kernel -------------------------------------------------------------------------------
@@ -175,11 +257,12 @@ __device__ __forceinline__ void tile_of(int bid, int nblk, int tiles_m, int tile
 }
 
 // 16 bytes per lane straight from a buffer into LDS at (wave-uniform) lds + 16 lane; offsets at or past
-// the buffer's size put zeros there.  Issued from asm so that the compiler's own waits do not count it:
-// the caller waits with stage_wait() and a barrier before the data is read.
+// the buffer's size put zeros there.  Issued from asm so that the compiler's own waits do not count it: the
+// kernel waits with copies_barrier(), which is also what keeps reads of the data behind it.  (No clobber of
+// memory here: nothing reads these bytes before that barrier, and fragments' reads may move past the copy.)
 __device__ __forceinline__ void dma16(unsigned off, i32x4 rsrc, unsigned lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-               :: "v"(off), "s"(rsrc), "s"(lds) : "memory", "m0");
+               :: "v"(off), "s"(rsrc), "s"(lds) : "m0");
 }
 __device__ __forceinline__ i32x4 buffer_of(const char* p, long long bytes) {
   const unsigned long long a = (unsigned long long)p;
@@ -191,29 +274,32 @@ __device__ __forceinline__ i32x4 buffer_of(const char* p, long long bytes) {
   r[3] = 0x00020000;
   return r;
 }
-constexpr unsigned DMA_NOWHERE = 0x80000000u;  // past any buffer_of
+constexpr unsigned DMA_NOWHERE = 0x80000000u;  // past any buffer_of; offsets are below
 
-// One operand's side of a tile: DIM rows of the output (RC) or columns (RS) by DENSE_BK bytes of
-// reduction, staged by NW waves.
+// One operand's side of a tile: DIM rows of the output (RC) or columns (RS) by BK bytes of reduction,
+// staged by NW waves.
 //
-// LDS of an RC operand: rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7), so that the 32 rows
-// of a fragment's read fall on all banks.  Of an RS operand: the reduction's rows of DIM values; for
-// bf16 the 32-byte unit u of row r at u ^ swz(r): a transposing read takes 32 bytes of four rows r..r + 3
-// (two such groups per half wave, of neighbouring units), and the swizzle puts those on all banks.
-template <int ES, int DIM, int NW, bool RC>
+// LDS of an RC operand: rows of BK bytes, 16-byte chunk c of row r at c ^ key(r).  A 16-byte read of 16
+// neighbouring rows takes each of the 16 chunks of a 256-byte bank row once, and rows 16..31 take them in
+// the same order: LDS then delivers 256 bytes a clock (half of it with c ^ (r & 7) at BK = 128: rows r and
+// r + 8 collide).  Of an RS operand: the reduction's rows of DIM values; for bf16 the 32-byte unit u of row
+// r at u ^ swz(r): a transposing read takes 32 bytes of four rows r..r + 3 (two such groups per half wave,
+// of neighbouring units), and the swizzle puts those on all banks.
+template <int ES, int DIM, int NW, bool RC, int BK>
 struct Side {
-  static constexpr int BYTES = DIM * DENSE_BK;
+  static constexpr int BYTES = DIM * BK;
   static constexpr int LOADS = BYTES / 1024 / NW;  // of one wave and stage
-  static constexpr int RROWS = DENSE_BK / ES;      // rows of an RS stage
+  static constexpr int RROWS = BK / ES;            // rows of an RS stage
   static constexpr int PITCH = DIM * ES;
-  static_assert(LOADS * NW * 1024 == BYTES, "whole loads");
+  static constexpr int CPR = BK / 16;
+  static_assert(LOADS * NW * 1024 == BYTES && NW % 2 == 0, "whole loads; key() of a lane's rows is the wave's");
 
   const char* p;
   long long ld, left;  // bytes: of a row; from p to the operand's end
   unsigned off[LOADS];
-  int k_lane;  // RC: this lane's first byte of the reduction in a stage
-  long long rbytes;
+  int k_lane, k_left;  // RC: this lane's first byte of the reduction in a stage; the reduction's bytes from p
 
+  static __device__ __forceinline__ int key(int r) { return BK == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
   static __device__ __forceinline__ int swz(int r) {
     if constexpr (ES == 2) return (((r & 3) << 1) | (((r >> 3) & 1) << 3)) & (DIM / 16 - 1);
     return 0;
@@ -227,14 +313,14 @@ struct Side {
     // of a 16-byte-aligned row are there (zeros behind an RC row's end, columns that nobody stores
     // behind an RS row's).
     ld = ldb;
-    rbytes = (R * ES + 15) & ~15LL;
     if constexpr (RC) {
-      p = (const char*)base + first * ld + (long long)step0 * DENSE_BK;
-      left = (dim - 1 - first) * ld + rbytes - (long long)step0 * DENSE_BK;
-      rbytes -= (long long)step0 * DENSE_BK;
-      k_lane = ((l & 7) ^ (l >> 3)) * 16;
+      const long long rbytes = (R * ES + 15) & ~15LL;  // at most GL_DENSE_MAX_FEATURES values
+      p = (const char*)base + first * ld + (long long)step0 * BK;
+      left = (dim - 1 - first) * ld + rbytes - (long long)step0 * BK;
+      k_left = (int)rbytes - step0 * BK;
+      k_lane = ((l % CPR) ^ key(w * (64 / CPR) + l / CPR)) * 16;
 #pragma unroll
-      for (int t = 0; t < LOADS; ++t) off[t] = (unsigned)((t * NW + w) * 8 + (l >> 3)) * (unsigned)ld + k_lane;
+      for (int t = 0; t < LOADS; ++t) off[t] = (unsigned)((t * NW + w) * (64 / CPR) + l / CPR) * (unsigned)ld + k_lane;
     } else {
       p = (const char*)base + (long long)step0 * RROWS * ld + first * ES;
       left = (R - 1 - (long long)step0 * RROWS) * ld + (((dim - first) * ES + 15) & ~15LL);
@@ -246,49 +332,56 @@ struct Side {
       }
     }
   }
-  // issue the loads of the next stage into LDS at `lds` and step on
-  __device__ __forceinline__ void issue(unsigned lds) {
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const i32x4 b = buffer_of(p, left);
-#pragma unroll
-    for (int t = 0; t < LOADS; ++t) {
-      unsigned o = off[t];
-      if constexpr (RC) o = k_lane < rbytes ? o : DMA_NOWHERE;
-      dma16(o, b, lds + (t * NW + w) * 1024);
-    }
+  // Copies of the next stage: prepare() and open() it, then copy() its parts in any order.  Stages past the
+  // reduction's end are zeros.
+  i32x4 rsrc, next_rsrc;
+  unsigned dead, next_dead;  // RC: bit 31 where the lane's chunk is past the reduction's end
+  __device__ __forceinline__ void prepare() {
+    next_rsrc = buffer_of(p, left);
+    const long long step = RC ? (long long)BK : RROWS * ld;
+    p += step;
+    left -= step;
     if constexpr (RC) {
-      p += DENSE_BK;
-      left -= DENSE_BK;
-      rbytes -= DENSE_BK;
-    } else {
-      p += RROWS * ld;
-      left -= RROWS * ld;
+      next_dead = k_lane < k_left ? 0u : DMA_NOWHERE;
+      k_left -= BK;
     }
+  }
+  __device__ __forceinline__ void open() {
+    rsrc = next_rsrc;
+    dead = next_dead;
+  }
+  __device__ __forceinline__ void copy(int t, unsigned lds) const {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    dma16(RC ? off[t] | dead : off[t], rsrc, lds + (t * NW + w) * 1024);
   }
 };
 
 // A lane's part of a 32-row fragment: row l % 32, and of the 32 bytes of reduction at kk * 32 the half l / 32.
 template <int ES> struct Frag;
 template <> struct Frag<2> {
+  static constexpr int STEPS = 1;  // matrix instructions
   bf16x8 v;
 };
 template <> struct Frag<4> {
+  static constexpr int STEPS = 4;
   f32x4 v;
 };
 
-template <int ES, int DIM, bool RC>
+template <int ES, int DIM, bool RC, int BK>
 struct Reader {
-  unsigned a[4];  // RC: byte of chunk kk; RS: see at()
+  static constexpr int READS = RC ? 1 : (ES == 2 ? 2 : 4);  // LDS instructions of a fragment
+  unsigned a[RC ? BK / 32 : 1];       // byte of chunk kk in the lane's row
   unsigned col[RC ? 1 : DIM / 32];
   // base: this wave's first row / column of the tile, a multiple of 32
   __device__ __forceinline__ void init(int base) {
     const int l = threadIdx.x & 63;
     if constexpr (RC) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) a[kk] = (base + (l & 31)) * DENSE_BK + (((2 * kk + (l >> 5)) ^ (l & 7)) * 16);
+      for (int kk = 0; kk < BK / 32; ++kk)
+        a[kk] = (base + (l & 31)) * BK + (((2 * kk + (l >> 5)) ^ Side<ES, DIM, 2, true, BK>::key(l & 31)) * 16);
     } else if constexpr (ES == 2) {
       const int g = l >> 4, i = l & 15, r = 8 * (g >> 1) + (i >> 2);
-      const int sw = Side<ES, DIM, 1, false>::swz(r);
+      const int sw = Side<ES, DIM, 2, false, BK>::swz(r);
 #pragma unroll
       for (int t = 0; t < DIM / 32; ++t)
         col[t] = r * (DIM * 2) + (((base / 16 + 2 * t + (g & 1)) ^ sw) * 32) + 8 * (i & 3);
@@ -299,7 +392,7 @@ struct Reader {
   __device__ __forceinline__ Frag<ES> read(const char* lds, int t, int kk) const {
     Frag<ES> f;
     if constexpr (RC) {
-      f.v = *reinterpret_cast<const decltype(f.v)*>(lds + a[kk] + t * 32 * DENSE_BK);
+      f.v = *reinterpret_cast<const decltype(f.v)*>(lds + a[kk] + t * 32 * BK);
     } else if constexpr (ES == 2) {
       typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
       union {
@@ -320,21 +413,25 @@ struct Reader {
 };
 
 // rows of the output are Q's (n), its columns P's (m): a lane then holds neighbours of a row of C
-__device__ __forceinline__ f32x16 mma(const Frag<2>& q, const Frag<2>& p, f32x16 c) {
+__device__ __forceinline__ f32x16 mma(const Frag<2>& q, const Frag<2>& p, int, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(q.v, p.v, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mma(const Frag<4>& q, const Frag<4>& p, f32x16 c) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(q.v[e], p.v[e], c, 0, 0, 0);
-  return c;
+__device__ __forceinline__ f32x16 mma(const Frag<4>& q, const Frag<4>& p, int x, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(q.v[x], p.v[x], c, 0, 0, 0);
 }
 
-template <int ES, int BM, int BN, int WM, int WN, bool PRC, bool QRC>
-__global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DenseK a) {
+// Every wave's LDS accesses and all but N of its copies done, then the workgroup's barrier.
+template <int N>
+__device__ __forceinline__ void copies_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <int ES, int BM, int BN, int WM, int WN, int BK, int NSP, int NSQ, bool PRC, bool QRC>
+__global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 8192 ? 1 : 2) void dense_tile_kernel(DenseK a) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
-  typedef Side<ES, BM, NW, PRC> SP;
-  typedef Side<ES, BN, NW, QRC> SQ;
-  constexpr int STAGE = SP::BYTES + SQ::BYTES;
+  typedef Side<ES, BM, NW, PRC, BK> SP;
+  typedef Side<ES, BN, NW, QRC, BK> SQ;
+  constexpr int LDS_Q = NSP * SP::BYTES, LDS = LDS_Q + NSQ * SQ::BYTES;  // P's stages, then Q's
   extern __shared__ __align__(1024) char smem[];
   int tm, tn, split;
   tile_of(blockIdx.x, gridDim.x, a.tiles_m, a.tiles_n, tm, tn, split);
@@ -348,8 +445,8 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DenseK a) {
   SQ sq;
   sp.init(a.P, a.ldp, m0, a.e.M, a.R, k0);
   sq.init(a.Q, a.ldq, n0, a.e.N, a.R, k0);
-  Reader<ES, BM, PRC> rp;
-  Reader<ES, BN, QRC> rq;
+  Reader<ES, BM, PRC, BK> rp;
+  Reader<ES, BN, QRC, BK> rq;
   rp.init(wm * TM * 32);
   rq.init(wn * TN * 32);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
@@ -362,86 +459,223 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DenseK a) {
 #pragma unroll
       for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.f;
 
-  sp.issue(lds0);
-  sq.issue(lds0 + SP::BYTES);
-  for (int k = 0; k < nk; ++k) {
-    const unsigned cur = (k & 1) * STAGE, nxt = STAGE - cur;
-    stage_wait();
-    __syncthreads();
-    if (k + 1 < nk) {
-      sp.issue(lds0 + nxt);
-      sq.issue(lds0 + nxt + SP::BYTES);
+  // A stage is KK parts of 32 bytes of reduction.  Fragments are read a part ahead of the products that
+  // take them, across stages too: the barrier that opens a stage stands before the last part of the stage
+  // ahead of it, whose products cover the barrier and the first reads.  From then on nobody reads the
+  // stage that ends, and copies of a stage further on go there: Q's NSQ on, with the last part, then P's NSP on,
+  // a share with each part (issued at once they hold up every wave behind the CU's one address unit).
+  constexpr int KK = BK / 32, LP = SP::LOADS, LQ = SQ::LOADS, COPIES = LP + LQ;
+  constexpr int SHARE = (COPIES + KK - 1) / KK, FIRST_SHARE = NSP > NSQ && LQ > SHARE ? LQ : SHARE;
+  constexpr int REST_SHARE = KK > 1 ? (COPIES - FIRST_SHARE + KK - 2) / (KK - 1) : 0;
+  // copies issued behind those of Q's next stage (and of P's, which is no later) when that has to be there
+  constexpr int BEHIND = (NSQ - 2) * COPIES + (NSP - NSQ) * LP;
+  static_assert(NSQ >= 2 && (NSP == NSQ || NSP == NSQ + 1) && BEHIND + FIRST_SHARE < 64 && KK % 2 == 0, "stages, parts");
+  Frag<ES> fp[2][TM], fq[2][TN];
+  auto copy = [&](int c, unsigned to_p, unsigned to_q) {
+    if (c < LQ) sq.copy(c, lds0 + to_q);
+    else sp.copy(c - LQ, lds0 + to_p);
+  };
+  unsigned cur_p = 0, cur_q = LDS_Q, to_p = (NSP - 1) * SP::BYTES, to_q = LDS_Q + (NSQ - 1) * SQ::BYTES;
+  // Products of the fragments of `set`, a row of the wave's tile at a time; with the first rows reads of
+  // part kk of the current stage into the other set, with the last the copies [c0, c1).  Reads come first so
+  // that a barrier behind the part finds them done.
+  constexpr int FIRST = TM > 1 ? TM / 2 : 1, LATER = TM - FIRST > 0 ? TM - FIRST : 1;
+  auto part_of = [&](int set, bool reads, int kk, int c0, int c1, bool prepare) {
+    const char* lp = smem + cur_p;
+    const char* lq = smem + cur_q;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int x = 0; x < Frag<ES>::STEPS; ++x)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mma(fq[set][j], fp[set][i], x, acc[i][j]);
+      if (reads && i < FIRST) {
+        if (i == 0)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) fq[set ^ 1][j] = rq.read(lq, j, kk);
+#pragma unroll
+        for (int h = i * TM / FIRST; h < (i + 1) * TM / FIRST; ++h) fp[set ^ 1][h] = rp.read(lp, h, kk);
+      }
+      if (i >= TM - LATER) {
+        const int y = i - (TM - LATER), n = c1 - c0;
+#pragma unroll
+        for (int c = y * n / LATER; c < (y + 1) * n / LATER; ++c)
+          if (c0 + c < COPIES) copy(c0 + c, to_p, to_q);
+      }
+      if (prepare && i == TM - 1) {
+        sp.prepare();
+        sq.prepare();
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const char* lp = smem + cur;
-    const char* lq = lp + SP::BYTES;
+  };
+  auto stage_of_p = [&](unsigned at) {
+    sp.prepare();
+    sp.open();
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      Frag<ES> fp[TM], fq[TN];
+    for (int c = 0; c < LP; ++c) sp.copy(c, lds0 + at);
+  };
+  if constexpr (NSP > NSQ) stage_of_p(0);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) fp[i] = rp.read(lp, i, kk);
+  for (int s = 0; s < NSQ - 1; ++s) {
+    sq.prepare();
+    sq.open();
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fq[j] = rq.read(lq, j, kk);
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mma(fq[j], fp[i], acc[i][j]);
-    }
+    for (int c = 0; c < LQ; ++c) sq.copy(c, lds0 + LDS_Q + s * SQ::BYTES);
+    stage_of_p((s + NSP - NSQ) * SP::BYTES);
   }
+  sp.prepare();
+  sq.prepare();
+  sp.open();
+  sq.open();
+#pragma unroll
+  for (int c = 0; c < FIRST_SHARE; ++c) copy(c, to_p, to_q);
+  copies_barrier<BEHIND + FIRST_SHARE>();
+#pragma unroll
+  for (int j = 0; j < TN; ++j) fq[0][j] = rq.read(smem + LDS_Q, j, 0);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) fp[0][i] = rp.read(smem, i, 0);
+  for (int k = 0; k < nk - 1; ++k) {
+#pragma unroll
+    for (int kk = 0; kk < KK - 1; ++kk)
+      part_of(kk & 1, true, kk + 1, FIRST_SHARE + kk * REST_SHARE, FIRST_SHARE + (kk + 1) * REST_SHARE, kk == KK - 2);
+    to_p = cur_p;
+    to_q = cur_q;
+    cur_p = cur_p == (NSP - 1) * SP::BYTES ? 0 : cur_p + SP::BYTES;
+    cur_q = cur_q == LDS_Q + (NSQ - 1) * SQ::BYTES ? LDS_Q : cur_q + SQ::BYTES;
+    sp.open();
+    sq.open();
+    copies_barrier<BEHIND>();
+    part_of((KK - 1) & 1, true, 0, 0, FIRST_SHARE, false);
+  }
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) part_of(kk & 1, kk + 1 < KK, kk + 1, 0, 0, false);
 
-  // The sums go through LDS, 32 rows of the wave's 64 columns at a time, so that a lane gets 4 neighbours
-  // of a row, 16 lanes a whole row (128 bytes of bf16), and the epilogue is a rolled loop.  Rows are 68
-  // floats apart: 16 rows of a store then fall on all banks.
-  static_assert(TN == 2 && NW * 32 * 68 * 4 <= 2 * STAGE, "a wave's rows of 64 columns");
-  __syncthreads();
+  // The sums go through LDS, 32 rows of 64 columns of the wave at a time, so that a lane gets 4 neighbours
+  // of a row and 16 lanes a whole row (128 bytes of bf16).  Rows are 68 floats apart: 16 rows of a store then
+  // fall on all banks.  What is added to 16 rows is loaded before the stores of the 16 ahead of them:
+  // stores and loads share a counter that runs in order, and a load behind a store waits for it.  A lane's rows
+  // are in registers four together, so types, kinds and edges are decided once for all of them.  (A row at a
+  // time, with its loads and branches, took 33,000 clocks a tile, as long as 12 stages of products.)
+  static_assert(TN % 2 == 0 && NW * 32 * 68 * 4 <= LDS, "a wave's rows of 64 columns");
+  constexpr bool FORWARD = PRC && QRC;  // bias, activation, residual and what is kept; else sums as they are
+  constexpr int ROWS = 4;               // of a lane at a time, 4 apart
+  copies_barrier<0>();
   const int l = threadIdx.x & 63;
   float* own = reinterpret_cast<float*>(smem) + w * 32 * 68;
-  float* part = a.part ? a.part + (long long)split * a.e.M * a.e.N : nullptr;
+  const bool split_up = a.part != nullptr;
+  const Added added = split_up ? Added{nullptr, 0, false} : dense_added(a.e);
+  char* C = split_up ? (char*)(a.part + (long long)split * a.e.M * a.e.N) : (char*)a.e.C;
+  const bool c_bf = !split_up && a.e.c_bf;
+  const long long c_step = (split_up ? a.e.N : a.e.sc) * (c_bf ? 2 : 4);
+  const bool inside = m0 + BM <= a.e.M && n0 + BN <= a.e.N;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
+  for (int jj = 0; jj < TN; jj += 2) {
+    const int n = n0 + (wn * TN + jj) * 32 + (l & 15) * 4, there = a.e.N - n;
+    const long long mw = m0 + wm * TM * 32 + (l >> 4);
+    float bias[4];
+    if constexpr (FORWARD) dense_bias(a.e, n, bias);
+    uv4 r[ROWS];
+    auto load_rows = [&](long long m) {
+      const char* p = added.p + m * added.step + (long long)n * (added.bf ? 2 : 4);
+      if (inside && added.bf) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+        for (int x = 0; x < ROWS; ++x) {
+          const uv2 t = reinterpret_cast<const bytes8*>(p + 4 * x * added.step)->v;
+          r[x] = uv4{t[0], t[1], 0u, 0u};
+        }
+      } else if (inside) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 t;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) t[x] = acc[i][j][4 * g + x];
-        *reinterpret_cast<f32x4*>(own + (l & 31) * 68 + 32 * j + 8 * g + 4 * (l >> 5)) = t;
-      }
-    const int n = n0 + wn * 64 + (l & 15) * 4;
-#pragma unroll 1
-    for (int r = l >> 4; r < 32; r += 4) {
-      const long long m = m0 + (wm * TM + i) * 32 + r;
-      const f32x4 t = *reinterpret_cast<const f32x4*>(own + r * 68 + (l & 15) * 4);
-      float v[4] = {t[0], t[1], t[2], t[3]};
-      if (part) {
-        if (m < a.e.M && n < a.e.N) store4(part, false, m * a.e.N + n, a.e.N - n, v);
+        for (int x = 0; x < ROWS; ++x) r[x] = reinterpret_cast<const bytes16*>(p + 4 * x * added.step)->v;
       } else {
-        dense_epilogue(a.e, m, n, v);
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x) {
+          r[x] = uv4{0u, 0u, 0u, 0u};
+          if (m + 4 * x < a.e.M && there > 0) r[x] = load_added(p + 4 * x * added.step, added.bf, there);
+        }
       }
+    };
+    if (added.p) load_rows(mw);
+#pragma unroll 1
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4 t;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) t[x] = acc[0][jj + j][4 * g + x];
+          *reinterpret_cast<f32x4*>(own + (l & 31) * 68 + 32 * j + 8 * g + 4 * (l >> 5)) = t;
+        }
+      // a rolled loop (its code is loaded once): the rows of accumulators move up
+#pragma unroll
+      for (int y = 0; y + 1 < TM; ++y)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[y][jj + j] = acc[y + 1][jj + j];
+#pragma unroll 1
+     for (int y = 0; y < 32; y += 4 * ROWS) {
+      const long long mi = mw + i * 32 + y;
+      float v[ROWS][4];
+#pragma unroll
+      for (int x = 0; x < ROWS; ++x) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(own + (y + 4 * x + (l >> 4)) * 68 + (l & 15) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[x][j] = t[j];
+      }
+      if constexpr (FORWARD) {
+        if (!split_up) dense_forward<ROWS>(a.e, mi, 4, n, v, bias);
+      }
+      if (added.p) {
+        if (added.bf) {
+#pragma unroll
+          for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], true);
+        } else {
+#pragma unroll
+          for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], false);
+        }
+        if (i + 1 < TM || y + 4 * ROWS < 32) load_rows(mi + 4 * ROWS);
+      }
+      char* c = C + mi * c_step + (long long)n * (c_bf ? 2 : 4);
+      if (inside && c_bf) {
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, true, 0, 4, v[x]);
+      } else if (inside) {
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, false, 0, 4, v[x]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x)
+          if (mi + 4 * x < a.e.M && there > 0) store4(c + 4 * x * c_step, c_bf, 0, there, v[x]);
+      }
+     }
     }
   }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------
 enum { DENSE_NT = 0, DENSE_NN = 1, DENSE_TN = 2 };  // P, Q: RC RC; RC RS; RS RS
-enum { DENSE_256 = 0, DENSE_128 = 1, DENSE_64 = 2, DENSE_TILES = 3 };
-constexpr int DENSE_BM[DENSE_TILES] = {256, 128, 64}, DENSE_BN[DENSE_TILES] = {256, 128, 128};
+constexpr int DENSE_BK = 128;                            // bytes of reduction of a stage: a cache line of an RC row
+// Tiles.  The large one keeps the matrix cores fed at the least traffic; the smaller ones fill the chip when
+// there are few.  DEEP: three stages (one workgroup a CU), which hides more of a load's latency where few
+// workgroups run.
+enum { DENSE_256 = 0, DENSE_256X128 = 1, DENSE_128 = 2, DENSE_128_DEEP = 3, DENSE_64 = 4, DENSE_TILES = 5 };
+constexpr int DENSE_BM[DENSE_TILES] = {256, 256, 128, 128, 64}, DENSE_BN[DENSE_TILES] = {256, 128, 128, 128, 128};
 
-template <int ES, int BM, int BN, int WM, int WN, bool PRC, bool QRC>
+template <int ES, int BM, int BN, int WM, int WN, int BK, int NSP, int NSQ, bool PRC, bool QRC>
 int launch_dense_tile_as(const DenseK& a, int splits, hipStream_t s) {
-  constexpr size_t lds = 2 * (BM + BN) * DENSE_BK;
-  const void* f = (const void*)dense_tile_kernel<ES, BM, BN, WM, WN, PRC, QRC>;
+  constexpr size_t lds = (NSP * BM + NSQ * BN) * BK;
+  const void* f = (const void*)dense_tile_kernel<ES, BM, BN, WM, WN, BK, NSP, NSQ, PRC, QRC>;
   GL_TRY(set_lds_limit(f, lds));
-  GL_LAUNCH(GL_KERNEL_DENSE, (dense_tile_kernel<ES, BM, BN, WM, WN, PRC, QRC>),
+  GL_LAUNCH(GL_KERNEL_DENSE, (dense_tile_kernel<ES, BM, BN, WM, WN, BK, NSP, NSQ, PRC, QRC>),
             dim3((unsigned)(a.tiles_m * a.tiles_n * splits)), dim3(64 * WM * WN), lds, s, a);
   GL_CHECK_LAUNCH();
   return 0;
 }
-template <int ES, int BM, int BN, int WM, int WN>
+template <int ES, int BM, int BN, int WM, int WN, int BK, int NSP, int NSQ>
 int launch_dense_tile_of(int form, const DenseK& a, int splits, hipStream_t s) {
-  if (form == DENSE_NT) return launch_dense_tile_as<ES, BM, BN, WM, WN, true, true>(a, splits, s);
-  if (form == DENSE_NN) return launch_dense_tile_as<ES, BM, BN, WM, WN, true, false>(a, splits, s);
-  return launch_dense_tile_as<ES, BM, BN, WM, WN, false, false>(a, splits, s);
+  if (form == DENSE_NT) return launch_dense_tile_as<ES, BM, BN, WM, WN, BK, NSP, NSQ, true, true>(a, splits, s);
+  if (form == DENSE_NN) return launch_dense_tile_as<ES, BM, BN, WM, WN, BK, NSP, NSQ, true, false>(a, splits, s);
+  return launch_dense_tile_as<ES, BM, BN, WM, WN, BK, NSP, NSQ, false, false>(a, splits, s);
 }
 int launch_dense_tile_bf16(int form, int tile, const DenseK& a, int splits, hipStream_t s);
 int launch_dense_tile_f32(int form, int tile, const DenseK& a, int splits, hipStream_t s);

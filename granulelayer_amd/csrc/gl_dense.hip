@@ -76,17 +76,24 @@ int launch_align(Operand& o, int es, void* dst, hipStream_t s) {
 // A lane holds 4 neighbouring columns and adds the splits in their order, then the epilogue.
 __global__ __launch_bounds__(256) void dense_join_kernel(const float* __restrict__ part, int splits, DenseEpi e) {
   const long long m = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int l = threadIdx.x & 63, n = blockIdx.y * 256 + l * 4;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  if (m < e.M && n < e.N) {
+  const int l = threadIdx.x & 63, n = blockIdx.y * 256 + l * 4, there = m < e.M ? e.N - n : 0;
+  float v[1][4] = {{0.f, 0.f, 0.f, 0.f}}, b[4];
+  dense_bias(e, n, b);
+  const Added added = dense_added(e);
+  uv4 r = {0u, 0u, 0u, 0u};
+  if (added.p && there > 0) r = load_added(added.p + m * added.step + (long long)n * (added.bf ? 2 : 4), added.bf, there);
+  if (there > 0) {
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
       float t[4];
-      load4(part, false, ((long long)s * e.M + m) * e.N + n, e.N - n, t);
+      load4(part, false, ((long long)s * e.M + m) * e.N + n, there, t);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += t[j];
+      for (int j = 0; j < 4; ++j) v[0][j] += t[j];
     }
   }
-  dense_epilogue(e, m, n, v);
+  dense_forward<1>(e, m, 1, n, v, b);
+  if (added.p) add_added(v[0], r, added.bf);
+  if (there > 0) store4(e.C, e.c_bf, m * e.sc + n, there, v[0]);
 }
 
 // ---- plan of a product --------------------------------------------------------------------------------
@@ -94,27 +101,37 @@ struct Product {
   int tile, splits, steps_per_split, steps, tiles_m, tiles_n;
   size_t part_bytes;
 };
+// What a tile costs, measured on whole problems of 16 to 256 stages: workgroups of a CU, microseconds of a stage
+// with one of them on each CU and with all, and of a tile's start and end.
+struct TileCost {
+  int per_cu;
+  double alone, full, ends;
+};
+constexpr TileCost COST_BF16[DENSE_TILES] = {
+    {1, 1.55, 1.55, 9}, {1, 0.88, 0.88, 7}, {2, 0.74, 1.05, 6}, {1, 0.57, 0.57, 6}, {2, 0.30, 0.68, 5}};
+constexpr TileCost COST_F32[DENSE_TILES] = {
+    {0, 0, 0, 0}, {0, 0, 0, 0}, {2, 2.15, 4.25, 6}, {0, 0, 0, 0}, {2, 1.10, 2.20, 5}};
+
+// Tile and splits of the reduction: the least of rounds x (stages x cost + ends), plus for a split product its
+// partial sums written and read (4 TB/s) and the launch that joins them.
 Product plan_product(int dtype, long long M, int N, long long R) {
-  const int es = es_of(dtype);
+  constexpr int CUS = 256;
+  const TileCost* cost = dtype == GL_DTYPE_BF16 ? COST_BF16 : COST_F32;
   Product best{};
   double best_t = 0;
-  const int steps = (int)((R * es + DENSE_BK - 1) / DENSE_BK);
-  for (int t = dtype == GL_DTYPE_BF16 ? DENSE_256 : DENSE_128; t < DENSE_TILES; ++t) {
+  const long long steps = (R * es_of(dtype) + DENSE_BK - 1) / DENSE_BK;
+  for (int t = 0; t < DENSE_TILES; ++t) {
     const long long tm = (M + DENSE_BM[t] - 1) / DENSE_BM[t], tn = (N + DENSE_BN[t] - 1) / DENSE_BN[t];
-    if (tm * tn > (1LL << 30)) continue;
-    // workgroups that run at once, and microseconds of a stage of each then
-    const double slots = t == DENSE_256 ? 256 : (t == DENSE_128 ? 512 : 768);
-    const double us = (t == DENSE_256 ? 2.1 : (t == DENSE_128 ? 1.4 : 1.2)) * (dtype == GL_DTYPE_BF16 ? 1.0 : 5.6);
-    for (int s = 1; s <= 32 && s <= steps; s = s < 4 ? s + 1 : s * 2) {
-      const int per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
-      if (splits != s || tm * tn * s > (1LL << 30)) continue;
-      const double rounds = (double)((tm * tn * s + (long long)slots - 1) / (long long)slots);
-      // a partly filled chip runs its workgroups a little faster each
-      double time = rounds * (per * us + 3.0);
-      if (s > 1) time += 4.0 + (double)s * M * N * 8 / 4.0e6;
+    if (!cost[t].per_cu || tm * tn > (1LL << 30)) continue;
+    for (long long s = 1; s <= 32 && s <= steps; s = s < 4 ? s + 1 : s * 2) {
+      const long long per = (steps + s - 1) / s, n = tm * tn * s, slots = CUS * cost[t].per_cu;
+      if ((steps + per - 1) / per != s || n > (1LL << 30)) continue;
+      const double stage = n <= CUS ? cost[t].alone : cost[t].full;
+      double time = (double)((n + slots - 1) / slots) * ((double)per * stage + cost[t].ends);
+      if (s > 1) time += 3.0 + (double)s * M * N * 8 / 4.0e6;
       if (best_t == 0 || time < best_t) {
         best_t = time;
-        best = Product{t, s, per, steps, (int)tm, (int)tn, s > 1 ? (size_t)round_up((long long)s * M * N * 4, 256) : 0};
+        best = Product{t, (int)s, (int)per, (int)steps, (int)tm, (int)tn, s > 1 ? (size_t)round_up(s * M * N * 4, 256) : 0};
       }
     }
   }
@@ -147,17 +164,13 @@ int run_product(int dtype, int form, const Operand& p, const Operand& q, long lo
 }
 
 // ---- dz = dY act'(z) and the sums of its columns -------------------------------------------------------
-__device__ __forceinline__ float dgelu_f(float z) {
-  const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-  return __builtin_fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), cdf);
-}
-
 constexpr int DZ_ROWS = 64, DZ_COLS = 256;  // of a workgroup; 32 lanes of 8 columns by 8 rows at a time
+constexpr int DZ_AHEAD = 4;                 // rows a lane has in flight
 
 // dz may be null (only the sums), part too (only dz).  Rows of dz are padded(N) apart, zeros behind N.
-template <bool YBF, bool OBF>
+template <bool YBF, bool OBF, int KEEP>
 __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ dY, long long sdy, const void* __restrict__ z,
-                                                       const uint8_t* __restrict__ ze, int keep, long long M, int N,
+                                                       const uint8_t* __restrict__ ze, long long M, int N,
                                                        void* __restrict__ dz, float* __restrict__ part) {
   __shared__ float sums[8][DZ_COLS];
   const int ct = threadIdx.x & 31, rt = threadIdx.x >> 5;
@@ -166,31 +179,49 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ 
   const int nblk = (N + 31) / 32;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (n < N) {
-    for (int i = 0; i < DZ_ROWS / 8; ++i) {
-      const long long m = (long long)blockIdx.x * DZ_ROWS + i * 8 + rt;
-      if (m >= M) break;
-      float g[8];
-      load8<YBF>(dY, m * sdy + n, N - n, g);
-      if (keep == GL_KEEP_SIGN) {
-        const unsigned w = ((const unsigned*)z)[m * nblk + (n >> 5)] >> (n & 31);
+#pragma unroll 1
+    for (int i = 0; i < DZ_ROWS / 8; i += DZ_AHEAD) {
+      const long long m0 = (long long)blockIdx.x * DZ_ROWS + i * 8 + rt;
+      if (m0 >= M) break;
+      float g[DZ_AHEAD][8], t[DZ_AHEAD][8];
+      unsigned bits[DZ_AHEAD];
+      uv2 codes[DZ_AHEAD];
+      int ex[DZ_AHEAD];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = (w >> j) & 1u ? g[j] : 0.f;
-      } else if (keep != GL_KEEP_NONE) {
-        float t[8];
-        if (keep == GL_KEEP_Z) {
-          load8<OBF>(z, m * ldz + n, N - n, t);
-        } else {
-          const uv2 w = *reinterpret_cast<const uv2*>((const uint8_t*)z + (m * nblk * 32 + n));
-          const float st = p8_step(ze[m * nblk + (n >> 5)]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) t[j] = p8_value(w[j >> 2], j & 3, st);
+      for (int x = 0; x < DZ_AHEAD; ++x) {
+        const long long m = m0 + 8 * x;
+        const int there = m < M ? N - n : 0;
+        load8<YBF>(dY, m * sdy + n, there, g[x]);
+        if constexpr (KEEP == GL_KEEP_SIGN) bits[x] = m < M ? ((const unsigned*)z)[m * nblk + (n >> 5)] >> (n & 31) : 0u;
+        if constexpr (KEEP == GL_KEEP_Z) load8<OBF>(z, m * ldz + n, there, t[x]);
+        if constexpr (KEEP == GL_KEEP_Z8) {
+          codes[x] = uv2{0u, 0u};
+          ex[x] = 1;
+          if (m < M) {
+            codes[x] = *reinterpret_cast<const uv2*>((const uint8_t*)z + (m * nblk * 32 + n));
+            ex[x] = ze[m * nblk + (n >> 5)];
+          }
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= n + j < N ? dgelu_f(t[j]) : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] += g[j];
-      if (dz) store8<OBF>(dz, m * ldz + n, 8, g);
+      for (int x = 0; x < DZ_AHEAD; ++x) {
+        const long long m = m0 + 8 * x;
+        if constexpr (KEEP == GL_KEEP_SIGN) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[x][j] = (bits[x] >> j) & 1u ? g[x][j] : 0.f;
+        } else if constexpr (KEEP != GL_KEEP_NONE) {
+          const float st = KEEP == GL_KEEP_Z8 ? p8_step(ex[x]) : 0.f;
+          // columns behind N hold dY's 0 and z's 0 (a code of 0 is NaN in a block without numbers)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float zj = KEEP == GL_KEEP_Z8 ? p8_value(codes[x][j >> 2], j & 3, st) : t[x][j];
+            g[x][j] = n + j < N ? g[x][j] * dgelu_f(zj) : 0.f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += g[x][j];
+        if (dz && m < M) store8<OBF>(dz, m * ldz + n, 8, g[x]);
+      }
     }
   }
   if (!part) return;
@@ -334,17 +365,25 @@ BwdPlan plan_bwd(const GlDenseBwdArgs* a) {
   return p;
 }
 
-template <bool YBF>
-int launch_dz(const GlDenseBwdArgs* a, void* dz, float* part, hipStream_t s) {
+template <bool YBF, bool OBF, int KEEP>
+int launch_dz_as(const GlDenseBwdArgs* a, void* dz, float* part, hipStream_t s) {
   const dim3 grid((unsigned)((a->M + DZ_ROWS - 1) / DZ_ROWS), (unsigned)ceil_div(a->N, DZ_COLS));
-  if (a->dtype == GL_DTYPE_BF16)
-    GL_LAUNCH(GL_KERNEL_DENSE_DZ, (dense_dz_kernel<YBF, true>), grid, dim3(256), 0, s, a->dY, a->sdy, a->z, a->z_exp, a->keep,
-              (long long)a->M, a->N, dz, part);
-  else
-    GL_LAUNCH(GL_KERNEL_DENSE_DZ, (dense_dz_kernel<YBF, false>), grid, dim3(256), 0, s, a->dY, a->sdy, a->z, a->z_exp,
-              a->keep, (long long)a->M, a->N, dz, part);
+  GL_LAUNCH(GL_KERNEL_DENSE_DZ, (dense_dz_kernel<YBF, OBF, KEEP>), grid, dim3(256), 0, s, a->dY, a->sdy, a->z, a->z_exp,
+            (long long)a->M, a->N, dz, part);
   GL_CHECK_LAUNCH();
   return 0;
+}
+template <bool YBF, bool OBF>
+int launch_dz_of(const GlDenseBwdArgs* a, void* dz, float* part, hipStream_t s) {
+  if (a->keep == GL_KEEP_NONE) return launch_dz_as<YBF, OBF, GL_KEEP_NONE>(a, dz, part, s);
+  if (a->keep == GL_KEEP_SIGN) return launch_dz_as<YBF, OBF, GL_KEEP_SIGN>(a, dz, part, s);
+  if (a->keep == GL_KEEP_Z) return launch_dz_as<YBF, OBF, GL_KEEP_Z>(a, dz, part, s);
+  return launch_dz_as<YBF, OBF, GL_KEEP_Z8>(a, dz, part, s);
+}
+int launch_dz(const GlDenseBwdArgs* a, void* dz, float* part, hipStream_t s) {
+  const bool o = a->dtype == GL_DTYPE_BF16;
+  if (a->dy_dtype == GL_DTYPE_BF16) return o ? launch_dz_of<true, true>(a, dz, part, s) : launch_dz_of<true, false>(a, dz, part, s);
+  return o ? launch_dz_of<false, true>(a, dz, part, s) : launch_dz_of<false, false>(a, dz, part, s);
 }
 
 DenseEpi store_epi(void* C, long long sc, int c_dtype, long long M, int N, int op_dtype, int accumulate) {
@@ -378,8 +417,8 @@ extern "C" int gl_dense_fwd(const GlDenseArgs* a, void* stream) {
   GL_TRY(check_fwd(a));
   if (a->M == 0) return 0;
   FwdPlan p = plan_fwd(a);
-  if (p.bytes && (!a->ws || ((uintptr_t)a->ws & 255))) return GL_ERR_ARG;
   if (a->ws_bytes < p.bytes) return GL_ERR_WORKSPACE;
+  if (p.bytes && (!a->ws || ((uintptr_t)a->ws & 255))) return GL_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   DenseEpi e = store_epi(a->Y, a->sy, a->y_dtype, a->M, a->N, a->dtype, 0);
   e.bias = a->bias;
@@ -409,14 +448,14 @@ extern "C" int gl_dense_bwd(const GlDenseBwdArgs* a, void* stream) {
   GL_TRY(check_bwd(a));
   if (a->M == 0) return 0;
   BwdPlan p = plan_bwd(a);
-  if (p.bytes && (!a->ws || ((uintptr_t)a->ws & 255))) return GL_ERR_ARG;
   if (a->ws_bytes < p.bytes) return GL_ERR_WORKSPACE;
+  if (p.bytes && (!a->ws || ((uintptr_t)a->ws & 255))) return GL_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   const int es = es_of(a->dtype);
   char* ws = (char*)a->ws;
   void* dz = p.own_dz ? ws : nullptr;
   float* db_part = a->db ? (float*)(ws + p.off_db) : nullptr;
-  if (dz || db_part) GL_TRY(a->dy_dtype == GL_DTYPE_BF16 ? launch_dz<true>(a, dz, db_part, s) : launch_dz<false>(a, dz, db_part, s));
+  if (dz || db_part) GL_TRY(launch_dz(a, dz, db_part, s));
   if (a->db) {
     GL_LAUNCH(GL_KERNEL_DENSE_DB, dense_db_kernel, dim3((unsigned)ceil_div(a->N, 32)), dim3(1024), 0, s, (const float*)db_part,
               p.chunks, a->N, a->db, (int)(a->g_dtype == GL_DTYPE_BF16), a->accumulate);

@@ -51,7 +51,9 @@ __device__ __forceinline__ unsigned short to_bf16(float x) {
   return __builtin_bit_cast(unsigned short, __float2bfloat16(x));
 }
 __device__ __forceinline__ unsigned to_bf16x2(float lo, float hi) {
-  return (unsigned)to_bf16(lo) | (unsigned)to_bf16(hi) << 16;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
 }
 // vectors at an element's own alignment: global memory takes 8- and 16-byte accesses at any address
 // that is a multiple of the element's size

@@ -1,7 +1,7 @@
 // Activations put into 8 bits and read back (gl_pack8, gl_unpack8); the format is in gl_pack8.h.
 //
 // Both kernels move each byte once and are bound by memory.  A lane holds 8 values of one 32-value
-// block, so four neighbouring lanes share a block and its maximum is two shuffles; a wave's
+// block, so four neighbouring lanes share a block and its maximum is two lane swaps; a wave's
 // accesses are contiguous along the row.
 #include "gl_internal.h"
 #include "gl_pack8.h"
@@ -40,8 +40,8 @@ __global__ __launch_bounds__(THREADS) void pack8_kernel(const void* __restrict__
     unsigned a = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) a = umax(a, abs_bits(v[s][j]));
-    a = umax(a, (unsigned)__shfl_xor((int)a, 1));
-    a = umax(a, (unsigned)__shfl_xor((int)a, 2));
+    a = umax(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0xB1, 0xf, 0xf, false));  // lane ^ 1
+    a = umax(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0x4E, 0xf, 0xf, false));  // lane ^ 2
     if (slot >= nb * 4) continue;
     const int ex = p8_exp(a);
     const float is = p8_inv_step(ex);

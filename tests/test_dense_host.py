@@ -85,7 +85,8 @@ def test_library_refuses_before_the_device():
         assert fwd(**bad) == -2, bad
     # odd rows are copied through workspace, which has to be there, aligned and large enough
     assert fwd(sx=65) == 0 and out.value >= 100 * 64 * 2
-    assert fwd(False, sx=65) == -1 and fwd(False, sx=65, ws=4096 + 16, ws_bytes=1 << 20) == -1
+    assert fwd(False, sx=65) == -3 and fwd(False, sx=65, ws_bytes=1 << 20) == -1
+    assert fwd(False, sx=65, ws=4096 + 16, ws_bytes=1 << 20) == -1
     assert fwd(False, sx=65, ws=4096, ws_bytes=100) == -3
     assert fwd(False, M=0, X=0, W=0, Y=0) == 0
 
