@@ -510,7 +510,7 @@ _DENSE_DTYPES = {torch.float32: N.GL_DTYPE_F32, torch.bfloat16: N.GL_DTYPE_BF16}
 
 def backend_for(device) -> HipBackend:
     """Backend of a device (the reference's backends.cuda.runtime.backend_for, runtime.py:188-197)."""
-    dev = torch.device(device)
+    dev = device if isinstance(device, torch.device) else torch.device(device)
     if dev.type != "cuda":
         raise RuntimeError(f"no HIP backend for {dev}: the MI355X path needs a ROCm GPU")
-    return HipBackend.get()
+    return HipBackend._instance or HipBackend.get()

@@ -98,6 +98,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(const float* __restrict
 
 // ---- plan of a product --------------------------------------------------------------------------------
 struct Product {
+  double us;  // what the plan expects
   int tile, splits, steps_per_split, steps, tiles_m, tiles_n;
   size_t part_bytes;
 };
@@ -110,16 +111,17 @@ struct TileCost {
 constexpr TileCost COST_BF16[DENSE_TILES] = {
     {1, 1.55, 1.55, 9}, {1, 0.88, 0.88, 7}, {2, 0.74, 1.05, 6}, {1, 0.57, 0.57, 6}, {2, 0.30, 0.68, 5}};
 constexpr TileCost COST_F32[DENSE_TILES] = {
-    {0, 0, 0, 0}, {0, 0, 0, 0}, {2, 2.15, 4.25, 6}, {0, 0, 0, 0}, {2, 1.10, 2.20, 5}};
+    {0, 0, 0, 0}, {0, 0, 0, 0}, {2, 2.15, 4.25, 6}, {1, 1.96, 1.96, 6}, {2, 1.10, 2.20, 5}};
 
-// Tile and splits of the reduction: the least of rounds x (stages x cost + ends), plus for a split product its
-// partial sums written and read (4 TB/s) and the launch that joins them.
+// Tile and splits of the reduction: the least of rounds x (stages x cost + ends), no less than the operands' bytes
+// take, plus for a split product its partial sums written and read (4 TB/s) and the launch that joins them.
 Product plan_product(int dtype, long long M, int N, long long R) {
   constexpr int CUS = 256;
   const TileCost* cost = dtype == GL_DTYPE_BF16 ? COST_BF16 : COST_F32;
   Product best{};
   double best_t = 0;
   const long long steps = (R * es_of(dtype) + DENSE_BK - 1) / DENSE_BK;
+  const double floor = (double)(M + N) * R * es_of(dtype) / 5.2e6;  // the operands' bytes
   for (int t = 0; t < DENSE_TILES; ++t) {
     const long long tm = (M + DENSE_BM[t] - 1) / DENSE_BM[t], tn = (N + DENSE_BN[t] - 1) / DENSE_BN[t];
     if (!cost[t].per_cu || tm * tn > (1LL << 30)) continue;
@@ -128,10 +130,11 @@ Product plan_product(int dtype, long long M, int N, long long R) {
       if ((steps + per - 1) / per != s || n > (1LL << 30)) continue;
       const double stage = n <= CUS ? cost[t].alone : cost[t].full;
       double time = (double)((n + slots - 1) / slots) * ((double)per * stage + cost[t].ends);
-      if (s > 1) time += 3.0 + (double)s * M * N * 8 / 4.0e6;
+      if (time < floor) time = floor;
+      if (s > 1) time += 4.0 + 0.15 * s + (double)s * M * N * 8 / 4.0e6;
       if (best_t == 0 || time < best_t) {
         best_t = time;
-        best = Product{t, (int)s, (int)per, (int)steps, (int)tm, (int)tn, s > 1 ? (size_t)round_up(s * M * N * 4, 256) : 0};
+        best = Product{time, t, (int)s, (int)per, (int)steps, (int)tm, (int)tn, s > 1 ? (size_t)round_up(s * M * N * 4, 256) : 0};
       }
     }
   }
@@ -281,12 +284,24 @@ struct FwdPlan {
 };
 FwdPlan plan_fwd(const GlDenseArgs* a) {
   FwdPlan p{};
-  p.few = a->M <= DENSE_FEW_ROWS && a->keep == GL_KEEP_NONE;
-  if (p.few) return p;
   const int es = es_of(a->dtype);
   p.x = operand(a->X, a->sx, a->M, a->K, true, es);
   p.w = operand(a->W, a->sw, a->N, a->K, true, es);
   p.pr = plan_product(a->dtype, a->M, a->N, a->K);
+  if (a->M <= DENSE_FEW_ROWS && a->keep == GL_KEEP_NONE) {
+    // Few rows: a workgroup's 16 features' weights at 25 bytes a ns of a CU, and 5 TB/s in all, then X from L2 at
+    // 40 bytes a ns; against the tiles and the copies they need.  4096 x 4096 bf16: 1 row 7.5 us (tiles 11.6),
+    // 16 rows 9.8 (12.3), 32 rows 13.8 (12.5), 64 rows 21.1 (13.4); from K 1024 64 rows 7.0 (8.4).
+    const double row = (double)a->K * es, w = a->N * row, rounds = ceil_div(ceil_div(a->N, 16), 256);
+    const double weights = w / 5.0e6 > rounds * 16 * row / 25e3 ? w / 5.0e6 : rounds * 16 * row / 25e3;
+    const double few = 1.5 + weights + rounds * (double)a->M * row / 40e3;
+    double tiles = p.pr.us;
+    if (p.x.copied || p.w.copied) tiles += 3.0 + 2.0 * w / 4.0e6;
+    if (few <= tiles) {
+      p.few = true;
+      return p;
+    }
+  }
   p.off_w = copy_bytes(p.x, es);
   p.off_part = p.off_w + copy_bytes(p.w, es);
   p.bytes = p.off_part + p.pr.part_bytes;

@@ -7,6 +7,7 @@ namespace gl {
 
 int launch_dense_tile_f32(int form, int tile, const DenseK& a, int splits, hipStream_t s) {
   if (tile == DENSE_128) return launch_dense_tile_of<4, 128, 128, 2, 2, DENSE_BK, 2, 2>(form, a, splits, s);
+  if (tile == DENSE_128_DEEP) return launch_dense_tile_of<4, 128, 128, 4, 2, DENSE_BK, 3, 3>(form, a, splits, s);
   return launch_dense_tile_of<4, 64, 128, 2, 2, DENSE_BK, 3, 3>(form, a, splits, s);
 }
 

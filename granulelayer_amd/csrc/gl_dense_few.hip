@@ -11,7 +11,7 @@ namespace gl {
 namespace {
 
 template <int ES>
-__device__ __forceinline__ uv4 load16(const char* row, long long k, long long kbytes, bool whole) {
+__device__ __forceinline__ uv4 load16(const char* row, int k, int kbytes, bool whole) {
   if (whole || k + 16 <= kbytes) return reinterpret_cast<const bytes16*>(row + k)->v;
   uv4 v = {0u, 0u, 0u, 0u};
   if constexpr (ES == 4) {
@@ -38,8 +38,8 @@ __device__ __forceinline__ f32x4 mma16(uv4 w, uv4 x, f32x4 c) {
   }
 }
 
-// MT: groups of 16 rows
-template <int ES, int MT>
+// MT: groups of 16 rows; PIECES: 256-byte pieces of a row that a wave has in flight
+template <int ES, int MT, int PIECES>
 __global__ __launch_bounds__(1024) void dense_few_kernel(const char* __restrict__ X, long long sxb, const char* __restrict__ W,
                                                          long long swb, int M, int K, DenseEpi e) {
   extern __shared__ __align__(16) float sums[];  // [waves][MT][16 m][16 n]
@@ -49,25 +49,32 @@ __global__ __launch_bounds__(1024) void dense_few_kernel(const char* __restrict_
   const char* xr[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) xr[t] = X + (long long)min(16 * t + (l & 15), M - 1) * sxb;
-  const long long kb = (long long)K * ES;
+  const int kb = K * ES;  // below 2^23
   f32x4 acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (long long p = (long long)wave * 256; p < kb; p += nw * 256) {
-    const bool whole = p + 256 <= kb;
-    const long long k = p + (l >> 4) * 16;
-    uv4 wf[4], xf[MT][4];
+  auto pieces = [&](int p, bool whole) {
+    uv4 wf[PIECES][4], xf[PIECES][MT][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) wf[u] = load16<ES>(wr, k + 64 * u, kb, whole);
+    for (int q = 0; q < PIECES; ++q)
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+      for (int u = 0; u < 4; ++u) wf[q][u] = load16<ES>(wr, p + q * nw * 256 + (l >> 4) * 16 + 64 * u, kb, whole);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) xf[t][u] = load16<ES>(xr[t], k + 64 * u, kb, whole);
+    for (int q = 0; q < PIECES; ++q)
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+      for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) acc[t] = mma16<ES>(wf[u], xf[t][u], acc[t]);
-  }
+        for (int u = 0; u < 4; ++u) xf[q][t][u] = load16<ES>(xr[t], p + q * nw * 256 + (l >> 4) * 16 + 64 * u, kb, whole);
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = mma16<ES>(wf[q][u], xf[q][t][u], acc[t]);
+  };
+  int p = wave * 256;
+  for (; p + ((PIECES - 1) * nw + 1) * 256 <= kb; p += PIECES * nw * 256) pieces(p, true);
+  if (p < kb) pieces(p, false);  // what is past the end is zero
 #pragma unroll
   for (int t = 0; t < MT; ++t)
     *reinterpret_cast<f32x4*>(sums + ((wave * MT + t) * 16 + (l & 15)) * 16 + 4 * (l >> 4)) = acc[t];
@@ -85,29 +92,28 @@ __global__ __launch_bounds__(1024) void dense_few_kernel(const char* __restrict_
   }
 }
 
-template <int ES, int MT>
+template <int ES, int MT, int PIECES>
 int launch_few(const GlDenseArgs* a, const DenseEpi& e, hipStream_t s) {
   // one 256-byte piece of every weight row per wave, up to the 16 waves of a workgroup
   int nw = ceil_div((long long)a->K * ES, 256);
   nw = nw < 4 ? 4 : (nw > 16 ? 16 : nw);
   const size_t lds = (size_t)nw * MT * 1024;
-  GL_LAUNCH(GL_KERNEL_DENSE_FEW, (dense_few_kernel<ES, MT>), dim3((unsigned)ceil_div(a->N, 16)), dim3(nw * 64), lds, s,
+  GL_LAUNCH(GL_KERNEL_DENSE_FEW, (dense_few_kernel<ES, MT, PIECES>), dim3((unsigned)ceil_div(a->N, 16)), dim3(nw * 64), lds, s,
             (const char*)a->X, a->sx * ES, (const char*)a->W, a->sw * ES, (int)a->M, a->K, e);
   GL_CHECK_LAUNCH();
   return 0;
+}
+template <int ES>
+int launch_few_of(const GlDenseArgs* a, const DenseEpi& e, hipStream_t s) {
+  if (a->M <= 16) return (long long)a->K * ES > 16 * 256 ? launch_few<ES, 1, 2>(a, e, s) : launch_few<ES, 1, 1>(a, e, s);
+  if (a->M <= 32) return launch_few<ES, 2, 1>(a, e, s);
+  return launch_few<ES, 4, 1>(a, e, s);
 }
 
 }  // namespace
 
 int launch_dense_few(const GlDenseArgs* a, const DenseEpi& e, hipStream_t s) {
-  if (a->dtype == GL_DTYPE_BF16) {
-    if (a->M <= 16) return launch_few<2, 1>(a, e, s);
-    if (a->M <= 32) return launch_few<2, 2>(a, e, s);
-    return launch_few<2, 4>(a, e, s);
-  }
-  if (a->M <= 16) return launch_few<4, 1>(a, e, s);
-  if (a->M <= 32) return launch_few<4, 2>(a, e, s);
-  return launch_few<4, 4>(a, e, s);
+  return a->dtype == GL_DTYPE_BF16 ? launch_few_of<2>(a, e, s) : launch_few_of<4>(a, e, s);
 }
 
 }  // namespace gl

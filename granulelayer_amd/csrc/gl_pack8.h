@@ -30,12 +30,16 @@ __device__ __forceinline__ int p8_exp(unsigned amax) {
 __device__ __forceinline__ float p8_inv_step(int e) { return e == 255 ? 0.f : __uint_as_float((unsigned)(254 - e) << 23); }
 __device__ __forceinline__ float p8_step(int e) { return __uint_as_float(e == 255 ? 0x7fc00000u : (unsigned)e << 23); }
 
+// Four codes.  1.5 x 2^23 has a last place of one: adding it rounds to a whole number (nearest even) and
+// leaves it in the low byte, two's complement; the product is exact, so the fused add rounds once.
 __device__ __forceinline__ unsigned p8_code(float x, float inv_step) {
-  const int q = __float2int_rn(x * inv_step);
-  return (unsigned)(q < -127 ? -127 : (q > 127 ? 127 : q)) & 0xffu;
+  constexpr float LIMIT = 127.f * 0x1p121f;  // of the largest step
+  return __float_as_uint(__builtin_fmaf(__builtin_amdgcn_fmed3f(x, -LIMIT, LIMIT), inv_step, 12582912.f));
 }
 __device__ __forceinline__ unsigned p8_codes4(float a, float b, float c, float d, float inv_step) {
-  return p8_code(a, inv_step) | p8_code(b, inv_step) << 8 | p8_code(c, inv_step) << 16 | p8_code(d, inv_step) << 24;
+  const unsigned lo = __builtin_amdgcn_perm(p8_code(b, inv_step), p8_code(a, inv_step), 0x0c0c0400u);
+  const unsigned hi = __builtin_amdgcn_perm(p8_code(d, inv_step), p8_code(c, inv_step), 0x04000c0cu);
+  return lo | hi;
 }
 // value i of four packed codes
 __device__ __forceinline__ float p8_value(unsigned codes, int i, float step) {
