@@ -9,6 +9,8 @@
 // transposed in memory.
 #pragma once
 
+#include <atomic>
+
 #include "gl_internal.h"
 #include "gl_pack8.h"
 
@@ -612,41 +614,41 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 8192 ? 1 : 2) v
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[y][jj + j] = acc[y + 1][jj + j];
 #pragma unroll 1
-     for (int y = 0; y < 32; y += 4 * ROWS) {
-      const long long mi = mw + i * 32 + y;
-      float v[ROWS][4];
+      for (int y = 0; y < 32; y += 4 * ROWS) {
+        const long long mi = mw + i * 32 + y;
+        float v[ROWS][4];
 #pragma unroll
-      for (int x = 0; x < ROWS; ++x) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(own + (y + 4 * x + (l >> 4)) * 68 + (l & 15) * 4);
+        for (int x = 0; x < ROWS; ++x) {
+          const f32x4 t = *reinterpret_cast<const f32x4*>(own + (y + 4 * x + (l >> 4)) * 68 + (l & 15) * 4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[x][j] = t[j];
-      }
-      if constexpr (FORWARD) {
-        if (!split_up) dense_forward<ROWS>(a.e, mi, 4, n, v, bias);
-      }
-      if (added.p) {
-        if (added.bf) {
+          for (int j = 0; j < 4; ++j) v[x][j] = t[j];
+        }
+        if constexpr (FORWARD) {
+          if (!split_up) dense_forward<ROWS>(a.e, mi, 4, n, v, bias);
+        }
+        if (added.p) {
+          if (added.bf) {
 #pragma unroll
-          for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], true);
+            for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], true);
+          } else {
+#pragma unroll
+            for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], false);
+          }
+          if (i + 1 < TM || y + 4 * ROWS < 32) load_rows(mi + 4 * ROWS);
+        }
+        char* c = C + mi * c_step + (long long)n * (c_bf ? 2 : 4);
+        if (inside && c_bf) {
+#pragma unroll
+          for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, true, 0, 4, v[x]);
+        } else if (inside) {
+#pragma unroll
+          for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, false, 0, 4, v[x]);
         } else {
 #pragma unroll
-          for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], false);
+          for (int x = 0; x < ROWS; ++x)
+            if (mi + 4 * x < a.e.M && there > 0) store4(c + 4 * x * c_step, c_bf, 0, there, v[x]);
         }
-        if (i + 1 < TM || y + 4 * ROWS < 32) load_rows(mi + 4 * ROWS);
       }
-      char* c = C + mi * c_step + (long long)n * (c_bf ? 2 : 4);
-      if (inside && c_bf) {
-#pragma unroll
-        for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, true, 0, 4, v[x]);
-      } else if (inside) {
-#pragma unroll
-        for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, false, 0, 4, v[x]);
-      } else {
-#pragma unroll
-        for (int x = 0; x < ROWS; ++x)
-          if (mi + 4 * x < a.e.M && there > 0) store4(c + 4 * x * c_step, c_bf, 0, there, v[x]);
-      }
-     }
     }
   }
 }
@@ -663,8 +665,14 @@ constexpr int DENSE_BM[DENSE_TILES] = {256, 256, 128, 128, 64}, DENSE_BN[DENSE_T
 template <int ES, int BM, int BN, int WM, int WN, int BK, int NSP, int NSQ, bool PRC, bool QRC>
 int launch_dense_tile_as(const DenseK& a, int splits, hipStream_t s) {
   constexpr size_t lds = (NSP * BM + NSQ * BN) * BK;
-  const void* f = (const void*)dense_tile_kernel<ES, BM, BN, WM, WN, BK, NSP, NSQ, PRC, QRC>;
-  GL_TRY(set_lds_limit(f, lds));
+  // the kernel's LDS limit is raised once a device
+  static std::atomic<unsigned long long> raised{0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return GL_ERR_DEVICE;
+  if (!(raised.load(std::memory_order_relaxed) >> dev & 1)) {
+    GL_TRY(set_lds_limit((const void*)dense_tile_kernel<ES, BM, BN, WM, WN, BK, NSP, NSQ, PRC, QRC>, lds));
+    raised.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   GL_LAUNCH(GL_KERNEL_DENSE, (dense_tile_kernel<ES, BM, BN, WM, WN, BK, NSP, NSQ, PRC, QRC>),
             dim3((unsigned)(a.tiles_m * a.tiles_n * splits)), dim3(64 * WM * WN), lds, s, a);
   GL_CHECK_LAUNCH();

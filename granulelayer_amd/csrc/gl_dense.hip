@@ -117,6 +117,7 @@ constexpr TileCost COST_F32[DENSE_TILES] = {
 // take, plus for a split product its partial sums written and read (4 TB/s) and the launch that joins them.
 Product plan_product(int dtype, long long M, int N, long long R) {
   constexpr int CUS = 256;
+  constexpr long long MAX_BLOCKS = 1LL << 23;  // a launch has fewer than 2^32 threads
   const TileCost* cost = dtype == GL_DTYPE_BF16 ? COST_BF16 : COST_F32;
   Product best{};
   double best_t = 0;
@@ -124,10 +125,10 @@ Product plan_product(int dtype, long long M, int N, long long R) {
   const double floor = (double)(M + N) * R * es_of(dtype) / 5.2e6;  // the operands' bytes
   for (int t = 0; t < DENSE_TILES; ++t) {
     const long long tm = (M + DENSE_BM[t] - 1) / DENSE_BM[t], tn = (N + DENSE_BN[t] - 1) / DENSE_BN[t];
-    if (!cost[t].per_cu || tm * tn > (1LL << 30)) continue;
+    if (!cost[t].per_cu) continue;
     for (long long s = 1; s <= 32 && s <= steps; s = s < 4 ? s + 1 : s * 2) {
       const long long per = (steps + s - 1) / s, n = tm * tn * s, slots = CUS * cost[t].per_cu;
-      if ((steps + per - 1) / per != s || n > (1LL << 30)) continue;
+      if ((steps + per - 1) / per != s || n >= MAX_BLOCKS) continue;
       const double stage = n <= CUS ? cost[t].alone : cost[t].full;
       double time = (double)((n + slots - 1) / slots) * ((double)per * stage + cost[t].ends);
       if (time < floor) time = floor;
@@ -167,14 +168,16 @@ int run_product(int dtype, int form, const Operand& p, const Operand& q, long lo
 }
 
 // ---- dz = dY act'(z) and the sums of its columns -------------------------------------------------------
-constexpr int DZ_ROWS = 64, DZ_COLS = 256;  // of a workgroup; 32 lanes of 8 columns by 8 rows at a time
-constexpr int DZ_AHEAD = 4;                 // rows a lane has in flight
+constexpr int DZ_COLS = 256;  // of a workgroup: 32 lanes of 8 columns by 8 rows at a time
+constexpr int DZ_AHEAD = 4;   // rows a lane has in flight
+// rows of a workgroup: one or two batches of loads, one where two would leave CUs without a workgroup
+inline int dz_rows(long long M, int N) { return (M + 63) / 64 * ceil_div(N, DZ_COLS) >= 512 ? 64 : 32; }
 
 // dz may be null (only the sums), part too (only dz).  Rows of dz are padded(N) apart, zeros behind N.
 template <bool YBF, bool OBF, int KEEP>
 __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ dY, long long sdy, const void* __restrict__ z,
                                                        const uint8_t* __restrict__ ze, long long M, int N,
-                                                       void* __restrict__ dz, float* __restrict__ part) {
+                                                       int rows, void* __restrict__ dz, float* __restrict__ part) {
   __shared__ float sums[8][DZ_COLS];
   const int ct = threadIdx.x & 31, rt = threadIdx.x >> 5;
   const int n = blockIdx.y * DZ_COLS + ct * 8;
@@ -183,8 +186,8 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ 
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (n < N) {
 #pragma unroll 1
-    for (int i = 0; i < DZ_ROWS / 8; i += DZ_AHEAD) {
-      const long long m0 = (long long)blockIdx.x * DZ_ROWS + i * 8 + rt;
+    for (int i = 0; i < rows; i += 8 * DZ_AHEAD) {
+      const long long m0 = (long long)blockIdx.x * rows + i + rt;
       if (m0 >= M) break;
       float g[DZ_AHEAD][8], t[DZ_AHEAD][8];
       unsigned bits[DZ_AHEAD];
@@ -288,6 +291,7 @@ FwdPlan plan_fwd(const GlDenseArgs* a) {
   p.x = operand(a->X, a->sx, a->M, a->K, true, es);
   p.w = operand(a->W, a->sw, a->N, a->K, true, es);
   p.pr = plan_product(a->dtype, a->M, a->N, a->K);
+  if (p.pr.splits == 0) return p;  // refused by the entry points
   if (a->M <= DENSE_FEW_ROWS && a->keep == GL_KEEP_NONE) {
     // Few rows: a workgroup's 16 features' weights at 25 bytes a ns of a CU, and 5 TB/s in all, then X from L2 at
     // 40 bytes a ns; against the tiles and the copies they need.  4096 x 4096 bf16: 1 row 7.5 us (tiles 11.6),
@@ -374,7 +378,7 @@ BwdPlan plan_bwd(const GlDenseBwdArgs* a) {
   p.off_part = at;
   at += part;
   p.off_db = at;
-  p.chunks = (a->M + DZ_ROWS - 1) / DZ_ROWS;
+  p.chunks = (a->M + dz_rows(a->M, a->N) - 1) / dz_rows(a->M, a->N);
   if (a->db) at += (size_t)round_up(p.chunks * a->N * 4, 256);
   p.bytes = at;
   return p;
@@ -382,9 +386,10 @@ BwdPlan plan_bwd(const GlDenseBwdArgs* a) {
 
 template <bool YBF, bool OBF, int KEEP>
 int launch_dz_as(const GlDenseBwdArgs* a, void* dz, float* part, hipStream_t s) {
-  const dim3 grid((unsigned)((a->M + DZ_ROWS - 1) / DZ_ROWS), (unsigned)ceil_div(a->N, DZ_COLS));
+  const int rows = dz_rows(a->M, a->N);
+  const dim3 grid((unsigned)((a->M + rows - 1) / rows), (unsigned)ceil_div(a->N, DZ_COLS));
   GL_LAUNCH(GL_KERNEL_DENSE_DZ, (dense_dz_kernel<YBF, OBF, KEEP>), grid, dim3(256), 0, s, a->dY, a->sdy, a->z, a->z_exp,
-            (long long)a->M, a->N, dz, part);
+            (long long)a->M, a->N, rows, dz, part);
   GL_CHECK_LAUNCH();
   return 0;
 }
@@ -424,7 +429,11 @@ using namespace gl;
 extern "C" int gl_dense_fwd_workspace(const GlDenseArgs* a, size_t* bytes) {
   GL_TRY(check_fwd(a));
   if (!bytes) return GL_ERR_ARG;
-  *bytes = a->M == 0 ? 0 : plan_fwd(a).bytes;
+  *bytes = 0;
+  if (a->M == 0) return 0;
+  const FwdPlan p = plan_fwd(a);
+  if (p.pr.splits == 0) return GL_ERR_UNSUPPORTED;
+  *bytes = p.bytes;
   return 0;
 }
 
@@ -432,6 +441,7 @@ extern "C" int gl_dense_fwd(const GlDenseArgs* a, void* stream) {
   GL_TRY(check_fwd(a));
   if (a->M == 0) return 0;
   FwdPlan p = plan_fwd(a);
+  if (p.pr.splits == 0) return GL_ERR_UNSUPPORTED;
   if (a->ws_bytes < p.bytes) return GL_ERR_WORKSPACE;
   if (p.bytes && (!a->ws || ((uintptr_t)a->ws & 255))) return GL_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
@@ -455,7 +465,11 @@ extern "C" int gl_dense_fwd(const GlDenseArgs* a, void* stream) {
 extern "C" int gl_dense_bwd_workspace(const GlDenseBwdArgs* a, size_t* bytes) {
   GL_TRY(check_bwd(a));
   if (!bytes) return GL_ERR_ARG;
-  *bytes = a->M == 0 ? 0 : plan_bwd(a).bytes;
+  *bytes = 0;
+  if (a->M == 0) return 0;
+  const BwdPlan p = plan_bwd(a);
+  if ((a->dX && p.px.splits == 0) || (a->dW && p.pw.splits == 0)) return GL_ERR_UNSUPPORTED;
+  *bytes = p.bytes;
   return 0;
 }
 
@@ -463,6 +477,7 @@ extern "C" int gl_dense_bwd(const GlDenseBwdArgs* a, void* stream) {
   GL_TRY(check_bwd(a));
   if (a->M == 0) return 0;
   BwdPlan p = plan_bwd(a);
+  if ((a->dX && p.px.splits == 0) || (a->dW && p.pw.splits == 0)) return GL_ERR_UNSUPPORTED;
   if (a->ws_bytes < p.bytes) return GL_ERR_WORKSPACE;
   if (p.bytes && (!a->ws || ((uintptr_t)a->ws & 255))) return GL_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;

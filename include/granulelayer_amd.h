@@ -303,7 +303,7 @@ int gl_window_build(const int32_t* idx, const int32_t* counts, int32_t D, int32_
  * every tensor are a stride apart (in elements, any stride of at least the width), features are
  * neighbours, and no address needs more than its element's alignment. */
 #define GL_DENSE_MAX_FEATURES 1048576 /* largest K, N and packed row */
-#define GL_DENSE_MAX_ROWS (1LL << 31) /* rows are fewer than this */
+#define GL_DENSE_MAX_ROWS (1LL << 26) /* rows are fewer than this */
 /* What the forward keeps of z for the backward, [M, *] in `z`: nothing; z > 0 as bits (word n / 32
  * of a row's ceil(N / 32) words, bit n % 32); z in the operands' type, rows round_up(N, 8) apart; z in
  * 8 bits (gl_pack8's codes in z and exponents in z_exp). */

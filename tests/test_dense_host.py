@@ -65,7 +65,7 @@ def test_library_refuses_before_the_device():
     for bad in (dict(rows=-1), dict(cols=0), dict(cols=N.DENSE_MAX_FEATURES + 1), dict(x=0), dict(q=0), dict(e=0), dict(sx=39),
                 dict(x=4098), dict(q=4100)):
         assert pack(**bad) == -1, bad
-    for bad in (dict(x_dtype=2), dict(rows=1 << 31)):
+    for bad in (dict(x_dtype=2), dict(rows=1 << 26)):
         assert pack(**bad) == -2, bad
     assert pack(rows=0, x=0, q=0, e=0) == 0
     assert L.gl_pack8(None, None) == -1 and L.gl_unpack8(None, None) == -1
@@ -81,8 +81,11 @@ def test_library_refuses_before_the_device():
                 dict(res=4096, sr=47, res_dtype=1), dict(res=4098, sr=48, res_dtype=0), dict(keep=1, z=4100)):
         assert fwd(**bad) == -1 and fwd(False, **bad) == -1, bad
     for bad in (dict(dtype=2), dict(y_dtype=7), dict(res=4096, sr=48, res_dtype=9), dict(N=N.DENSE_MAX_FEATURES + 1),
-                dict(M=1 << 31)):
+                dict(M=1 << 26)):
         assert fwd(**bad) == -2, bad
+    # more workgroups than a launch has
+    big = dict(M=(1 << 26) - 1, N=1 << 20, K=1 << 20, sx=1 << 20, sw=1 << 20, sy=1 << 20)
+    assert fwd(**big) == -2 and fwd(False, **big) == -2
     # odd rows are copied through workspace, which has to be there, aligned and large enough
     assert fwd(sx=65) == 0 and out.value >= 100 * 64 * 2
     assert fwd(False, sx=65) == -3 and fwd(False, sx=65, ws_bytes=1 << 20) == -1
@@ -103,6 +106,8 @@ def test_library_refuses_before_the_device():
         assert bwd(**bad) == -1 and bwd(False, **bad) == -1, bad
     for bad in (dict(dtype=3), dict(dy_dtype=3), dict(g_dtype=3), dict(K=N.DENSE_MAX_FEATURES + 1)):
         assert bwd(**bad) == -2, bad
+    big = dict(M=(1 << 26) - 1, N=1 << 20, K=1 << 20, sx=1 << 20, sw=1 << 20, sdy=1 << 20)
+    assert bwd(**big) == -2 and bwd(False, **big) == -2
     assert bwd(False, ws=4096, ws_bytes=8) == -3
     assert bwd(False, M=0, dY=0) == 0
 
