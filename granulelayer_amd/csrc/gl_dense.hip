@@ -12,13 +12,20 @@ inline long long padded(long long n) { return round_up(n, 8); }  // row of a cop
 // The tile kernel loads 16 bytes at a time straight into LDS.  An operand whose rows do not start at
 // 16-byte addresses, or (reduction along the row) end inside 16 bytes, is copied to rows of padded(cols)
 // elements first, zeros behind the last: one pass over an operand that the product reads many times.
+// Up to two operands a launch (blockIdx.z).
+struct AlignK {
+  const void* src[2];
+  void* dst[2];
+  long long ld[2], rows[2];
+  int cols[2];
+};
 template <typename T>
-__global__ __launch_bounds__(256) void dense_align_kernel(const T* __restrict__ src, long long ld, long long rows, int cols,
-                                                          T* __restrict__ dst) {
-  const int ldd = (cols + 7) / 8 * 8;
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void dense_align_kernel(AlignK a) {
+  const int z = blockIdx.z, cols = a.cols[z], ldd = (cols + 7) / 8 * 8;
+  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), ld = a.ld[z];
   const int c0 = (blockIdx.y * 64 + (threadIdx.x & 63)) * 8;
-  if (r >= rows || c0 >= ldd) return;
+  if (r >= a.rows[z] || c0 >= ldd) return;
+  const T* src = (const T*)a.src[z];
   T v[8];
   if (c0 + 8 <= cols) {
     struct __attribute__((packed, aligned(2))) U { T x[8]; };
@@ -29,7 +36,7 @@ __global__ __launch_bounds__(256) void dense_align_kernel(const T* __restrict__ 
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = c0 + j < cols ? src[r * ld + c0 + j] : T(0);
   }
-  T* d = dst + r * ldd + c0;
+  T* d = (T*)a.dst[z] + r * ldd + c0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) d[j] = v[j];
 }
@@ -58,17 +65,32 @@ inline size_t copy_bytes(const Operand& o, int es) {
   return o.copied ? (size_t)round_up(o.rows * padded(o.cols) * es, 256) : 0;
 }
 
-int launch_align(Operand& o, int es, void* dst, hipStream_t s) {
-  const dim3 grid((unsigned)((o.rows + 3) / 4), (unsigned)ceil_div(padded(o.cols), 512));
-  if (es == 2)
-    GL_LAUNCH(GL_KERNEL_DENSE_ALIGN, dense_align_kernel<unsigned short>, grid, dim3(256), 0, s, (const unsigned short*)o.p,
-              o.ld, o.rows, o.cols, (unsigned short*)dst);
-  else
-    GL_LAUNCH(GL_KERNEL_DENSE_ALIGN, dense_align_kernel<unsigned>, grid, dim3(256), 0, s, (const unsigned*)o.p, o.ld, o.rows,
-              o.cols, (unsigned*)dst);
+// copies those of the operands (null or not) that need it to their places; they then are the copies
+int launch_align(Operand* o0, void* dst0, Operand* o1, void* dst1, int es, hipStream_t s) {
+  AlignK k{};
+  int n = 0, cols = 0;
+  long long rows = 0;
+  Operand* const ops[2] = {o0, o1};
+  void* const dst[2] = {dst0, dst1};
+  for (int i = 0; i < 2; ++i) {
+    Operand* o = ops[i];
+    if (!o || !o->copied) continue;
+    k.src[n] = o->p;
+    k.dst[n] = dst[i];
+    k.ld[n] = o->ld;
+    k.rows[n] = o->rows;
+    k.cols[n] = o->cols;
+    rows = o->rows > rows ? o->rows : rows;
+    cols = o->cols > cols ? o->cols : cols;
+    ++n;
+    o->p = dst[i];
+    o->ld = padded(o->cols);
+  }
+  if (n == 0) return 0;
+  const dim3 grid((unsigned)((rows + 3) / 4), (unsigned)ceil_div(padded(cols), 512), (unsigned)n);
+  if (es == 2) GL_LAUNCH(GL_KERNEL_DENSE_ALIGN, dense_align_kernel<unsigned short>, grid, dim3(256), 0, s, k);
+  else GL_LAUNCH(GL_KERNEL_DENSE_ALIGN, dense_align_kernel<unsigned>, grid, dim3(256), 0, s, k);
   GL_CHECK_LAUNCH();
-  o.p = dst;
-  o.ld = padded(o.cols);
   return 0;
 }
 
@@ -169,8 +191,11 @@ int run_product(int dtype, int form, const Operand& p, const Operand& q, long lo
 
 // ---- dz = dY act'(z) and the sums of its columns -------------------------------------------------------
 constexpr int DZ_COLS = 256;  // of a workgroup: 32 lanes of 8 columns by 8 rows at a time
-constexpr int DZ_AHEAD = 4;   // rows a lane has in flight
-// rows of a workgroup: one or two batches of loads, one where two would leave CUs without a workgroup
+// Rows a lane has in flight.  The 8-bit form costs more instructions and fewer bytes: more waves instead of rows.
+// 16384 x 4096 bf16, 340 MB: 2 rows 81 us, 4 rows 88, 8 rows 120; z as it was, 4096 x 4096: 2 rows 23.2, 4 rows 22.5, 8
+// rows 30.5.  (About 30 slots an element, 58 us of the 81, beside 70 of memory.)
+constexpr int dz_ahead(int keep) { return keep == GL_KEEP_Z8 ? 2 : 4; }
+// rows of a workgroup: half where the whole would leave CUs without a workgroup
 inline int dz_rows(long long M, int N) { return (M + 63) / 64 * ceil_div(N, DZ_COLS) >= 512 ? 64 : 32; }
 
 // dz may be null (only the sums), part too (only dz).  Rows of dz are padded(N) apart, zeros behind N.
@@ -178,6 +203,7 @@ template <bool YBF, bool OBF, int KEEP>
 __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ dY, long long sdy, const void* __restrict__ z,
                                                        const uint8_t* __restrict__ ze, long long M, int N,
                                                        int rows, void* __restrict__ dz, float* __restrict__ part) {
+  constexpr int AHEAD = dz_ahead(KEEP);
   __shared__ float sums[8][DZ_COLS];
   const int ct = threadIdx.x & 31, rt = threadIdx.x >> 5;
   const int n = blockIdx.y * DZ_COLS + ct * 8;
@@ -186,15 +212,15 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ 
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (n < N) {
 #pragma unroll 1
-    for (int i = 0; i < rows; i += 8 * DZ_AHEAD) {
+    for (int i = 0; i < rows; i += 8 * AHEAD) {
       const long long m0 = (long long)blockIdx.x * rows + i + rt;
       if (m0 >= M) break;
-      float g[DZ_AHEAD][8], t[DZ_AHEAD][8];
-      unsigned bits[DZ_AHEAD];
-      uv2 codes[DZ_AHEAD];
-      int ex[DZ_AHEAD];
+      float g[AHEAD][8], t[AHEAD][8];
+      unsigned bits[AHEAD];
+      uv2 codes[AHEAD];
+      int ex[AHEAD];
 #pragma unroll
-      for (int x = 0; x < DZ_AHEAD; ++x) {
+      for (int x = 0; x < AHEAD; ++x) {
         const long long m = m0 + 8 * x;
         const int there = m < M ? N - n : 0;
         load8<YBF>(dY, m * sdy + n, there, g[x]);
@@ -210,19 +236,20 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ 
         }
       }
 #pragma unroll
-      for (int x = 0; x < DZ_AHEAD; ++x) {
+      for (int x = 0; x < AHEAD; ++x) {
         const long long m = m0 + 8 * x;
         if constexpr (KEEP == GL_KEEP_SIGN) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) g[x][j] = (bits[x] >> j) & 1u ? g[x][j] : 0.f;
         } else if constexpr (KEEP != GL_KEEP_NONE) {
           const float st = KEEP == GL_KEEP_Z8 ? p8_step(ex[x]) : 0.f;
-          // columns behind N hold dY's 0 and z's 0 (a code of 0 is NaN in a block without numbers)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float zj = KEEP == GL_KEEP_Z8 ? p8_value(codes[x][j >> 2], j & 3, st) : t[x][j];
-            g[x][j] = n + j < N ? g[x][j] * dgelu_f(zj) : 0.f;
-          }
+          for (int j = 0; j < 8; ++j)
+            g[x][j] *= dgelu_f(KEEP == GL_KEEP_Z8 ? p8_value(codes[x][j >> 2], j & 3, st) : t[x][j]);
+          // columns behind N hold dY's 0, but a code of 0 is NaN in a block without numbers
+          if (KEEP == GL_KEEP_Z8 && n + 8 > N)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[x][j] = n + j < N ? g[x][j] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[j] += g[x][j];
@@ -457,8 +484,7 @@ extern "C" int gl_dense_fwd(const GlDenseArgs* a, void* stream) {
   if (p.few) return launch_dense_few(a, e, s);
   const int es = es_of(a->dtype);
   char* ws = (char*)a->ws;
-  if (p.x.copied) GL_TRY(launch_align(p.x, es, ws, s));
-  if (p.w.copied) GL_TRY(launch_align(p.w, es, ws + p.off_w, s));
+  GL_TRY(launch_align(&p.x, ws, &p.w, ws + p.off_w, es, s));
   return run_product(a->dtype, DENSE_NT, p.x, p.w, a->K, p.pr, ws + p.off_part, e, s);
 }
 
@@ -492,8 +518,8 @@ extern "C" int gl_dense_bwd(const GlDenseBwdArgs* a, void* stream) {
     GL_CHECK_LAUNCH();
   }
   if (dz) p.dz_nn.p = p.dz_tn.p = dz;
+  GL_TRY(launch_align(a->dW && a->X ? &p.x : nullptr, ws + p.off_x, a->dX ? &p.w : nullptr, ws + p.off_w, es, s));
   if (a->dX) {
-    if (p.w.copied) GL_TRY(launch_align(p.w, es, ws + p.off_w, s));
     GL_TRY(run_product(a->dtype, DENSE_NN, p.dz_nn, p.w, a->N, p.px, ws + p.off_part,
                        store_epi(a->dX, a->K, a->dtype, a->M, a->K, a->dtype, 0), s));
   }
@@ -501,8 +527,6 @@ extern "C" int gl_dense_bwd(const GlDenseBwdArgs* a, void* stream) {
     if (!a->X) {
       GL_TRY(launch_unpack8(a->xq, a->xe, a->M, a->K, ws + p.off_x, p.x.ld, a->dtype, s));
       p.x.p = ws + p.off_x;
-    } else if (p.x.copied) {
-      GL_TRY(launch_align(p.x, es, ws + p.off_x, s));
     }
     GL_TRY(run_product(a->dtype, DENSE_TN, p.dz_tn, p.x, a->M, p.pw, ws + p.off_part,
                        store_epi(a->dW, a->K, a->g_dtype, a->N, a->K, a->dtype, a->accumulate), s));

@@ -425,3 +425,31 @@ def test_refusals_on_the_gpu():
     w2.main_grad = torch.zeros(24, 16, device=DEV, dtype=BF)
     with pytest.raises(ValueError, match="main_grad"):
         dense_projection(x, w2).backward(t["dy"])
+
+
+@pytest.mark.parametrize("ckpt", ["exact", "int8"])
+def test_gelu_over_the_whole_line(ckpt):
+    """gelu and its derivative by themselves: a product with one weight of 1 hands every fp32 z through (exactly, 1 z
+    has one term), from subnormals to the largest numbers, infinities and NaN."""
+    f = torch.finfo(F32)
+    z = torch.cat([torch.linspace(-15, 15, 200001), torch.tensor([0.0, -0.0, f.tiny, -f.tiny, 1e-40, 7.99, 8.01, -8.01, 6.49, 6.51,
+                   -6.51, 40.0, -40.0, 1e4, -1e4, 1e19, -1e19, f.max, -f.max, float("inf"), float("-inf"), float("nan")])])
+    z = z.to(DEV).reshape(-1, 1).requires_grad_(True)
+    one = torch.ones(1, 1, device=DEV)
+    y = dense_projection(z, one, None, None, "gelu", ckpt)
+    served = dense_projection(z.detach()[:50], one, None, None, "gelu")
+    assert torch.equal(served, y.detach()[:50])
+    z6 = z.detach().double()
+    want = torch.where(z6 == float("-inf"), 0.0, act64(z6, "gelu"))
+    fine = ~want.isnan()
+    assert bool(want[:-1].isnan().logical_not().all()) and bool(y[-1].isnan())
+    # the last place of z (z - a Q(a) is rounded there) and 1e-7 of the polynomial
+    err = (y.detach().double() - want).abs()[fine & want.isfinite()]
+    assert bool((err <= 2 * U * z6.abs()[fine & want.isfinite()] + 1e-7).all())
+    assert float(y.detach()[-3]) == float("inf")
+    g, = torch.autograd.grad(y, z, torch.ones_like(y))
+    if ckpt == "exact":
+        w = torch.where(z6.abs() > 1e3, (z6 > 0).double(), dact64(z6, "gelu"))
+        assert bool(((g.double() - w).abs()[:-1] <= 4e-7).all()) and bool(g[-1].isnan())
+    else:
+        assert bool(g[-3:].isnan().all()) and bool(g[:-3].isfinite().all())
