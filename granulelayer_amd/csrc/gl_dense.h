@@ -22,6 +22,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
+// Bytes of reduction of a stage: a cache line of an RC row (half lines are fetched twice), 64 bf16 or 32 fp32.
+constexpr int DENSE_BK = 128;
+
 // What becomes of a product's sums.
 struct DenseEpi {
   const void* bias;  // operands' type, or null
@@ -44,14 +47,14 @@ struct DenseK {
   long long ldp, ldq;  // bytes between rows
   long long R;         // reduction; behind it an RC operand's rows have zeros up to 16 bytes
   int tiles_m, tiles_n;
-  int steps, steps_per_split;  // stages of the tile's dense_bk() bytes
+  int steps, steps_per_split;  // stages
   float* part;                 // split products: sums [split][M][N], joined by dense_join_kernel
   DenseEpi e;
 };
 
 // ---- activations -----------------------------------------------------------------------------------
 // GELU from the normal distribution's upper tail: with a = |z| and Q(a) = 1 - Phi(a),
-//     gelu(z) = max(z, 0) - a Q(a)        gelu'(z) = Phi(z) + z phi(z)
+//     gelu(z) = max(z, 0) - a Q(a)
 // and Q(a) = 2^R(a): log2 of the tail is smooth, and a polynomial of degree 8, fitted on [0, 8] by least squares
 // weighted with a Q(a), leaves 8e-9 in a Q(a).  Evaluated in fp32 gelu is within 2.5e-7 of the exact values over
 // [-14, 14] (the last place of z near 4), and keeps its relative accuracy in the negative tail, where 1 + erf
@@ -74,12 +77,24 @@ __device__ __forceinline__ float gelu_f(float z) {
   const float a = __builtin_fminf(__builtin_fabsf(z), 8.f);
   return __builtin_fmaf(-a, upper_tail(a), relu_f(z));
 }
+// gelu'(z) = D(a) for z < 0 and 1 - D(a) else, D(a) = Q(a) - a phi(a) = exp(-a^2 / 2) P(a): P of degree 10, by
+// least squares weighted with the exponential, leaves 7e-8 on [0, 6.5], and D(6.5) is below 2e-9; within 1.7e-7 in
+// fp32.  One exponential, 18 slots.
 __device__ __forceinline__ float dgelu_f(float z) {
-  // past 20 the density is below 1e-87, zero in fp32; NaN passes the comparison
-  const float c = __builtin_fabsf(z) > 20.f ? __builtin_copysignf(20.f, z) : z;
-  const float q = upper_tail(__builtin_fminf(__builtin_fabsf(z), 8.f));
-  const float phi = 0.39894228f * __builtin_amdgcn_exp2f(c * c * -0.72134752f);
-  return __builtin_fmaf(c, phi, c < 0.f ? q : 1.f - q);
+  const float m = __builtin_fabsf(z), a = m > 6.5f ? 6.5f : m;  // NaN stays
+  float p = 1.63169273e-06f;
+  p = __builtin_fmaf(p, a, -3.5207835e-05f);
+  p = __builtin_fmaf(p, a, 0.000339738821f);
+  p = __builtin_fmaf(p, a, -0.00197462901f);
+  p = __builtin_fmaf(p, a, 0.00793939456f);
+  p = __builtin_fmaf(p, a, -0.024313936f);
+  p = __builtin_fmaf(p, a, 0.0611548908f);
+  p = __builtin_fmaf(p, a, -0.132513806f);
+  p = __builtin_fmaf(p, a, 0.249916792f);
+  p = __builtin_fmaf(p, a, -0.797878802f);
+  p = __builtin_fmaf(p, a, 0.49999994f);
+  const float d = p * __builtin_amdgcn_exp2f(a * a * -0.72134752f);
+  return z < 0.f ? d : 1.f - d;
 }
 __device__ __forceinline__ float act_rt(int act, float z) {
   return act == GL_ACT_RELU ? relu_f(z) : (act == GL_ACT_GELU ? gelu_f(z) : z);
@@ -277,17 +292,18 @@ __device__ __forceinline__ i32x4 buffer_of(const char* p, long long bytes) {
 }
 constexpr unsigned DMA_NOWHERE = 0x80000000u;  // past any buffer_of; offsets are below
 
-// One operand's side of a tile: DIM rows of the output (RC) or columns (RS) by BK bytes of reduction,
+// One operand's side of a tile: DIM rows of the output (RC) or columns (RS) by DENSE_BK bytes of reduction,
 // staged by NW waves.
 //
-// LDS of an RC operand: rows of BK bytes, 16-byte chunk c of row r at c ^ key(r).  A 16-byte read of 16
+// LDS of an RC operand: rows of 128 bytes, 16-byte chunk c of row r at c ^ key(r).  A 16-byte read of 16
 // neighbouring rows takes each of the 16 chunks of a 256-byte bank row once, and rows 16..31 take them in
-// the same order: LDS then delivers 256 bytes a clock (half of it with c ^ (r & 7) at BK = 128: rows r and
-// r + 8 collide).  Of an RS operand: the reduction's rows of DIM values; for bf16 the 32-byte unit u of row
-// r at u ^ swz(r): a transposing read takes 32 bytes of four rows r..r + 3 (two such groups per half wave,
-// of neighbouring units), and the swizzle puts those on all banks.
-template <int ES, int DIM, int NW, bool RC, int BK>
+// the same order: LDS then delivers 256 bytes a clock (half of it with c ^ (r & 7): rows r and r + 8
+// collide).  Of an RS operand: the reduction's rows of DIM values; for bf16 the 32-byte unit u of row r at
+// u ^ swz(r): a transposing read takes 32 bytes of four rows r..r + 3 (two such groups per half wave, of
+// neighbouring units), and the swizzle puts those on all banks.
+template <int ES, int DIM, int NW, bool RC>
 struct Side {
+  static constexpr int BK = DENSE_BK;
   static constexpr int BYTES = DIM * BK;
   static constexpr int LOADS = BYTES / 1024 / NW;  // of one wave and stage
   static constexpr int RROWS = BK / ES;            // rows of an RS stage
@@ -300,7 +316,7 @@ struct Side {
   unsigned off[LOADS];
   int k_lane, k_left;  // RC: this lane's first byte of the reduction in a stage; the reduction's bytes from p
 
-  static __device__ __forceinline__ int key(int r) { return BK == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+  static __device__ __forceinline__ int key(int r) { return (r >> 1) & 7; }
   static __device__ __forceinline__ int swz(int r) {
     if constexpr (ES == 2) return (((r & 3) << 1) | (((r >> 3) & 1) << 3)) & (DIM / 16 - 1);
     return 0;
@@ -368,9 +384,9 @@ template <> struct Frag<4> {
   f32x4 v;
 };
 
-template <int ES, int DIM, bool RC, int BK>
+template <int ES, int DIM, bool RC>
 struct Reader {
-  static constexpr int READS = RC ? 1 : (ES == 2 ? 2 : 4);  // LDS instructions of a fragment
+  static constexpr int BK = DENSE_BK;
   unsigned a[RC ? BK / 32 : 1];       // byte of chunk kk in the lane's row
   unsigned col[RC ? 1 : DIM / 32];
   // base: this wave's first row / column of the tile, a multiple of 32
@@ -379,10 +395,10 @@ struct Reader {
     if constexpr (RC) {
 #pragma unroll
       for (int kk = 0; kk < BK / 32; ++kk)
-        a[kk] = (base + (l & 31)) * BK + (((2 * kk + (l >> 5)) ^ Side<ES, DIM, 2, true, BK>::key(l & 31)) * 16);
+        a[kk] = (base + (l & 31)) * BK + (((2 * kk + (l >> 5)) ^ Side<ES, DIM, 2, true>::key(l & 31)) * 16);
     } else if constexpr (ES == 2) {
       const int g = l >> 4, i = l & 15, r = 8 * (g >> 1) + (i >> 2);
-      const int sw = Side<ES, DIM, 2, false, BK>::swz(r);
+      const int sw = Side<ES, DIM, 2, false>::swz(r);
 #pragma unroll
       for (int t = 0; t < DIM / 32; ++t)
         col[t] = r * (DIM * 2) + (((base / 16 + 2 * t + (g & 1)) ^ sw) * 32) + 8 * (i & 3);
@@ -427,11 +443,11 @@ __device__ __forceinline__ void copies_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <int ES, int BM, int BN, int WM, int WN, int BK, int NSP, int NSQ, bool PRC, bool QRC>
-__global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 8192 ? 1 : 2) void dense_tile_kernel(DenseK a) {
-  constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
-  typedef Side<ES, BM, NW, PRC, BK> SP;
-  typedef Side<ES, BN, NW, QRC, BK> SQ;
+template <int ES, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC>
+__global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
+  constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, BK = DENSE_BK;
+  typedef Side<ES, BM, NW, PRC> SP;
+  typedef Side<ES, BN, NW, QRC> SQ;
   constexpr int LDS_Q = NSP * SP::BYTES, LDS = LDS_Q + NSQ * SQ::BYTES;  // P's stages, then Q's
   extern __shared__ __align__(1024) char smem[];
   int tm, tn, split;
@@ -446,8 +462,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 8192 ? 1 : 2) v
   SQ sq;
   sp.init(a.P, a.ldp, m0, a.e.M, a.R, k0);
   sq.init(a.Q, a.ldq, n0, a.e.N, a.R, k0);
-  Reader<ES, BM, PRC, BK> rp;
-  Reader<ES, BN, QRC, BK> rq;
+  Reader<ES, BM, PRC> rp;
+  Reader<ES, BN, QRC> rq;
   rp.init(wm * TM * 32);
   rq.init(wn * TN * 32);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
@@ -558,7 +574,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 8192 ? 1 : 2) v
   // stores and loads share a counter that runs in order, and a load behind a store waits for it.  A lane's rows
   // are in registers four together, so types, kinds and edges are decided once for all of them.  (A row at a
   // time, with its loads and branches, took 33,000 clocks a tile, as long as 12 stages of products.)
-  static_assert(TN % 2 == 0 && NW * 32 * 68 * 4 <= LDS, "a wave's rows of 64 columns");
+  static_assert(TN == 2 && NW * 32 * 68 * 4 <= LDS, "a wave's rows of 64 columns");
   constexpr bool FORWARD = PRC && QRC;  // bias, activation, residual and what is kept; else sums as they are
   constexpr int ROWS = 4;               // of a lane at a time, 4 apart
   copies_barrier<0>();
@@ -570,84 +586,81 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 8192 ? 1 : 2) v
   const bool c_bf = !split_up && a.e.c_bf;
   const long long c_step = (split_up ? a.e.N : a.e.sc) * (c_bf ? 2 : 4);
   const bool inside = m0 + BM <= a.e.M && n0 + BN <= a.e.N;
+  const int n = n0 + wn * 64 + (l & 15) * 4, there = a.e.N - n;
+  const long long mw = m0 + wm * TM * 32 + (l >> 4);
+  float bias[4];
+  if constexpr (FORWARD) dense_bias(a.e, n, bias);
+  uv4 r[ROWS];
+  auto load_rows = [&](long long m) {
+    const char* p = added.p + m * added.step + (long long)n * (added.bf ? 2 : 4);
+    if (inside && added.bf) {
 #pragma unroll
-  for (int jj = 0; jj < TN; jj += 2) {
-    const int n = n0 + (wn * TN + jj) * 32 + (l & 15) * 4, there = a.e.N - n;
-    const long long mw = m0 + wm * TM * 32 + (l >> 4);
-    float bias[4];
-    if constexpr (FORWARD) dense_bias(a.e, n, bias);
-    uv4 r[ROWS];
-    auto load_rows = [&](long long m) {
-      const char* p = added.p + m * added.step + (long long)n * (added.bf ? 2 : 4);
-      if (inside && added.bf) {
-#pragma unroll
-        for (int x = 0; x < ROWS; ++x) {
-          const uv2 t = reinterpret_cast<const bytes8*>(p + 4 * x * added.step)->v;
-          r[x] = uv4{t[0], t[1], 0u, 0u};
-        }
-      } else if (inside) {
-#pragma unroll
-        for (int x = 0; x < ROWS; ++x) r[x] = reinterpret_cast<const bytes16*>(p + 4 * x * added.step)->v;
-      } else {
-#pragma unroll
-        for (int x = 0; x < ROWS; ++x) {
-          r[x] = uv4{0u, 0u, 0u, 0u};
-          if (m + 4 * x < a.e.M && there > 0) r[x] = load_added(p + 4 * x * added.step, added.bf, there);
-        }
+      for (int x = 0; x < ROWS; ++x) {
+        const uv2 t = reinterpret_cast<const bytes8*>(p + 4 * x * added.step)->v;
+        r[x] = uv4{t[0], t[1], 0u, 0u};
       }
-    };
-    if (added.p) load_rows(mw);
+    } else if (inside) {
+#pragma unroll
+      for (int x = 0; x < ROWS; ++x) r[x] = reinterpret_cast<const bytes16*>(p + 4 * x * added.step)->v;
+    } else {
+#pragma unroll
+      for (int x = 0; x < ROWS; ++x) {
+        r[x] = uv4{0u, 0u, 0u, 0u};
+        if (m + 4 * x < a.e.M && there > 0) r[x] = load_added(p + 4 * x * added.step, added.bf, there);
+      }
+    }
+  };
+  if (added.p) load_rows(mw);
 #pragma unroll 1
-    for (int i = 0; i < TM; ++i) {
+  for (int i = 0; i < TM; ++i) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          f32x4 t;
+      for (int g = 0; g < 4; ++g) {
+        f32x4 t;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) t[x] = acc[0][jj + j][4 * g + x];
-          *reinterpret_cast<f32x4*>(own + (l & 31) * 68 + 32 * j + 8 * g + 4 * (l >> 5)) = t;
-        }
-      // a rolled loop (its code is loaded once): the rows of accumulators move up
+        for (int x = 0; x < 4; ++x) t[x] = acc[0][j][4 * g + x];
+        *reinterpret_cast<f32x4*>(own + (l & 31) * 68 + 32 * j + 8 * g + 4 * (l >> 5)) = t;
+      }
+    // a rolled loop (its code is loaded once): the rows of accumulators move up
 #pragma unroll
-      for (int y = 0; y + 1 < TM; ++y)
+    for (int y = 0; y + 1 < TM; ++y)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[y][jj + j] = acc[y + 1][jj + j];
+      for (int j = 0; j < 2; ++j) acc[y][j] = acc[y + 1][j];
 #pragma unroll 1
-      for (int y = 0; y < 32; y += 4 * ROWS) {
-        const long long mi = mw + i * 32 + y;
-        float v[ROWS][4];
+    for (int y = 0; y < 32; y += 4 * ROWS) {
+      const long long mi = mw + i * 32 + y;
+      float v[ROWS][4];
 #pragma unroll
-        for (int x = 0; x < ROWS; ++x) {
-          const f32x4 t = *reinterpret_cast<const f32x4*>(own + (y + 4 * x + (l >> 4)) * 68 + (l & 15) * 4);
+      for (int x = 0; x < ROWS; ++x) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(own + (y + 4 * x + (l >> 4)) * 68 + (l & 15) * 4);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[x][j] = t[j];
-        }
-        if constexpr (FORWARD) {
-          if (!split_up) dense_forward<ROWS>(a.e, mi, 4, n, v, bias);
-        }
-        if (added.p) {
-          if (added.bf) {
+        for (int j = 0; j < 4; ++j) v[x][j] = t[j];
+      }
+      if constexpr (FORWARD) {
+        if (!split_up) dense_forward<ROWS>(a.e, mi, 4, n, v, bias);
+      }
+      if (added.p) {
+        if (added.bf) {
 #pragma unroll
-            for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], true);
-          } else {
-#pragma unroll
-            for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], false);
-          }
-          if (i + 1 < TM || y + 4 * ROWS < 32) load_rows(mi + 4 * ROWS);
-        }
-        char* c = C + mi * c_step + (long long)n * (c_bf ? 2 : 4);
-        if (inside && c_bf) {
-#pragma unroll
-          for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, true, 0, 4, v[x]);
-        } else if (inside) {
-#pragma unroll
-          for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, false, 0, 4, v[x]);
+          for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], true);
         } else {
 #pragma unroll
-          for (int x = 0; x < ROWS; ++x)
-            if (mi + 4 * x < a.e.M && there > 0) store4(c + 4 * x * c_step, c_bf, 0, there, v[x]);
+          for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], false);
         }
+        if (i + 1 < TM || y + 4 * ROWS < 32) load_rows(mi + 4 * ROWS);
+      }
+      char* c = C + mi * c_step + (long long)n * (c_bf ? 2 : 4);
+      if (inside && c_bf) {
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, true, 0, 4, v[x]);
+      } else if (inside) {
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, false, 0, 4, v[x]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x)
+          if (mi + 4 * x < a.e.M && there > 0) store4(c + 4 * x * c_step, c_bf, 0, there, v[x]);
       }
     }
   }
@@ -655,34 +668,33 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 8192 ? 1 : 2) v
 
 // ---- host side ---------------------------------------------------------------------------------------
 enum { DENSE_NT = 0, DENSE_NN = 1, DENSE_TN = 2 };  // P, Q: RC RC; RC RS; RS RS
-constexpr int DENSE_BK = 128;                            // bytes of reduction of a stage: a cache line of an RC row
 // Tiles.  The large one keeps the matrix cores fed at the least traffic; the smaller ones fill the chip when
 // there are few.  DEEP: three stages (one workgroup a CU), which hides more of a load's latency where few
 // workgroups run.
 enum { DENSE_256 = 0, DENSE_256X128 = 1, DENSE_128 = 2, DENSE_128_DEEP = 3, DENSE_64 = 4, DENSE_TILES = 5 };
 constexpr int DENSE_BM[DENSE_TILES] = {256, 256, 128, 128, 64}, DENSE_BN[DENSE_TILES] = {256, 128, 128, 128, 128};
 
-template <int ES, int BM, int BN, int WM, int WN, int BK, int NSP, int NSQ, bool PRC, bool QRC>
+template <int ES, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC>
 int launch_dense_tile_as(const DenseK& a, int splits, hipStream_t s) {
-  constexpr size_t lds = (NSP * BM + NSQ * BN) * BK;
+  constexpr size_t lds = (NSP * BM + NSQ * BN) * DENSE_BK;
   // the kernel's LDS limit is raised once a device
   static std::atomic<unsigned long long> raised{0};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return GL_ERR_DEVICE;
   if (!(raised.load(std::memory_order_relaxed) >> dev & 1)) {
-    GL_TRY(set_lds_limit((const void*)dense_tile_kernel<ES, BM, BN, WM, WN, BK, NSP, NSQ, PRC, QRC>, lds));
+    GL_TRY(set_lds_limit((const void*)dense_tile_kernel<ES, BM, BN, WM, WN, NSP, NSQ, PRC, QRC>, lds));
     raised.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  GL_LAUNCH(GL_KERNEL_DENSE, (dense_tile_kernel<ES, BM, BN, WM, WN, BK, NSP, NSQ, PRC, QRC>),
+  GL_LAUNCH(GL_KERNEL_DENSE, (dense_tile_kernel<ES, BM, BN, WM, WN, NSP, NSQ, PRC, QRC>),
             dim3((unsigned)(a.tiles_m * a.tiles_n * splits)), dim3(64 * WM * WN), lds, s, a);
   GL_CHECK_LAUNCH();
   return 0;
 }
-template <int ES, int BM, int BN, int WM, int WN, int BK, int NSP, int NSQ>
+template <int ES, int BM, int BN, int WM, int WN, int NSP, int NSQ>
 int launch_dense_tile_of(int form, const DenseK& a, int splits, hipStream_t s) {
-  if (form == DENSE_NT) return launch_dense_tile_as<ES, BM, BN, WM, WN, BK, NSP, NSQ, true, true>(a, splits, s);
-  if (form == DENSE_NN) return launch_dense_tile_as<ES, BM, BN, WM, WN, BK, NSP, NSQ, true, false>(a, splits, s);
-  return launch_dense_tile_as<ES, BM, BN, WM, WN, BK, NSP, NSQ, false, false>(a, splits, s);
+  if (form == DENSE_NT) return launch_dense_tile_as<ES, BM, BN, WM, WN, NSP, NSQ, true, true>(a, splits, s);
+  if (form == DENSE_NN) return launch_dense_tile_as<ES, BM, BN, WM, WN, NSP, NSQ, true, false>(a, splits, s);
+  return launch_dense_tile_as<ES, BM, BN, WM, WN, NSP, NSQ, false, false>(a, splits, s);
 }
 int launch_dense_tile_bf16(int form, int tile, const DenseK& a, int splits, hipStream_t s);
 int launch_dense_tile_f32(int form, int tile, const DenseK& a, int splits, hipStream_t s);

@@ -95,7 +95,8 @@ int launch_align(Operand* o0, void* dst0, Operand* o1, void* dst1, int es, hipSt
 }
 
 // ---- the sums of a split product --------------------------------------------------------------------
-// A lane holds 4 neighbouring columns and adds the splits in their order, then the epilogue.
+// A lane holds 4 neighbouring columns and adds the splits in their order, then the epilogue.  Bound by the sums'
+// bytes: 2 x 2048 x 1024 fp32 in 5.7 us (4.4 TB/s).
 __global__ __launch_bounds__(256) void dense_join_kernel(const float* __restrict__ part, int splits, DenseEpi e) {
   const long long m = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int l = threadIdx.x & 63, n = blockIdx.y * 256 + l * 4, there = m < e.M ? e.N - n : 0;
@@ -191,19 +192,19 @@ int run_product(int dtype, int form, const Operand& p, const Operand& q, long lo
 
 // ---- dz = dY act'(z) and the sums of its columns -------------------------------------------------------
 constexpr int DZ_COLS = 256;  // of a workgroup: 32 lanes of 8 columns by 8 rows at a time
-// Rows a lane has in flight.  The 8-bit form costs more instructions and fewer bytes: more waves instead of rows.
-// 16384 x 4096 bf16, 340 MB: 2 rows 81 us, 4 rows 88, 8 rows 120; z as it was, 4096 x 4096: 2 rows 23.2, 4 rows 22.5, 8
-// rows 30.5.  (About 30 slots an element, 58 us of the 81, beside 70 of memory.)
-constexpr int dz_ahead(int keep) { return keep == GL_KEEP_Z8 ? 2 : 4; }
+// Rows a lane has in flight: more of them leave fewer waves.  16384 x 4096 bf16 with z in 8 bits, 340 MB: 2 rows 68 us
+// (5.0 TB/s), 4 rows 78, 8 rows 120; z as it was, 4096 x 4096: 2 and 4 rows 22, 8 rows 30.
+constexpr int DZ_AHEAD = 2;
 // rows of a workgroup: half where the whole would leave CUs without a workgroup
 inline int dz_rows(long long M, int N) { return (M + 63) / 64 * ceil_div(N, DZ_COLS) >= 512 ? 64 : 32; }
 
+// One pass over dY and what was kept; memory bound.  dz is rounded to the operands' type, which the matrix
+// instructions of dX and dW take (half a step of bf16 an element, beside W's and X's own); db sums it unrounded in fp32.
 // dz may be null (only the sums), part too (only dz).  Rows of dz are padded(N) apart, zeros behind N.
 template <bool YBF, bool OBF, int KEEP>
 __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ dY, long long sdy, const void* __restrict__ z,
                                                        const uint8_t* __restrict__ ze, long long M, int N,
                                                        int rows, void* __restrict__ dz, float* __restrict__ part) {
-  constexpr int AHEAD = dz_ahead(KEEP);
   __shared__ float sums[8][DZ_COLS];
   const int ct = threadIdx.x & 31, rt = threadIdx.x >> 5;
   const int n = blockIdx.y * DZ_COLS + ct * 8;
@@ -212,15 +213,15 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ 
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (n < N) {
 #pragma unroll 1
-    for (int i = 0; i < rows; i += 8 * AHEAD) {
+    for (int i = 0; i < rows; i += 8 * DZ_AHEAD) {
       const long long m0 = (long long)blockIdx.x * rows + i + rt;
       if (m0 >= M) break;
-      float g[AHEAD][8], t[AHEAD][8];
-      unsigned bits[AHEAD];
-      uv2 codes[AHEAD];
-      int ex[AHEAD];
+      float g[DZ_AHEAD][8], t[DZ_AHEAD][8];
+      unsigned bits[DZ_AHEAD];
+      uv2 codes[DZ_AHEAD];
+      int ex[DZ_AHEAD];
 #pragma unroll
-      for (int x = 0; x < AHEAD; ++x) {
+      for (int x = 0; x < DZ_AHEAD; ++x) {
         const long long m = m0 + 8 * x;
         const int there = m < M ? N - n : 0;
         load8<YBF>(dY, m * sdy + n, there, g[x]);
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ 
         }
       }
 #pragma unroll
-      for (int x = 0; x < AHEAD; ++x) {
+      for (int x = 0; x < DZ_AHEAD; ++x) {
         const long long m = m0 + 8 * x;
         if constexpr (KEEP == GL_KEEP_SIGN) {
 #pragma unroll
@@ -269,7 +270,8 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ 
   part[(long long)blockIdx.x * N + c] = t;
 }
 
-// db from the sums of `chunks` row blocks: 32 columns a workgroup, 32 rows of lanes, then LDS
+// db from the sums of `chunks` row blocks: 32 columns a workgroup, 32 rows of lanes, then LDS.  256 x 4096 sums: 6 us,
+// the latency of 8 dependent loads.
 __global__ __launch_bounds__(1024) void dense_db_kernel(const float* __restrict__ part, long long chunks, int N,
                                                         void* __restrict__ db, int g_bf, int accumulate) {
   __shared__ float sums[32][33];
