@@ -453,3 +453,29 @@ def test_gelu_over_the_whole_line(ckpt):
         assert bool(((g.double() - w).abs()[:-1] <= 4e-7).all()) and bool(g[-1].isnan())
     else:
         assert bool(g[-3:].isnan().all()) and bool(g[:-3].isfinite().all())
+
+
+def test_past_32_bits():
+    """Rows whose elements and bytes are past 2^31 and 2^32 of x, y, z and dy.  dy is zero but on those rows, and sums
+    with zeros are exact, so the gradients' bounds are those of the rows alone."""
+    M, K, N = 2 ** 21 + 3, 1032, 2056
+    x = torch.randn(M, K, device=DEV, dtype=BF)
+    t = inputs(1, K, N, BF)
+    rows = torch.tensor(sorted({0, 1, 255, 256, M - 1, M - 4, *(e // n + d for e in (2 ** 30, 2 ** 31, 2 ** 32) for n in (K, N)
+                                                                for d in (-1, 0, 1) if e // n + d < M)}), device=DEV)
+    dy = torch.zeros(M, N, device=DEV, dtype=BF)
+    dy[rows] = torch.randn(len(rows), N, device=DEV).to(BF)
+    leaves = [x.requires_grad_(True), t["w"].requires_grad_(True), t["b"].requires_grad_(True)]
+    y = dense_projection(*leaves, None, "gelu", "int8")
+    xq, xe, z, ze = (y.grad_fn.saved_tensors[i] for i in (1, 2, 5, 6))
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    x, w, b, y = x.detach(), t["w"].detach(), t["b"].detach(), y.detach()
+    check_forward(y[rows], x[rows], w, b, None, "gelu")
+    be = backend_for(y.device)
+    kept = [be.unpack8(q[rows], e[rows], n, F32) for q, e, n in ((xq, xe, K), (z, ze, N))]
+    assert torch.equal(kept[0], pack_activation(x[rows]).unpack(F32))
+    sub = dict(x=x[rows], w=w, b=b, dy=dy[rows])
+    check_gradients(dict(dx=dx[rows], dw=dw, db=db), sub, "gelu", kept[1].double(), kept[0], None)
+    others = torch.ones(M, dtype=torch.bool, device=DEV)
+    others[rows] = False
+    assert not bool(dx[others].any())
