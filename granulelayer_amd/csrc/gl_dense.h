@@ -296,11 +296,11 @@ constexpr unsigned DMA_NOWHERE = 0x80000000u;  // past any buffer_of; offsets ar
 // staged by NW waves.
 //
 // LDS of an RC operand: rows of 128 bytes, 16-byte chunk c of row r at c ^ key(r).  A 16-byte read of 16
-// neighbouring rows takes each of the 16 chunks of a 256-byte bank row once, and rows 16..31 take them in
-// the same order: LDS then delivers 256 bytes a clock (half of it with c ^ (r & 7): rows r and r + 8
-// collide).  Of an RS operand: the reduction's rows of DIM values; for bf16 the 32-byte unit u of row r at
-// u ^ swz(r): a transposing read takes 32 bytes of four rows r..r + 3 (two such groups per half wave, of
-// neighbouring units), and the swizzle puts those on all banks.
+// neighbouring rows takes each of the 16 chunks of a 256-byte bank row once: LDS then delivers 256 bytes a clock
+// (half of it with c ^ (r & 7): rows r and r + 8 collide).  Of an RS operand: the reduction's rows of DIM values, the
+// 32-byte unit u of row r at u ^ swz(r).  bf16: a transposing read takes 32 bytes of four rows r..r + 3, and in each half
+// wave the same of rows 8 further on, or the next unit of these; fp32: 16 values of rows 4 apart.  The swizzle
+// puts them on all banks.
 template <int ES, int DIM, int NW, bool RC>
 struct Side {
   static constexpr int BK = DENSE_BK;
@@ -318,8 +318,9 @@ struct Side {
 
   static __device__ __forceinline__ int key(int r) { return (r >> 1) & 7; }
   static __device__ __forceinline__ int swz(int r) {
-    if constexpr (ES == 2) return (((r & 3) << 1) | (((r >> 3) & 1) << 3)) & (DIM / 16 - 1);
-    return 0;
+    if constexpr (ES == 4) return ((r >> 2) & 3) << 1;
+    // (64 columns: rows r and r + 1 are in different halves of a bank row as it is)
+    return DIM == 64 ? (r & 2) | ((r >> 3) & 1) : ((r & 3) << 1) | ((r >> 3) & 1);
   }
 
   // base: the operand; first: the tile's first row (RC) or column (RS); dim, R: the operand's size
@@ -373,7 +374,8 @@ struct Side {
   }
 };
 
-// A lane's part of a 32-row fragment: row l % 32, and of the 32 bytes of reduction at kk * 32 the half l / 32.
+// A fragment: MS rows (16 or 32) of an operand by what a matrix instruction of MS x MS takes in 16 bytes a lane,
+// 64 or 32 bytes of the reduction.  Lane l has row l % MS and the 16 bytes l / MS.
 template <int ES> struct Frag;
 template <> struct Frag<2> {
   static constexpr int STEPS = 1;  // matrix instructions
@@ -384,32 +386,29 @@ template <> struct Frag<4> {
   f32x4 v;
 };
 
-template <int ES, int DIM, bool RC>
+template <int ES, int MS, int DIM, bool RC>
 struct Reader {
-  static constexpr int BK = DENSE_BK;
-  unsigned a[RC ? BK / 32 : 1];       // byte of chunk kk in the lane's row
-  unsigned col[RC ? 1 : DIM / 32];
-  // base: this wave's first row / column of the tile, a multiple of 32
+  static_assert(MS == 16 || (MS == 32 && ES == 2), "fp32 rows are read 16 at a time");
+  unsigned at;  // byte of this lane's part of fragment 0, part 0
+  // base: this wave's first row / column of the tile, a multiple of its rows / columns
   __device__ __forceinline__ void init(int base) {
-    const int l = threadIdx.x & 63;
+    const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
     if constexpr (RC) {
-#pragma unroll
-      for (int kk = 0; kk < BK / 32; ++kk)
-        a[kk] = (base + (l & 31)) * BK + (((2 * kk + (l >> 5)) ^ Side<ES, DIM, 2, true>::key(l & 31)) * 16);
+      at = (base + l % MS) * DENSE_BK + ((l / MS ^ Side<ES, DIM, 2, true>::key(l % MS)) * 16);
     } else if constexpr (ES == 2) {
-      const int g = l >> 4, i = l & 15, r = 8 * (g >> 1) + (i >> 2);
-      const int sw = Side<ES, DIM, 2, false>::swz(r);
-#pragma unroll
-      for (int t = 0; t < DIM / 32; ++t)
-        col[t] = r * (DIM * 2) + (((base / 16 + 2 * t + (g & 1)) ^ sw) * 32) + 8 * (i & 3);
+      const int r = 8 * (MS == 16 ? g : g >> 1) + (i >> 2), u = base / 16 + (MS == 16 ? 0 : g & 1);
+      at = r * (DIM * 2) + (u ^ Side<ES, DIM, 2, false>::swz(r)) * 32 + 8 * (i & 3);
     } else {
-      col[0] = (l >> 5) * 4 * (DIM * 4) + (base + (l & 31)) * 4;
+      at = 4 * g * (DIM * 4) + ((base / 8 + (i >> 3)) ^ Side<ES, DIM, 2, false>::swz(4 * g)) * 32 + (i & 7) * 4;
     }
   }
-  __device__ __forceinline__ Frag<ES> read(const char* lds, int t, int kk) const {
+  // part kk of fragment t of the wave, from the stage at LDS address lds: a step of swizzled bits is an exclusive or
+  __device__ __forceinline__ Frag<ES> read(unsigned lds, int t, int kk) const {
+    constexpr int PART = 1024 / MS;  // bytes of reduction
     Frag<ES> f;
     if constexpr (RC) {
-      f.v = *reinterpret_cast<const decltype(f.v)*>(lds + a[kk] + t * 32 * BK);
+      typedef const __attribute__((address_space(3))) decltype(f.v) lds_vec;
+      f.v = *(lds_vec*)(((lds + at) ^ kk * PART) + t * MS * DENSE_BK);
     } else if constexpr (ES == 2) {
       typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
       union {
@@ -418,24 +417,36 @@ struct Reader {
       } u;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds + col[t] + (16 * kk + 4 * h) * (DIM * 2)));
+        u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_i16x4*)(((lds + at) ^ t * MS * 2) + (PART / 2 * kk + 4 * h) * (DIM * 2)));
       f.v = u.v;
     } else {
+      typedef const __attribute__((address_space(3))) float lds_float;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        f.v[e] = *reinterpret_cast<const float*>(lds + col[0] + (8 * kk + e) * (DIM * 4) + t * 128);
+      for (int e = 0; e < 4; ++e) f.v[e] = *(lds_float*)(((lds + at) ^ t * 64) + (16 * kk + e) * (DIM * 4));
     }
     return f;
   }
 };
 
-// rows of the output are Q's (n), its columns P's (m): a lane then holds neighbours of a row of C
+// rows of the output are Q's (n), its columns P's (m): a lane then holds neighbours of a row of C.
+//
+// 16 x 16 or 32 x 32: an instruction of 16 x 16 reads and writes its sums for twice the products, which takes less
+// power, and power sets the clock of large bf16 products: from registers alone 2,120 TFLOP/s against 1,890.  But it is
+// half as long, and a wave that is alone on its SIMD has less to hide its reads behind.  16384 x 4096 over 4096 in 256 x
+// 256 tiles: 399 us against 409 (407 against 430 on a card with a lower clock); 4096 x 1024 over 4096 in 128 x 128 tiles, a
+// wave a SIMD: 39.4 against 36.9.  fp32: 1040 against 1060 us (4096 x 4096 over 4096, NN).
+__device__ __forceinline__ f32x4 mma(const Frag<2>& q, const Frag<2>& p, int, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(q.v, p.v, c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x16 mma(const Frag<2>& q, const Frag<2>& p, int, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(q.v, p.v, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mma(const Frag<4>& q, const Frag<4>& p, int x, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x2f32(q.v[x], p.v[x], c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mma(const Frag<4>& q, const Frag<4>& p, int x, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(q.v[x], p.v[x], c, 0, 0, 0);
 }
+template <int MS> struct Sums { typedef f32x4 type; };  // a lane's of an instruction
+template <> struct Sums<32> { typedef f32x16 type; };
 
 // Every wave's LDS accesses and all but N of its copies done, then the workgroup's barrier.
 template <int N>
@@ -443,9 +454,9 @@ __device__ __forceinline__ void copies_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <int ES, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC>
+template <int ES, int MS, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC>
 __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
-  constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, BK = DENSE_BK;
+  constexpr int NW = WM * WN, TM = BM / WM / MS, TN = BN / WN / MS;  // fragments of a wave
   typedef Side<ES, BM, NW, PRC> SP;
   typedef Side<ES, BN, NW, QRC> SQ;
   constexpr int LDS_Q = NSP * SP::BYTES, LDS = LDS_Q + NSQ * SQ::BYTES;  // P's stages, then Q's
@@ -462,26 +473,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   SQ sq;
   sp.init(a.P, a.ldp, m0, a.e.M, a.R, k0);
   sq.init(a.Q, a.ldq, n0, a.e.N, a.R, k0);
-  Reader<ES, BM, PRC> rp;
-  Reader<ES, BN, QRC> rq;
-  rp.init(wm * TM * 32);
-  rq.init(wn * TN * 32);
+  Reader<ES, MS, BM, PRC> rp;
+  Reader<ES, MS, BN, QRC> rq;
+  rp.init(wm * TM * MS);
+  rq.init(wn * TN * MS);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
 
-  f32x16 acc[TM][TN];
+  typename Sums<MS>::type acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.f;
+      for (int x = 0; x < MS * MS / 64; ++x) acc[i][j][x] = 0.f;
 
-  // A stage is KK parts of 32 bytes of reduction.  Fragments are read a part ahead of the products that
+  // A stage is KK parts of 64 (or 32) bytes of reduction.  Fragments are read a part ahead of the products that
   // take them, across stages too: the barrier that opens a stage stands before the last part of the stage
   // ahead of it, whose products cover the barrier and the first reads.  From then on nobody reads the
   // stage that ends, and copies of a stage further on go there: Q's NSQ on, with the last part, then P's NSP on,
   // a share with each part (issued at once they hold up every wave behind the CU's one address unit).
-  constexpr int KK = BK / 32, LP = SP::LOADS, LQ = SQ::LOADS, COPIES = LP + LQ;
+  constexpr int KK = DENSE_BK * MS / 1024, LP = SP::LOADS, LQ = SQ::LOADS, COPIES = LP + LQ;
   constexpr int SHARE = (COPIES + KK - 1) / KK, FIRST_SHARE = NSP > NSQ && LQ > SHARE ? LQ : SHARE;
   constexpr int REST_SHARE = KK > 1 ? (COPIES - FIRST_SHARE + KK - 2) / (KK - 1) : 0;
   // copies issued behind those of Q's next stage (and of P's, which is no later) when that has to be there
@@ -493,37 +504,34 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
     else sp.copy(c - LQ, lds0 + to_p);
   };
   unsigned cur_p = 0, cur_q = LDS_Q, to_p = (NSP - 1) * SP::BYTES, to_q = LDS_Q + (NSQ - 1) * SQ::BYTES;
-  // Products of the fragments of `set`, a row of the wave's tile at a time; with the first rows reads of
-  // part kk of the current stage into the other set, with the last the copies [c0, c1).  Reads come first so
-  // that a barrier behind the part finds them done.
-  constexpr int FIRST = TM > 1 ? TM / 2 : 1, LATER = TM - FIRST > 0 ? TM - FIRST : 1;
+  // Products of the fragments of `set`; among the first half of them reads of part kk of the current stage into
+  // the other set, so that a barrier behind the part finds them done, among the second half the copies [c0, c1).
+  // FENCE: products that the compiler may move them over.  (bf16: in bunches they take 2 to 5% more clocks; fp32: a
+  // fence behind each of its long instructions takes 4% more.)
   auto part_of = [&](int set, bool reads, int kk, int c0, int c1, bool prepare) {
-    const char* lp = smem + cur_p;
-    const char* lq = smem + cur_q;
+    constexpr int SLOTS = TM * TN * Frag<ES>::STEPS, HALF = SLOTS / 2, READS = TM + TN, FENCE = ES == 4 ? 16 : 32 / MS;
+    const unsigned lp = lds0 + cur_p, lq = lds0 + cur_q;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    for (int s = 0; s < SLOTS; ++s) {
+      const int j = s % TN, x = s / TN % Frag<ES>::STEPS, i = s / TN / Frag<ES>::STEPS;
+      acc[i][j] = mma(fq[set][j], fp[set][i], x, acc[i][j]);
+      if (s < HALF) {
 #pragma unroll
-      for (int x = 0; x < Frag<ES>::STEPS; ++x)
+        for (int h = s * READS / HALF; reads && h < (s + 1) * READS / HALF; ++h) {
+          if (h < TN) fq[set ^ 1][h] = rq.read(lq, h, kk);
+          else fp[set ^ 1][h - TN] = rp.read(lp, h - TN, kk);
+        }
+      } else {
+        const int y = s - HALF, n = c1 - c0;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mma(fq[set][j], fp[set][i], x, acc[i][j]);
-      if (reads && i < FIRST) {
-        if (i == 0)
-#pragma unroll
-          for (int j = 0; j < TN; ++j) fq[set ^ 1][j] = rq.read(lq, j, kk);
-#pragma unroll
-        for (int h = i * TM / FIRST; h < (i + 1) * TM / FIRST; ++h) fp[set ^ 1][h] = rp.read(lp, h, kk);
-      }
-      if (i >= TM - LATER) {
-        const int y = i - (TM - LATER), n = c1 - c0;
-#pragma unroll
-        for (int c = y * n / LATER; c < (y + 1) * n / LATER; ++c)
+        for (int c = y * n / HALF; c < (y + 1) * n / HALF; ++c)
           if (c0 + c < COPIES) copy(c0 + c, to_p, to_q);
       }
-      if (prepare && i == TM - 1) {
+      if (prepare && s == SLOTS - 1) {
         sp.prepare();
         sq.prepare();
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (s % FENCE == FENCE - 1) __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto stage_of_p = [&](unsigned at) {
@@ -549,9 +557,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   for (int c = 0; c < FIRST_SHARE; ++c) copy(c, to_p, to_q);
   copies_barrier<BEHIND + FIRST_SHARE>();
 #pragma unroll
-  for (int j = 0; j < TN; ++j) fq[0][j] = rq.read(smem + LDS_Q, j, 0);
+  for (int j = 0; j < TN; ++j) fq[0][j] = rq.read(lds0 + LDS_Q, j, 0);
 #pragma unroll
-  for (int i = 0; i < TM; ++i) fp[0][i] = rp.read(smem, i, 0);
+  for (int i = 0; i < TM; ++i) fp[0][i] = rp.read(lds0, i, 0);
   for (int k = 0; k < nk - 1; ++k) {
 #pragma unroll
     for (int kk = 0; kk < KK - 1; ++kk)
@@ -574,7 +582,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   // stores and loads share a counter that runs in order, and a load behind a store waits for it.  A lane's rows
   // are in registers four together, so types, kinds and edges are decided once for all of them.  (A row at a
   // time, with its loads and branches, took 33,000 clocks a tile, as long as 12 stages of products.)
-  static_assert(TN == 2 && NW * 32 * 68 * 4 <= LDS, "a wave's rows of 64 columns");
+  static_assert(TN * MS == 64 && TM * MS % 32 == 0 && NW * 32 * 68 * 4 <= LDS, "a wave's rows of 64 columns");
   constexpr bool FORWARD = PRC && QRC;  // bias, activation, residual and what is kept; else sums as they are
   constexpr int ROWS = 4;               // of a lane at a time, 4 apart
   copies_barrier<0>();
@@ -587,7 +595,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   const long long c_step = (split_up ? a.e.N : a.e.sc) * (c_bf ? 2 : 4);
   const bool inside = m0 + BM <= a.e.M && n0 + BN <= a.e.N;
   const int n = n0 + wn * 64 + (l & 15) * 4, there = a.e.N - n;
-  const long long mw = m0 + wm * TM * 32 + (l >> 4);
+  const long long mw = m0 + wm * TM * MS + (l >> 4);
   float bias[4];
   if constexpr (FORWARD) dense_bias(a.e, n, bias);
   uv4 r[ROWS];
@@ -612,21 +620,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   };
   if (added.p) load_rows(mw);
 #pragma unroll 1
-  for (int i = 0; i < TM; ++i) {
+  for (int i = 0; i < TM * MS / 32; ++i) {
+    // acc[h][j], four at a time: row l % MS, columns from 4 (l / MS)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int h = 0; h < 32 / MS; ++h)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 t;
+      for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) t[x] = acc[0][j][4 * g + x];
-        *reinterpret_cast<f32x4*>(own + (l & 31) * 68 + 32 * j + 8 * g + 4 * (l >> 5)) = t;
-      }
+        for (int g = 0; g < MS * MS / 256; ++g) {
+          f32x4 t;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) t[x] = acc[h][j][4 * g + x];
+          *reinterpret_cast<f32x4*>(own + (MS * h + l % MS) * 68 + MS * j + 8 * g + 4 * (l / MS)) = t;
+        }
     // a rolled loop (its code is loaded once): the rows of accumulators move up
 #pragma unroll
-    for (int y = 0; y + 1 < TM; ++y)
+    for (int y = 0; y + 32 / MS < TM; ++y)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[y][j] = acc[y + 1][j];
+      for (int j = 0; j < TN; ++j) acc[y][j] = acc[y + 32 / MS][j];
 #pragma unroll 1
     for (int y = 0; y < 32; y += 4 * ROWS) {
       const long long mi = mw + i * 32 + y;
@@ -648,7 +659,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
 #pragma unroll
           for (int x = 0; x < ROWS; ++x) add_added(v[x], r[x], false);
         }
-        if (i + 1 < TM || y + 4 * ROWS < 32) load_rows(mi + 4 * ROWS);
+        if (i + 1 < TM * MS / 32 || y + 4 * ROWS < 32) load_rows(mi + 4 * ROWS);
       }
       char* c = C + mi * c_step + (long long)n * (c_bf ? 2 : 4);
       if (inside && c_bf) {
@@ -674,7 +685,7 @@ enum { DENSE_NT = 0, DENSE_NN = 1, DENSE_TN = 2 };  // P, Q: RC RC; RC RS; RS RS
 enum { DENSE_256 = 0, DENSE_256X128 = 1, DENSE_128 = 2, DENSE_128_DEEP = 3, DENSE_64 = 4, DENSE_TILES = 5 };
 constexpr int DENSE_BM[DENSE_TILES] = {256, 256, 128, 128, 64}, DENSE_BN[DENSE_TILES] = {256, 128, 128, 128, 128};
 
-template <int ES, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC>
+template <int ES, int MS, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC>
 int launch_dense_tile_as(const DenseK& a, int splits, hipStream_t s) {
   constexpr size_t lds = (NSP * BM + NSQ * BN) * DENSE_BK;
   // the kernel's LDS limit is raised once a device
@@ -682,19 +693,19 @@ int launch_dense_tile_as(const DenseK& a, int splits, hipStream_t s) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return GL_ERR_DEVICE;
   if (!(raised.load(std::memory_order_relaxed) >> dev & 1)) {
-    GL_TRY(set_lds_limit((const void*)dense_tile_kernel<ES, BM, BN, WM, WN, NSP, NSQ, PRC, QRC>, lds));
+    GL_TRY(set_lds_limit((const void*)dense_tile_kernel<ES, MS, BM, BN, WM, WN, NSP, NSQ, PRC, QRC>, lds));
     raised.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  GL_LAUNCH(GL_KERNEL_DENSE, (dense_tile_kernel<ES, BM, BN, WM, WN, NSP, NSQ, PRC, QRC>),
+  GL_LAUNCH(GL_KERNEL_DENSE, (dense_tile_kernel<ES, MS, BM, BN, WM, WN, NSP, NSQ, PRC, QRC>),
             dim3((unsigned)(a.tiles_m * a.tiles_n * splits)), dim3(64 * WM * WN), lds, s, a);
   GL_CHECK_LAUNCH();
   return 0;
 }
-template <int ES, int BM, int BN, int WM, int WN, int NSP, int NSQ>
+template <int ES, int MS, int BM, int BN, int WM, int WN, int NSP, int NSQ>
 int launch_dense_tile_of(int form, const DenseK& a, int splits, hipStream_t s) {
-  if (form == DENSE_NT) return launch_dense_tile_as<ES, BM, BN, WM, WN, NSP, NSQ, true, true>(a, splits, s);
-  if (form == DENSE_NN) return launch_dense_tile_as<ES, BM, BN, WM, WN, NSP, NSQ, true, false>(a, splits, s);
-  return launch_dense_tile_as<ES, BM, BN, WM, WN, NSP, NSQ, false, false>(a, splits, s);
+  if (form == DENSE_NT) return launch_dense_tile_as<ES, MS, BM, BN, WM, WN, NSP, NSQ, true, true>(a, splits, s);
+  if (form == DENSE_NN) return launch_dense_tile_as<ES, MS, BM, BN, WM, WN, NSP, NSQ, true, false>(a, splits, s);
+  return launch_dense_tile_as<ES, MS, BM, BN, WM, WN, NSP, NSQ, false, false>(a, splits, s);
 }
 int launch_dense_tile_bf16(int form, int tile, const DenseK& a, int splits, hipStream_t s);
 int launch_dense_tile_f32(int form, int tile, const DenseK& a, int splits, hipStream_t s);
