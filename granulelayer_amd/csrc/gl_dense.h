@@ -120,18 +120,24 @@ __device__ __forceinline__ void load4(const void* p, bool bf, long long i, int n
     for (int j = 0; j < 4; ++j) v[j] = j < n ? ld_param((const float*)p, bf, i + j) : 0.f;
   }
 }
+typedef unsigned uv4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned uv2_any __attribute__((ext_vector_type(2), aligned(2)));
+// STREAM: a hint that the caches need not keep it
+template <bool STREAM = false>
 __device__ __forceinline__ void store4(void* p, bool bf, long long i, int n, const float (&v)[4]) {
   if (n >= 4) {
     if (bf) {
       uv2 w;
       w[0] = to_bf16x2(v[0], v[1]);
       w[1] = to_bf16x2(v[2], v[3]);
-      reinterpret_cast<bytes8*>((char*)p + 2 * i)->v = w;
+      if constexpr (STREAM) __builtin_nontemporal_store(w, reinterpret_cast<uv2_any*>((char*)p + 2 * i));
+      else reinterpret_cast<bytes8*>((char*)p + 2 * i)->v = w;
     } else {
       uv4 w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(v[j]);
-      reinterpret_cast<bytes16*>((char*)p + 4 * i)->v = w;
+      if constexpr (STREAM) __builtin_nontemporal_store(w, reinterpret_cast<uv4_any*>((char*)p + 4 * i));
+      else reinterpret_cast<bytes16*>((char*)p + 4 * i)->v = w;
     }
   } else {
 #pragma unroll
@@ -585,6 +591,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   static_assert(TN * MS == 64 && TM * MS % 32 == 0 && NW * 32 * 68 * 4 <= LDS, "a wave's rows of 64 columns");
   constexpr bool FORWARD = PRC && QRC;  // bias, activation, residual and what is kept; else sums as they are
   constexpr int ROWS = 4;               // of a lane at a time, 4 apart
+  // The caches need not keep the large tile's results and what is added to them, but the operands of the tiles that
+  // still run: 8192 x 8192 over 4096 with an fp32 residual 538 -> 500 us.  (Without it where outputs are smaller and
+  // still there for who reads them next: fp32 2048 x 4096 over 1024 takes 2% longer with it.)
+  constexpr bool STREAM = BM * BN == 65536;
   copies_barrier<0>();
   const int l = threadIdx.x & 63;
   float* own = reinterpret_cast<float*>(smem) + w * 32 * 68;
@@ -604,12 +614,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
     if (inside && added.bf) {
 #pragma unroll
       for (int x = 0; x < ROWS; ++x) {
-        const uv2 t = reinterpret_cast<const bytes8*>(p + 4 * x * added.step)->v;
+        const char* px = p + 4 * x * added.step;
+        const uv2 t = STREAM ? (uv2)__builtin_nontemporal_load(reinterpret_cast<const uv2_any*>(px))
+                             : reinterpret_cast<const bytes8*>(px)->v;
         r[x] = uv4{t[0], t[1], 0u, 0u};
       }
     } else if (inside) {
 #pragma unroll
-      for (int x = 0; x < ROWS; ++x) r[x] = reinterpret_cast<const bytes16*>(p + 4 * x * added.step)->v;
+      for (int x = 0; x < ROWS; ++x) {
+        const char* px = p + 4 * x * added.step;
+        r[x] = STREAM ? (uv4)__builtin_nontemporal_load(reinterpret_cast<const uv4_any*>(px))
+                      : reinterpret_cast<const bytes16*>(px)->v;
+      }
     } else {
 #pragma unroll
       for (int x = 0; x < ROWS; ++x) {
@@ -664,10 +680,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
       char* c = C + mi * c_step + (long long)n * (c_bf ? 2 : 4);
       if (inside && c_bf) {
 #pragma unroll
-        for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, true, 0, 4, v[x]);
+        for (int x = 0; x < ROWS; ++x) store4<STREAM>(c + 4 * x * c_step, true, 0, 4, v[x]);
       } else if (inside) {
 #pragma unroll
-        for (int x = 0; x < ROWS; ++x) store4(c + 4 * x * c_step, false, 0, 4, v[x]);
+        for (int x = 0; x < ROWS; ++x) store4<STREAM>(c + 4 * x * c_step, false, 0, 4, v[x]);
       } else {
 #pragma unroll
         for (int x = 0; x < ROWS; ++x)
