@@ -347,7 +347,8 @@ class SparsePoolFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        kept, (w, b, *svals) = ctx.saved_tensors[:ctx.n_x], ctx.saved_tensors[ctx.n_x:]
+        tensors = ctx.saved_tensors  # once: a checkpointed region hands them out a single time
+        kept, (w, b, *svals) = tensors[:ctx.n_x], tensors[ctx.n_x:]
         saved = dict(zip(ctx.saved_keys, svals))
         rt: Level1Runtime = ctx.rt
         x, x_dtype = _kept_input(ctx, kept)

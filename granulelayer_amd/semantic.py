@@ -127,7 +127,8 @@ class SemanticPoolFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        kept, (w, b, *rest) = ctx.saved_tensors[:ctx.n_x], ctx.saved_tensors[ctx.n_x:]
+        tensors = ctx.saved_tensors  # once: a checkpointed region hands them out a single time
+        kept, (w, b, *rest) = tensors[:ctx.n_x], tensors[ctx.n_x:]
         tparams = rest[: ctx.n_t]
         saved = dict(zip(ctx.saved_keys, rest[ctx.n_t:]))
         rt: Level1Runtime = ctx.rt
