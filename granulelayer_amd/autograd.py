@@ -244,10 +244,20 @@ def _grad_buffers(w, b):
             torch.zeros(b.shape, device=b.device, dtype=torch.float32), False)
 
 
-def _saved_stats(level: LevelSpec, out: Dict[str, torch.Tensor], policy: str) -> Dict[str, torch.Tensor]:
+# pools whose backward divides each neuron's term by what the forward summed (pre, L2)
+NORMALISED_POOLS = ("logmeanexp", "power_mean", "softmax_weighted")
+
+
+def _saved_stats(level: LevelSpec, out: Dict[str, torch.Tensor], policy: str,
+                 rounded_input: bool = False) -> Dict[str, torch.Tensor]:
     """What the forward keeps for backward (autograd.py:366-377): pre, with save_winners the
-    max-pooling winner ids or the top-k slots, and softmax-weighted pooling's L2."""
-    if policy == "recompute_stats":
+    max-pooling winner ids or the top-k slots, and softmax-weighted pooling's L2.
+
+    With rounded_input the backward recomputes z from the input's 8-bit form.  A smooth pool's terms are
+    then exp(act(z^) scale - L2) or (z^ / pre)^(p - 1): with pre and L2 of the exact input they would not sum
+    to 1 (off by exp(scale dz), without bound at low temperatures), so nothing is kept and the backward's
+    own forward gives those of the kept input."""
+    if policy == "recompute_stats" or (rounded_input and level.type in NORMALISED_POOLS):
         return {}
     keep = {"pre": out["pre"]}
     if "relu_mask" in out:  # the forward's ReLU bits (1/32 of the hidden tensor): dW skips the recompute
@@ -260,14 +270,18 @@ def _saved_stats(level: LevelSpec, out: Dict[str, torch.Tensor], policy: str) ->
     return keep
 
 
+def _rounds_input(ctx, rt: Level1Runtime) -> bool:
+    """Whether the backward gets the input in 8 bits: activation_checkpoint="int8", and a backward can run."""
+    return (rt.activation_checkpoint == "int8" and getattr(rt, "grad_call", True) and any(ctx.needs_input_grad)
+            and rt.backend is not None)
+
+
 def _keep_input(ctx, rt: Level1Runtime, x, xc) -> list:
-    """Tensors that stand for the input in ctx's saved ones: x itself, or with
-    activation_checkpoint="int8" the 8-bit form of the kernels' operand xc when a backward can run.
-    The gradients are then those at the values that were kept: dW sums over them, and neurons whose
-    z the backward recomputes are recomputed from them."""
+    """Tensors that stand for the input in ctx's saved ones: x itself, or the 8-bit form of the kernels'
+    operand xc (_rounds_input).  The gradients are then those at the values that were kept: dW sums over
+    them, and neurons whose z the backward recomputes are recomputed from them."""
     ctx.x_kept = None
-    if (rt.activation_checkpoint == "int8" and getattr(rt, "grad_call", True) and any(ctx.needs_input_grad)
-            and rt.backend is not None):
+    if _rounds_input(ctx, rt):
         ctx.x_kept = (xc.shape, xc.dtype, x.dtype)
         kept = list(rt.backend.pack8(xc))
     else:
@@ -338,7 +352,7 @@ class SparsePoolFunction(torch.autograd.Function):
         out = rt.forward(xc, wc, bc, track_ids=(policy == "save_winners"), relu_mask=keep_bits)
         pre = out["pre"]
         y = act_torch(pre, lv.out_activation)
-        saved = _saved_stats(lv, out, policy)
+        saved = _saved_stats(lv, out, policy, _rounds_input(ctx, rt))
         ctx.rt, ctx.policy, ctx.compute_dtype = rt, policy, compute_dtype
         ctx.saved_keys = list(saved.keys())
         ctx.save_for_backward(*_keep_input(ctx, rt, x, xc), w, b, *saved.values())

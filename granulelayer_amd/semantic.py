@@ -22,7 +22,7 @@ from typing import Dict, List
 import torch
 
 from .autograd import (CHECKPOINT_BUDGET, Level1Runtime, _compute_operands, _grad_buffers, _ids_per_token,
-                       _keep_input, _kept_input, _level1_backward, _saved_stats, act_torch, fit_policy)
+                       _keep_input, _kept_input, _level1_backward, _rounds_input, _saved_stats, act_torch, fit_policy)
 from .config import LevelSpec, PoolingConfig
 
 
@@ -99,7 +99,8 @@ class SemanticPoolFunction(torch.autograd.Function):
     """Two-level: F = out_act(level1(x)) [B, G, S]; y = level2(transform(F)) (autograd.py:417-476).
 
     level1_checkpoint "save": pre (and the level-1 statistics the policy keeps) saved by the
-    forward; "recompute": only x / W / b, the backward reruns the level-1 forward."""
+    forward; "recompute": only x / W / b, the backward reruns the level-1 forward.  A smooth level 1 with its
+    input in 8 bits always reruns it (_saved_stats)."""
 
     @staticmethod
     def forward(ctx, x, w, b, rt: Level1Runtime, cfg: PoolingConfig, policy: str, compute_dtype,
@@ -115,7 +116,8 @@ class SemanticPoolFunction(torch.autograd.Function):
         with torch.no_grad():
             y = level2_forward(F, cfg, tp)
         if cfg.level1_checkpoint == "save":
-            saved = _saved_stats(l1, out, policy if policy != "recompute_stats" else "minimal_stats")
+            saved = _saved_stats(l1, out, policy if policy != "recompute_stats" else "minimal_stats",
+                                 _rounds_input(ctx, rt))
         else:
             saved = {}
         ctx.rt, ctx.cfg, ctx.policy, ctx.compute_dtype, ctx.tnames = rt, cfg, policy, compute_dtype, tnames

@@ -64,3 +64,24 @@ def test_under_activation_checkpointing(pooling, eight):
     got = torch.autograd.grad(checkpoint(call, x, use_reentrant=False).sum(), (x, *params))
     for g, t in zip(got, want):
         assert torch.equal(g, t)
+
+
+LEVELS = {"lme": dict(type="logmeanexp", temperature=0.05), "softmax": dict(type="softmax_weighted"),
+          "power": dict(type="power_mean", p=4.0)}
+
+
+@pytest.mark.parametrize("two", [False, True], ids=["one level", "two levels"])
+@pytest.mark.parametrize("eight", ["exact", "int8"])
+@pytest.mark.parametrize("level", LEVELS.values(), ids=LEVELS.keys())
+def test_normalisers_and_terms_are_of_one_input(level, eight, two):
+    """What a smooth pool's backward divides by was summed over the input that its terms are recomputed from."""
+    pooling = dict(levels=[dict(level, neurons_per_shard=32), dict(type="sum")], level1_checkpoint="save") if two else level
+    call, be, _ = _layer(pooling, eight)
+    x = torch.randn(5, 24, requires_grad=True)
+    call(x).sum().backward()
+    (xb, stats), = be.backwards
+    assert torch.equal(xb, x.detach().round() if eight == "int8" else x.detach())
+    assert torch.equal(stats["pre"], xb.sum(1, keepdim=True).expand_as(stats["pre"]))
+    if "L2" in stats:
+        assert torch.equal(stats["L2"], 2 * stats["pre"])
+    assert len(be.forwards) == (2 if eight == "int8" else 1)

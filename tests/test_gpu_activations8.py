@@ -242,3 +242,49 @@ def test_a_block_of_layers_trains_in_8_bits():
     opt = FusedAdamW(m.parameters(), lr=1e-3)
     opt.step()
     assert all(not bool(p.main_grad.any()) for p in m.parameters())
+
+
+SMOOTH = {
+    "lme": dict(type="logmeanexp"),
+    "lme cold": dict(type="logmeanexp", temperature=0.05),
+    "lme gelu": dict(type="logmeanexp", temperature=0.1, activation="gelu", out_activation="gelu"),
+    "softmax": dict(type="softmax_weighted", beta=10.0),
+    "softmax gelu": dict(type="softmax_weighted", activation="gelu"),
+    "power": dict(type="power_mean", p=4.0),
+    "power odd": dict(type="power_mean", p=2.5),
+    "two": dict(levels=[dict(type="softmax_weighted", beta=10.0, neurons_per_shard=128), dict(type="logmeanexp")],
+                level1_checkpoint="save"),
+    "two power": dict(levels=[dict(type="power_mean", p=4.0, neurons_per_shard=128, out_activation="gelu"), dict(type="sum")],
+                      level1_checkpoint="save"),
+}
+
+
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("pooling", SMOOTH.values(), ids=SMOOTH.keys())
+def test_smooth_pools_take_their_normalisers_from_the_kept_input(pooling, large):
+    """A smooth pool's gradient divides by what its forward summed: with an input kept in 8 bits, that of the kept
+    values, also under the default policy, which keeps the exact input's.  The gradients have the bits of an exact layer at the
+    kept values that recomputes its statistics; one large feature a block makes the kept values coarse."""
+    import granulelayer_amd as G
+
+    def layer(ckpt, pooling, **kw):
+        return G.SparsePoolingLayer(250, 6144, 12, shared_neurons=None, pooling=pooling, dtype=torch.float32, device=DEV,
+                                    seed=4, bias_std=0.3, activation_checkpoint=ckpt, **kw)
+
+    eight = layer("int8", pooling)
+    if "levels" in pooling:
+        exact = layer("exact", dict(pooling, level1_checkpoint="recompute"))
+    else:
+        exact = layer("exact", pooling, checkpoint_policy="recompute_stats")
+    x = torch.randn(3, 17, 250, generator=torch.Generator().manual_seed(1)).to(DEV)
+    if large:
+        x[..., ::32] *= 30
+    xe = x.clone().requires_grad_(True)
+    xk = pack_activation(x).unpack().requires_grad_(True)
+    y = eight(xe)
+    assert torch.equal(y, exact(x))
+    dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(6)).to(DEV)
+    got = torch.autograd.grad(y, [xe, eight.weight, eight.bias], dy)
+    want = torch.autograd.grad(exact(xk), [xk, exact.weight, exact.bias], dy)
+    for g, w in zip(got, want):
+        assert g.dtype == w.dtype and torch.equal(g, w)
