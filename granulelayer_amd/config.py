@@ -194,7 +194,8 @@ class PhysicalPlan:
     only the pooled statistics between forward and backward and the backward recomputes z;
     ``"keep"`` also keeps the forward's ReLU bit of every (token, neuron) -- 1/32 of the [B, N]
     hidden tensor's fp32 bytes -- for ReLU mean / sum layers at fan-in 8, so the backward's dW
-    pass skips the recompute (same results, bit for bit).
+    pass skips the recompute (same results, bit for bit).  With ``activation_checkpoint="int8"``
+    the kept bits are those of the exact input, and mask dW, db and dX alike.
     """
 
     phys_splits: int = 0

@@ -288,3 +288,57 @@ def test_smooth_pools_take_their_normalisers_from_the_kept_input(pooling, large)
     want = torch.autograd.grad(exact(xk), [xk, exact.weight, exact.bias], dy)
     for g, w in zip(got, want):
         assert g.dtype == w.dtype and torch.equal(g, w)
+
+
+@pytest.mark.parametrize("pool", ["mean", "sum"])
+def test_kept_relu_bits_are_the_mask_of_every_gradient(pool):
+    """PhysicalPlan(relu_bits="keep") with an input in 8 bits: the exact input's bits mask dW, db and dX alike.  dX and db do
+    not multiply the input, so they have the exact layer's bits; dW is dz^T x over those neurons, in the kept x."""
+    import granulelayer_amd as G
+
+    D, H, U = 200, 4096, 8
+    lay = [G.SparsePoolingLayer(D, H, U, shared_neurons=None, pooling=pool, dtype=torch.float32, device=DEV, seed=1,
+                                bias_std=0.2, activation_checkpoint=c, plan=G.PhysicalPlan(relu_bits="keep"))
+           for c in ("exact", "int8")]
+    x = torch.randn(37, D, generator=torch.Generator().manual_seed(2)).to(DEV)
+    dy = torch.randn(37, U, generator=torch.Generator().manual_seed(3)).to(DEV)
+    grads = []
+    for m in lay:
+        xl = x.clone().requires_grad_(True)
+        grads.append(torch.autograd.grad(m(xl), [xl, m.weight, m.bias], dy))
+        assert m.last_info["backward_relu_mask"]
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][2], grads[1][2])
+    m = lay[1]
+    idx = m.indices.reshape(-1, 8).long()
+    w6, b6 = m.weight.detach().double().reshape(-1, 8), m.bias.detach().double().reshape(-1)
+    z = torch.stack([(x[t].double()[idx] * w6).sum(-1) + b6 for t in range(37)])  # [37, slots]
+    slots = z.shape[1] // U
+    counts = m.layout.counts_tensor(DEV).double()
+    there = torch.arange(slots, device=DEV).repeat(U) < counts.repeat_interleave(slots)
+    c1 = (dy.double() / (counts if pool == "mean" else 1.0)).repeat_interleave(slots, 1)
+    dz = torch.where((z > 0) & there, c1, 0.0)
+    # neurons with a z within its rounding of 0 (9 roundings of at most the terms' sum) may go either way: a few at most
+    mag = torch.stack([(x[t].double()[idx] * w6).abs().sum(-1) + b6.abs() for t in range(37)])
+    sure = ~((z.abs() <= 9 * 2.0 ** -24 * mag) & there).any(0)
+    assert float(sure.double().mean()) > 0.99
+    xk = pack_activation(x).unpack().double()
+    want = torch.stack([(dz[:, :, None] * v[:, idx]).sum(0) for v in (x.double(), xk)])
+    # 37 products of fp32 added in fp32, from a coefficient that is rounded once
+    bound = 40 * 2.0 ** -24 * (dz.abs()[:, :, None] * xk[:, idx].abs()).sum(0)
+    got = grads[1][1].double().reshape(-1, 8)
+    assert bool(((got - want[1]).abs() <= bound)[sure].all())
+    assert bool(((got - want[0]).abs() > bound)[sure].any())  # and the kept x's, not the exact one's
+
+
+@pytest.mark.parametrize("kind", ["mean", "lme", "two", "cover"])
+@pytest.mark.parametrize("ckpt", ["exact", "int8"])
+def test_layers_under_activation_checkpointing(kind, ckpt):
+    from torch.utils.checkpoint import checkpoint
+
+    lay = sparse_layer(kind, ckpt)
+    x = torch.randn(9, 256 if kind == "cover" else 250, device=DEV, requires_grad=True)
+    leaves = [x, lay.weight, lay.bias]
+    want = torch.autograd.grad(lay(x).square().sum(), leaves)
+    got = torch.autograd.grad(checkpoint(lay, x, use_reentrant=False).square().sum(), leaves)
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
