@@ -479,3 +479,22 @@ def test_past_32_bits():
     others = torch.ones(M, dtype=torch.bool, device=DEV)
     others[rows] = False
     assert not bool(dx[others].any())
+
+
+# Sizes whose forward product takes each tile, whole and with its reduction split (the rest of them are in the tests above);
+# dX and dW take it with the sizes in turn.
+TILES = [
+    (BF, "256 x 256 split", 8200, 8200, 1001), (BF, "256 x 128", 4104, 520, 1001), (BF, "256 x 128 split", 8200, 3001, 130),
+    (BF, "128 x 128", 1001, 100, 4104), (BF, "128 x 128 split", 777, 8200, 3001), (BF, "deep", 8200, 1001, 130),
+    (BF, "deep split", 3001, 8200, 257),
+    (F32, "128 x 128", 1001, 100, 4104), (F32, "128 x 128 split", 8200, 1001, 130), (F32, "deep", 2500, 130, 777),
+    (F32, "deep split", 4104, 777, 130),
+]
+
+
+@pytest.mark.parametrize("turn", ["forward", "dx", "dw"])
+@pytest.mark.parametrize("dtype,tile,M,K,N", TILES, ids=[f"{str(t[0])[6:]} {t[1]}" for t in TILES])
+def test_every_tile_of_every_product(dtype, tile, M, K, N, turn):
+    """The products are M x N over K, M x K over N and N x K over M."""
+    size = {"forward": (M, K, N), "dx": (M, N, K), "dw": (K, N, M)}[turn]
+    check_training(inputs(*size, dtype), "gelu", "int8")
