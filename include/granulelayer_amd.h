@@ -303,7 +303,8 @@ int gl_window_build(const int32_t* idx, const int32_t* counts, int32_t D, int32_
  * every tensor are a stride apart (in elements, any stride of at least the width), features are
  * neighbours, and no address needs more than its element's alignment. */
 #define GL_DENSE_MAX_FEATURES 1048576 /* largest K, N and packed row */
-#define GL_DENSE_MAX_ROWS (1LL << 26) /* rows are fewer than this */
+/* rows are fewer than this: 64 threads a row, in workgroups of 4 rows, stay below the 2^32 of a launch */
+#define GL_DENSE_MAX_ROWS ((1LL << 26) - 3)
 /* What the forward keeps of z for the backward, [M, *] in `z`: nothing; z > 0 as bits (word n / 32
  * of a row's ceil(N / 32) words, bit n % 32); z in the operands' type, rows round_up(N, 8) apart; z in
  * 8 bits (gl_pack8's codes in z and exponents in z_exp). */

@@ -123,3 +123,20 @@ def test_sparse_layers_take_the_option(form):
     assert make(activation_checkpoint="int8").activation_checkpoint == "int8"
     with pytest.raises(ValueError, match="activation_checkpoint"):
         make(activation_checkpoint="int2")
+
+
+def test_row_limit_is_what_launches_hold():
+    """64 threads a row in workgroups of 4 rows: from 2^26 - 3 rows on that is 2^32 threads, more than a launch has.  Such
+    calls are refused before they reach the device, with a query and without."""
+    L = N.library().lib
+    out = ctypes.c_size_t()
+    for M, code in (((1 << 26) - 4, 0), ((1 << 26) - 3, -2), ((1 << 26) - 1, -2)):
+        f = N.GlDenseArgs(X=4096, sx=9, W=8192, sw=9, Y=16384, sy=8, M=M, N=8, K=9, dtype=1, y_dtype=1)
+        assert L.gl_dense_fwd_workspace(ctypes.byref(f), ctypes.byref(out)) == code
+        b = N.GlDenseBwdArgs(dY=4096, sdy=8, X=4096, sx=9, W=8192, sw=9, M=M, N=8, K=9, dtype=1, dy_dtype=1, dX=4096, dW=4096,
+                             db=4096, g_dtype=1)
+        assert L.gl_dense_bwd_workspace(ctypes.byref(b), ctypes.byref(out)) == code
+        if code:
+            p = N.GlPack8Args(x=4096, sx=512, rows=M, cols=512, x_dtype=1, q=4096, e=4096)
+            assert L.gl_dense_fwd(ctypes.byref(f), None) == code and L.gl_dense_bwd(ctypes.byref(b), None) == code
+            assert L.gl_pack8(ctypes.byref(p), None) == code and L.gl_unpack8(ctypes.byref(p), None) == code
