@@ -20,6 +20,7 @@ GL_POOL = {"mean": 0, "sum": 1, "max": 2, "topk_mean": 3, "logmeanexp": 4, "powe
 GL_DTYPE_F32, GL_DTYPE_BF16 = 0, 1
 GL_KEEP = {"none": 0, "sign": 1, "z": 2, "z8": 3}
 DENSE_MAX_FEATURES = 1 << 20  # GL_DENSE_MAX_FEATURES
+GL_ERR_WORKSPACE = -3
 GL_ERR_SCRATCH = -8
 FWD_STATIC_SCRATCH_BYTES = 64 << 20  # GL_FWD_STATIC_SCRATCH_BYTES
 
@@ -164,9 +165,10 @@ class Library:
     def error(self, code: int) -> str:
         return self.lib.gl_error_string(code).decode()
 
-    def call(self, name: str, *args):
+    def call(self, name: str, *args, accept: int = 0):
+        """The entry point's code, 0 or ``accept``; any other raises."""
         r = getattr(self.lib, name)(*args)
-        if r != 0:
+        if r != 0 and r != accept:
             raise NativeError(f"{name} failed (code {r}: {self.error(r)})")
         return r
 

@@ -469,8 +469,9 @@ class HipBackend:
         a = N.GlDenseArgs(_ptr(x), sx, _ptr(w), sw, _ptr(b), _ptr(res), sr, _ptr(y), F, M, F, K, code, rcode, ycode,
                           N.GL_ACT[activation], N.GL_KEEP[keep], _ptr(z), _ptr(z_exp), 0, 0)
         with _on(dev):
-            # few rows and whole tiles need no workspace: the call says so faster than a query before it
-            if self.lib.lib.gl_dense_fwd(ctypes.byref(a), _stream(dev)) != 0:
+            # few rows and whole tiles need no workspace: the call says so, before it enqueues anything, faster than
+            # a query before it
+            if self.lib.call("gl_dense_fwd", ctypes.byref(a), _stream(dev), accept=N.GL_ERR_WORKSPACE) != 0:
                 need = self.lib.size_query("gl_dense_fwd_workspace", a)
                 ws = torch.empty(need, device=dev, dtype=torch.uint8)
                 a.ws, a.ws_bytes = _ptr(ws), need

@@ -140,3 +140,35 @@ def test_row_limit_is_what_launches_hold():
             p = N.GlPack8Args(x=4096, sx=512, rows=M, cols=512, x_dtype=1, q=4096, e=4096)
             assert L.gl_dense_fwd(ctypes.byref(f), None) == code and L.gl_dense_bwd(ctypes.byref(b), None) == code
             assert L.gl_pack8(ctypes.byref(p), None) == code and L.gl_unpack8(ctypes.byref(p), None) == code
+
+
+@pytest.mark.parametrize("answers,calls", [([0], 1), ([-3, 0], 2), ([-1], 1), ([2], 1), ([719, 0], 1), ([-3, 2], 2)])
+def test_only_a_missing_workspace_is_asked_for(monkeypatch, answers, calls):
+    """The forward is issued a second time where the first one wants a workspace, and for no other error: kernels may have
+    been enqueued before it."""
+    from types import SimpleNamespace
+
+    from granulelayer_amd import backend as B
+
+    seen = []
+
+    def fwd(a, stream):
+        seen.append(a._obj.ws_bytes)
+        return answers[len(seen) - 1]
+
+    def query(a, out):
+        out._obj.value = 512
+        return 0
+
+    lib = N.Library.__new__(N.Library)
+    lib.lib = SimpleNamespace(gl_dense_fwd=fwd, gl_dense_fwd_workspace=query, gl_error_string=lambda code: b"it failed")
+    monkeypatch.setattr(B, "_on", lambda dev: B._NO_SWITCH)
+    monkeypatch.setattr(B, "_stream", lambda dev: 0)
+    be = B.HipBackend(lib)
+    args = (torch.zeros(3, 8), torch.zeros(5, 8), None, None, "identity", "none")
+    if answers[-1] == 0 and calls == len(answers):
+        assert be.dense_forward(*args)[0].shape == (3, 5)
+    else:
+        with pytest.raises(N.NativeError, match=f"gl_dense_fwd failed .code {answers[calls - 1]}: it failed"):
+            be.dense_forward(*args)
+    assert seen == [0, 512][:calls]
