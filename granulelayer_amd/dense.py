@@ -67,8 +67,8 @@ def _main_grads(w, b, need_w, need_b):
 
 
 class DenseProjectionFunction(torch.autograd.Function):
-    """x [M, K], residual [M, N] or None -> y [M, N]; keeps x (or its 8-bit form) and what the activation's
-    derivative needs of z."""
+    """x [M, K], residual [M, N] or None -> y [M, N]; keeps x (or its 8-bit form), W and what the activation's
+    derivative needs of z.  The bias may change before the backward, which reads only its shape and main_grad."""
 
     @staticmethod
     def forward(ctx, x, w, b, res, activation, activation_checkpoint):
@@ -82,7 +82,9 @@ class DenseProjectionFunction(torch.autograd.Function):
         xs = (None, None, None)  # x, or its codes and exponents
         if need_w:
             xs = (None, *be.pack8(x)) if packed else (x, None, None)
-        ctx.save_for_backward(*xs, w, b, z, z_exp)
+        ctx.save_for_backward(*xs, w, None, z, z_exp)
+        # a computed bias stands there by its shape and type alone
+        ctx.bias = b if b is None or b.is_leaf or hasattr(b, "main_grad") else torch.empty_like(b, device="meta")
         ctx.activation, ctx.keep, ctx.x_shape, ctx.x_dtype = activation, keep, x.shape, x.dtype
         ctx.res_dtype = None if res is None else res.dtype
         return y
@@ -90,7 +92,8 @@ class DenseProjectionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, xq, xe, w, b, z, z_exp = ctx.saved_tensors
+        x, xq, xe, w, _, z, z_exp = ctx.saved_tensors
+        b = ctx.bias
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dy = dy.resolve_neg()
         dres = dy.to(ctx.res_dtype) if need_r else None

@@ -172,3 +172,63 @@ def test_only_a_missing_workspace_is_asked_for(monkeypatch, answers, calls):
         with pytest.raises(N.NativeError, match=f"gl_dense_fwd failed .code {answers[calls - 1]}: it failed"):
             be.dense_forward(*args)
     assert seen == [0, 512][:calls]
+
+
+class _Products:
+    """The dense products of an identity projection in plain torch."""
+
+    def dense_forward(self, x, w, b, res, activation, keep):
+        return x @ w.t() + (0 if b is None else b), None, None
+
+    def dense_backward(self, dy, activation, keep, z, z_exp, x, xq, xe, w, dx, dw, db, accumulate):
+        for out, grad, add in ((dx, lambda: dy @ w, False), (dw, lambda: dy.t() @ x, accumulate),
+                               (db, lambda: dy.sum(0), accumulate)):
+            if out is not None:
+                out.copy_(grad() + out if add else grad())
+
+
+@pytest.fixture
+def plain_products(monkeypatch):
+    from granulelayer_amd import dense
+
+    monkeypatch.setattr(dense, "backend_for", lambda dev: _Products())
+
+
+@pytest.mark.parametrize("main_grad", [False, True])
+@pytest.mark.parametrize("x_grad", [False, True])
+def test_the_bias_may_change_before_the_backward(plain_products, x_grad, main_grad):
+    """No gradient is computed from it, so F.linear allows it too; a changed weight is refused."""
+    x = torch.randn(5, 3, requires_grad=x_grad)
+    w, b = torch.randn(4, 3, requires_grad=True), torch.randn(4, requires_grad=True)
+    dy = torch.randn(5, 4)
+    y = dense_projection(x, w, b)
+    if main_grad:
+        w.main_grad, b.main_grad = torch.ones(4, 3), torch.ones(4)
+    with torch.no_grad():
+        b.add_(1)
+    y.backward(dy)
+    got = (w.main_grad - 1, b.main_grad - 1) if main_grad else (w.grad, b.grad)
+    torch.testing.assert_close(got[0], dy.t() @ x.detach())
+    torch.testing.assert_close(got[1], dy.sum(0))
+    assert not main_grad or (w.grad is None and b.grad is None)
+    if x_grad:
+        assert torch.equal(x.grad, dy @ w.detach())
+    y = dense_projection(x, w, b)
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward(dy)
+
+
+def test_a_computed_bias_is_not_held(plain_products):
+    import weakref
+
+    x, w, b = torch.randn(5, 3), torch.randn(4, 3), torch.randn(4, requires_grad=True)
+    b2 = b * 2
+    y = dense_projection(x, w, b2)
+    gone = weakref.ref(b2)
+    del b2
+    assert gone() is None
+    dy = torch.randn(5, 4)
+    y.backward(dy)
+    torch.testing.assert_close(b.grad, 2 * dy.sum(0))

@@ -498,3 +498,18 @@ def test_every_tile_of_every_product(dtype, tile, M, K, N, turn):
     """The products are M x N over K, M x K over N and N x K over M."""
     size = {"forward": (M, K, N), "dx": (M, N, K), "dw": (K, N, M)}[turn]
     check_training(inputs(*size, dtype), "gelu", "int8")
+
+
+@pytest.mark.parametrize("asked", ["w", "b", "wb", "xwb"])
+def test_computed_parameters(asked):
+    """bf16 parameters cast from fp32 ones: the gradients of the cast ones, cast; the bias may change before the backward."""
+    t = inputs(70, 48, 40, BF)
+    leaves = {k: t[k].float().requires_grad_(k in asked) for k in "xwb"}
+    cast = {k: v.bfloat16() for k, v in leaves.items()}
+    y = dense_projection(cast["x"], cast["w"], cast["b"], None, "gelu")
+    with torch.no_grad():
+        cast["b"].add_(1)
+    got = torch.autograd.grad(y, [leaves[k] for k in asked], t["dy"])
+    want = run_training(t, "gelu", "exact")[1]
+    for k, g in zip(asked, got):
+        assert g.dtype == F32 and torch.equal(g, want["d" + k].float())
