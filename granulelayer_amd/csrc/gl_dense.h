@@ -56,9 +56,11 @@ struct DenseK {
 // GELU from the normal distribution's upper tail: with a = |z| and Q(a) = 1 - Phi(a),
 //     gelu(z) = max(z, 0) - a Q(a)
 // and Q(a) = 2^R(a): log2 of the tail is smooth, and a polynomial of degree 8, fitted on [0, 8] by least squares
-// weighted with a Q(a), leaves 8e-9 in a Q(a).  Evaluated in fp32 gelu is within 2.5e-7 of the exact values over
-// [-14, 14] (the last place of z near 4), and keeps its relative accuracy in the negative tail, where 1 + erf
-// cancels.  15 instruction slots, against about 40 with erff; past 8, a Q(a) is below 5e-15.
+// weighted with a Q(a), leaves 1.3e-8 in a Q(a) with its coefficients in fp32.  That weight evens out the absolute error:
+// evaluated in fp32 gelu is within 2.5e-7 of the exact values over [-14, 14] (the last place of z near 4), and within 5e-8
+// for z < 0.  Relative to gelu the tail is off by 2e-5 down to z = -4, 0.4% at -5, 5% at -6 and 84% at -8, where
+// gelu is -5e-15; 1 + erf in fp32 cancels there (5e-4 at -4, 5% at -5, nothing left from about -5.5).  Below -8, at -inf
+// too, the result stays at -8e-16.  15 instruction slots, against about 40 with erff.
 // max(z, 0) by comparison: NaN stays NaN.
 __device__ __forceinline__ float upper_tail(float a) {
   float r = -1.8003542e-06f;
@@ -78,7 +80,7 @@ __device__ __forceinline__ float gelu_f(float z) {
   return __builtin_fmaf(-a, upper_tail(a), relu_f(z));
 }
 // gelu'(z) = D(a) for z < 0 and 1 - D(a) else, D(a) = Q(a) - a phi(a) = exp(-a^2 / 2) P(a): P of degree 10, by
-// least squares weighted with the exponential, leaves 7e-8 on [0, 6.5], and D(6.5) is below 2e-9; within 1.7e-7 in
+// least squares weighted with the exponential, leaves 8e-8 on [0, 6.5], and D(6.5) is below 2e-9; within 1.7e-7 in
 // fp32.  One exponential, 18 slots.
 __device__ __forceinline__ float dgelu_f(float z) {
   const float m = __builtin_fabsf(z), a = m > 6.5f ? 6.5f : m;  // NaN stays

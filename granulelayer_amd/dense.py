@@ -2,9 +2,10 @@
 
 What a model around a sparse layer needs next to it: the map from its width into the layer's inputs,
 and from the pooled outputs back onto a residual stream.  Bias, activation and residual are the
-product's epilogue on the GPU, activations are the sparse layer's (identity, relu, erf gelu), operands
-fp32 or bf16 with products and sums in fp32, and gradients go to ``main_grad`` where the parameters have
-it, as the sparse layer's do (no counterpart in the reference).
+product's epilogue on the GPU, activations are the sparse layer's (identity, relu, erf gelu; gelu by a
+polynomial, within 2.5e-7 of erf's, and about 0 at -inf where erf's form gives NaN), operands fp32 or bf16 with
+products and sums in fp32, and gradients go to ``main_grad`` where the parameters have it, as the sparse layer's do (no
+counterpart in the reference).
 
 The backward needs x and, through the activation, z = x W^T + b.  ReLU keeps one bit of z an element.
 GELU keeps z in the operands' type, or in 8 bits (``activation_checkpoint="int8"``, activations8.py),

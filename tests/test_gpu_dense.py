@@ -513,3 +513,14 @@ def test_computed_parameters(asked):
     want = run_training(t, "gelu", "exact")[1]
     for k, g in zip(asked, got):
         assert g.dtype == F32 and torch.equal(g, want["d" + k].float())
+
+
+def test_gelu_in_the_negative_tail():
+    """Relative to gelu, down to z = -4: the fit's 2e-5, and the last places of a log2 of magnitude 15 (2e-6)."""
+    z = torch.linspace(-4, -1e-3, 100001).to(DEV).reshape(-1, 1)
+    y = dense_projection(z, torch.ones(1, 1, device=DEV), None, None, "gelu")
+    want = act64(z.double(), "gelu")
+    assert bool(((y.double() - want).abs() <= 2.5e-5 * want.abs()).all())
+    below = torch.tensor([[-9.0], [-1e4], [float("-inf")]], device=DEV)
+    y = dense_projection(below, torch.ones(1, 1, device=DEV), None, None, "gelu")
+    assert bool((y.abs() < 1e-14).all())
