@@ -10,6 +10,10 @@ counterpart in the reference).
 The backward needs x and, through the activation, z = x W^T + b.  ReLU keeps one bit of z an element.
 GELU keeps z in the operands' type, or in 8 bits (``activation_checkpoint="int8"``, activations8.py),
 which also keeps x in 8 bits; the gradients are then those at the values that were kept.
+
+With bf16 operands the gradient at z, dz = dy act'(z), is rounded to bf16 before dX and dW (the matrix
+instructions take two operands of one type), also where dy is fp32 because the residual is: half a step, 2^-8, of each
+term at most, so 2.3e-3 of dX and dW in all where the rounding of the result alone gives 1.7e-3.  db sums dz unrounded.
 """
 from __future__ import annotations
 
@@ -116,7 +120,8 @@ def dense_projection(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
 
     x [..., K] and weight [N, K], both float32 or both bfloat16 (products and sums in fp32); bias [N] of
     their type; residual [..., N] float32 or bfloat16.  The result has x's type, or float32 with a
-    float32 residual, and is rounded once.  Rows may be any stride apart."""
+    float32 residual, and is rounded once.  Rows may be any stride apart.  The backward of bfloat16
+    operands rounds the gradient at the product to bfloat16 before the products for x and the weight."""
     _check(x, weight, bias, residual, activation, activation_checkpoint)
     N, K = weight.shape
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
