@@ -442,8 +442,8 @@ struct Reader {
 // 16 x 16 or 32 x 32: an instruction of 16 x 16 reads and writes its sums for twice the products, which takes less
 // power, and power sets the clock of large bf16 products: from registers alone 2,120 TFLOP/s against 1,890.  But it is
 // half as long, and a wave that is alone on its SIMD has less to hide its reads behind.  16384 x 4096 over 4096 in 256 x
-// 256 tiles: 399 us against 409 (407 against 430 on a card with a lower clock); 4096 x 1024 over 4096 in 128 x 128 tiles, a
-// wave a SIMD: 39.4 against 36.9.  fp32: 1040 against 1060 us (4096 x 4096 over 4096, NN).
+// 256 tiles, on the card where both were timed: 399 us against 409 (407 against 430 on one with a lower clock); 4096 x 1024
+// over 4096 in 128 x 128 tiles, a wave a SIMD: 39.4 against 36.9.  fp32: 1040 against 1060 us (4096 x 4096 over 4096, NN).
 __device__ __forceinline__ f32x4 mma(const Frag<2>& q, const Frag<2>& p, int, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(q.v, p.v, c, 0, 0, 0);
 }
@@ -594,8 +594,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   constexpr bool FORWARD = PRC && QRC;  // bias, activation, residual and what is kept; else sums as they are
   constexpr int ROWS = 4;               // of a lane at a time, 4 apart
   // The caches need not keep the large tile's results and what is added to them, but the operands of the tiles that
-  // still run: 8192 x 8192 over 4096 with an fp32 residual 538 -> 500 us.  (Without it where outputs are smaller and
-  // still there for who reads them next: fp32 2048 x 4096 over 1024 takes 2% longer with it.)
+  // still run.  By tile, not by the outputs' size.  With it and without, us: 8192 x 8192 over 4096 with an fp32 residual
+  // 480 / 525, 4096 x 4096 over 16384 (TN) 372 / 387, forward and backward of 8192 x 4096 over 4096 with GELU 647 / 668, of 4096
+  // x 4096 over 1024 no different (161 to 169), that forward alone 43.5 / 45.3.  What it loses: a next product that reads 32 MB of
+  // results at once, 4096 x 1024 -> 4096 -> 1024 in a graph 80 / 75.  The smaller tiles go without: fp32 2048 x 4096
+  // over 1024 takes 2% longer with it.
   constexpr bool STREAM = BM * BN == 65536;
   copies_barrier<0>();
   const int l = threadIdx.x & 63;

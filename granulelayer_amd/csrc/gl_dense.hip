@@ -323,8 +323,8 @@ FwdPlan plan_fwd(const GlDenseArgs* a) {
   if (p.pr.splits == 0) return p;  // refused by the entry points
   if (a->M <= DENSE_FEW_ROWS && a->keep == GL_KEEP_NONE) {
     // Few rows: a workgroup's 16 features' weights at 25 bytes a ns of a CU, and 5 TB/s in all, then X from L2 at
-    // 40 bytes a ns; against the tiles and the copies they need.  4096 x 4096 bf16: 1 row 7.5 us (tiles 11.6),
-    // 16 rows 9.8 (12.3), 32 rows 13.8 (12.5), 64 rows 21.1 (13.4); from K 1024 64 rows 7.0 (8.4).
+    // 40 bytes a ns; against the tiles and the copies they need.  4096 x 4096 bf16, in a graph: 1 row 6.9 us (tiles
+    // 11.6), 16 rows 9.6 (12.3), 32 rows 13.8 (12.5), 64 rows 21.1 (12.7); from K 1024 64 rows 7.0 (8.4).
     const double row = (double)a->K * es, w = a->N * row, rounds = ceil_div(ceil_div(a->N, 16), 256);
     const double weights = w / 5.0e6 > rounds * 16 * row / 25e3 ? w / 5.0e6 : rounds * 16 * row / 25e3;
     const double few = 1.5 + weights + rounds * (double)a->M * row / 40e3;

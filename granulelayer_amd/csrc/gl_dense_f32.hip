@@ -1,6 +1,6 @@
 // fp32 instances of the dense tile kernel (gl_dense.h): fp32 MFMA, 1/16 of the bf16 rate, so a stage's LDS reads
-// and copies are a small part of its products and no tile past 128 x 128 is needed.  2048 x 4096 over 1024: 134 us,
-// 128 TFLOP/s; 4096 x 4096 over 4096: 1002 us, 137 TFLOP/s (a large library product reaches 154).  The deep tile has
+// and copies are a small part of its products and no tile past 128 x 128 is needed.  2048 x 4096 over 1024: 133 us,
+// 129 TFLOP/s; 4096 x 4096 over 4096: 994 us, 138 TFLOP/s (a large library product reaches 154).  The deep tile has
 // eight waves: one workgroup a CU then keeps as many waves as two of the plain one.
 #include "gl_dense.h"
 
