@@ -276,12 +276,12 @@ def _rounds_input(ctx, rt: Level1Runtime) -> bool:
             and rt.backend is not None)
 
 
-def _keep_input(ctx, rt: Level1Runtime, x, xc) -> list:
-    """Tensors that stand for the input in ctx's saved ones: x itself, or the 8-bit form of the kernels'
-    operand xc (_rounds_input).  The gradients are then those at the values that were kept: dW sums over
+def _keep_input(ctx, rt: Level1Runtime, x, xc, rounded: bool) -> list:
+    """Tensors that stand for the input in ctx's saved ones: x itself, or (rounded) the 8-bit form of the kernels'
+    operand xc.  The gradients are then those at the values that were kept: dW sums over
     them, and neurons whose z the backward recomputes are recomputed from them."""
     ctx.x_kept = None
-    if _rounds_input(ctx, rt):
+    if rounded:
         ctx.x_kept = (xc.shape, xc.dtype, x.dtype)
         kept = list(rt.backend.pack8(xc))
     else:
@@ -352,10 +352,11 @@ class SparsePoolFunction(torch.autograd.Function):
         out = rt.forward(xc, wc, bc, track_ids=(policy == "save_winners"), relu_mask=keep_bits)
         pre = out["pre"]
         y = act_torch(pre, lv.out_activation)
-        saved = _saved_stats(lv, out, policy, _rounds_input(ctx, rt))
+        rounded = _rounds_input(ctx, rt)
+        saved = _saved_stats(lv, out, policy, rounded)
         ctx.rt, ctx.policy, ctx.compute_dtype = rt, policy, compute_dtype
         ctx.saved_keys = list(saved.keys())
-        ctx.save_for_backward(*_keep_input(ctx, rt, x, xc), w, b, *saved.values())
+        ctx.save_for_backward(*_keep_input(ctx, rt, x, xc, rounded), w, b, *saved.values())
         rt.last_info["checkpoint_bytes"] = sum(t.numel() * t.element_size() for t in saved.values())
         return y
 

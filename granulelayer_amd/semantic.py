@@ -115,15 +115,15 @@ class SemanticPoolFunction(torch.autograd.Function):
         tp = dict(zip(tnames, tparams))
         with torch.no_grad():
             y = level2_forward(F, cfg, tp)
+        rounded = _rounds_input(ctx, rt)
         if cfg.level1_checkpoint == "save":
-            saved = _saved_stats(l1, out, policy if policy != "recompute_stats" else "minimal_stats",
-                                 _rounds_input(ctx, rt))
+            saved = _saved_stats(l1, out, policy if policy != "recompute_stats" else "minimal_stats", rounded)
         else:
             saved = {}
         ctx.rt, ctx.cfg, ctx.policy, ctx.compute_dtype, ctx.tnames = rt, cfg, policy, compute_dtype, tnames
         ctx.saved_keys = list(saved.keys())
         ctx.n_t = len(tparams)
-        ctx.save_for_backward(*_keep_input(ctx, rt, x, xc), w, b, *tparams, *saved.values())
+        ctx.save_for_backward(*_keep_input(ctx, rt, x, xc, rounded), w, b, *tparams, *saved.values())
         rt.last_info["checkpoint_bytes"] = sum(t.numel() * t.element_size() for t in saved.values())
         return y
 

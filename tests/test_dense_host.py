@@ -232,3 +232,17 @@ def test_a_computed_bias_is_not_held(plain_products):
     dy = torch.randn(5, 4)
     y.backward(dy)
     torch.testing.assert_close(b.grad, 2 * dy.sum(0))
+
+
+def test_under_activation_checkpointing(plain_products):
+    from torch.utils.checkpoint import checkpoint
+
+    x, w, b = (torch.randn(*s, requires_grad=True) for s in ((5, 3), (4, 3), (4,)))
+
+    def call(x):
+        return dense_projection(x, w * 2, b * 2)
+
+    want = torch.autograd.grad(call(x).sum(), (x, w, b))
+    got = torch.autograd.grad(checkpoint(call, x, use_reentrant=False).sum(), (x, w, b))
+    for g, t in zip(got, want):
+        assert torch.equal(g, t)
