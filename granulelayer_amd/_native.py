@@ -13,11 +13,12 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libgranulelayer_amd.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 GL_ACT = {"identity": 0, "relu": 1, "gelu": 2}
 GL_POOL = {"mean": 0, "sum": 1, "max": 2, "topk_mean": 3, "logmeanexp": 4, "power_mean": 5, "softmax_weighted": 6}
 GL_DTYPE_F32, GL_DTYPE_BF16 = 0, 1
+GL_MOMENTS_INT8 = 2
 GL_KEEP = {"none": 0, "sign": 1, "z": 2, "z8": 3}
 DENSE_MAX_FEATURES = 1 << 20  # GL_DENSE_MAX_FEATURES
 GL_ERR_WORKSPACE = -3
@@ -25,6 +26,7 @@ GL_ERR_SCRATCH = -8
 FWD_STATIC_SCRATCH_BYTES = 64 << 20  # GL_FWD_STATIC_SCRATCH_BYTES
 
 _P, _I32, _I64, _SZ, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
+_D = ctypes.c_double
 
 
 class GlFwdArgs(ctypes.Structure):
@@ -81,8 +83,20 @@ class GlDenseBwdArgs(ctypes.Structure):
                 ("accumulate", _I32), ("ws", _P), ("ws_bytes", _SZ)]
 
 
-# gl_struct_layout ids 0..7
-STRUCTS = (GlFwdArgs, GlBwdArgs, GlEdgeArgs, GlAdamArgs, GlCoverArgs, GlPack8Args, GlDenseArgs, GlDenseBwdArgs)
+class GlAdamTensor(ctypes.Structure):
+    _fields_ = [("p", _P), ("g", _P), ("m", _P), ("v", _P), ("master", _P), ("m_scale", _P), ("v_scale", _P),
+                ("n", _I64), ("seed", ctypes.c_uint64), ("bc1", _F), ("bc2", _F)]
+
+
+class GlAdamManyArgs(ctypes.Structure):
+    _fields_ = [("t", _P), ("count", _I32), ("p_dtype", _I32), ("g_dtype", _I32), ("moments_dtype", _I32),
+                ("stochastic", _I32), ("clear", _I32), ("lr", _D), ("beta1", _D), ("beta2", _D), ("eps", _D),
+                ("weight_decay", _D)]
+
+
+# gl_struct_layout ids 0..9
+STRUCTS = (GlFwdArgs, GlBwdArgs, GlEdgeArgs, GlAdamArgs, GlCoverArgs, GlPack8Args, GlDenseArgs, GlDenseBwdArgs,
+           GlAdamTensor, GlAdamManyArgs)
 # every symbol include/granulelayer_amd.h declares
 EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_workspace", "gl_fwd", "gl_fwd_static",
            "gl_fwd_mask_bytes",
@@ -90,14 +104,14 @@ EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_work
            "gl_edges_build", "gl_bwd_workspace", "gl_bwd", "gl_adam", "gl_sched_size", "gl_sched_build_host",
            "gl_sched_build", "gl_window_build_host", "gl_window_build", "gl_cover_select", "gl_trace_begin",
            "gl_trace_end", "gl_pack8", "gl_unpack8", "gl_dense_fwd_workspace", "gl_dense_fwd", "gl_dense_bwd_workspace",
-           "gl_dense_bwd")
+           "gl_dense_bwd", "gl_adam_many", "gl_adam_values")
 KERNEL_NAMES = {1: "tile_x_kernel", 2: "fwd_kernel", 3: "fwd_finalize_kernel", 4: "c1t_kernel", 5: "bwd_w_kernel",
                 6: "dx_kernel", 7: "dx_reduce_kernel", 8: "adam_kernel", 9: "edges_build", 10: "fwd_kernel_win",
                 11: "bwd_w_kernel_win", 12: "max_events_dw_kernel", 13: "max_events_dx_kernel",
                 14: "cover_select_kernel", 15: "sched_build_kernel", 16: "dx_dense_kernel",
                 17: "dx_dma_kernel", 18: "pack8_kernel", 19: "unpack8_kernel", 20: "dense_tile_kernel",
                 21: "dense_few_kernel", 22: "dense_join_kernel", 23: "dense_dz_kernel", 24: "dense_db_kernel",
-                25: "dense_align_kernel"}
+                25: "dense_align_kernel", 26: "adam_values_kernel"}
 
 
 class NativeError(RuntimeError):
@@ -125,7 +139,8 @@ class Library:
         L.gl_error_string.argtypes = [ctypes.c_int]
         for name, st in (("gl_fwd", GlFwdArgs), ("gl_fwd_static", GlFwdArgs), ("gl_bwd", GlBwdArgs),
                          ("gl_edges_build", GlEdgeArgs), ("gl_adam", GlAdamArgs), ("gl_cover_select", GlCoverArgs), ("gl_pack8", GlPack8Args), ("gl_unpack8", GlPack8Args),
-                         ("gl_dense_fwd", GlDenseArgs), ("gl_dense_bwd", GlDenseBwdArgs)):
+                         ("gl_dense_fwd", GlDenseArgs), ("gl_dense_bwd", GlDenseBwdArgs),
+                         ("gl_adam_many", GlAdamManyArgs), ("gl_adam_values", GlAdamManyArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), _P]
         for name, st in (("gl_fwd_workspace", GlFwdArgs), ("gl_bwd_workspace", GlBwdArgs),

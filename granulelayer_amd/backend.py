@@ -404,6 +404,24 @@ class HipBackend:
         with _on(p.device):
             self.lib.call("gl_adam", ctypes.byref(a), ctypes.c_void_p(_stream(p.device)))
 
+    def adam_many(self, device, rows, p_dtype, g_dtype, m_dtype, lr, beta1, beta2, eps, weight_decay, stochastic=False,
+                  clear=False):
+        """In-place fused AdamW over the tensors of ``rows``, tuples in GlAdamTensor's order (addresses, elements,
+        seed, bias corrections); all of one dtype of parameters, gradients and moments (int8: codes), all with a
+        master or none."""
+        t = np.array(rows, dtype=_ADAM_TENSOR)
+        a = N.GlAdamManyArgs(t.ctypes.data, len(rows), _DENSE_DTYPES[p_dtype], _DENSE_DTYPES[g_dtype], _MOMENTS[m_dtype],
+                             int(stochastic), int(clear), lr, beta1, beta2, eps, weight_decay)
+        with _on(device):
+            self.lib.call("gl_adam_many", ctypes.byref(a), _stream(device))
+
+    def adam_values(self, device, rows):
+        """The fp32 values of 8-bit moments: ``rows`` as for ``adam_many``, with m's values going to g and v's to p."""
+        t = np.array(rows, dtype=_ADAM_TENSOR)
+        a = N.GlAdamManyArgs(t.ctypes.data, len(rows), 0, 0, N.GL_MOMENTS_INT8)
+        with _on(device):
+            self.lib.call("gl_adam_values", ctypes.byref(a), _stream(device))
+
     # ------------------------------------------------------------------ activations in 8 bits
     def pack8(self, x):
         """x [rows, features] in 8 bits: (codes [rows, round_up(features, 32)] int8, exponents
@@ -507,6 +525,8 @@ class HipBackend:
 
 
 _DENSE_DTYPES = {torch.float32: N.GL_DTYPE_F32, torch.bfloat16: N.GL_DTYPE_BF16}
+_MOMENTS = {**_DENSE_DTYPES, torch.int8: N.GL_MOMENTS_INT8}
+_ADAM_TENSOR = np.dtype(N.GlAdamTensor)
 
 
 def backend_for(device) -> HipBackend:

@@ -162,6 +162,21 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       for (long long x : t) v[c++] = x;
       break;
     }
+    case 8: {
+      typedef GlAdamTensor S;
+      long long t[] = {(long long)sizeof(S), OFF(S, p), OFF(S, g), OFF(S, m), OFF(S, v), OFF(S, master), OFF(S, m_scale),
+                       OFF(S, v_scale), OFF(S, n), OFF(S, seed), OFF(S, bc1), OFF(S, bc2)};
+      for (long long x : t) v[c++] = x;
+      break;
+    }
+    case 9: {
+      typedef GlAdamManyArgs S;
+      long long t[] = {(long long)sizeof(S), OFF(S, t), OFF(S, count), OFF(S, p_dtype), OFF(S, g_dtype),
+                       OFF(S, moments_dtype), OFF(S, stochastic), OFF(S, clear), OFF(S, lr), OFF(S, beta1), OFF(S, beta2),
+                       OFF(S, eps), OFF(S, weight_decay)};
+      for (long long x : t) v[c++] = x;
+      break;
+    }
     default:
       return GL_ERR_ARG;
   }

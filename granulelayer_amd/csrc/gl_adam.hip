@@ -1,9 +1,21 @@
-// Fused AdamW: one streaming pass reads p, g, m, v (and an fp32 master copy) and writes p, m, v and
-// g = 0 (32 bytes per element with fp32 parameters and moments, 24 with bf16 moments).
+// Fused AdamW over a list of tensors: one streaming pass reads p, g, m, v (and an fp32 master copy) and writes
+// p, m, v and, of main_grad buffers, g = 0.  Bytes an element: 32 with fp32 parameters, gradient buffers and
+// moments, 24 with bf16 moments, 20 with moments in 8 bits; 10 with parameters and gradients in bf16 and moments in 8 bits.
 // Reference: _adamw_kernel, sparse_pooling/optim.py:26-64 (fp32 parameters; bf16 parameters with
-// HAS_MASTER, with STOCH, or rounded to nearest even).  The
+// HAS_MASTER, with STOCH, or rounded to nearest even), a launch a tensor.  With fp32 and bf16 moments the
 // update is evaluated unfused in the reference's operation order; every element is read and
 // written by the same thread, so the in-place race fixed at optim.py:43-50 cannot occur.
+//
+// Moments in 8 bits (no counterpart in the reference): blocks of 256 neighbouring elements of a tensor share two
+// fp32 scales,
+//     m = s c |c|      c from -127 to 127    s = max |m| / 127^2
+//     v = (r c^2)^2    c from 0 to 255       r = sqrt(max v) / 255^2
+// with the codes nearest in their root: a value is off by 1 / c of itself, 0.8% of m and 0.4% of sqrt(v) next to the
+// maximum, more towards zero, and sqrt(v) reaches down to 1.5e-5 of the largest.  Codes of v are 1 at least where v > 0: a
+// sqrt(v) rounded to nothing would leave m / eps.  The update itself takes the moments before they are put into 8 bits.
+// A value next to a border between two codes must not depend on how its sums are rounded, so moments and
+// codes are computed in 64 bits, which this chip does as fast as unpacked 32.  A block with an infinity or a NaN in m or v has
+// the scale NaN; one whose largest |m| is below 2^-100 (v: 2^-126) the scale 0.
 #include "gl_common.h"
 #include "gl_internal.h"
 
@@ -13,6 +25,31 @@ struct AdamK {
   float lr, b1, b2, eps, wd, bc1, bc2;
 };
 
+// The tensors of a launch travel as kernel arguments: nothing to copy to the device, nothing to keep alive.
+constexpr int ADAM_TENSORS = 40;      // of a launch: 3.7 of the 4 KB that arguments may take
+constexpr int ADAM_BLOCK = 256;       // elements that share a scale
+constexpr int ADAM_CHUNK = 4096;      // elements of a workgroup: 4 vectors of 4 a thread
+struct AdamTensorK {
+  void* p;
+  void* g;
+  void* m;
+  void* v;
+  float* master;
+  float* m_scale;
+  float* v_scale;
+  long long n;
+  unsigned long long seed;
+  float bc1, bc2;
+};
+struct AdamTable {
+  float lr, b1, b2, eps, wd;
+  int count, clear;
+  double b1d, a1d, b2d, a2d;           // of the 8-bit moments: betas and 1 - beta
+  unsigned first[ADAM_TENSORS + 1];    // first workgroup of every tensor
+  AdamTensorK t[ADAM_TENSORS];
+};
+static_assert(sizeof(AdamTable) <= 4096, "kernel arguments");
+
 __device__ __forceinline__ float bf16_bits_to_f32(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
 __device__ __forceinline__ unsigned short f32_to_bf16_rne(float f) {
   unsigned u = __float_as_uint(f);
@@ -21,25 +58,87 @@ __device__ __forceinline__ unsigned short f32_to_bf16_rne(float f) {
   return (unsigned short)(u >> 16);
 }
 
+__device__ __forceinline__ void adam_param(const AdamK& c, float& p, float m, float v) {
+#pragma clang fp contract(off)
+  const float upd = (m / c.bc1) / (__builtin_sqrtf(v / c.bc2) + c.eps);
+  p = p * (1.0f - c.lr * c.wd) - c.lr * upd;
+}
 __device__ __forceinline__ void adam_elem(const AdamK& c, float& p, float g, float& m, float& v) {
 #pragma clang fp contract(off)
   m = c.b1 * m + (1.0f - c.b1) * g;
   v = c.b2 * v + (1.0f - c.b2) * g * g;
-  const float upd = (m / c.bc1) / (__builtin_sqrtf(v / c.bc2) + c.eps);
-  p = p * (1.0f - c.lr * c.wd) - c.lr * upd;
+  adam_param(c, p, m, v);
 }
 
 // Streams are read and written with non-temporal loads and stores (each element is touched once;
 // at C2's 805M elements this ran at 6.3 TB/s against 5.4 with plain accesses in a measurement of
-// this access pattern), one 16-byte vector of each stream per thread.
-typedef float f4v __attribute__((ext_vector_type(4)));
-template <typename T>
-__device__ __forceinline__ T ld_nt(const void* p, long long i) {
-  return __builtin_nontemporal_load(reinterpret_cast<const T*>(p) + i);
+// this access pattern).  Vectors are at the elements' own alignment, so a tensor may begin anywhere.
+typedef unsigned w4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned w2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned w1 __attribute__((aligned(1)));
+
+// four neighbours from element i, of which the first n are there
+template <bool BF>
+__device__ __forceinline__ void adam_load(const void* p, long long i, int n, float (&v)[4]) {
+  if (n >= 4) {
+    if constexpr (BF) {
+      const w2 w = __builtin_nontemporal_load(reinterpret_cast<const w2*>((const char*)p + 2 * i));
+      v[0] = __uint_as_float(w[0] << 16);
+      v[1] = __uint_as_float(w[0] & 0xffff0000u);
+      v[2] = __uint_as_float(w[1] << 16);
+      v[3] = __uint_as_float(w[1] & 0xffff0000u);
+    } else {
+      const w4 w = __builtin_nontemporal_load(reinterpret_cast<const w4*>((const char*)p + 4 * i));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(w[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < n ? ld_param_t<BF>((const float*)p, i + j) : 0.f;
+  }
 }
-template <typename T>
-__device__ __forceinline__ void st_nt(void* p, long long i, T v) {
-  __builtin_nontemporal_store(v, reinterpret_cast<T*>(p) + i);
+__device__ __forceinline__ void adam_store(float* p, long long i, int n, const float (&v)[4]) {
+  if (n >= 4) {
+    w4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(v[j]);
+    __builtin_nontemporal_store(w, reinterpret_cast<w4*>(p + i));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[i + j] = v[j];
+  }
+}
+__device__ __forceinline__ void adam_store(unsigned short* p, long long i, int n, const unsigned short (&v)[4]) {
+  if (n >= 4) {
+    w2 w;
+    w[0] = (unsigned)v[0] | (unsigned)v[1] << 16;
+    w[1] = (unsigned)v[2] | (unsigned)v[3] << 16;
+    __builtin_nontemporal_store(w, reinterpret_cast<w2*>(p + i));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[i + j] = v[j];
+  }
+}
+__device__ __forceinline__ unsigned adam_load_codes(const void* p, long long i, int n) {
+  const unsigned char* c = (const unsigned char*)p + i;
+  if (n >= 4) return __builtin_nontemporal_load(reinterpret_cast<const w1*>(c));
+  unsigned w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < n) w |= (unsigned)c[j] << (8 * j);
+  return w;
+}
+__device__ __forceinline__ void adam_store_codes(void* p, long long i, int n, unsigned w) {
+  unsigned char* c = (unsigned char*)p + i;
+  if (n >= 4) {
+    __builtin_nontemporal_store((w1)w, reinterpret_cast<w1*>(c));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) c[j] = (unsigned char)(w >> (8 * j));
+  }
 }
 
 // Parameter storage of the update: fp32, or bf16 rounded to nearest even, bf16 with an fp32
@@ -78,121 +177,301 @@ __device__ __forceinline__ unsigned short round_param(float p, unsigned long lon
   }
 }
 
-template <bool BF16M, int PM>
-__global__ void __launch_bounds__(256) adam_kernel(void* __restrict__ P, float* __restrict__ Gr, void* __restrict__ M,
-                                                   void* __restrict__ V, float* __restrict__ MS, long long n, AdamK c,
-                                                   unsigned long long seed) {
-  constexpr bool BP = PM != PM_F32;  // bf16 parameter storage
-  const long long n4 = n >> 2;
-  const long long stride = (long long)gridDim.x * blockDim.x;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += stride) {
-    const f4v g = ld_nt<f4v>(Gr, i);
-    float4 p;
-    if constexpr (PM == PM_F32) {
-      const f4v pv = ld_nt<f4v>(P, i);
-      p = make_float4(pv.x, pv.y, pv.z, pv.w);
-    } else if constexpr (PM == PM_BF16_MASTER) {
-      const f4v pv = ld_nt<f4v>(MS, i);
-      p = make_float4(pv.x, pv.y, pv.z, pv.w);
-    } else {
-      const unsigned long long pb = ld_nt<unsigned long long>(P, i);
-      p = make_float4(bf16_bits_to_f32((unsigned short)pb), bf16_bits_to_f32((unsigned short)(pb >> 16)),
-                      bf16_bits_to_f32((unsigned short)(pb >> 32)), bf16_bits_to_f32((unsigned short)(pb >> 48)));
+// ---- 8-bit moments -----------------------------------------------------------------------------------
+// the largest of 64 lanes, integer order (of values >= 0: the values' order, infinities and NaN above every number)
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+  auto up = [](unsigned a, unsigned b) { return a > b ? a : b; };
+  v = up(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));   // lane ^ 1
+  v = up(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));   // lane ^ 2
+  v = up(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));  // row_ror:4
+  v = up(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // row_ror:8
+  const auto p16 = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = up(p16[0], p16[1]);
+  const auto p32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return up(p32[0], p32[1]);
+}
+// scales of a block from the bits of its largest fp32 |m| and v
+__device__ __forceinline__ float scale_m(unsigned top) {
+  if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return top < 0x0d800000u ? 0.f : (float)((double)__uint_as_float(top) * (1.0 / 16129.0));
+}
+__device__ __forceinline__ float scale_v(unsigned top) {
+  if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return top < 0x00800000u ? 0.f : (float)(__builtin_sqrt((double)__uint_as_float(top)) * (1.0 / 65025.0));
+}
+// floor(x + 1/2) of the root x of y >= 0: an estimate decides all but which side of i + 1/2 it is on, the square
+// (i + 1/2)^2, exact in 64 bits, decides that
+__device__ __forceinline__ unsigned code_m(double y) {
+  const float i = __builtin_floorf(__builtin_amdgcn_sqrtf((float)y) + 0.25f), h = i + 0.5f;
+  return (unsigned)i + (y >= (double)(h * h) ? 1u : 0u);
+}
+// of the fourth root
+__device__ __forceinline__ unsigned code_v(double y) {
+  const float i = __builtin_floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y)) + 0.25f), h = i + 0.5f;
+  const double h2 = (double)(h * h);
+  return (unsigned)i + (y >= h2 * h2 ? 1u : 0u);
+}
+// values of codes
+__device__ __forceinline__ double value_m(unsigned codes, int j, double s) {
+  const int c = (int)(codes << (24 - 8 * j)) >> 24;
+  return (double)(c * __builtin_abs(c)) * s;
+}
+__device__ __forceinline__ double value_v(unsigned codes, int j, double r) {
+  const unsigned c = (codes >> (8 * j)) & 255u;
+  const double t = (double)(c * c) * r;
+  return t * t;
+}
+
+// MOM: GL_DTYPE_F32, GL_DTYPE_BF16 or GL_MOMENTS_INT8; GBF: bf16 gradients.  A workgroup takes a chunk of one
+// tensor; wave w the vectors of its w-th quarter, AHEAD of them in flight.  With 8-bit moments a wave's vector is a block.
+template <int MOM, int PM, bool GBF>
+__global__ void __launch_bounds__(256) adam_kernel(AdamTable a) {
+  constexpr bool I8 = MOM == GL_MOMENTS_INT8, BM = MOM == GL_DTYPE_BF16;
+  constexpr int AHEAD = 2, VECS = ADAM_CHUNK / 1024;
+  int ti = 0;
+  for (int step = 32; step > 0; step >>= 1)
+    if (ti + step < a.count && a.first[ti + step] <= blockIdx.x) ti += step;
+  const AdamTensorK& t = a.t[ti];
+  const AdamK c{a.lr, a.b1, a.b2, a.eps, a.wd, t.bc1, t.bc2};
+  const int lane = threadIdx.x & 63;
+  const long long base = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + (threadIdx.x >> 6) * (VECS * 256);
+  const void* P = PM == PM_BF16_MASTER ? (const void*)t.master : t.p;
+  constexpr bool PBF = PM == PM_BF16_RNE || PM == PM_BF16_SR;
+#pragma unroll 1
+  for (int y = 0; y < VECS; y += AHEAD) {
+    float p[AHEAD][4], g[AHEAD][4], m[AHEAD][4], v[AHEAD][4];
+    unsigned cm[AHEAD], cv[AHEAD];
+    float sm[AHEAD], sv[AHEAD];
+    int there[AHEAD];
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) {
+      const long long block = base + (y + x) * 256, i = block + 4 * lane;
+      const long long left = t.n - i;
+      there[x] = left > 4 ? 4 : (left < 0 ? 0 : (int)left);
+      adam_load<PBF>(P, i, there[x], p[x]);
+      adam_load<GBF>(t.g, i, there[x], g[x]);
+      if constexpr (I8) {
+        cm[x] = adam_load_codes(t.m, i, there[x]);
+        cv[x] = adam_load_codes(t.v, i, there[x]);
+        sm[x] = sv[x] = 0.f;
+        if (block < t.n) {
+          sm[x] = t.m_scale[block / ADAM_BLOCK];
+          sv[x] = t.v_scale[block / ADAM_BLOCK];
+        }
+      } else {
+        adam_load<BM>(t.m, i, there[x], m[x]);
+        adam_load<BM>(t.v, i, there[x], v[x]);
+      }
     }
-    float4 m, v;
-    if constexpr (BF16M) {
-      const unsigned long long mb = ld_nt<unsigned long long>(M, i), vb = ld_nt<unsigned long long>(V, i);
-      m = make_float4(bf16_bits_to_f32((unsigned short)mb), bf16_bits_to_f32((unsigned short)(mb >> 16)),
-                      bf16_bits_to_f32((unsigned short)(mb >> 32)), bf16_bits_to_f32((unsigned short)(mb >> 48)));
-      v = make_float4(bf16_bits_to_f32((unsigned short)vb), bf16_bits_to_f32((unsigned short)(vb >> 16)),
-                      bf16_bits_to_f32((unsigned short)(vb >> 32)), bf16_bits_to_f32((unsigned short)(vb >> 48)));
-    } else {
-      const f4v mv = ld_nt<f4v>(M, i), vv = ld_nt<f4v>(V, i);
-      m = make_float4(mv.x, mv.y, mv.z, mv.w);
-      v = make_float4(vv.x, vv.y, vv.z, vv.w);
-    }
-    adam_elem(c, p.x, g.x, m.x, v.x);
-    adam_elem(c, p.y, g.y, m.y, v.y);
-    adam_elem(c, p.z, g.z, m.z, v.z);
-    adam_elem(c, p.w, g.w, m.w, v.w);
-    if constexpr (BF16M) {
-      const unsigned long long mo = (unsigned long long)f32_to_bf16_rne(m.x) | (unsigned long long)f32_to_bf16_rne(m.y) << 16 |
-                                    (unsigned long long)f32_to_bf16_rne(m.z) << 32 | (unsigned long long)f32_to_bf16_rne(m.w) << 48;
-      const unsigned long long vo = (unsigned long long)f32_to_bf16_rne(v.x) | (unsigned long long)f32_to_bf16_rne(v.y) << 16 |
-                                    (unsigned long long)f32_to_bf16_rne(v.z) << 32 | (unsigned long long)f32_to_bf16_rne(v.w) << 48;
-      st_nt<unsigned long long>(M, i, mo);
-      st_nt<unsigned long long>(V, i, vo);
-    } else {
-      st_nt<f4v>(M, i, (f4v){m.x, m.y, m.z, m.w});
-      st_nt<f4v>(V, i, (f4v){v.x, v.y, v.z, v.w});
-    }
-    st_nt<f4v>(Gr, i, (f4v){0.f, 0.f, 0.f, 0.f});
-    if constexpr (BP) {
-      if constexpr (PM == PM_BF16_MASTER) st_nt<f4v>(MS, i, (f4v){p.x, p.y, p.z, p.w});
-      const long long e = i << 2;
-      const unsigned long long po = (unsigned long long)round_param<PM>(p.x, seed, e) |
-                                    (unsigned long long)round_param<PM>(p.y, seed, e + 1) << 16 |
-                                    (unsigned long long)round_param<PM>(p.z, seed, e + 2) << 32 |
-                                    (unsigned long long)round_param<PM>(p.w, seed, e + 3) << 48;
-      st_nt<unsigned long long>(P, i, po);
-    } else {
-      st_nt<f4v>(P, i, (f4v){p.x, p.y, p.z, p.w});
-    }
-  }
-  // tail (n % 4 elements), handled by the first threads of block 0
-  const long long t = (n4 << 2) + threadIdx.x;
-  if (blockIdx.x == 0 && t < n) {
-    float g = Gr[t], m, v, p;
-    if constexpr (PM == PM_F32) p = reinterpret_cast<float*>(P)[t];
-    else if constexpr (PM == PM_BF16_MASTER) p = MS[t];
-    else p = bf16_bits_to_f32(reinterpret_cast<unsigned short*>(P)[t]);
-    if constexpr (BF16M) {
-      m = bf16_bits_to_f32(reinterpret_cast<unsigned short*>(M)[t]);
-      v = bf16_bits_to_f32(reinterpret_cast<unsigned short*>(V)[t]);
-    } else {
-      m = reinterpret_cast<float*>(M)[t];
-      v = reinterpret_cast<float*>(V)[t];
-    }
-    adam_elem(c, p, g, m, v);
-    if constexpr (BF16M) {
-      reinterpret_cast<unsigned short*>(M)[t] = f32_to_bf16_rne(m);
-      reinterpret_cast<unsigned short*>(V)[t] = f32_to_bf16_rne(v);
-    } else {
-      reinterpret_cast<float*>(M)[t] = m;
-      reinterpret_cast<float*>(V)[t] = v;
-    }
-    Gr[t] = 0.f;
-    if constexpr (BP) {
-      if constexpr (PM == PM_BF16_MASTER) MS[t] = p;
-      reinterpret_cast<unsigned short*>(P)[t] = round_param<PM>(p, seed, t);
-    } else {
-      reinterpret_cast<float*>(P)[t] = p;
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) {
+      const long long block = base + (y + x) * 256, i = block + 4 * lane;
+      const int n = there[x];
+      if constexpr (I8) {
+        if (block >= t.n) break;  // of the whole wave
+        double dm[4], dv[4];
+        unsigned tm = 0, tv = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double gj = (double)g[x][j];
+          dm[j] = __builtin_fma(a.b1d, value_m(cm[x], j, (double)sm[x]), a.a1d * gj);
+          dv[j] = __builtin_fma(a.b2d, value_v(cv[x], j, (double)sv[x]), a.a2d * (gj * gj));
+          if (j >= n) dm[j] = dv[j] = 0.0;  // behind the end a code of 0 is NaN too in a block without numbers
+          m[x][j] = (float)dm[j];
+          v[x][j] = (float)dv[j];
+          const unsigned bm = __float_as_uint(m[x][j]) & 0x7fffffffu, bv = __float_as_uint(v[x][j]) & 0x7fffffffu;
+          tm = tm > bm ? tm : bm;
+          tv = tv > bv ? tv : bv;
+        }
+        tm = wave_umax(tm);
+        tv = wave_umax(tv);
+        const float fs = scale_m(tm), fr = scale_v(tv);
+        unsigned om = 0, ov = 0;
+        if (fs > 0.f) {
+          const double im = 1.0 / (double)fs;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int q = (int)code_m(__builtin_fabs(dm[j]) * im);
+            om |= ((unsigned)(dm[j] < 0.0 ? -q : q) & 255u) << (8 * j);
+          }
+        }
+        if (fr > 0.f) {
+          const double ir = 1.0 / (double)fr, iv = ir * ir;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const unsigned u = code_v(dv[j] * iv);
+            ov |= (u == 0 && dv[j] > 0.0 ? 1u : u) << (8 * j);
+          }
+        }
+        adam_store_codes(t.m, i, n, om);
+        adam_store_codes(t.v, i, n, ov);
+        if (lane == 0) {
+          t.m_scale[block / ADAM_BLOCK] = fs;
+          t.v_scale[block / ADAM_BLOCK] = fr;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) adam_param(c, p[x][j], m[x][j], v[x][j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) adam_elem(c, p[x][j], g[x][j], m[x][j], v[x][j]);
+        if constexpr (BM) {
+          unsigned short om[4], ov[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            om[j] = f32_to_bf16_rne(m[x][j]);
+            ov[j] = f32_to_bf16_rne(v[x][j]);
+          }
+          adam_store((unsigned short*)t.m, i, n, om);
+          adam_store((unsigned short*)t.v, i, n, ov);
+        } else {
+          adam_store((float*)t.m, i, n, m[x]);
+          adam_store((float*)t.v, i, n, v[x]);
+        }
+      }
+      if constexpr (!GBF) {
+        const float none[4] = {0.f, 0.f, 0.f, 0.f};
+        if (a.clear) adam_store((float*)t.g, i, n, none);
+      }
+      if constexpr (PM == PM_F32) {
+        adam_store((float*)t.p, i, n, p[x]);
+      } else {
+        if constexpr (PM == PM_BF16_MASTER) adam_store(t.master, i, n, p[x]);
+        unsigned short o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = round_param<PM>(p[x][j], t.seed, i + j);
+        adam_store((unsigned short*)t.p, i, n, o);
+      }
     }
   }
 }
 
-template <bool BF16M>
-static int launch_adam(int pm, dim3 grid, hipStream_t s, const GlAdamArgs* a, const AdamK& c) {
-  void* P = a->p;
-  if (pm == PM_F32)
-    GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<BF16M, PM_F32>), grid, dim3(256), 0, s, P, a->g, a->m, a->v, a->master, a->n, c,
-              a->seed);
-  else if (pm == PM_BF16_RNE)
-    GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<BF16M, PM_BF16_RNE>), grid, dim3(256), 0, s, P, a->g, a->m, a->v, a->master,
-              a->n, c, a->seed);
-  else if (pm == PM_BF16_MASTER)
-    GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<BF16M, PM_BF16_MASTER>), grid, dim3(256), 0, s, P, a->g, a->m, a->v, a->master,
-              a->n, c, a->seed);
-  else
-    GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<BF16M, PM_BF16_SR>), grid, dim3(256), 0, s, P, a->g, a->m, a->v, a->master,
-              a->n, c, a->seed);
-  GL_CHECK_LAUNCH();
+// The fp32 values of 8-bit moments (into g: m's, into p: v's).
+__global__ void __launch_bounds__(256) adam_values_kernel(AdamTable a) {
+  int ti = 0;
+  for (int step = 32; step > 0; step >>= 1)
+    if (ti + step < a.count && a.first[ti + step] <= blockIdx.x) ti += step;
+  const AdamTensorK& t = a.t[ti];
+  const long long base = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + threadIdx.x * 4;
+#pragma unroll
+  for (int x = 0; x < ADAM_CHUNK / 1024; ++x) {
+    const long long i = base + x * 1024, left = t.n - i;
+    if (left <= 0) return;
+    const int n = left > 4 ? 4 : (int)left;
+    const unsigned cm = adam_load_codes(t.m, i, n), cv = adam_load_codes(t.v, i, n);
+    const double sm = (double)t.m_scale[i / ADAM_BLOCK], sv = (double)t.v_scale[i / ADAM_BLOCK];
+    float m[4], v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = (float)value_m(cm, j, sm);
+      v[j] = (float)value_v(cv, j, sv);
+    }
+    adam_store((float*)t.g, i, n, m);
+    adam_store((float*)t.p, i, n, v);
+  }
+}
+
+template <int MOM, int PM>
+void launch_adam_as(bool gbf, dim3 grid, hipStream_t s, const AdamTable& a) {
+  if (gbf) GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<MOM, PM, true>), grid, dim3(256), 0, s, a);
+  else GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<MOM, PM, false>), grid, dim3(256), 0, s, a);
+}
+template <int MOM>
+void launch_adam_of(int pm, bool gbf, dim3 grid, hipStream_t s, const AdamTable& a) {
+  if (pm == PM_F32) launch_adam_as<MOM, PM_F32>(gbf, grid, s, a);
+  else if (pm == PM_BF16_RNE) launch_adam_as<MOM, PM_BF16_RNE>(gbf, grid, s, a);
+  else if (pm == PM_BF16_MASTER) launch_adam_as<MOM, PM_BF16_MASTER>(gbf, grid, s, a);
+  else launch_adam_as<MOM, PM_BF16_SR>(gbf, grid, s, a);
+}
+
+// one launch for every ADAM_TENSORS tensors; `values`: their moments' values instead of a step
+int launch_adam(const GlAdamManyArgs* a, bool values, hipStream_t s) {
+  AdamTable k{};
+  k.lr = (float)a->lr;
+  k.b1 = (float)a->beta1;
+  k.b2 = (float)a->beta2;
+  k.eps = (float)a->eps;
+  k.wd = (float)a->weight_decay;
+  k.clear = a->clear;
+  k.b1d = a->beta1;
+  k.a1d = 1.0 - a->beta1;
+  k.b2d = a->beta2;
+  k.a2d = 1.0 - a->beta2;
+  constexpr long long MAX_GROUPS = 1LL << 23;  // of a launch: fewer than 2^32 threads
+  int next = 0;
+  while (next < a->count) {
+    long long groups = 0;
+    k.count = 0;
+    while (next < a->count && k.count < ADAM_TENSORS) {
+      const GlAdamTensor& t = a->t[next];
+      const long long need = (t.n + ADAM_CHUNK - 1) / ADAM_CHUNK;
+      if (groups + need > MAX_GROUPS) break;  // (a tensor has at most MAX_GROUPS: check_adam)
+      ++next;
+      if (need == 0) continue;
+      k.first[k.count] = (unsigned)groups;
+      k.t[k.count++] = AdamTensorK{t.p, t.g, t.m, t.v, t.master, t.m_scale, t.v_scale, (long long)t.n,
+                                   (unsigned long long)t.seed, t.bc1, t.bc2};
+      groups += need;
+    }
+    if (groups == 0) continue;
+    k.first[k.count] = (unsigned)groups;
+    const dim3 grid((unsigned)groups);
+    if (values) {
+      GL_LAUNCH(GL_KERNEL_ADAM_VALUES, adam_values_kernel, grid, dim3(256), 0, s, k);
+    } else {
+      const AdamTensorK& t = k.t[0];
+      const int pm = a->p_dtype == GL_DTYPE_F32 ? PM_F32 : (t.master ? PM_BF16_MASTER : (a->stochastic ? PM_BF16_SR : PM_BF16_RNE));
+      const bool gbf = a->g_dtype == GL_DTYPE_BF16;
+      if (a->moments_dtype == GL_DTYPE_F32) launch_adam_of<GL_DTYPE_F32>(pm, gbf, grid, s, k);
+      else if (a->moments_dtype == GL_DTYPE_BF16) launch_adam_of<GL_DTYPE_BF16>(pm, gbf, grid, s, k);
+      else launch_adam_of<GL_MOMENTS_INT8>(pm, gbf, grid, s, k);
+    }
+    GL_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+int check_adam(const GlAdamManyArgs* a, bool values) {
+  if (!a || a->count < 0 || (a->count > 0 && !a->t)) return GL_ERR_ARG;
+  if (a->moments_dtype != GL_DTYPE_F32 && a->moments_dtype != GL_DTYPE_BF16 && a->moments_dtype != GL_MOMENTS_INT8)
+    return GL_ERR_UNSUPPORTED;
+  const bool i8 = a->moments_dtype == GL_MOMENTS_INT8;
+  if (values && !i8) return GL_ERR_ARG;
+  if (!values) {
+    if ((a->p_dtype != GL_DTYPE_F32 && a->p_dtype != GL_DTYPE_BF16) || (a->g_dtype != GL_DTYPE_F32 && a->g_dtype != GL_DTYPE_BF16))
+      return GL_ERR_UNSUPPORTED;
+    if (a->clear && a->g_dtype != GL_DTYPE_F32) return GL_ERR_ARG;
+    if (a->p_dtype == GL_DTYPE_F32 && a->stochastic) return GL_ERR_ARG;  // fp32 parameters round nothing
+  }
+  const uintptr_t pe = values || a->p_dtype == GL_DTYPE_F32 ? 3 : 1, ge = values || a->g_dtype == GL_DTYPE_F32 ? 3 : 1;
+  const uintptr_t me = i8 ? 0 : (a->moments_dtype == GL_DTYPE_F32 ? 3 : 1);
+  const bool master = a->count > 0 && a->t[0].master;
+  for (int i = 0; i < a->count; ++i) {
+    const GlAdamTensor& t = a->t[i];
+    if (t.n < 0) return GL_ERR_ARG;
+    if (t.n == 0) continue;
+    if (t.n > GL_ADAM_MAX_ELEMENTS) return GL_ERR_UNSUPPORTED;
+    if (!t.p || !t.g || !t.m || !t.v || (i8 && (!t.m_scale || !t.v_scale))) return GL_ERR_ARG;
+    if (!values && ((t.master != nullptr) != master || (master && a->p_dtype == GL_DTYPE_F32))) return GL_ERR_ARG;
+    if (((uintptr_t)t.p & pe) || ((uintptr_t)t.g & ge) || (((uintptr_t)t.m | (uintptr_t)t.v) & me) ||
+        (((uintptr_t)t.master | (uintptr_t)t.m_scale | (uintptr_t)t.v_scale) & 3))
+      return GL_ERR_ARG;
+  }
   return 0;
 }
 
 }  // namespace gl
 
 using namespace gl;
+
+extern "C" int gl_adam_many(const GlAdamManyArgs* a, void* stream) {
+  GL_TRY(check_adam(a, false));
+  return launch_adam(a, false, (hipStream_t)stream);
+}
+
+extern "C" int gl_adam_values(const GlAdamManyArgs* a, void* stream) {
+  GL_TRY(check_adam(a, true));
+  return launch_adam(a, true, (hipStream_t)stream);
+}
 
 extern "C" int gl_adam(const GlAdamArgs* a, void* stream) {
   if (!a || a->n < 0) return GL_ERR_ARG;
@@ -201,19 +480,14 @@ extern "C" int gl_adam(const GlAdamArgs* a, void* stream) {
   if (a->moments_dtype != GL_DTYPE_F32 && a->moments_dtype != GL_DTYPE_BF16) return GL_ERR_UNSUPPORTED;
   if (a->p_dtype != GL_DTYPE_F32 && a->p_dtype != GL_DTYPE_BF16) return GL_ERR_UNSUPPORTED;
   if (a->p_dtype == GL_DTYPE_F32 && (a->master || a->stochastic)) return GL_ERR_ARG;  // fp32 parameters round nothing
-  const int pm = a->p_dtype == GL_DTYPE_F32 ? PM_F32 : (a->master ? PM_BF16_MASTER : (a->stochastic ? PM_BF16_SR : PM_BF16_RNE));
-  // vector path: 16-byte fp32 streams (g, fp32 p, master), 8-byte bf16 streams (bf16 p, bf16 moments)
-  const uintptr_t a16 = (uintptr_t)a->g | (pm == PM_F32 ? (uintptr_t)a->p : 0) | (uintptr_t)a->master;
-  const uintptr_t a8 = (pm == PM_F32 ? 0 : (uintptr_t)a->p);
+  const bool f32p = a->p_dtype == GL_DTYPE_F32;
+  // this entry point's tensors are at whole vectors: 16-byte fp32 streams, 8-byte bf16 streams
+  const uintptr_t a16 = (uintptr_t)a->g | (f32p ? (uintptr_t)a->p : 0) | (uintptr_t)a->master;
+  const uintptr_t a8 = f32p ? 0 : (uintptr_t)a->p;
   const uintptr_t alm = (uintptr_t)a->m | (uintptr_t)a->v;
   if ((a16 & 15) || (a8 & 7) || (alm & (a->moments_dtype == GL_DTYPE_F32 ? 15 : 7))) return GL_ERR_ARG;
-  AdamK c{a->lr, a->beta1, a->beta2, a->eps, a->weight_decay, a->bc1, a->bc2};
-  hipStream_t s = (hipStream_t)stream;
-  // one vector per thread (a grid-stride loop covers grids past the launch limit)
-  long long n4 = a->n >> 2;
-  long long blocks = (n4 + 255) / 256;
-  if (blocks > (1LL << 30)) blocks = 1LL << 30;
-  if (blocks < 1) blocks = 1;
-  const dim3 grid((unsigned)blocks);
-  return a->moments_dtype == GL_DTYPE_F32 ? launch_adam<false>(pm, grid, s, a, c) : launch_adam<true>(pm, grid, s, a, c);
+  const GlAdamTensor t{a->p, a->g, a->m, a->v, a->master, nullptr, nullptr, a->n, a->seed, a->bc1, a->bc2};
+  const GlAdamManyArgs k{&t, 1, a->p_dtype, GL_DTYPE_F32, a->moments_dtype, a->master ? 0 : a->stochastic, 1,
+                         a->lr, a->beta1, a->beta2, a->eps, a->weight_decay};
+  return gl_adam_many(&k, stream);
 }

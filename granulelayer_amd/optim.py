@@ -1,32 +1,46 @@
 """Fused AdamW for the layer parameters, mirroring sparse_pooling/optim.py (FusedAdamW).
 
-Reads the fp32 ``main_grad`` buffers written by the fused backward (or ``.grad``), updates the
-parameters and zeroes the gradient in the same streaming pass (the HIP kernel gl_adam).
+Reads the fp32 ``main_grad`` buffers written by the fused backward (zeroed in the same streaming pass) or
+``.grad`` in its own type, and updates the tensors of a parameter group together: a launch of the HIP kernel
+takes 40 of them (gl_adam_many).
 Semantics are dense AdamW for every element (optim.py:1-15): m = b1 m + (1-b1) g,
 v = b2 v + (1-b2) g^2, p = p (1 - lr wd) - lr (m / bc1) / (sqrt(v / bc2) + eps), bc_i = 1 - b_i^t.
 
-Moments are fp32 (``moments="fp32"``) or bf16 (``"bf16"``, the reference default).  Parameters
-are fp32, or bf16 with the reference's three variants (optim.py:5-9, 52-62): an fp32 master copy
+Moments are fp32 (``moments="fp32"``), bf16 (``"bf16"``, the reference default) or 8 bits (``"int8"``, no
+counterpart in the reference): blocks of 256 neighbouring elements of a tensor share two fp32 scales,
+
+    m = s c |c|       c from -127 to 127    s = max |m| / 127^2
+    v = (r c^2)^2     c from 0 to 255       r = sqrt(max v) / 255^2
+
+with c the nearest by its root and 1 at least where v > 0.  A step takes the new moments before they are put
+into 8 bits; a block with an infinity or a NaN in its moments is NaN from then on.  The state of a parameter has codes
+``m`` (int8) and ``v`` (uint8) and scales ``m_scale`` and ``v_scale``; ``moment_values`` gives what they stand for.
+
+Parameters are fp32, or bf16 with the reference's three variants (optim.py:5-9, 52-62): an fp32 master copy
 in the optimizer state (``master_weights=True``; the update runs on it and the parameter gets its
 nearest-even rounding), stochastic rounding (the default without masters: noise from Triton's
-``tl.randint(seed, element)`` below the bf16 cut, the seed counting launches as the reference's
+``tl.randint(seed, element)`` below the bf16 cut, the seed counting tensors as the reference's
 ``_seed`` does), or nearest-even rounding (``stochastic_rounding=False``).
 """
 from __future__ import annotations
 
-from typing import Iterable
+from typing import Iterable, List, Tuple
 
 import torch
 
 from .backend import backend_for
+
+_MOMENTS = {"bf16": torch.bfloat16, "fp32": torch.float32, "int8": torch.int8}
+_TYPES = (torch.float32, torch.bfloat16)
+_BLOCK = 256  # elements of a tensor that share the scales of 8-bit moments
 
 
 class FusedAdamW(torch.optim.Optimizer):
     def __init__(self, params: Iterable[torch.nn.Parameter], lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
                  weight_decay=0.0, moments: str = "bf16", master_weights: bool = False,
                  stochastic_rounding: bool = True):
-        if moments not in ("bf16", "fp32"):
-            raise ValueError("moments must be 'bf16' or 'fp32'")
+        if moments not in _MOMENTS:
+            raise ValueError("moments must be 'bf16', 'fp32' or 'int8'")
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
         self.moments = moments
@@ -42,38 +56,135 @@ class FusedAdamW(torch.optim.Optimizer):
                     n += t.numel() * t.element_size()
         return n
 
+    def load_state_dict(self, state_dict):
+        """As torch's, but every tensor of the state keeps its own type (torch's casts it to the parameter's)."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            for key, value in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(value):
+                    self.state[p][key] = value.detach().to(p.device, copy=True)
+
+    def _new_state(self, p):
+        st = dict(step=0)
+        if self.moments == "int8":
+            st["m"] = torch.zeros(p.shape, device=p.device, dtype=torch.int8)
+            st["v"] = torch.zeros(p.shape, device=p.device, dtype=torch.uint8)
+            for key in ("m_scale", "v_scale"):
+                st[key] = torch.zeros(-(-p.numel() // _BLOCK), device=p.device)
+        else:
+            for key in ("m", "v"):
+                st[key] = torch.zeros(p.shape, device=p.device, dtype=_MOMENTS[self.moments])
+        if self.master_weights and p.dtype != torch.float32:
+            st["master"] = p.detach().float().clone()
+        return st
+
+    @staticmethod
+    def _check_state(p, st):
+        """The moments' type; raises where the state does not fit the parameter."""
+        m, v, master = st["m"], st["v"], st.get("master")
+        if m.dtype not in _MOMENTS.values() or v.dtype != (torch.uint8 if m.dtype == torch.int8 else m.dtype):
+            raise TypeError(f"moments must both be float32, both bfloat16, or codes in int8 and uint8 (got {m.dtype}, {v.dtype})")
+        of = [(m, p.numel()), (v, p.numel())]
+        if m.dtype == torch.int8:
+            for key in ("m_scale", "v_scale"):
+                if st[key].dtype != torch.float32:
+                    raise TypeError(f"{key} must be float32 (got {st[key].dtype})")
+                of.append((st[key], -(-p.numel() // _BLOCK)))
+        if master is not None:
+            if p.dtype != torch.bfloat16 or master.dtype != torch.float32:
+                raise TypeError("master must be a float32 copy of a bfloat16 parameter")
+            of.append((master, p.numel()))
+        for t, n in of:
+            if t.numel() != n or t.get_device() != p.get_device() or not t.is_contiguous():
+                raise ValueError("the optimizer state must be contiguous tensors of the parameter's size and device")
+        return m.dtype
+
+    def _gradient(self, p):
+        """(gradient, whether it is a main_grad) as the kernel reads it, or None."""
+        g = getattr(p, "main_grad", None)
+        main = g is not None
+        if not main:
+            g = p.grad
+            if g is None:
+                return None
+        if p.dtype not in _TYPES:
+            raise NotImplementedError(f"FusedAdamW updates fp32 or bf16 parameters (got {p.dtype})")
+        if not p.is_contiguous():
+            raise ValueError("FusedAdamW needs contiguous parameters and gradients")
+        if main:
+            if not g.is_contiguous():
+                raise ValueError("FusedAdamW needs contiguous parameters and gradients")
+            if g.dtype != torch.float32:
+                raise TypeError("grad must be a contiguous float32 tensor")
+        else:
+            if g.dtype not in _TYPES:
+                g = g.float()
+            g = g.resolve_neg().contiguous()
+        if g.numel() != p.numel() or g.get_device() != p.get_device():
+            raise ValueError("param and grad must have the same number of elements and be on one device")
+        return g, main
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        mdt = torch.bfloat16 if self.moments == "bf16" else torch.float32
         for group in self.param_groups:
-            b1, b2 = group["betas"]
-            for p in group["params"]:
-                g = getattr(p, "main_grad", None)
-                if g is None:
-                    if p.grad is None:
-                        continue
-                    g = p.grad.float().contiguous()
-                if p.dtype not in (torch.float32, torch.bfloat16):
-                    raise NotImplementedError(f"FusedAdamW updates fp32 or bf16 parameters (got {p.dtype})")
-                if not p.is_contiguous() or not g.is_contiguous():
-                    raise ValueError("FusedAdamW needs contiguous parameters and gradients")
-                st = self.state[p]
-                if not st:
-                    st["step"] = 0
-                    st["m"] = torch.zeros(p.shape, device=p.device, dtype=mdt)
-                    st["v"] = torch.zeros(p.shape, device=p.device, dtype=mdt)
-                    if self.master_weights and p.dtype != torch.float32:
-                        st["master"] = p.detach().float().clone()
-                st["step"] += 1
-                t = st["step"]
-                self._seed += 1
-                backend_for(p.device).adam(p, g, st["m"], st["v"], group["lr"], b1, b2, group["eps"],
-                                           group["weight_decay"], 1 - b1 ** t, 1 - b2 ** t, master=st.get("master"),
-                                           stochastic=self.stochastic_rounding, seed=self._seed)
-                if getattr(p, "main_grad", None) is None:
-                    p.grad = None
+            self._step_group(group)
         return loss
+
+    def _step_group(self, group):
+        b1, b2 = group["betas"]
+        calls, keep, corrections = {}, [], {}
+        todo = [(p, got) for p in group["params"] if (got := self._gradient(p)) is not None]
+        for p, (g, main) in todo:
+            backend_for(p.device)
+            st = self.state[p]
+            if not st:
+                st.update(self._new_state(p))
+            mdt = self._check_state(p, st)
+            master = st.get("master")
+            t = st["step"] + 1
+            if t not in corrections:
+                corrections[t] = (1 - b1 ** t, 1 - b2 ** t)
+            i8 = mdt == torch.int8
+            self._seed += 1
+            keep.append((st, t))
+            calls.setdefault((p.device, p.dtype, g.dtype, mdt, main, master is not None), []).append(
+                (p.data_ptr(), g.data_ptr(), st["m"].data_ptr(), st["v"].data_ptr(),
+                 0 if master is None else master.data_ptr(), st["m_scale"].data_ptr() if i8 else 0,
+                 st["v_scale"].data_ptr() if i8 else 0, p.numel(), self._seed & (2**64 - 1), *corrections[t]))
+        for (dev, pdt, gdt, mdt, main, master), rows in calls.items():
+            backend_for(dev).adam_many(dev, rows, pdt, gdt, mdt, group["lr"], b1, b2, group["eps"], group["weight_decay"],
+                                       stochastic=self.stochastic_rounding and pdt == torch.bfloat16 and not master,
+                                       clear=main)
+        for st, t in keep:
+            st["step"] = t
+        for p, (g, main) in todo:
+            if not main:
+                p.grad = None
+
+    @torch.no_grad()
+    def moment_values(self) -> List[Tuple[torch.Tensor, torch.Tensor]]:
+        """fp32 copies of the moments (m, v), of the parameters' shapes, in the order of the parameters that have
+        made a step."""
+        out, calls = [], {}
+        for group in self.param_groups:
+            for p in group["params"]:
+                st = self.state.get(p)
+                if not st:
+                    continue
+                if self._check_state(p, st) != torch.int8:
+                    out.append((st["m"].to(torch.float32, copy=True), st["v"].to(torch.float32, copy=True)))
+                    continue
+                m, v = (torch.empty(p.shape, device=p.device) for _ in range(2))
+                out.append((m, v))
+                calls.setdefault(p.device, []).append(
+                    (v.data_ptr(), m.data_ptr(), st["m"].data_ptr(), st["v"].data_ptr(), 0, st["m_scale"].data_ptr(),
+                     st["v_scale"].data_ptr(), p.numel(), 0, 1.0, 1.0))
+        for dev, rows in calls.items():
+            backend_for(dev).adam_values(dev, rows)
+        return out

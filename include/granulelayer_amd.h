@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define GL_ABI_VERSION 14
+#define GL_ABI_VERSION 15
 
 enum {
   GL_OK = 0,
@@ -224,8 +224,9 @@ int gl_cover_select(const GlCoverArgs* a, void* stream);
 /* ABI identity: version and struct layouts (sizeof, then every field offset in declaration
  * order) so a binding can refuse a mismatched library.  Replaces sp_abi_version /
  * sp_struct_layout (sparse_pooling/kernels/cuda/abi.cu:17-62, checked in runtime.py:103-120).
- * which: 0 GlFwdArgs, 1 GlBwdArgs, 2 GlEdgeArgs, 3 GlAdamArgs, 4 GlCoverArgs.  Returns the number of values
- * written (or needed, when n is too small), negative on an unknown struct. */
+ * which: 0 GlFwdArgs, 1 GlBwdArgs, 2 GlEdgeArgs, 3 GlAdamArgs, 4 GlCoverArgs, 5 GlPack8Args, 6 GlDenseArgs,
+ * 7 GlDenseBwdArgs, 8 GlAdamTensor, 9 GlAdamManyArgs.  Returns the number of values written
+ * (or needed, when n is too small), negative on an unknown struct. */
 int gl_abi_version(void);
 int gl_struct_layout(int which, long long* out, int n);
 const char* gl_error_string(int code);
@@ -264,6 +265,39 @@ int gl_bwd(const GlBwdArgs* a, void* stream);
 
 /* Fused AdamW (in place). */
 int gl_adam(const GlAdamArgs* a, void* stream);
+
+/* The same step over many tensors: a launch takes 40 of them, which travel as its arguments, so nothing is
+ * copied to the device and `t` may go when the call returns.  No address needs more than its element's
+ * alignment.  Moments of GL_MOMENTS_INT8 are codes of one byte, m's signed, with two fp32 scales for every
+ * 256 neighbouring elements (the last block of a tensor may be shorter):
+ *   m = m_scale c |c|,  m_scale = max |m| / 127^2;   v = (v_scale c^2)^2,  v_scale = sqrt(max v) / 255^2
+ * with the maxima rounded to fp32, c the nearest by its root, 1 at least where v > 0. */
+#define GL_MOMENTS_INT8 2
+#define GL_ADAM_MAX_ELEMENTS (1LL << 35) /* of a tensor */
+typedef struct GlAdamTensor {
+  void* p;                /* [n] of p_dtype */
+  void* g;                /* [n] of g_dtype */
+  void* m;                /* [n] of moments_dtype */
+  void* v;
+  float* master;          /* as GlAdamArgs.master: all tensors of a call, or none */
+  float* m_scale;         /* [ceil(n / 256)] of 8-bit moments */
+  float* v_scale;
+  int64_t n;
+  uint64_t seed;          /* as GlAdamArgs.seed */
+  float bc1, bc2;
+} GlAdamTensor;
+typedef struct GlAdamManyArgs {
+  const GlAdamTensor* t;  /* in host memory */
+  int32_t count;
+  int32_t p_dtype, g_dtype; /* GL_DTYPE_F32 | GL_DTYPE_BF16 */
+  int32_t moments_dtype;  /* GL_DTYPE_F32 | GL_DTYPE_BF16 | GL_MOMENTS_INT8 */
+  int32_t stochastic;     /* as GlAdamArgs.stochastic */
+  int32_t clear;          /* 1: fp32 gradients are zeroed */
+  double lr, beta1, beta2, eps, weight_decay;
+} GlAdamManyArgs;
+int gl_adam_many(const GlAdamManyArgs* a, void* stream);
+/* The fp32 values that 8-bit moments stand for: m's into g, v's into p (both [n] fp32). */
+int gl_adam_values(const GlAdamManyArgs* a, void* stream);
 
 /* Gather schedule of the forward and dW kernels (K = 8 only), built on the HOST once per index
  * tensor from host copies of idx [G*S, 8] and counts [G] (rec_shift 0); upload the result and pass it as
@@ -392,7 +426,8 @@ enum {
   GL_KERNEL_DENSE = 20, GL_KERNEL_DENSE_FEW = 21,      /* dense products: tiled; few rows */
   GL_KERNEL_DENSE_JOIN = 22,                           /* sums of a split product, with its epilogue */
   GL_KERNEL_DENSE_DZ = 23, GL_KERNEL_DENSE_DB = 24,    /* dz and the partial sums of db; their sum */
-  GL_KERNEL_DENSE_ALIGN = 25                           /* operands copied to 16-byte rows */
+  GL_KERNEL_DENSE_ALIGN = 25,                          /* operands copied to 16-byte rows */
+  GL_KERNEL_ADAM_VALUES = 26                           /* 8-bit moments to fp32 */
 };
 
 /* Launch trace for benchmarks and tests (process-wide, not for concurrent callers): after
