@@ -18,6 +18,7 @@
 // the scale NaN; one whose largest |m| is below 2^-100 (v: 2^-126) the scale 0.
 #include "gl_common.h"
 #include "gl_internal.h"
+#include "gl_pack8.h"
 
 namespace gl {
 
@@ -28,7 +29,7 @@ struct AdamK {
 // The tensors of a launch travel as kernel arguments: nothing to copy to the device, nothing to keep alive.
 constexpr int ADAM_TENSORS = 40;      // of a launch: 3.7 of the 4 KB that arguments may take
 constexpr int ADAM_BLOCK = 256;       // elements that share a scale
-constexpr int ADAM_CHUNK = 4096;      // elements of a workgroup: 4 vectors of 4 a thread
+constexpr int ADAM_CHUNK = 1024;      // elements of a workgroup: a vector of 4 a thread
 struct AdamTensorK {
   void* p;
   void* g;
@@ -50,24 +51,12 @@ struct AdamTable {
 };
 static_assert(sizeof(AdamTable) <= 4096, "kernel arguments");
 
-__device__ __forceinline__ float bf16_bits_to_f32(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
-__device__ __forceinline__ unsigned short f32_to_bf16_rne(float f) {
-  unsigned u = __float_as_uint(f);
-  if ((u & 0x7f800000u) == 0x7f800000u) return (unsigned short)((u | ((u & 0x007fffffu) ? 0x00400000u : 0u)) >> 16);
-  u += 0x7fffu + ((u >> 16) & 1u);
-  return (unsigned short)(u >> 16);
-}
-
-__device__ __forceinline__ void adam_param(const AdamK& c, float& p, float m, float v) {
-#pragma clang fp contract(off)
-  const float upd = (m / c.bc1) / (__builtin_sqrtf(v / c.bc2) + c.eps);
-  p = p * (1.0f - c.lr * c.wd) - c.lr * upd;
-}
 __device__ __forceinline__ void adam_elem(const AdamK& c, float& p, float g, float& m, float& v) {
 #pragma clang fp contract(off)
   m = c.b1 * m + (1.0f - c.b1) * g;
   v = c.b2 * v + (1.0f - c.b2) * g * g;
-  adam_param(c, p, m, v);
+  const float upd = (m / c.bc1) / (__builtin_sqrtf(v / c.bc2) + c.eps);
+  p = p * (1.0f - c.lr * c.wd) - c.lr * upd;
 }
 
 // Streams are read and written with non-temporal loads and stores (each element is touched once;
@@ -109,16 +98,14 @@ __device__ __forceinline__ void adam_store(float* p, long long i, int n, const f
       if (j < n) p[i + j] = v[j];
   }
 }
-__device__ __forceinline__ void adam_store(unsigned short* p, long long i, int n, const unsigned short (&v)[4]) {
+// four bf16 in two words
+__device__ __forceinline__ void adam_store(unsigned short* p, long long i, int n, unsigned lo, unsigned hi) {
   if (n >= 4) {
-    w2 w;
-    w[0] = (unsigned)v[0] | (unsigned)v[1] << 16;
-    w[1] = (unsigned)v[2] | (unsigned)v[3] << 16;
-    __builtin_nontemporal_store(w, reinterpret_cast<w2*>(p + i));
+    __builtin_nontemporal_store((w2){lo, hi}, reinterpret_cast<w2*>(p + i));
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (j < n) p[i + j] = v[j];
+      if (j < n) p[i + j] = (unsigned short)((j < 2 ? lo : hi) >> (16 * (j & 1)));
   }
 }
 __device__ __forceinline__ unsigned adam_load_codes(const void* p, long long i, int n) {
@@ -167,14 +154,8 @@ __device__ __forceinline__ unsigned philox_randint(unsigned long long seed, unsi
 }
 
 // the bf16 parameter of element i from its fp32 update p
-template <int PM>
-__device__ __forceinline__ unsigned short round_param(float p, unsigned long long seed, long long i) {
-  if constexpr (PM == PM_BF16_SR) {
-    const unsigned u = (__float_as_uint(p) + (philox_randint(seed, (unsigned long long)i) & 0xffffu)) & 0xffff0000u;
-    return (unsigned short)(u >> 16);
-  } else {
-    return f32_to_bf16_rne(p);
-  }
+__device__ __forceinline__ unsigned round_stochastic(float p, unsigned long long seed, long long i) {
+  return (__float_as_uint(p) + (philox_randint(seed, (unsigned long long)i) & 0xffffu)) >> 16;
 }
 
 // ---- 8-bit moments -----------------------------------------------------------------------------------
@@ -222,152 +203,130 @@ __device__ __forceinline__ double value_v(unsigned codes, int j, double r) {
   return t * t;
 }
 
-// MOM: GL_DTYPE_F32, GL_DTYPE_BF16 or GL_MOMENTS_INT8; GBF: bf16 gradients.  A workgroup takes a chunk of one
-// tensor; wave w the vectors of its w-th quarter, AHEAD of them in flight.  With 8-bit moments a wave's vector is a block.
+// the tensor of this workgroup
+__device__ __forceinline__ int adam_tensor(const AdamTable& a) {
+  int t = 0;
+  for (int step = 32; step > 0; step >>= 1)
+    if (t + step < a.count && a.first[t + step] <= blockIdx.x) t += step;
+  return t;
+}
+
+// MOM: GL_DTYPE_F32, GL_DTYPE_BF16 or GL_MOMENTS_INT8; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
+// thread one vector of each stream; with 8-bit moments a wave's vectors are a block.
 template <int MOM, int PM, bool GBF>
 __global__ void __launch_bounds__(256) adam_kernel(AdamTable a) {
   constexpr bool I8 = MOM == GL_MOMENTS_INT8, BM = MOM == GL_DTYPE_BF16;
-  constexpr int AHEAD = 2, VECS = ADAM_CHUNK / 1024;
-  int ti = 0;
-  for (int step = 32; step > 0; step >>= 1)
-    if (ti + step < a.count && a.first[ti + step] <= blockIdx.x) ti += step;
+  const int ti = adam_tensor(a);
   const AdamTensorK& t = a.t[ti];
   const AdamK c{a.lr, a.b1, a.b2, a.eps, a.wd, t.bc1, t.bc2};
   const int lane = threadIdx.x & 63;
-  const long long base = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + (threadIdx.x >> 6) * (VECS * 256);
-  const void* P = PM == PM_BF16_MASTER ? (const void*)t.master : t.p;
-  constexpr bool PBF = PM == PM_BF16_RNE || PM == PM_BF16_SR;
-#pragma unroll 1
-  for (int y = 0; y < VECS; y += AHEAD) {
-    float p[AHEAD][4], g[AHEAD][4], m[AHEAD][4], v[AHEAD][4];
-    unsigned cm[AHEAD], cv[AHEAD];
-    float sm[AHEAD], sv[AHEAD];
-    int there[AHEAD];
+  const long long block = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + (threadIdx.x >> 6) * 256, i = block + 4 * lane;
+  if (block >= t.n) return;  // of the whole wave
+  const int n = t.n - i > 4 ? 4 : (t.n - i < 0 ? 0 : (int)(t.n - i));
+  float p[4], g[4], m[4], v[4];
+  unsigned cm, cv;
+  float sm, sv;
+  adam_load<PM == PM_BF16_RNE || PM == PM_BF16_SR>(PM == PM_BF16_MASTER ? (const void*)t.master : t.p, i, n, p);
+  adam_load<GBF>(t.g, i, n, g);
+  if constexpr (I8) {
+    cm = adam_load_codes(t.m, i, n);
+    cv = adam_load_codes(t.v, i, n);
+    sm = t.m_scale[block / ADAM_BLOCK];
+    sv = t.v_scale[block / ADAM_BLOCK];
+    double dm[4], dv[4];
+    unsigned tm = 0, tv = 0;
 #pragma unroll
-    for (int x = 0; x < AHEAD; ++x) {
-      const long long block = base + (y + x) * 256, i = block + 4 * lane;
-      const long long left = t.n - i;
-      there[x] = left > 4 ? 4 : (left < 0 ? 0 : (int)left);
-      adam_load<PBF>(P, i, there[x], p[x]);
-      adam_load<GBF>(t.g, i, there[x], g[x]);
-      if constexpr (I8) {
-        cm[x] = adam_load_codes(t.m, i, there[x]);
-        cv[x] = adam_load_codes(t.v, i, there[x]);
-        sm[x] = sv[x] = 0.f;
-        if (block < t.n) {
-          sm[x] = t.m_scale[block / ADAM_BLOCK];
-          sv[x] = t.v_scale[block / ADAM_BLOCK];
-        }
-      } else {
-        adam_load<BM>(t.m, i, there[x], m[x]);
-        adam_load<BM>(t.v, i, there[x], v[x]);
+    for (int j = 0; j < 4; ++j) {
+      const double gj = (double)g[j];
+      dm[j] = __builtin_fma(a.b1d, value_m(cm, j, (double)sm), a.a1d * gj);
+      dv[j] = __builtin_fma(a.b2d, value_v(cv, j, (double)sv), a.a2d * (gj * gj));
+      if (j >= n) dm[j] = dv[j] = 0.0;  // behind the end a code of 0 is NaN too in a block without numbers
+      m[j] = (float)dm[j];
+      v[j] = (float)dv[j];
+      const unsigned bm = __float_as_uint(m[j]) & 0x7fffffffu, bv = __float_as_uint(v[j]) & 0x7fffffffu;
+      tm = tm > bm ? tm : bm;
+      tv = tv > bv ? tv : bv;
+    }
+    const float fs = scale_m(wave_umax(tm)), fr = scale_v(wave_umax(tv));
+    unsigned om = 0, ov = 0;
+    if (fs > 0.f) {
+      const double im = 1.0 / (double)fs;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int q = (int)code_m(__builtin_fabs(dm[j]) * im);
+        om |= ((unsigned)(dm[j] < 0.0 ? -q : q) & 255u) << (8 * j);
       }
     }
+    if (fr > 0.f) {
+      const double ir = 1.0 / (double)fr, iv = ir * ir;
 #pragma unroll
-    for (int x = 0; x < AHEAD; ++x) {
-      const long long block = base + (y + x) * 256, i = block + 4 * lane;
-      const int n = there[x];
-      if constexpr (I8) {
-        if (block >= t.n) break;  // of the whole wave
-        double dm[4], dv[4];
-        unsigned tm = 0, tv = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const double gj = (double)g[x][j];
-          dm[j] = __builtin_fma(a.b1d, value_m(cm[x], j, (double)sm[x]), a.a1d * gj);
-          dv[j] = __builtin_fma(a.b2d, value_v(cv[x], j, (double)sv[x]), a.a2d * (gj * gj));
-          if (j >= n) dm[j] = dv[j] = 0.0;  // behind the end a code of 0 is NaN too in a block without numbers
-          m[x][j] = (float)dm[j];
-          v[x][j] = (float)dv[j];
-          const unsigned bm = __float_as_uint(m[x][j]) & 0x7fffffffu, bv = __float_as_uint(v[x][j]) & 0x7fffffffu;
-          tm = tm > bm ? tm : bm;
-          tv = tv > bv ? tv : bv;
-        }
-        tm = wave_umax(tm);
-        tv = wave_umax(tv);
-        const float fs = scale_m(tm), fr = scale_v(tv);
-        unsigned om = 0, ov = 0;
-        if (fs > 0.f) {
-          const double im = 1.0 / (double)fs;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int q = (int)code_m(__builtin_fabs(dm[j]) * im);
-            om |= ((unsigned)(dm[j] < 0.0 ? -q : q) & 255u) << (8 * j);
-          }
-        }
-        if (fr > 0.f) {
-          const double ir = 1.0 / (double)fr, iv = ir * ir;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const unsigned u = code_v(dv[j] * iv);
-            ov |= (u == 0 && dv[j] > 0.0 ? 1u : u) << (8 * j);
-          }
-        }
-        adam_store_codes(t.m, i, n, om);
-        adam_store_codes(t.v, i, n, ov);
-        if (lane == 0) {
-          t.m_scale[block / ADAM_BLOCK] = fs;
-          t.v_scale[block / ADAM_BLOCK] = fr;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) adam_param(c, p[x][j], m[x][j], v[x][j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) adam_elem(c, p[x][j], g[x][j], m[x][j], v[x][j]);
-        if constexpr (BM) {
-          unsigned short om[4], ov[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            om[j] = f32_to_bf16_rne(m[x][j]);
-            ov[j] = f32_to_bf16_rne(v[x][j]);
-          }
-          adam_store((unsigned short*)t.m, i, n, om);
-          adam_store((unsigned short*)t.v, i, n, ov);
-        } else {
-          adam_store((float*)t.m, i, n, m[x]);
-          adam_store((float*)t.v, i, n, v[x]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const unsigned u = code_v(dv[j] * iv);
+        ov |= (u == 0 && dv[j] > 0.0 ? 1u : u) << (8 * j);
       }
-      if constexpr (!GBF) {
-        const float none[4] = {0.f, 0.f, 0.f, 0.f};
-        if (a.clear) adam_store((float*)t.g, i, n, none);
-      }
-      if constexpr (PM == PM_F32) {
-        adam_store((float*)t.p, i, n, p[x]);
-      } else {
-        if constexpr (PM == PM_BF16_MASTER) adam_store(t.master, i, n, p[x]);
-        unsigned short o[4];
+    }
+    adam_store_codes(t.m, i, n, om);
+    adam_store_codes(t.v, i, n, ov);
+    if (lane == 0) {
+      t.m_scale[block / ADAM_BLOCK] = fs;
+      t.v_scale[block / ADAM_BLOCK] = fr;
+    }
+    // the update by estimates of the root and the quotient, each within a last place
+    const float i1 = 1.f / c.bc1, i2 = __builtin_sqrtf(1.f / c.bc2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = round_param<PM>(p[x][j], t.seed, i + j);
-        adam_store((unsigned short*)t.p, i, n, o);
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[j]), i2, c.eps);
+      p[j] = __builtin_fmaf(-c.lr, m[j] * i1 * __builtin_amdgcn_rcpf(d), p[j] * (1.f - c.lr * c.wd));
+    }
+  } else {
+    adam_load<BM>(t.m, i, n, m);
+    adam_load<BM>(t.v, i, n, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) adam_elem(c, p[j], g[j], m[j], v[j]);
+    if constexpr (BM) {
+      adam_store((unsigned short*)t.m, i, n, to_bf16x2(m[0], m[1]), to_bf16x2(m[2], m[3]));
+      adam_store((unsigned short*)t.v, i, n, to_bf16x2(v[0], v[1]), to_bf16x2(v[2], v[3]));
+    } else {
+      adam_store((float*)t.m, i, n, m);
+      adam_store((float*)t.v, i, n, v);
+    }
+  }
+  if constexpr (!GBF) {
+    const float none[4] = {0.f, 0.f, 0.f, 0.f};
+    if (a.clear) adam_store((float*)t.g, i, n, none);
+  }
+  if constexpr (PM == PM_F32) {
+    adam_store((float*)t.p, i, n, p);
+  } else {
+    if constexpr (PM == PM_BF16_MASTER) adam_store(t.master, i, n, p);
+    if constexpr (PM == PM_BF16_SR) {
+      unsigned o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = round_stochastic(p[j], t.seed, i + j);
+      adam_store((unsigned short*)t.p, i, n, o[0] | o[1] << 16, o[2] | o[3] << 16);
+    } else {
+      adam_store((unsigned short*)t.p, i, n, to_bf16x2(p[0], p[1]), to_bf16x2(p[2], p[3]));
     }
   }
 }
 
 // The fp32 values of 8-bit moments (into g: m's, into p: v's).
 __global__ void __launch_bounds__(256) adam_values_kernel(AdamTable a) {
-  int ti = 0;
-  for (int step = 32; step > 0; step >>= 1)
-    if (ti + step < a.count && a.first[ti + step] <= blockIdx.x) ti += step;
+  const int ti = adam_tensor(a);
   const AdamTensorK& t = a.t[ti];
-  const long long base = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + threadIdx.x * 4;
+  const long long i = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + threadIdx.x * 4;
+  if (i >= t.n) return;
+  const int n = t.n - i > 4 ? 4 : (int)(t.n - i);
+  const unsigned cm = adam_load_codes(t.m, i, n), cv = adam_load_codes(t.v, i, n);
+  const double sm = (double)t.m_scale[i / ADAM_BLOCK], sv = (double)t.v_scale[i / ADAM_BLOCK];
+  float m[4], v[4];
 #pragma unroll
-  for (int x = 0; x < ADAM_CHUNK / 1024; ++x) {
-    const long long i = base + x * 1024, left = t.n - i;
-    if (left <= 0) return;
-    const int n = left > 4 ? 4 : (int)left;
-    const unsigned cm = adam_load_codes(t.m, i, n), cv = adam_load_codes(t.v, i, n);
-    const double sm = (double)t.m_scale[i / ADAM_BLOCK], sv = (double)t.v_scale[i / ADAM_BLOCK];
-    float m[4], v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      m[j] = (float)value_m(cm, j, sm);
-      v[j] = (float)value_v(cv, j, sv);
-    }
-    adam_store((float*)t.g, i, n, m);
-    adam_store((float*)t.p, i, n, v);
+  for (int j = 0; j < 4; ++j) {
+    m[j] = (float)value_m(cm, j, sm);
+    v[j] = (float)value_v(cv, j, sv);
   }
+  adam_store((float*)t.g, i, n, m);
+  adam_store((float*)t.p, i, n, v);
 }
 
 template <int MOM, int PM>

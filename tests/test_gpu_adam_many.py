@@ -149,10 +149,11 @@ class Reference8:
             upd = (m / (1 - b1 ** t)) / (np.sqrt(v / (1 - b2 ** t)) + HP["eps"])
             self.state = _encode(m, v)
             p = p_from.astype(np.float64) * (1 - lr * HP["weight_decay"]) - lr * upd
-        # p: its product with 1 - lr wd (itself off by a rounding of lr wd and one of the difference) and the last
-        # subtraction, half a step each: 4.  upd: m, v, two quotients, the root, the sum, the quotient, lr and its product,
-        # bc1 and bc2 as fp32, at most one each: 11
-        tol = 2.0 ** -24 * (4 * np.abs(p_from) + 11 * lr * np.abs(upd) + np.abs(p))
+        # In halves of a last place, 2^-24.  p: its product with 1 - lr wd (itself off by lr, wd, their product and the
+        # difference), 5, and the last sum, of p.  upd: m, v under a root, 1 / bc1 and 1 / bc2 (each as fp32 and its
+        # quotient; the second's root with half of them), lr and five products or sums, 12, and an estimated root and
+        # quotient of two each: 16
+        tol = 2.0 ** -24 * (5 * np.abs(p_from) + 16 * lr * np.abs(upd) + np.abs(p))
         return p, tol
 
 
