@@ -66,9 +66,9 @@ typedef unsigned w4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned w2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef unsigned w1 __attribute__((aligned(1)));
 
-// four neighbours from element i, of which the first n are there
+// four neighbours from element i of a wave's part p, of which the first n are there
 template <bool BF>
-__device__ __forceinline__ void adam_load(const void* p, long long i, int n, float (&v)[4]) {
+__device__ __forceinline__ void adam_load(const void* p, unsigned i, int n, float (&v)[4]) {
   if (n >= 4) {
     if constexpr (BF) {
       const w2 w = __builtin_nontemporal_load(reinterpret_cast<const w2*>((const char*)p + 2 * i));
@@ -86,7 +86,7 @@ __device__ __forceinline__ void adam_load(const void* p, long long i, int n, flo
     for (int j = 0; j < 4; ++j) v[j] = j < n ? ld_param_t<BF>((const float*)p, i + j) : 0.f;
   }
 }
-__device__ __forceinline__ void adam_store(float* p, long long i, int n, const float (&v)[4]) {
+__device__ __forceinline__ void adam_store(float* p, unsigned i, int n, const float (&v)[4]) {
   if (n >= 4) {
     w4 w;
 #pragma unroll
@@ -99,7 +99,7 @@ __device__ __forceinline__ void adam_store(float* p, long long i, int n, const f
   }
 }
 // four bf16 in two words
-__device__ __forceinline__ void adam_store(unsigned short* p, long long i, int n, unsigned lo, unsigned hi) {
+__device__ __forceinline__ void adam_store(unsigned short* p, unsigned i, int n, unsigned lo, unsigned hi) {
   if (n >= 4) {
     __builtin_nontemporal_store((w2){lo, hi}, reinterpret_cast<w2*>(p + i));
   } else {
@@ -108,7 +108,7 @@ __device__ __forceinline__ void adam_store(unsigned short* p, long long i, int n
       if (j < n) p[i + j] = (unsigned short)((j < 2 ? lo : hi) >> (16 * (j & 1)));
   }
 }
-__device__ __forceinline__ unsigned adam_load_codes(const void* p, long long i, int n) {
+__device__ __forceinline__ unsigned adam_load_codes(const void* p, unsigned i, int n) {
   const unsigned char* c = (const unsigned char*)p + i;
   if (n >= 4) return __builtin_nontemporal_load(reinterpret_cast<const w1*>(c));
   unsigned w = 0;
@@ -117,7 +117,7 @@ __device__ __forceinline__ unsigned adam_load_codes(const void* p, long long i, 
     if (j < n) w |= (unsigned)c[j] << (8 * j);
   return w;
 }
-__device__ __forceinline__ void adam_store_codes(void* p, long long i, int n, unsigned w) {
+__device__ __forceinline__ void adam_store_codes(void* p, unsigned i, int n, unsigned w) {
   unsigned char* c = (unsigned char*)p + i;
   if (n >= 4) {
     __builtin_nontemporal_store((w1)w, reinterpret_cast<w1*>(c));
@@ -171,6 +171,18 @@ __device__ __forceinline__ unsigned wave_umax(unsigned v) {
   const auto p32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return up(p32[0], p32[1]);
 }
+// 1 / x of a positive normal fp32 x to 2^-45, and sqrt(x) to about 2^-51: estimates of 2^-23 and one or two steps of Newton's
+__device__ __forceinline__ double reciprocal(float x) {
+  const double r = (double)__builtin_amdgcn_rcpf(x);
+  return __builtin_fma(r, __builtin_fma(-(double)x, r, 1.0), r);
+}
+__device__ __forceinline__ double root(float x) {
+  const float e = __builtin_amdgcn_sqrtf(x);
+  const double d = (double)x, h = 0.5 * (double)__builtin_amdgcn_rcpf(e);
+  double r = (double)e;
+  r = __builtin_fma(h, __builtin_fma(-r, r, d), r);
+  return __builtin_fma(h, __builtin_fma(-r, r, d), r);
+}
 // scales of a block from the bits of its largest fp32 |m| and v
 __device__ __forceinline__ float scale_m(unsigned top) {
   if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
@@ -178,10 +190,18 @@ __device__ __forceinline__ float scale_m(unsigned top) {
 }
 __device__ __forceinline__ float scale_v(unsigned top) {
   if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-  return top < 0x00800000u ? 0.f : (float)(__builtin_sqrt((double)__uint_as_float(top)) * (1.0 / 65025.0));
+  return top < 0x00800000u ? 0.f : (float)(root(__uint_as_float(top)) * (1.0 / 65025.0));
 }
-// floor(x + 1/2) of the root x of y >= 0: an estimate decides all but which side of i + 1/2 it is on, the square
-// (i + 1/2)^2, exact in 64 bits, decides that
+// Codes.  In fp32, where a root is within 6e-5 of its own: adding 1.5 x 2^23 rounds it to a whole number, which is left in
+// the low byte in two's complement, and `near` gathers how far roots are from whole numbers.  Where one is within
+// CODE_NEAR of a border between two codes (a wave in nine) all of the wave's are decided in 64 bits instead: of floor(x + 1/2),
+// x the root, an estimate decides all but which side of i + 1/2 x is on, and (i + 1/2)^2, exact in 64 bits, decides that.
+constexpr float CODE_NEAR = 0x1p-13f;
+__device__ __forceinline__ unsigned code_of(float x, float& near) {
+  const float r = x + 12582912.f;
+  near = __builtin_fmaxf(near, __builtin_fabsf(x - (r - 12582912.f)));
+  return __float_as_uint(r);
+}
 __device__ __forceinline__ unsigned code_m(double y) {
   const float i = __builtin_floorf(__builtin_amdgcn_sqrtf((float)y) + 0.25f), h = i + 0.5f;
   return (unsigned)i + (y >= (double)(h * h) ? 1u : 0u);
@@ -191,6 +211,9 @@ __device__ __forceinline__ unsigned code_v(double y) {
   const float i = __builtin_floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y)) + 0.25f), h = i + 0.5f;
   const double h2 = (double)(h * h);
   return (unsigned)i + (y >= h2 * h2 ? 1u : 0u);
+}
+__device__ __forceinline__ unsigned low_bytes(const unsigned (&c)[4]) {
+  return __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u) | __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
 }
 // values of codes
 __device__ __forceinline__ double value_m(unsigned codes, int j, double s) {
@@ -213,120 +236,125 @@ __device__ __forceinline__ int adam_tensor(const AdamTable& a) {
 
 // MOM: GL_DTYPE_F32, GL_DTYPE_BF16 or GL_MOMENTS_INT8; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
 // thread one vector of each stream; with 8-bit moments a wave's vectors are a block.
-template <int MOM, int PM, bool GBF>
-__global__ void __launch_bounds__(256) adam_kernel(AdamTable a) {
+// WHOLE: all of the wave's 256 elements are there (no lane's ends are looked at).
+template <int MOM, int PM, bool GBF, bool WHOLE>
+__device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensorK& t, long long block) {
   constexpr bool I8 = MOM == GL_MOMENTS_INT8, BM = MOM == GL_DTYPE_BF16;
-  const int ti = adam_tensor(a);
-  const AdamTensorK& t = a.t[ti];
   const AdamK c{a.lr, a.b1, a.b2, a.eps, a.wd, t.bc1, t.bc2};
-  const int lane = threadIdx.x & 63;
-  const long long block = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + (threadIdx.x >> 6) * 256, i = block + 4 * lane;
-  if (block >= t.n) return;  // of the whole wave
-  const int n = t.n - i > 4 ? 4 : (t.n - i < 0 ? 0 : (int)(t.n - i));
+  constexpr int PB = PM == PM_BF16_RNE || PM == PM_BF16_SR ? 2 : 4, MB = I8 ? 1 : (BM ? 2 : 4);
+  const unsigned i = 4 * (threadIdx.x & 63);
+  const int n = WHOLE || t.n - block - i > 4 ? 4 : (t.n - block < i ? 0 : (int)(t.n - block - i));
   float p[4], g[4], m[4], v[4];
-  unsigned cm, cv;
-  float sm, sv;
-  adam_load<PM == PM_BF16_RNE || PM == PM_BF16_SR>(PM == PM_BF16_MASTER ? (const void*)t.master : t.p, i, n, p);
-  adam_load<GBF>(t.g, i, n, g);
+  char* P = (PM == PM_BF16_MASTER ? (char*)t.master : (char*)t.p) + block * PB;
+  char* G = (char*)t.g + block * (GBF ? 2 : 4);
+  char* M = (char*)t.m + block * MB;
+  char* V = (char*)t.v + block * MB;
+  adam_load<PB == 2>(P, i, n, p);
+  adam_load<GBF>(G, i, n, g);
   if constexpr (I8) {
-    cm = adam_load_codes(t.m, i, n);
-    cv = adam_load_codes(t.v, i, n);
-    sm = t.m_scale[block / ADAM_BLOCK];
-    sv = t.v_scale[block / ADAM_BLOCK];
+    const unsigned cm = adam_load_codes(M, i, n), cv = adam_load_codes(V, i, n);
+    const double sm = (double)t.m_scale[block / ADAM_BLOCK], sv = (double)t.v_scale[block / ADAM_BLOCK];
+    // (behind the end: 0, and NaN in a block that is NaN anyway)
     double dm[4], dv[4];
     unsigned tm = 0, tv = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double gj = (double)g[j];
-      dm[j] = __builtin_fma(a.b1d, value_m(cm, j, (double)sm), a.a1d * gj);
-      dv[j] = __builtin_fma(a.b2d, value_v(cv, j, (double)sv), a.a2d * (gj * gj));
-      if (j >= n) dm[j] = dv[j] = 0.0;  // behind the end a code of 0 is NaN too in a block without numbers
+      dm[j] = __builtin_fma(a.b1d, value_m(cm, j, sm), a.a1d * gj);
+      dv[j] = __builtin_fma(a.b2d, value_v(cv, j, sv), a.a2d * (gj * gj));
       m[j] = (float)dm[j];
       v[j] = (float)dv[j];
-      const unsigned bm = __float_as_uint(m[j]) & 0x7fffffffu, bv = __float_as_uint(v[j]) & 0x7fffffffu;
-      tm = tm > bm ? tm : bm;
-      tv = tv > bv ? tv : bv;
+      tm = umax(tm, abs_bits(m[j]));
+      tv = umax(tv, __float_as_uint(v[j]));  // of v >= 0; a NaN is above every number with either sign
     }
     const float fs = scale_m(wave_umax(tm)), fr = scale_v(wave_umax(tv));
-    unsigned om = 0, ov = 0;
-    if (fs > 0.f) {
-      const double im = 1.0 / (double)fs;
+    const bool live_m = fs > 0.f, live_v = fr > 0.f;  // of the whole wave
+    const double im = reciprocal(live_m ? fs : 1.f), ir = reciprocal(live_v ? fr : 1.f);
+    const float imf = (float)im, irf = (float)ir;
+    unsigned om[4], ov[4];
+    float near = 0.f, rv[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      om[j] = code_of(__builtin_copysignf(__builtin_amdgcn_sqrtf(__builtin_fabsf(m[j]) * imf), m[j]), near);
+      rv[j] = __builtin_amdgcn_sqrtf(v[j] * irf * irf);
+      ov[j] = code_of(__builtin_fmaxf(__builtin_amdgcn_sqrtf(rv[j]), dv[j] > 0.0 ? 0.75f : 0.f), near);
+    }
+    if (__builtin_amdgcn_ballot_w64(near > 0.5f - CODE_NEAR)) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int q = (int)code_m(__builtin_fabs(dm[j]) * im);
-        om |= ((unsigned)(dm[j] < 0.0 ? -q : q) & 255u) << (8 * j);
+        const unsigned q = live_m ? code_m(__builtin_fabs(dm[j]) * im) : 0u, u = live_v ? code_v(dv[j] * ir * ir) : 0u;
+        om[j] = dm[j] < 0.0 ? 0u - q : q;
+        ov[j] = u == 0 && dv[j] > 0.0 ? 1u : u;
       }
     }
-    if (fr > 0.f) {
-      const double ir = 1.0 / (double)fr, iv = ir * ir;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned u = code_v(dv[j] * iv);
-        ov |= (u == 0 && dv[j] > 0.0 ? 1u : u) << (8 * j);
-      }
-    }
-    adam_store_codes(t.m, i, n, om);
-    adam_store_codes(t.v, i, n, ov);
-    if (lane == 0) {
+    adam_store_codes(M, i, n, live_m ? low_bytes(om) : 0u);
+    adam_store_codes(V, i, n, live_v ? low_bytes(ov) : 0u);
+    if (i == 0) {
       t.m_scale[block / ADAM_BLOCK] = fs;
       t.v_scale[block / ADAM_BLOCK] = fr;
     }
-    // the update by estimates of the root and the quotient, each within a last place
-    const float i1 = 1.f / c.bc1, i2 = __builtin_sqrtf(1.f / c.bc2);
+    // the update by the root that v's code has and an estimated quotient, within a few last places; bc1 and bc2 come as
+    // lr / bc1 and 1 / sqrt(bc2)
+    const float up = (live_v ? fr : 1.f) * c.bc2, keep = 1.f - c.lr * c.wd;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[j]), i2, c.eps);
-      p[j] = __builtin_fmaf(-c.lr, m[j] * i1 * __builtin_amdgcn_rcpf(d), p[j] * (1.f - c.lr * c.wd));
-    }
+    for (int j = 0; j < 4; ++j)
+      p[j] = __builtin_fmaf(-(m[j] * c.bc1), __builtin_amdgcn_rcpf(__builtin_fmaf(rv[j], up, c.eps)), p[j] * keep);
   } else {
-    adam_load<BM>(t.m, i, n, m);
-    adam_load<BM>(t.v, i, n, v);
+    adam_load<BM>(M, i, n, m);
+    adam_load<BM>(V, i, n, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) adam_elem(c, p[j], g[j], m[j], v[j]);
     if constexpr (BM) {
-      adam_store((unsigned short*)t.m, i, n, to_bf16x2(m[0], m[1]), to_bf16x2(m[2], m[3]));
-      adam_store((unsigned short*)t.v, i, n, to_bf16x2(v[0], v[1]), to_bf16x2(v[2], v[3]));
+      adam_store((unsigned short*)M, i, n, to_bf16x2(m[0], m[1]), to_bf16x2(m[2], m[3]));
+      adam_store((unsigned short*)V, i, n, to_bf16x2(v[0], v[1]), to_bf16x2(v[2], v[3]));
     } else {
-      adam_store((float*)t.m, i, n, m);
-      adam_store((float*)t.v, i, n, v);
+      adam_store((float*)M, i, n, m);
+      adam_store((float*)V, i, n, v);
     }
   }
   if constexpr (!GBF) {
     const float none[4] = {0.f, 0.f, 0.f, 0.f};
-    if (a.clear) adam_store((float*)t.g, i, n, none);
+    if (a.clear) adam_store((float*)G, i, n, none);
   }
-  if constexpr (PM == PM_F32) {
-    adam_store((float*)t.p, i, n, p);
-  } else {
-    if constexpr (PM == PM_BF16_MASTER) adam_store(t.master, i, n, p);
-    if constexpr (PM == PM_BF16_SR) {
-      unsigned o[4];
+  if constexpr (PM == PM_F32 || PM == PM_BF16_MASTER) adam_store((float*)P, i, n, p);
+  unsigned short* O = (unsigned short*)t.p + block;
+  if constexpr (PM == PM_BF16_SR) {
+    unsigned o[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = round_stochastic(p[j], t.seed, i + j);
-      adam_store((unsigned short*)t.p, i, n, o[0] | o[1] << 16, o[2] | o[3] << 16);
-    } else {
-      adam_store((unsigned short*)t.p, i, n, to_bf16x2(p[0], p[1]), to_bf16x2(p[2], p[3]));
-    }
+    for (int j = 0; j < 4; ++j) o[j] = round_stochastic(p[j], t.seed, block + i + j);
+    adam_store(O, i, n, o[0] | o[1] << 16, o[2] | o[3] << 16);
+  } else if constexpr (PM != PM_F32) {
+    adam_store(O, i, n, to_bf16x2(p[0], p[1]), to_bf16x2(p[2], p[3]));
   }
+}
+template <int MOM, int PM, bool GBF>
+__global__ void __launch_bounds__(256) adam_kernel(AdamTable a) {
+  const int ti = adam_tensor(a);
+  const AdamTensorK& t = a.t[ti];
+  const long long block = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + wave_uniform(threadIdx.x >> 6) * 256;
+  if (block + 256 <= t.n) adam_vector<MOM, PM, GBF, true>(a, t, block);
+  else if (block < t.n) adam_vector<MOM, PM, GBF, false>(a, t, block);
 }
 
 // The fp32 values of 8-bit moments (into g: m's, into p: v's).
 __global__ void __launch_bounds__(256) adam_values_kernel(AdamTable a) {
   const int ti = adam_tensor(a);
   const AdamTensorK& t = a.t[ti];
-  const long long i = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + threadIdx.x * 4;
-  if (i >= t.n) return;
-  const int n = t.n - i > 4 ? 4 : (int)(t.n - i);
-  const unsigned cm = adam_load_codes(t.m, i, n), cv = adam_load_codes(t.v, i, n);
-  const double sm = (double)t.m_scale[i / ADAM_BLOCK], sv = (double)t.v_scale[i / ADAM_BLOCK];
+  const long long block = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + wave_uniform(threadIdx.x >> 6) * 256;
+  const unsigned i = 4 * (threadIdx.x & 63);
+  const long long left = t.n - block - i;
+  if (left <= 0) return;
+  const int n = left > 4 ? 4 : (int)left;
+  const unsigned cm = adam_load_codes((char*)t.m + block, i, n), cv = adam_load_codes((char*)t.v + block, i, n);
+  const double sm = (double)t.m_scale[block / ADAM_BLOCK], sv = (double)t.v_scale[block / ADAM_BLOCK];
   float m[4], v[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     m[j] = (float)value_m(cm, j, sm);
     v[j] = (float)value_v(cv, j, sv);
   }
-  adam_store((float*)t.g, i, n, m);
-  adam_store((float*)t.p, i, n, v);
+  adam_store((float*)t.g + block, i, n, m);
+  adam_store((float*)t.p + block, i, n, v);
 }
 
 template <int MOM, int PM>
@@ -367,8 +395,12 @@ int launch_adam(const GlAdamManyArgs* a, bool values, hipStream_t s) {
       ++next;
       if (need == 0) continue;
       k.first[k.count] = (unsigned)groups;
-      k.t[k.count++] = AdamTensorK{t.p, t.g, t.m, t.v, t.master, t.m_scale, t.v_scale, (long long)t.n,
-                                   (unsigned long long)t.seed, t.bc1, t.bc2};
+      AdamTensorK& d = k.t[k.count++];
+      d = AdamTensorK{t.p, t.g, t.m, t.v, t.master, t.m_scale, t.v_scale, (long long)t.n, (unsigned long long)t.seed, t.bc1, t.bc2};
+      if (a->moments_dtype == GL_MOMENTS_INT8) {  // as that update takes them
+        d.bc1 = (float)(a->lr / t.bc1);
+        d.bc2 = (float)(1.0 / __builtin_sqrt((double)t.bc2));
+      }
       groups += need;
     }
     if (groups == 0) continue;
