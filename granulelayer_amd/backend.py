@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import struct
 import threading
 from typing import Dict, Optional
 
@@ -406,19 +407,18 @@ class HipBackend:
 
     def adam_many(self, device, rows, p_dtype, g_dtype, m_dtype, lr, beta1, beta2, eps, weight_decay, stochastic=False,
                   clear=False):
-        """In-place fused AdamW over the tensors of ``rows``, tuples in GlAdamTensor's order (addresses, elements,
-        seed, bias corrections); all of one dtype of parameters, gradients and moments (int8: codes), all with a
-        master or none."""
-        t = np.array(rows, dtype=_ADAM_TENSOR)
-        a = N.GlAdamManyArgs(t.ctypes.data, len(rows), _DENSE_DTYPES[p_dtype], _DENSE_DTYPES[g_dtype], _MOMENTS[m_dtype],
+        """In-place fused AdamW over the tensors of ``rows`` (``adam_row``); all of one dtype of parameters, gradients
+        and moments (int8: codes), all with a master or none."""
+        t = b"".join(rows)
+        a = N.GlAdamManyArgs(ctypes.cast(t, ctypes.c_void_p), len(rows), _DENSE_DTYPES[p_dtype], _DENSE_DTYPES[g_dtype], _MOMENTS[m_dtype],
                              int(stochastic), int(clear), lr, beta1, beta2, eps, weight_decay)
         with _on(device):
             self.lib.call("gl_adam_many", ctypes.byref(a), _stream(device))
 
     def adam_values(self, device, rows):
         """The fp32 values of 8-bit moments: ``rows`` as for ``adam_many``, with m's values going to g and v's to p."""
-        t = np.array(rows, dtype=_ADAM_TENSOR)
-        a = N.GlAdamManyArgs(t.ctypes.data, len(rows), 0, 0, N.GL_MOMENTS_INT8)
+        t = b"".join(rows)
+        a = N.GlAdamManyArgs(ctypes.cast(t, ctypes.c_void_p), len(rows), 0, 0, N.GL_MOMENTS_INT8)
         with _on(device):
             self.lib.call("gl_adam_values", ctypes.byref(a), _stream(device))
 
@@ -526,7 +526,10 @@ class HipBackend:
 
 _DENSE_DTYPES = {torch.float32: N.GL_DTYPE_F32, torch.bfloat16: N.GL_DTYPE_BF16}
 _MOMENTS = {**_DENSE_DTYPES, torch.int8: N.GL_MOMENTS_INT8}
-_ADAM_TENSOR = np.dtype(N.GlAdamTensor)
+# a GlAdamTensor as bytes: p, g, m, v, master, m_scale, v_scale, n, seed, bc1, bc2
+_ADAM_ROW = struct.Struct("7QqQ2f")
+assert _ADAM_ROW.size == ctypes.sizeof(N.GlAdamTensor)
+adam_row = _ADAM_ROW.pack
 
 
 def backend_for(device) -> HipBackend:

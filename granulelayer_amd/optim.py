@@ -28,7 +28,7 @@ from typing import Iterable, List, Tuple
 
 import torch
 
-from .backend import backend_for
+from .backend import adam_row as _ROW, backend_for
 
 _MOMENTS = {"bf16": torch.bfloat16, "fp32": torch.float32, "int8": torch.int8}
 _TYPES = (torch.float32, torch.bfloat16)
@@ -47,6 +47,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self.master_weights = master_weights
         self.stochastic_rounding = stochastic_rounding
         self._seed = 0
+        self._known, self._kinds = {}, {}
 
     def state_bytes(self) -> int:
         n = 0
@@ -59,6 +60,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As torch's, but every tensor of the state keeps its own type (torch's casts it to the parameter's)."""
         super().load_state_dict(state_dict)
+        self._known.clear()
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
@@ -101,30 +103,36 @@ class FusedAdamW(torch.optim.Optimizer):
                 raise ValueError("the optimizer state must be contiguous tensors of the parameter's size and device")
         return m.dtype
 
-    def _gradient(self, p):
-        """(gradient, whether it is a main_grad) as the kernel reads it, or None."""
-        g = getattr(p, "main_grad", None)
-        main = g is not None
-        if not main:
-            g = p.grad
-            if g is None:
-                return None
+    def _known_state(self, p, st):
+        """What a step needs of a parameter's state, checked: held for the next step, which looks whether the tensors
+        are still these and where they were."""
+        if not st:
+            st.update(self._new_state(p))
+        mdt = self._check_state(p, st)
+        backend = backend_for(p.device)
+        of = (st["m"], st["v"], st.get("master"), st.get("m_scale"), st.get("v_scale"))
+        rest = tuple(0 if t is None else t.data_ptr() for t in of[2:])
+        kind = (backend, p.device, p.dtype, mdt, of[2] is not None)
+        kind = self._kinds.setdefault(kind, kind)
+        known = (of, of[0].data_ptr(), of[1].data_ptr(), rest, p.numel(), p.dtype, p.get_device(), kind)
+        self._known[id(p)] = (p, known)  # (p is held, so that its id is its own)
+        return known
+
+    @staticmethod
+    def _gradient(p, g, main):
+        """g as the kernel reads it, checked."""
         if p.dtype not in _TYPES:
             raise NotImplementedError(f"FusedAdamW updates fp32 or bf16 parameters (got {p.dtype})")
-        if not p.is_contiguous():
+        if not p.is_contiguous() or (main and not g.is_contiguous()):
             raise ValueError("FusedAdamW needs contiguous parameters and gradients")
         if main:
-            if not g.is_contiguous():
-                raise ValueError("FusedAdamW needs contiguous parameters and gradients")
             if g.dtype != torch.float32:
                 raise TypeError("grad must be a contiguous float32 tensor")
         else:
-            if g.dtype not in _TYPES:
-                g = g.float()
-            g = g.resolve_neg().contiguous()
+            g = (g if g.dtype in _TYPES else g.float()).resolve_neg().contiguous()
         if g.numel() != p.numel() or g.get_device() != p.get_device():
             raise ValueError("param and grad must have the same number of elements and be on one device")
-        return g, main
+        return g
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -138,32 +146,53 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _step_group(self, group):
         b1, b2 = group["betas"]
-        calls, keep, corrections = {}, [], {}
-        todo = [(p, got) for p in group["params"] if (got := self._gradient(p)) is not None]
-        for p, (g, main) in todo:
-            backend_for(p.device)
-            st = self.state[p]
-            if not st:
-                st.update(self._new_state(p))
-            mdt = self._check_state(p, st)
-            master = st.get("master")
+        f32, bf16 = torch.float32, torch.bfloat16
+        todo = []
+        for p in group["params"]:  # everything is checked before anything changes
+            g = getattr(p, "main_grad", None)
+            main = g is not None
+            if not main:
+                g = p.grad
+                if g is None:
+                    continue
+            gdt = g.dtype
+            if (not (gdt is f32 or (gdt is bf16 and not main)) or not g.is_contiguous() or g.is_neg()
+                    or not p.is_contiguous() or not (p.dtype is f32 or p.dtype is bf16)
+                    or g.numel() != p.numel() or g.get_device() != p.get_device()):
+                g = self._gradient(p, g, main)
+                gdt = g.dtype
+            todo.append((p, g, gdt, main))
+        calls, states, corrections = {}, [], {}
+        state, known_of, seed, last = self.state, self._known, self._seed, (None, None, None)
+        for p, g, gdt, main in todo:
+            st = state[p]
+            known = known_of.get(id(p))
+            known = None if known is None else known[1]
+            if (known is None or not st or st["m"] is not known[0][0] or st["v"] is not known[0][1]
+                    or st.get("master") is not known[0][2] or st.get("m_scale") is not known[0][3]
+                    or st.get("v_scale") is not known[0][4] or known[0][0].data_ptr() != known[1]
+                    or known[0][1].data_ptr() != known[2] or p.numel() != known[4] or p.dtype is not known[5]
+                    or p.get_device() != known[6]):
+                known = self._known_state(p, st)
+            _, m, v, rest, n, _, _, kind = known
             t = st["step"] + 1
-            if t not in corrections:
-                corrections[t] = (1 - b1 ** t, 1 - b2 ** t)
-            i8 = mdt == torch.int8
-            self._seed += 1
-            keep.append((st, t))
-            calls.setdefault((p.device, p.dtype, g.dtype, mdt, main, master is not None), []).append(
-                (p.data_ptr(), g.data_ptr(), st["m"].data_ptr(), st["v"].data_ptr(),
-                 0 if master is None else master.data_ptr(), st["m_scale"].data_ptr() if i8 else 0,
-                 st["v_scale"].data_ptr() if i8 else 0, p.numel(), self._seed & (2**64 - 1), *corrections[t]))
-        for (dev, pdt, gdt, mdt, main, master), rows in calls.items():
-            backend_for(dev).adam_many(dev, rows, pdt, gdt, mdt, group["lr"], b1, b2, group["eps"], group["weight_decay"],
-                                       stochastic=self.stochastic_rounding and pdt == torch.bfloat16 and not master,
-                                       clear=main)
-        for st, t in keep:
-            st["step"] = t
-        for p, (g, main) in todo:
+            c = corrections.get(t)
+            if c is None:
+                c = corrections[t] = (1 - b1 ** t, 1 - b2 ** t)
+            seed += 1
+            states.append(st)
+            row = _ROW(p.data_ptr(), g.data_ptr(), m, v, *rest, n, seed & 0xffffffffffffffff, *c)
+            if kind is not last[0] or gdt is not last[1] or main is not last[2]:
+                last = (kind, gdt, main)
+                rows = calls.setdefault(last, [])
+            rows.append(row)
+        self._seed = seed
+        for ((backend, dev, pdt, mdt, has_master), gdt, main), rows in calls.items():
+            backend.adam_many(dev, rows, pdt, gdt, mdt, group["lr"], b1, b2, group["eps"], group["weight_decay"],
+                              stochastic=self.stochastic_rounding and pdt is bf16 and not has_master, clear=main)
+        for st in states:
+            st["step"] += 1
+        for p, _, _, main in todo:
             if not main:
                 p.grad = None
 
@@ -183,8 +212,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 m, v = (torch.empty(p.shape, device=p.device) for _ in range(2))
                 out.append((m, v))
                 calls.setdefault(p.device, []).append(
-                    (v.data_ptr(), m.data_ptr(), st["m"].data_ptr(), st["v"].data_ptr(), 0, st["m_scale"].data_ptr(),
-                     st["v_scale"].data_ptr(), p.numel(), 0, 1.0, 1.0))
+                    _ROW(v.data_ptr(), m.data_ptr(), st["m"].data_ptr(), st["v"].data_ptr(), 0, st["m_scale"].data_ptr(),
+                         st["v_scale"].data_ptr(), p.numel(), 0, 1.0, 1.0))
         for dev, rows in calls.items():
             backend_for(dev).adam_values(dev, rows)
         return out

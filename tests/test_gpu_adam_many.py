@@ -3,8 +3,6 @@
 fp32 and bf16 moments: bit for bit the single-tensor step, whatever the tensors' number, sizes, places and kinds of
 gradients.  8-bit moments: codes and scales equal to a restatement in float64; parameters within the roundings of
 an fp32 update."""
-import ctypes
-
 import numpy as np
 import pytest
 import torch
@@ -12,8 +10,7 @@ import torch
 from conftest import gpu_available
 
 from granulelayer_amd import FusedAdamW
-from granulelayer_amd import _native as N
-from granulelayer_amd.backend import HipBackend, _ptr, _stream
+from granulelayer_amd.backend import HipBackend, adam_row
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a ROCm GPU")]
 DEV = "cuda"
@@ -323,8 +320,8 @@ def test_another_stream_and_a_graph():
     # a captured call replays its own numbers; here the same as an eager call's of the third step
     st = opts[0].state[ps[0]]
     b1, b2 = HP["betas"]
-    row = (ps[0].data_ptr(), ps[0].main_grad.data_ptr(), st["m"].data_ptr(), st["v"].data_ptr(), 0,
-           st["m_scale"].data_ptr(), st["v_scale"].data_ptr(), n, 0, 1 - b1 ** 3, 1 - b2 ** 3)
+    row = adam_row(ps[0].data_ptr(), ps[0].main_grad.data_ptr(), st["m"].data_ptr(), st["v"].data_ptr(), 0,
+                   st["m_scale"].data_ptr(), st["v_scale"].data_ptr(), n, 0, 1 - b1 ** 3, 1 - b2 ** 3)
 
     def call():
         HipBackend.get().adam_many(ps[0].device, [row], torch.float32, torch.float32, torch.int8, HP["lr"], b1, b2,
