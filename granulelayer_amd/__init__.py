@@ -9,7 +9,8 @@ library granulelayer_amd/lib/libgranulelayer_amd.so through its C ABI
 
 Beside them, without a counterpart in the reference: ``DenseProjection`` / ``dense_projection`` (a dense
 product with bias, activation and residual in its epilogue) and ``pack_activation`` /
-``PackedActivation`` (activations kept in 8 bits, also ``activation_checkpoint="int8"`` of the layers).
+``PackedActivation`` (activations kept in 8 bits, also ``activation_checkpoint="int8"`` of the layers),
+``LayerNorm`` / ``layer_norm``.
 """
 from .activations8 import PackedActivation, pack_activation
 from .config import LevelSpec, PhysicalPlan, PoolingConfig
@@ -17,7 +18,9 @@ from .cover_topk16 import CoverTopK16Layer
 from .dense import DenseProjection, dense_projection
 from .layer import SparsePoolingLayer
 from .layout import SparseLayout, init_parameters
+from .norm import LayerNorm, layer_norm
 from .optim import FusedAdamW
 
 __all__ = ["SparsePoolingLayer", "PoolingConfig", "LevelSpec", "PhysicalPlan", "SparseLayout", "init_parameters",
-           "CoverTopK16Layer", "FusedAdamW", "DenseProjection", "dense_projection", "PackedActivation", "pack_activation"]
+           "CoverTopK16Layer", "FusedAdamW", "DenseProjection", "dense_projection", "PackedActivation", "pack_activation",
+           "LayerNorm", "layer_norm"]

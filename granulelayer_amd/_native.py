@@ -94,9 +94,20 @@ class GlAdamManyArgs(ctypes.Structure):
                 ("weight_decay", _D)]
 
 
-# gl_struct_layout ids 0..9
+class GlNormArgs(ctypes.Structure):
+    _fields_ = [("X", _P), ("sx", _I64), ("weight", _P), ("bias", _P), ("Y", _P), ("sy", _I64), ("stats", _P), ("M", _I64),
+                ("D", _I32), ("x_dtype", _I32), ("w_dtype", _I32), ("y_dtype", _I32), ("eps", _F)]
+
+
+class GlNormBwdArgs(ctypes.Structure):
+    _fields_ = [("dY", _P), ("sdy", _I64), ("X", _P), ("sx", _I64), ("weight", _P), ("stats", _P), ("dX", _P),
+                ("dweight", _P), ("dbias", _P), ("M", _I64), ("D", _I32), ("x_dtype", _I32), ("w_dtype", _I32),
+                ("dy_dtype", _I32), ("g_dtype", _I32), ("accumulate", _I32), ("ws", _P), ("ws_bytes", _SZ)]
+
+
+# gl_struct_layout ids 0..11
 STRUCTS = (GlFwdArgs, GlBwdArgs, GlEdgeArgs, GlAdamArgs, GlCoverArgs, GlPack8Args, GlDenseArgs, GlDenseBwdArgs,
-           GlAdamTensor, GlAdamManyArgs)
+           GlAdamTensor, GlAdamManyArgs, GlNormArgs, GlNormBwdArgs)
 # every symbol include/granulelayer_amd.h declares
 EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_workspace", "gl_fwd", "gl_fwd_static",
            "gl_fwd_mask_bytes",
@@ -104,14 +115,16 @@ EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_work
            "gl_edges_build", "gl_bwd_workspace", "gl_bwd", "gl_adam", "gl_sched_size", "gl_sched_build_host",
            "gl_sched_build", "gl_window_build_host", "gl_window_build", "gl_cover_select", "gl_trace_begin",
            "gl_trace_end", "gl_pack8", "gl_unpack8", "gl_dense_fwd_workspace", "gl_dense_fwd", "gl_dense_bwd_workspace",
-           "gl_dense_bwd", "gl_adam_many", "gl_adam_values")
+           "gl_dense_bwd", "gl_adam_many", "gl_adam_values", "gl_norm_fwd", "gl_norm_bwd_workspace",
+           "gl_norm_bwd")
 KERNEL_NAMES = {1: "tile_x_kernel", 2: "fwd_kernel", 3: "fwd_finalize_kernel", 4: "c1t_kernel", 5: "bwd_w_kernel",
                 6: "dx_kernel", 7: "dx_reduce_kernel", 8: "adam_kernel", 9: "edges_build", 10: "fwd_kernel_win",
                 11: "bwd_w_kernel_win", 12: "max_events_dw_kernel", 13: "max_events_dx_kernel",
                 14: "cover_select_kernel", 15: "sched_build_kernel", 16: "dx_dense_kernel",
                 17: "dx_dma_kernel", 18: "pack8_kernel", 19: "unpack8_kernel", 20: "dense_tile_kernel",
                 21: "dense_few_kernel", 22: "dense_join_kernel", 23: "dense_dz_kernel", 24: "dense_db_kernel",
-                25: "dense_align_kernel", 26: "adam_values_kernel"}
+                25: "dense_align_kernel", 26: "adam_values_kernel", 27: "norm_fwd_kernel", 28: "norm_bwd_kernel",
+                29: "norm_dw_kernel"}
 
 
 class NativeError(RuntimeError):
@@ -140,11 +153,13 @@ class Library:
         for name, st in (("gl_fwd", GlFwdArgs), ("gl_fwd_static", GlFwdArgs), ("gl_bwd", GlBwdArgs),
                          ("gl_edges_build", GlEdgeArgs), ("gl_adam", GlAdamArgs), ("gl_cover_select", GlCoverArgs), ("gl_pack8", GlPack8Args), ("gl_unpack8", GlPack8Args),
                          ("gl_dense_fwd", GlDenseArgs), ("gl_dense_bwd", GlDenseBwdArgs),
-                         ("gl_adam_many", GlAdamManyArgs), ("gl_adam_values", GlAdamManyArgs)):
+                         ("gl_adam_many", GlAdamManyArgs), ("gl_adam_values", GlAdamManyArgs),
+                         ("gl_norm_fwd", GlNormArgs), ("gl_norm_bwd", GlNormBwdArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), _P]
         for name, st in (("gl_fwd_workspace", GlFwdArgs), ("gl_bwd_workspace", GlBwdArgs),
-                         ("gl_dense_fwd_workspace", GlDenseArgs), ("gl_dense_bwd_workspace", GlDenseBwdArgs)):
+                         ("gl_dense_fwd_workspace", GlDenseArgs), ("gl_dense_bwd_workspace", GlDenseBwdArgs),
+                         ("gl_norm_bwd_workspace", GlNormBwdArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), ctypes.POINTER(_SZ)]
         L.gl_trace_begin.restype = ctypes.c_int

@@ -523,6 +523,53 @@ class HipBackend:
                 a.ws, a.ws_bytes = _ptr(ws), need
             self.lib.call("gl_dense_bwd", ctypes.byref(a), _stream(dev))
 
+    # ------------------------------------------------------------------ layer norm
+    def norm_forward(self, x, w, b, eps, out_dtype, keep):
+        """(y [M, D] of ``out_dtype``, what the backward takes: [M, 2] fp32 with ``keep``) of x [M, D], w and b [D]
+        of one dtype or None."""
+        x, code, sx = _x_operand(x.resolve_neg())
+        M, D = x.shape
+        dev = x.device
+        w, b, wcode = _norm_params(w, b)
+        y = torch.empty((M, D), device=dev, dtype=out_dtype)
+        stats = torch.empty((M, 2), device=dev) if keep else None
+        a = N.GlNormArgs(_ptr(x), sx, _ptr(w), _ptr(b), _ptr(y), D, _ptr(stats), M, D, code, wcode, _DENSE_DTYPES[out_dtype],
+                         eps)
+        with _on(dev):
+            self.lib.call("gl_norm_fwd", ctypes.byref(a), _stream(dev))
+        return y, stats
+
+    def norm_backward(self, dy, x, w, stats, dx, dw, db, accumulate):
+        """Gradients of ``norm_forward`` into dx [M, D] (x's dtype), dw and db [D] (one dtype, or fp32 and added to
+        with ``accumulate``); None for what is not needed."""
+        dy, ycode, sdy = _x_operand(dy)
+        x, code, sx = _x_operand(x.resolve_neg())
+        M, D = x.shape
+        dev = x.device
+        w, _, wcode = _norm_params(w, None)
+        if M == 0:  # sums over no rows
+            for t in (dw, db):
+                if t is not None and not accumulate:
+                    t.zero_()
+            return
+        gcode = next((_DENSE_DTYPES[t.dtype] for t in (dw, db) if t is not None), 0)
+        a = N.GlNormBwdArgs(_ptr(dy), sdy, _ptr(x), sx, _ptr(w), _ptr(stats), _ptr(dx), _ptr(dw), _ptr(db), M, D, code, wcode,
+                            ycode, gcode, int(accumulate), 0, 0)
+        with _on(dev):
+            need = self.lib.size_query("gl_norm_bwd_workspace", a)
+            if need:
+                ws = torch.empty(need, device=dev, dtype=torch.uint8)
+                a.ws, a.ws_bytes = _ptr(ws), need
+            self.lib.call("gl_norm_bwd", ctypes.byref(a), _stream(dev))
+
+
+def _norm_params(w, b):
+    """Contiguous w and b and their dtype's code."""
+    w = None if w is None else w.resolve_neg().contiguous()
+    b = None if b is None else b.resolve_neg().contiguous()
+    t = b if w is None else w
+    return w, b, 0 if t is None else _DENSE_DTYPES[t.dtype]
+
 
 _DENSE_DTYPES = {torch.float32: N.GL_DTYPE_F32, torch.bfloat16: N.GL_DTYPE_BF16}
 _MOMENTS = {**_DENSE_DTYPES, torch.int8: N.GL_MOMENTS_INT8}

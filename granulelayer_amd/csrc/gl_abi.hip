@@ -177,6 +177,21 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       for (long long x : t) v[c++] = x;
       break;
     }
+    case 10: {
+      typedef GlNormArgs S;
+      long long t[] = {(long long)sizeof(S), OFF(S, X), OFF(S, sx), OFF(S, weight), OFF(S, bias), OFF(S, Y), OFF(S, sy),
+                       OFF(S, stats), OFF(S, M), OFF(S, D), OFF(S, x_dtype), OFF(S, w_dtype), OFF(S, y_dtype), OFF(S, eps)};
+      for (long long x : t) v[c++] = x;
+      break;
+    }
+    case 11: {
+      typedef GlNormBwdArgs S;
+      long long t[] = {(long long)sizeof(S), OFF(S, dY), OFF(S, sdy), OFF(S, X), OFF(S, sx), OFF(S, weight), OFF(S, stats),
+                       OFF(S, dX), OFF(S, dweight), OFF(S, dbias), OFF(S, M), OFF(S, D), OFF(S, x_dtype), OFF(S, w_dtype),
+                       OFF(S, dy_dtype), OFF(S, g_dtype), OFF(S, accumulate), OFF(S, ws), OFF(S, ws_bytes)};
+      for (long long x : t) v[c++] = x;
+      break;
+    }
     default:
       return GL_ERR_ARG;
   }

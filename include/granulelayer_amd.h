@@ -225,7 +225,7 @@ int gl_cover_select(const GlCoverArgs* a, void* stream);
  * order) so a binding can refuse a mismatched library.  Replaces sp_abi_version /
  * sp_struct_layout (sparse_pooling/kernels/cuda/abi.cu:17-62, checked in runtime.py:103-120).
  * which: 0 GlFwdArgs, 1 GlBwdArgs, 2 GlEdgeArgs, 3 GlAdamArgs, 4 GlCoverArgs, 5 GlPack8Args, 6 GlDenseArgs,
- * 7 GlDenseBwdArgs, 8 GlAdamTensor, 9 GlAdamManyArgs.  Returns the number of values written
+ * 7 GlDenseBwdArgs, 8 GlAdamTensor, 9 GlAdamManyArgs, 10 GlNormArgs, 11 GlNormBwdArgs.  Returns the number of values written
  * (or needed, when n is too small), negative on an unknown struct. */
 int gl_abi_version(void);
 int gl_struct_layout(int which, long long* out, int n);
@@ -412,6 +412,49 @@ typedef struct GlDenseBwdArgs {
 int gl_dense_bwd_workspace(const GlDenseBwdArgs* a, size_t* bytes);
 int gl_dense_bwd(const GlDenseBwdArgs* a, void* stream);
 
+/* ---- layer norm --------------------------------------------------------------------------------
+ *
+ *   Y[m,d] = (X[m,d] - mean) r weight[d] + bias[d],   r = 1 / sqrt(variance + eps)
+ *
+ * with the row's mean and variance (over D).  Rows are a stride apart, features are neighbours, no address
+ * needs more than its element's alignment; sums are fp32. */
+#define GL_NORM_MAX_ROWS (1LL << 40)
+typedef struct GlNormArgs {
+  const void* X;       /* [M, D] of x_dtype */
+  int64_t sx;
+  const void* weight;  /* [D] of w_dtype, or NULL: ones */
+  const void* bias;    /* [D] of w_dtype, or NULL: zeros */
+  void* Y;             /* [M, D] of y_dtype */
+  int64_t sy;
+  float* stats;        /* out [M, 2], every row's mean and r, for the backward; or NULL */
+  int64_t M;
+  int32_t D;           /* up to GL_DENSE_MAX_FEATURES */
+  int32_t x_dtype, w_dtype, y_dtype;
+  float eps;
+} GlNormArgs;
+int gl_norm_fwd(const GlNormArgs* a, void* stream);
+
+/* The backward, from dY, X and the forward's stats.  Gradients that are NULL are not computed. */
+typedef struct GlNormBwdArgs {
+  const void* dY;      /* [M, D] of dy_dtype */
+  int64_t sdy;
+  const void* X;
+  int64_t sx;
+  const void* weight;
+  const float* stats;
+  void* dX;            /* [M, D] of x_dtype, contiguous */
+  void* dweight;       /* [D] of g_dtype */
+  void* dbias;
+  int64_t M;
+  int32_t D;
+  int32_t x_dtype, w_dtype, dy_dtype, g_dtype;
+  int32_t accumulate;  /* dweight and dbias (fp32) are added to */
+  void* ws;            /* 256-byte aligned */
+  size_t ws_bytes;
+} GlNormBwdArgs;
+int gl_norm_bwd_workspace(const GlNormBwdArgs* a, size_t* bytes);
+int gl_norm_bwd(const GlNormBwdArgs* a, void* stream);
+
 /* Kernel ids reported by the trace below. */
 enum {
   GL_KERNEL_TILE_X = 1, GL_KERNEL_FWD = 2, GL_KERNEL_FWD_FINALIZE = 3, GL_KERNEL_C1T = 4, GL_KERNEL_BWD_W = 5,
@@ -427,7 +470,9 @@ enum {
   GL_KERNEL_DENSE_JOIN = 22,                           /* sums of a split product, with its epilogue */
   GL_KERNEL_DENSE_DZ = 23, GL_KERNEL_DENSE_DB = 24,    /* dz and the partial sums of db; their sum */
   GL_KERNEL_DENSE_ALIGN = 25,                          /* operands copied to 16-byte rows */
-  GL_KERNEL_ADAM_VALUES = 26                           /* 8-bit moments to fp32 */
+  GL_KERNEL_ADAM_VALUES = 26,                          /* 8-bit moments to fp32 */
+  GL_KERNEL_NORM = 27, GL_KERNEL_NORM_BWD = 28,        /* layer norm; dX and the workgroups' sums of dW, db */
+  GL_KERNEL_NORM_DW = 29                               /* their sum */
 };
 
 /* Launch trace for benchmarks and tests (process-wide, not for concurrent callers): after
