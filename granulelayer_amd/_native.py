@@ -9,6 +9,7 @@ entry point of the product path raises if the library is missing or refuses a ca
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -131,6 +132,17 @@ class NativeError(RuntimeError):
     pass
 
 
+_FORMAT = {_P: "Q", _I32: "i", _I64: "q", _SZ: "Q", _F: "f", _D: "d", ctypes.c_uint64: "Q"}
+
+
+def packer(st):
+    """A function of all of a structure's fields, in order, to its bytes: a fraction of the time that making a ctypes
+    structure of as many fields takes.  (The trailing pad is the structure's.)"""
+    s = struct.Struct("@" + "".join(_FORMAT[t] for _, t in st._fields_) + "0q")
+    assert s.size == ctypes.sizeof(st)
+    return s.pack
+
+
 def struct_layout(st) -> list:
     return [ctypes.sizeof(st)] + [getattr(st, name).offset for name, _ in st._fields_]
 
@@ -201,6 +213,18 @@ class Library:
         if r != 0 and r != accept:
             raise NativeError(f"{name} failed (code {r}: {self.error(r)})")
         return r
+
+    def entry(self, name: str):
+        """The entry point as a function of a ``packer``'s bytes and a stream; raises on any code but 0."""
+        f = self.lib[name]  # a function object of its own
+        f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p, _P]
+
+        def call(args, stream):
+            r = f(args, stream)
+            if r != 0:
+                raise NativeError(f"{name} failed (code {r}: {self.error(r)})")
+
+        return call
 
     def size_query(self, name: str, args) -> int:
         out = _SZ(0)

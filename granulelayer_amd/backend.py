@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import struct
+import functools
 import threading
 from typing import Dict, Optional
 
@@ -53,7 +53,7 @@ _NO_SWITCH = contextlib.nullcontext()
 def _on(dev):
     """``torch.cuda.device(dev)``, or nothing when dev is the current device already (the switch and
     its return cost the smallest calls several microseconds)."""
-    return _NO_SWITCH if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _NO_SWITCH if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def _x_operand(x: torch.Tensor):
@@ -101,6 +101,8 @@ class HipBackend:
         self.lib = lib or N.library()
         # stage only each pool's input window in LDS when the windows are narrow (same results)
         self.window_staging = window_staging
+        self._norm_fwd, self._norm_bwd = self.lib.entry("gl_norm_fwd"), self.lib.entry("gl_norm_bwd")
+        self._norm_bytes = functools.lru_cache(256)(self._norm_bytes_of)
 
     @classmethod
     def get(cls) -> "HipBackend":
@@ -533,10 +535,10 @@ class HipBackend:
         w, b, wcode = _norm_params(w, b)
         y = torch.empty((M, D), device=dev, dtype=out_dtype)
         stats = torch.empty((M, 2), device=dev) if keep else None
-        a = N.GlNormArgs(_ptr(x), sx, _ptr(w), _ptr(b), _ptr(y), D, _ptr(stats), M, D, code, wcode, _DENSE_DTYPES[out_dtype],
-                         eps)
+        a = _NORM(x.data_ptr(), sx, _ptr(w), _ptr(b), y.data_ptr(), D, _ptr(stats), M, D, code, wcode,
+                  _DENSE_DTYPES[out_dtype], eps)
         with _on(dev):
-            self.lib.call("gl_norm_fwd", ctypes.byref(a), _stream(dev))
+            self._norm_fwd(a, _stream(dev))
         return y, stats
 
     def norm_backward(self, dy, x, w, stats, dx, dw, db, accumulate):
@@ -547,20 +549,22 @@ class HipBackend:
         M, D = x.shape
         dev = x.device
         w, _, wcode = _norm_params(w, None)
+        sums = db if dw is None else dw
         if M == 0:  # sums over no rows
             for t in (dw, db):
                 if t is not None and not accumulate:
                     t.zero_()
             return
-        gcode = next((_DENSE_DTYPES[t.dtype] for t in (dw, db) if t is not None), 0)
-        a = N.GlNormBwdArgs(_ptr(dy), sdy, _ptr(x), sx, _ptr(w), _ptr(stats), _ptr(dx), _ptr(dw), _ptr(db), M, D, code, wcode,
-                            ycode, gcode, int(accumulate), 0, 0)
+        need = self._norm_bytes(M, D, dx is not None, sums is not None)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+        a = _NORM_BWD(dy.data_ptr(), sdy, x.data_ptr(), sx, _ptr(w), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), M, D,
+                      code, wcode, ycode, 0 if sums is None else _DENSE_DTYPES[sums.dtype], accumulate, _ptr(ws), need)
         with _on(dev):
-            need = self.lib.size_query("gl_norm_bwd_workspace", a)
-            if need:
-                ws = torch.empty(need, device=dev, dtype=torch.uint8)
-                a.ws, a.ws_bytes = _ptr(ws), need
-            self.lib.call("gl_norm_bwd", ctypes.byref(a), _stream(dev))
+            self._norm_bwd(a, _stream(dev))
+
+    def _norm_bytes_of(self, M, D, dx, sums):
+        a = N.GlNormBwdArgs(dY=16, X=16, stats=16, sdy=D, sx=D, dX=16 * dx, dweight=16 * sums, M=M, D=D)
+        return self.lib.size_query("gl_norm_bwd_workspace", a)
 
 
 def _norm_params(w, b):
@@ -572,11 +576,9 @@ def _norm_params(w, b):
 
 
 _DENSE_DTYPES = {torch.float32: N.GL_DTYPE_F32, torch.bfloat16: N.GL_DTYPE_BF16}
+_NORM, _NORM_BWD = N.packer(N.GlNormArgs), N.packer(N.GlNormBwdArgs)
 _MOMENTS = {**_DENSE_DTYPES, torch.int8: N.GL_MOMENTS_INT8}
-# a GlAdamTensor as bytes: p, g, m, v, master, m_scale, v_scale, n, seed, bc1, bc2
-_ADAM_ROW = struct.Struct("7QqQ2f")
-assert _ADAM_ROW.size == ctypes.sizeof(N.GlAdamTensor)
-adam_row = _ADAM_ROW.pack
+adam_row = N.packer(N.GlAdamTensor)  # p, g, m, v, master, m_scale, v_scale, n, seed, bc1, bc2
 
 
 def backend_for(device) -> HipBackend:

@@ -52,12 +52,98 @@ __device__ __forceinline__ void norm_params(const void* p, bool bf, int c, int n
   }
 }
 
-// T threads a row (a wave, or the workgroup), V vectors a thread: rows of up to 8 T V features.
-template <int T, int V, bool XBF, bool YBF>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void norm_fwd_kernel(NormK a) {
-  constexpr int ROWS = T < 256 ? 256 / T : 1, NW = T / 64;  // rows of a workgroup at a time, waves of a row
-  __shared__ float red[2][NW];
-  const int t = threadIdx.x % T;
+// Eight features as they are stored: a row that is on its way to the next turn, and one that is read twice.
+template <bool BF>
+struct Eight {
+  uv4 w[BF ? 1 : 2];
+};
+typedef unsigned uv4_at __attribute__((ext_vector_type(4), aligned(2)));
+// STREAM: the caches need not keep it
+template <bool BF, bool STREAM>
+__device__ __forceinline__ Eight<BF> load_eight(const void* p, long long i, int n) {
+  Eight<BF> e;
+  if (n >= 8) {
+#pragma unroll
+    for (int h = 0; h < (BF ? 1 : 2); ++h) {
+      const uv4_at* q = reinterpret_cast<const uv4_at*>((const char*)p + (BF ? 2 : 4) * i + 16 * h);
+      if constexpr (STREAM) e.w[h] = __builtin_nontemporal_load(q);
+      else e.w[h] = *q;
+    }
+  } else {
+    float v[8];
+    load8<BF>(p, i, n, v);
+    if constexpr (BF) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e.w[0][j] = __float_as_uint(v[2 * j]) >> 16 | __float_as_uint(v[2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e.w[j >> 2][j & 3] = __float_as_uint(v[j]);
+    }
+  }
+  return e;
+}
+template <bool BF>
+__device__ __forceinline__ float value(const Eight<BF>& e, int j) {
+  if constexpr (BF) return __uint_as_float(j & 1 ? e.w[0][j >> 1] & 0xffff0000u : e.w[0][j >> 1] << 16);
+  else return __uint_as_float(e.w[j >> 2][j & 3]);
+}
+template <bool BF, bool STREAM>
+__device__ __forceinline__ void store_eight(void* p, long long i, int n, const float (&v)[8]) {
+  if (!STREAM || n < 8) {
+    store8<BF>(p, i, n, v);
+  } else if constexpr (BF) {
+    uv4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = to_bf16x2(v[2 * j], v[2 * j + 1]);
+    __builtin_nontemporal_store(w, reinterpret_cast<uv4_at*>((char*)p + 2 * i));
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uv4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(v[4 * h + j]);
+      __builtin_nontemporal_store(w, reinterpret_cast<uv4_at*>((char*)p + 4 * i + 16 * h));
+    }
+  }
+}
+
+// Totals over the threads of a row, the same bits in all of them: a wave's, or (WAVE false) those of up to 16 waves, of
+// which this is number `wave`, through `red`, 16 pairs that are 0 where there is no wave.
+template <bool WAVE>
+__device__ __forceinline__ void row_totals(float& a, float& b, float (*red)[2], int wave) {
+  a = wave_total(a);
+  b = wave_total(b);
+  if constexpr (!WAVE) {
+    const int l = threadIdx.x & 63;
+    if (l == 0) {
+      red[wave][0] = a;
+      red[wave][1] = b;
+    }
+    __syncthreads();
+    a = red[l & 15][0];
+    b = red[l & 15][1];
+    a += dpp<0xB1>(a);
+    b += dpp<0xB1>(b);
+    a += dpp<0x4E>(a);
+    b += dpp<0x4E>(b);
+    a += dpp<0x141>(a);
+    b += dpp<0x141>(b);
+    a += dpp<0x140>(a);
+    b += dpp<0x140>(b);
+  }
+}
+
+// A row is a wave's (WAVE: four rows a workgroup) or a workgroup's, with V vectors a thread.  The next turn's row is
+// loaded before this one's sums, so a workgroup always has a row on its way.
+template <bool WAVE, int V, bool XBF, bool YBF, bool STREAM>
+__global__ __launch_bounds__(WAVE ? 256 : V == 1 ? 1024 : 512) void norm_fwd_kernel(NormK a) {
+  __shared__ float red[2][16][2];
+  constexpr int ROWS = WAVE ? 4 : 1;
+  const int T = WAVE ? 64 : blockDim.x, t = WAVE ? threadIdx.x & 63 : threadIdx.x;
+  if constexpr (!WAVE) {
+    if (threadIdx.x < 64) (&red[0][0][0])[threadIdx.x] = 0.f;
+    __syncthreads();
+  }
   float w[V][8], b[V][8];
 #pragma unroll
   for (int y = 0; y < V; ++y) {
@@ -65,30 +151,26 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_fwd_kernel(NormK a) {
     norm_params(a.w, a.w_bf, c, a.D - c, 1.f, w[y]);
     norm_params(a.b, a.w_bf, c, a.D - c, 0.f, b[y]);
   }
-  auto total = [&](float v, int which) {
-    v = wave_total(v);
-    if constexpr (NW > 1) {
-      if ((threadIdx.x & 63) == 0) red[which][threadIdx.x >> 6] = v;
-      __syncthreads();
-      v = 0.f;
-#pragma unroll
-      for (int k = 0; k < NW; ++k) v += red[which][k];
-    }
-    return v;
-  };
-  // (a row's threads leave together: rows of a workgroup share no barrier)
-  for (long long m = (long long)blockIdx.x * ROWS + threadIdx.x / T; m < a.M; m += (long long)gridDim.x * ROWS) {
-    float x[V][8], s = 0.f;
+  const long long step = (long long)gridDim.x * ROWS;
+  long long m = (long long)blockIdx.x * ROWS + (WAVE ? threadIdx.x >> 6 : 0);
+  Eight<XBF> next[V];
+  auto fetch = [&](long long row) {
 #pragma unroll
     for (int y = 0; y < V; ++y) {
       const int c = (y * T + t) * 8;
-      load8<XBF>(a.X, m * a.sx + c, a.D - c, x[y]);
+      next[y] = load_eight<XBF, STREAM>(a.X, row * a.sx + c, a.D - c);
     }
+  };
+  if (m < a.M) fetch(m);
+  for (; m < a.M; m += step) {
+    float x[V][8], s = 0.f, none = 0.f;
 #pragma unroll
     for (int y = 0; y < V; ++y)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += x[y][j];
-    const float mean = total(s, 0) / (float)a.D;  // (by 1 / D a constant row's would be off its value)
+      for (int j = 0; j < 8; ++j) s += x[y][j] = value<XBF>(next[y], j);
+    if (m + step < a.M) fetch(m + step);
+    row_totals<WAVE>(s, none, red[0], t >> 6);
+    const float mean = s / (float)a.D;  // (by 1 / D a constant row's would be off its value)
     s = 0.f;
 #pragma unroll
     for (int y = 0; y < V; ++y) {
@@ -99,13 +181,14 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_fwd_kernel(NormK a) {
         if (left >= 8 || j < left) s = __builtin_fmaf(x[y][j], x[y][j], s);
       }
     }
-    const float r = 1.f / __builtin_sqrtf(total(s, 1) / (float)a.D + a.eps);
+    row_totals<WAVE>(s, none, red[1], t >> 6);
+    const float r = 1.f / __builtin_sqrtf(s / (float)a.D + a.eps);
 #pragma unroll
     for (int y = 0; y < V; ++y) {
       const int c = (y * T + t) * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[y][j] = __builtin_fmaf(x[y][j] * r, w[y][j], b[y][j]);
-      store8<YBF>(a.Y, m * a.sy + c, a.D - c, x[y]);
+      store_eight<YBF, STREAM>(a.Y, m * a.sy + c, a.D - c, x[y]);
     }
     if (a.stats && t == 0) {
       a.stats[2 * m] = mean;
@@ -114,12 +197,20 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_fwd_kernel(NormK a) {
   }
 }
 
-template <int T, int V, bool XBF, bool YBF>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void norm_bwd_kernel(NormK a) {
-  constexpr int ROWS = T < 256 ? 256 / T : 1, NW = T / 64;
-  __shared__ float red[2][NW][2];
-  extern __shared__ __align__(16) float sums[];  // [ROWS][8 T V] of rows that share a workgroup
-  const int t = threadIdx.x % T;
+// The backward's workgroups have `teams` rows at a time, T threads each (WAVE: one), that add their sums of dw and db
+// up in LDS at the end: a workgroup leaves 8 D bytes of them however many rows it has at a time.
+// AHEAD: the next turn's row is loaded before this one's sums; with two vectors a thread there are no registers for it.
+template <bool WAVE, int V, bool XBF, bool YBF, bool STREAM>
+__global__ __launch_bounds__(1024) void norm_bwd_kernel(NormK a, int T, int teams) {
+  constexpr bool AHEAD = V == 1;
+  constexpr int MOST = WAVE ? 16 : V == 1 ? 8 : 1;  // teams (of 128 threads and more, or 1024)
+  __shared__ float red[2][WAVE ? 1 : MOST][16][2];
+  __shared__ float sums[V == 1 ? 8192 : 1];
+  const int team = WAVE ? wave_uniform(threadIdx.x >> 6) : wave_uniform(threadIdx.x / (unsigned)T), t = threadIdx.x - team * T;
+  if constexpr (!WAVE) {
+    for (int i = threadIdx.x; i < MOST * 64; i += blockDim.x) (&red[0][0][0][0])[i] = 0.f;
+    __syncthreads();
+  }
   float w[V][8], dw[V][8], db[V][8];
 #pragma unroll
   for (int y = 0; y < V; ++y) {
@@ -129,70 +220,77 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_bwd_kernel(NormK a) {
     for (int j = 0; j < 8; ++j) dw[y][j] = db[y][j] = 0.f;
   }
   const float inv = 1.f / (float)a.D;
-  int turn = 0;
-  for (long long m = (long long)blockIdx.x * ROWS + threadIdx.x / T; m < a.M; m += (long long)gridDim.x * ROWS) {
-    float x[V][8], g[V][8];
-    const float mean = a.stats[2 * m], r = a.stats[2 * m + 1];
+  const long long step = (long long)gridDim.x * teams;
+  Eight<XBF> nx[V], x[V];
+  Eight<YBF> ng[V], g[V];
+  float next_mean = 0.f, next_r = 0.f;
+  auto fetch = [&](long long row) {
+    if (row >= a.M) return;
 #pragma unroll
     for (int y = 0; y < V; ++y) {
       const int c = (y * T + t) * 8;
-      load8<XBF>(a.X, m * a.sx + c, a.D - c, x[y]);
-      load8<YBF>(a.dY, m * a.sdy + c, a.D - c, g[y]);
+      nx[y] = load_eight<XBF, STREAM>(a.X, row * a.sx + c, a.D - c);
+      ng[y] = load_eight<YBF, STREAM>(a.dY, row * a.sdy + c, a.D - c);
     }
+    next_mean = a.stats[2 * row];
+    next_r = a.stats[2 * row + 1];
+  };
+  if constexpr (AHEAD) fetch((long long)blockIdx.x * teams + team);
+  int turn = 0;
+  for (long long first = (long long)blockIdx.x * teams; first < a.M; first += step) {  // the workgroup's turns
+    const long long m = first + team;
+    if constexpr (!AHEAD) fetch(m);
+    const float mean = next_mean, r = next_r;
+#pragma unroll
+    for (int y = 0; y < V; ++y) {
+      x[y] = nx[y];
+      g[y] = ng[y];
+    }
+    if constexpr (AHEAD) fetch(m + step);
     float s0 = 0.f, s1 = 0.f;
+    if (m < a.M) {
 #pragma unroll
-    for (int y = 0; y < V; ++y)
+      for (int y = 0; y < V; ++y)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {  // (behind the row g is 0)
-        x[y][j] = (x[y][j] - mean) * r;
-        dw[y][j] = __builtin_fmaf(g[y][j], x[y][j], dw[y][j]);
-        db[y][j] += g[y][j];
-        g[y][j] *= w[y][j];
-        s0 += g[y][j];
-        s1 = __builtin_fmaf(g[y][j], x[y][j], s1);
-      }
-    if (!a.Y) continue;
-    s0 = wave_total(s0);
-    s1 = wave_total(s1);
-    if constexpr (NW > 1) {  // the other half is written when every thread has passed a barrier after it read this one
-      if ((threadIdx.x & 63) == 0) {
-        red[turn][threadIdx.x >> 6][0] = s0;
-        red[turn][threadIdx.x >> 6][1] = s1;
-      }
-      __syncthreads();
-      s0 = s1 = 0.f;
-#pragma unroll
-      for (int k = 0; k < NW; ++k) {
-        s0 += red[turn][k][0];
-        s1 += red[turn][k][1];
-      }
-      turn ^= 1;
+        for (int j = 0; j < 8; ++j) {  // (behind the row g is 0)
+          const float h = (value<XBF>(x[y], j) - mean) * r, d = value<YBF>(g[y], j), e = d * w[y][j];
+          dw[y][j] = __builtin_fmaf(d, h, dw[y][j]);
+          db[y][j] += d;
+          s0 += e;
+          s1 = __builtin_fmaf(e, h, s1);
+        }
     }
+    if (!a.Y) continue;
+    // (red's other half is written when every thread has passed a barrier since it read this one)
+    row_totals<WAVE>(s0, s1, red[turn][WAVE ? 0 : team], t >> 6);
+    turn ^= 1;
     s0 *= inv;
     s1 *= inv;
+    if (m < a.M) {
 #pragma unroll
-    for (int y = 0; y < V; ++y) {
-      const int c = (y * T + t) * 8;
+      for (int y = 0; y < V; ++y) {
+        const int c = (y * T + t) * 8;
+        float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[y][j] = r * (g[y][j] - s0 - x[y][j] * s1);
-      store8<XBF>(a.Y, m * a.D + c, a.D - c, x[y]);
+        for (int j = 0; j < 8; ++j) {
+          const float h = (value<XBF>(x[y], j) - mean) * r;
+          v[j] = r * (value<YBF>(g[y], j) * w[y][j] - s0 - h * s1);
+        }
+        store_eight<XBF, STREAM>(a.Y, m * a.D + c, a.D - c, v);
+      }
     }
   }
   if (!a.part) return;
   float* part = a.part + (long long)blockIdx.x * 2 * a.D;
   auto write = [&](float (&v)[V][8], float* to) {
-    if constexpr (ROWS > 1) {
-      float* own = sums + (threadIdx.x / T) * (8 * T * V);
+    if (V == 1 && teams > 1) {
       __syncthreads();
 #pragma unroll
-      for (int y = 0; y < V; ++y)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) own[(y * T + t) * 8 + j] = v[y][j];
+      for (int j = 0; j < 8; ++j) sums[threadIdx.x * 8 + j] = v[0][j];  // (teams are T threads apart)
       __syncthreads();
-      for (int c = threadIdx.x; c < a.D; c += 256) {
-        float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < ROWS; ++k) s += sums[k * (8 * T * V) + c];
+      for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
+        float s = sums[c];
+        for (int k = 1; k < teams; ++k) s += sums[k * 8 * T + c];
         to[c] = s;
       }
     } else {
@@ -335,70 +433,87 @@ __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__
 }
 
 // ---- plans -----------------------------------------------------------------------------------------------------
-// Widest row of T threads with V vectors each.  T and V are the least that hold the row.
-enum { NORM_512 = 0, NORM_1K, NORM_2K, NORM_4K, NORM_8K, NORM_16K, NORM_WIDE };
-inline int norm_form(int D) {
-  int f = NORM_512;
-  while (f < NORM_WIDE && D > (512 << f)) ++f;
-  return f;
-}
-inline int norm_rows(int form) { return form <= NORM_1K ? 4 : 1; }  // of a workgroup at a time
 constexpr int CUS = 256;
+constexpr int NORM_MOST = 16384;  // features that the registers of a workgroup hold
+// bytes of x and y past which they go around the caches: 32768 x 8192 bf16 backward 268 us, 300 without; of 67 MB
+// (16384 x 1024) a forward that does takes 16 us, 13.5 without
+constexpr long long NORM_STREAM = 256LL << 20;
 inline long long least(long long a, long long b) { return a < b ? a : b; }
+
+// Forward: vectors of a thread (rows of up to 1024 features are a wave's), threads, and workgroups: as many as run at
+// once, no more than rows.
+inline int fwd_vectors(int D) { return D <= 512 ? 1 : D <= 1024 ? 2 : D <= 4096 ? 1 : D <= 8192 ? 2 : 4; }
+inline int fwd_threads(int D) { return D <= 1024 ? 256 : 64 * ceil_div(D, 512 * fwd_vectors(D)); }
 inline int fwd_groups(long long M, int D) {
-  const int f = norm_form(D);
-  return (int)least((M + norm_rows(f) - 1) / norm_rows(f), f == NORM_WIDE ? 2 * CUS : (f == NORM_16K ? 2 : f == NORM_8K ? 4 : 8) * CUS);
+  if (D > NORM_MOST) return (int)least(M, 2 * CUS);
+  return (int)least(D <= 1024 ? (M + 3) / 4 : M, 2048 / fwd_threads(D) * CUS);
 }
-// workgroups of the backward that keep sums (each leaves 8 D bytes of them)
+// Backward: threads of a row (up to 512 features are a wave's), its teams (fewer where rows are: every CU has some),
+// and workgroups, one a CU, or two where half a CU's threads are enough for one.
+inline int bwd_threads(int D) { return D > 8192 ? 1024 : 64 * ceil_div(D, 512); }
+inline int bwd_teams(long long M, int D) { return (int)least(1024 / bwd_threads(D), (M + CUS - 1) / CUS); }
 inline int bwd_groups(long long M, int D) {
-  const int f = norm_form(D);
-  if (f == NORM_WIDE) return (int)least(M, 64);
-  return (int)least((M + norm_rows(f) - 1) / norm_rows(f), 2 * CUS);
+  if (D > NORM_MOST) return (int)least(M, 64);
+  const int teams = bwd_teams(M, D);
+  return (int)least((M + teams - 1) / teams, bwd_threads(D) * teams <= 768 ? 2 * CUS : CUS);
 }
 
-template <bool BWD, int T, int V, bool XBF, bool YBF>
-int launch_norm_as(const NormK& k, int groups, hipStream_t s) {
-  constexpr int threads = T < 256 ? 256 : T;
-  if constexpr (BWD) {
-    constexpr size_t lds = T < 256 ? 256 * 8 * V * 4 : 0;
-    GL_LAUNCH(GL_KERNEL_NORM_BWD, (norm_bwd_kernel<T, V, XBF, YBF>), dim3((unsigned)groups), dim3(threads), lds, s, k);
-  } else {
-    GL_LAUNCH(GL_KERNEL_NORM, (norm_fwd_kernel<T, V, XBF, YBF>), dim3((unsigned)groups), dim3(threads), 0, s, k);
-  }
+template <bool WAVE, int V, bool XBF, bool YBF, bool STREAM>
+int launch_fwd_as(const NormK& k, hipStream_t s) {
+  GL_LAUNCH(GL_KERNEL_NORM, (norm_fwd_kernel<WAVE, V, XBF, YBF, STREAM>), dim3((unsigned)fwd_groups(k.M, k.D)),
+            dim3((unsigned)fwd_threads(k.D)), 0, s, k);
   GL_CHECK_LAUNCH();
   return 0;
 }
-template <bool BWD, bool XBF, bool YBF>
-int launch_norm_of(const NormK& k, int groups, float* means, hipStream_t s) {
-  switch (norm_form(k.D)) {
-    case NORM_512: return launch_norm_as<BWD, 64, 1, XBF, YBF>(k, groups, s);
-    case NORM_1K: return launch_norm_as<BWD, 64, 2, XBF, YBF>(k, groups, s);
-    case NORM_2K: return launch_norm_as<BWD, 256, 1, XBF, YBF>(k, groups, s);
-    case NORM_4K: return launch_norm_as<BWD, 256, 2, XBF, YBF>(k, groups, s);
-    case NORM_8K: return launch_norm_as<BWD, 512, 2, XBF, YBF>(k, groups, s);
-    case NORM_16K: return launch_norm_as<BWD, 1024, 2, XBF, YBF>(k, groups, s);
-    default: break;
+template <bool WAVE, int V, bool XBF, bool YBF, bool STREAM>
+int launch_bwd_as(const NormK& k, hipStream_t s) {
+  const int T = bwd_threads(k.D), teams = bwd_teams(k.M, k.D);
+  GL_LAUNCH(GL_KERNEL_NORM_BWD, (norm_bwd_kernel<WAVE, V, XBF, YBF, STREAM>), dim3((unsigned)bwd_groups(k.M, k.D)),
+            dim3((unsigned)(T * teams)), 0, s, k, T, teams);
+  GL_CHECK_LAUNCH();
+  return 0;
+}
+template <bool BWD, bool XBF, bool YBF, bool STREAM>
+int launch_norm_rows(const NormK& k, hipStream_t s) {
+  if constexpr (BWD) {
+    if (k.D <= 512) return launch_bwd_as<true, 1, XBF, YBF, STREAM>(k, s);
+    if (k.D <= 8192) return launch_bwd_as<false, 1, XBF, YBF, STREAM>(k, s);
+    return launch_bwd_as<false, 2, XBF, YBF, STREAM>(k, s);
+  } else {
+    if (k.D <= 512) return launch_fwd_as<true, 1, XBF, YBF, STREAM>(k, s);
+    if (k.D <= 1024) return launch_fwd_as<true, 2, XBF, YBF, STREAM>(k, s);
+    if (k.D <= 4096) return launch_fwd_as<false, 1, XBF, YBF, STREAM>(k, s);
+    if (k.D <= 8192) return launch_fwd_as<false, 2, XBF, YBF, STREAM>(k, s);
+    return launch_fwd_as<false, 4, XBF, YBF, STREAM>(k, s);
   }
+}
+template <bool BWD, bool XBF, bool YBF>
+int launch_norm_of(const NormK& k, float* means, hipStream_t s) {
+  if (k.D <= NORM_MOST) {
+    const bool stream = k.M * k.D * ((XBF ? 2 : 4) + (YBF ? 2 : 4)) > NORM_STREAM;
+    return stream ? launch_norm_rows<BWD, XBF, YBF, true>(k, s) : launch_norm_rows<BWD, XBF, YBF, false>(k, s);
+  }
+  const unsigned groups = (unsigned)(BWD ? bwd_groups(k.M, k.D) : fwd_groups(k.M, k.D));
   if constexpr (BWD) {
     if (k.Y) {
       GL_LAUNCH(GL_KERNEL_NORM_BWD, (norm_wide_kernel<XBF, YBF, true>), dim3((unsigned)least(k.M, 2 * CUS)), dim3(WIDE_T), 0, s,
                 k, means);
       GL_CHECK_LAUNCH();
     }
-    GL_LAUNCH(GL_KERNEL_NORM_BWD, (norm_wide_dx_kernel<XBF, YBF>), dim3((unsigned)groups, (unsigned)ceil_div(k.D, 2048)),
+    GL_LAUNCH(GL_KERNEL_NORM_BWD, (norm_wide_dx_kernel<XBF, YBF>), dim3(groups, (unsigned)ceil_div(k.D, 2048)),
               dim3(256), 0, s, k, (const float*)means);
   } else {
-    GL_LAUNCH(GL_KERNEL_NORM, (norm_wide_kernel<XBF, YBF, false>), dim3((unsigned)groups), dim3(WIDE_T), 0, s, k, means);
+    GL_LAUNCH(GL_KERNEL_NORM, (norm_wide_kernel<XBF, YBF, false>), dim3(groups), dim3(WIDE_T), 0, s, k, means);
   }
   GL_CHECK_LAUNCH();
   return 0;
 }
 template <bool BWD>
-int launch_norm(const NormK& k, int x_dtype, int y_dtype, int groups, float* means, hipStream_t s) {
+int launch_norm(const NormK& k, int x_dtype, int y_dtype, float* means, hipStream_t s) {
   const bool y = y_dtype == GL_DTYPE_BF16;
   if (x_dtype == GL_DTYPE_BF16)
-    return y ? launch_norm_of<BWD, true, true>(k, groups, means, s) : launch_norm_of<BWD, true, false>(k, groups, means, s);
-  return y ? launch_norm_of<BWD, false, true>(k, groups, means, s) : launch_norm_of<BWD, false, false>(k, groups, means, s);
+    return y ? launch_norm_of<BWD, true, true>(k, means, s) : launch_norm_of<BWD, true, false>(k, means, s);
+  return y ? launch_norm_of<BWD, false, true>(k, means, s) : launch_norm_of<BWD, false, false>(k, means, s);
 }
 
 bool dtype_ok(int d) { return d == GL_DTYPE_F32 || d == GL_DTYPE_BF16; }
@@ -434,7 +549,7 @@ size_t part_bytes(const GlNormBwdArgs* a) {
   return a->dweight || a->dbias ? (size_t)round_up((long long)bwd_groups(a->M, a->D) * 8 * a->D, 256) : 0;
 }
 size_t bwd_bytes(const GlNormBwdArgs* a) {
-  return part_bytes(a) + (norm_form(a->D) == NORM_WIDE && a->dX ? (size_t)round_up(a->M * 8, 256) : 0);
+  return part_bytes(a) + (a->D > NORM_MOST && a->dX ? (size_t)round_up(a->M * 8, 256) : 0);
 }
 
 }  // namespace
@@ -458,7 +573,7 @@ extern "C" int gl_norm_fwd(const GlNormArgs* a, void* stream) {
   k.D = a->D;
   k.w_bf = a->w_dtype == GL_DTYPE_BF16;
   k.eps = a->eps;
-  return launch_norm<false>(k, a->x_dtype, a->y_dtype, fwd_groups(a->M, a->D), nullptr, (hipStream_t)stream);
+  return launch_norm<false>(k, a->x_dtype, a->y_dtype, nullptr, (hipStream_t)stream);
 }
 
 extern "C" int gl_norm_bwd_workspace(const GlNormBwdArgs* a, size_t* bytes) {
@@ -489,7 +604,7 @@ extern "C" int gl_norm_bwd(const GlNormBwdArgs* a, void* stream) {
   k.M = a->M;
   k.D = a->D;
   k.w_bf = a->w_dtype == GL_DTYPE_BF16;
-  GL_TRY(launch_norm<true>(k, a->x_dtype, a->dy_dtype, groups, (float*)((char*)a->ws + part), s));
+  GL_TRY(launch_norm<true>(k, a->x_dtype, a->dy_dtype, (float*)((char*)a->ws + part), s));
   if (part) {
     GL_LAUNCH(GL_KERNEL_NORM_DW, norm_dw_kernel, dim3((unsigned)ceil_div(2LL * a->D, 64)), dim3(1024), 0, s,
               (const float*)k.part, groups, a->D, a->dweight, a->dbias, (int)(a->g_dtype == GL_DTYPE_BF16), a->accumulate);

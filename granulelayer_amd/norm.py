@@ -30,7 +30,7 @@ def _check(x, weight, bias, eps, out_dtype):
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        if tuple(t.shape) != (D,):
+        if t.shape != (D,):
             raise ValueError(f"{name} must be [{D}] (got {tuple(t.shape)})")
         if t.dtype not in _DTYPES:
             raise TypeError(f"{name} must be float32 or bfloat16 (got {t.dtype})")
@@ -53,17 +53,27 @@ class LayerNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, w, stats = ctx.saved_tensors
-        b = ctx.bias
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        mg_w, mg_b, use_main = _main_grads(w, b, need_w, need_b)
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
-        dw = mg_w if use_main else (torch.empty(w.shape, device=x.device, dtype=w.dtype) if need_w else None)
-        db = mg_b if use_main else (torch.empty(b.shape, device=x.device, dtype=b.dtype) if need_b else None)
-        backend_for(x.device).norm_backward(dy.resolve_neg(), x, w, stats, dx, dw, db, use_main)
-        return dx, None if use_main else dw, None if use_main else db, None, None
+        # what once_differentiable adds is needed where a graph of the backward is made
+        return _graph_gradients(ctx, dy) if torch.is_grad_enabled() else _gradients(ctx, dy)
+
+
+def _gradients(ctx, dy):
+    x, w, stats = ctx.saved_tensors
+    b = ctx.bias
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+    mg_w, mg_b, use_main = _main_grads(w, b, need_w, need_b)
+    if use_main:
+        dw, db = mg_w, mg_b
+    else:
+        dw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if need_w else None
+        db = torch.empty(b.shape, device=x.device, dtype=b.dtype) if need_b else None
+    backend_for(x.device).norm_backward(dy.resolve_neg(), x, w, stats, dx, dw, db, use_main)
+    return dx, None if use_main else dw, None if use_main else db, None, None
+
+
+_graph_gradients = once_differentiable(_gradients)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
