@@ -101,7 +101,6 @@ class HipBackend:
         self.lib = lib or N.library()
         # stage only each pool's input window in LDS when the windows are narrow (same results)
         self.window_staging = window_staging
-        self._norm_fwd, self._norm_bwd = self.lib.entry("gl_norm_fwd"), self.lib.entry("gl_norm_bwd")
         self._norm_bytes = functools.lru_cache(256)(self._norm_bytes_of)
 
     @classmethod
@@ -526,6 +525,9 @@ class HipBackend:
             self.lib.call("gl_dense_bwd", ctypes.byref(a), _stream(dev))
 
     # ------------------------------------------------------------------ layer norm
+    _norm_fwd = functools.cached_property(lambda self: self.lib.entry("gl_norm_fwd"))
+    _norm_bwd = functools.cached_property(lambda self: self.lib.entry("gl_norm_bwd"))
+
     def norm_forward(self, x, w, b, eps, out_dtype, keep):
         """(y [M, D] of ``out_dtype``, what the backward takes: [M, 2] fp32 with ``keep``) of x [M, D], w and b [D]
         of one dtype or None."""
