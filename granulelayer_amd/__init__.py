@@ -10,11 +10,13 @@ library granulelayer_amd/lib/libgranulelayer_amd.so through its C ABI
 Beside them, without a counterpart in the reference: ``DenseProjection`` / ``dense_projection`` (a dense
 product with bias, activation and residual in its epilogue) and ``pack_activation`` /
 ``PackedActivation`` (activations kept in 8 bits, also ``activation_checkpoint="int8"`` of the layers),
-``LayerNorm`` / ``layer_norm``.
+``LayerNorm`` / ``layer_norm``, and ``DenseCrossEntropy`` / ``dense_cross_entropy`` (the loss of a dense head over
+many classes, without its logits).
 """
 from .activations8 import PackedActivation, pack_activation
 from .config import LevelSpec, PhysicalPlan, PoolingConfig
 from .cover_topk16 import CoverTopK16Layer
+from .cross_entropy import DenseCrossEntropy, dense_cross_entropy
 from .dense import DenseProjection, dense_projection
 from .layer import SparsePoolingLayer
 from .layout import SparseLayout, init_parameters
@@ -23,4 +25,4 @@ from .optim import FusedAdamW
 
 __all__ = ["SparsePoolingLayer", "PoolingConfig", "LevelSpec", "PhysicalPlan", "SparseLayout", "init_parameters",
            "CoverTopK16Layer", "FusedAdamW", "DenseProjection", "dense_projection", "PackedActivation", "pack_activation",
-           "LayerNorm", "layer_norm"]
+           "LayerNorm", "layer_norm", "DenseCrossEntropy", "dense_cross_entropy"]

@@ -20,6 +20,7 @@ GL_ACT = {"identity": 0, "relu": 1, "gelu": 2}
 GL_POOL = {"mean": 0, "sum": 1, "max": 2, "topk_mean": 3, "logmeanexp": 4, "power_mean": 5, "softmax_weighted": 6}
 GL_DTYPE_F32, GL_DTYPE_BF16 = 0, 1
 GL_MOMENTS_INT8 = 2
+GL_CE = {"none": 0, "mean": 1, "sum": 2}
 GL_KEEP = {"none": 0, "sign": 1, "z": 2, "z8": 3}
 DENSE_MAX_FEATURES = 1 << 20  # GL_DENSE_MAX_FEATURES
 GL_ERR_WORKSPACE = -3
@@ -106,9 +107,22 @@ class GlNormBwdArgs(ctypes.Structure):
                 ("dy_dtype", _I32), ("g_dtype", _I32), ("accumulate", _I32), ("ws", _P), ("ws_bytes", _SZ)]
 
 
-# gl_struct_layout ids 0..11
+class GlCeArgs(ctypes.Structure):
+    _fields_ = [("X", _P), ("sx", _I64), ("W", _P), ("sw", _I64), ("bias", _P), ("target", _P), ("ignore_index", _I64),
+                ("M", _I64), ("N", _I32), ("K", _I32), ("dtype", _I32), ("reduction", _I32), ("loss", _P), ("kept", _P),
+                ("ws", _P), ("ws_bytes", _SZ)]
+
+
+class GlCeBwdArgs(ctypes.Structure):
+    _fields_ = [("X", _P), ("sx", _I64), ("W", _P), ("sw", _I64), ("bias", _P), ("target", _P), ("ignore_index", _I64),
+                ("M", _I64), ("N", _I32), ("K", _I32), ("dtype", _I32), ("reduction", _I32), ("kept", _P), ("dloss", _P),
+                ("sdl", _I64), ("dX", _P), ("dW", _P), ("db", _P), ("g_dtype", _I32), ("accumulate", _I32),
+                ("piece_bytes", _SZ), ("ws", _P), ("ws_bytes", _SZ)]
+
+
+# gl_struct_layout ids 0..13
 STRUCTS = (GlFwdArgs, GlBwdArgs, GlEdgeArgs, GlAdamArgs, GlCoverArgs, GlPack8Args, GlDenseArgs, GlDenseBwdArgs,
-           GlAdamTensor, GlAdamManyArgs, GlNormArgs, GlNormBwdArgs)
+           GlAdamTensor, GlAdamManyArgs, GlNormArgs, GlNormBwdArgs, GlCeArgs, GlCeBwdArgs)
 # every symbol include/granulelayer_amd.h declares
 EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_workspace", "gl_fwd", "gl_fwd_static",
            "gl_fwd_mask_bytes",
@@ -117,7 +131,7 @@ EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_work
            "gl_sched_build", "gl_window_build_host", "gl_window_build", "gl_cover_select", "gl_trace_begin",
            "gl_trace_end", "gl_pack8", "gl_unpack8", "gl_dense_fwd_workspace", "gl_dense_fwd", "gl_dense_bwd_workspace",
            "gl_dense_bwd", "gl_adam_many", "gl_adam_values", "gl_norm_fwd", "gl_norm_bwd_workspace",
-           "gl_norm_bwd")
+           "gl_norm_bwd", "gl_ce_fwd_workspace", "gl_ce_fwd", "gl_ce_bwd_workspace", "gl_ce_bwd")
 KERNEL_NAMES = {1: "tile_x_kernel", 2: "fwd_kernel", 3: "fwd_finalize_kernel", 4: "c1t_kernel", 5: "bwd_w_kernel",
                 6: "dx_kernel", 7: "dx_reduce_kernel", 8: "adam_kernel", 9: "edges_build", 10: "fwd_kernel_win",
                 11: "bwd_w_kernel_win", 12: "max_events_dw_kernel", 13: "max_events_dx_kernel",
@@ -125,7 +139,7 @@ KERNEL_NAMES = {1: "tile_x_kernel", 2: "fwd_kernel", 3: "fwd_finalize_kernel", 4
                 17: "dx_dma_kernel", 18: "pack8_kernel", 19: "unpack8_kernel", 20: "dense_tile_kernel",
                 21: "dense_few_kernel", 22: "dense_join_kernel", 23: "dense_dz_kernel", 24: "dense_db_kernel",
                 25: "dense_align_kernel", 26: "adam_values_kernel", 27: "norm_fwd_kernel", 28: "norm_bwd_kernel",
-                29: "norm_dw_kernel"}
+                29: "norm_dw_kernel", 30: "ce_stats_kernel", 31: "ce_grad_kernel", 32: "ce_gather_kernel", 33: "ce_rows_kernel"}
 
 
 class NativeError(RuntimeError):
@@ -166,12 +180,14 @@ class Library:
                          ("gl_edges_build", GlEdgeArgs), ("gl_adam", GlAdamArgs), ("gl_cover_select", GlCoverArgs), ("gl_pack8", GlPack8Args), ("gl_unpack8", GlPack8Args),
                          ("gl_dense_fwd", GlDenseArgs), ("gl_dense_bwd", GlDenseBwdArgs),
                          ("gl_adam_many", GlAdamManyArgs), ("gl_adam_values", GlAdamManyArgs),
-                         ("gl_norm_fwd", GlNormArgs), ("gl_norm_bwd", GlNormBwdArgs)):
+                         ("gl_norm_fwd", GlNormArgs), ("gl_norm_bwd", GlNormBwdArgs),
+                         ("gl_ce_fwd", GlCeArgs), ("gl_ce_bwd", GlCeBwdArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), _P]
         for name, st in (("gl_fwd_workspace", GlFwdArgs), ("gl_bwd_workspace", GlBwdArgs),
                          ("gl_dense_fwd_workspace", GlDenseArgs), ("gl_dense_bwd_workspace", GlDenseBwdArgs),
-                         ("gl_norm_bwd_workspace", GlNormBwdArgs)):
+                         ("gl_norm_bwd_workspace", GlNormBwdArgs),
+                         ("gl_ce_fwd_workspace", GlCeArgs), ("gl_ce_bwd_workspace", GlCeBwdArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), ctypes.POINTER(_SZ)]
         L.gl_trace_begin.restype = ctypes.c_int

@@ -101,7 +101,10 @@ class HipBackend:
         self.lib = lib or N.library()
         # stage only each pool's input window in LDS when the windows are narrow (same results)
         self.window_staging = window_staging
+        # workspaces' sizes by what decides them
         self._norm_bytes = functools.lru_cache(256)(self._norm_bytes_of)
+        self._ce_bytes = functools.lru_cache(256)(self._ce_bytes_of)
+        self._ce_bwd_bytes = functools.lru_cache(256)(self._ce_bwd_bytes_of)
 
     @classmethod
     def get(cls) -> "HipBackend":
@@ -568,6 +571,68 @@ class HipBackend:
         a = N.GlNormBwdArgs(dY=16, X=16, stats=16, sdy=D, sx=D, dX=16 * dx, dweight=16 * sums, M=M, D=D)
         return self.lib.size_query("gl_norm_bwd_workspace", a)
 
+    # ------------------------------------------------------------------ cross entropy of a dense head
+    _ce_fwd = functools.cached_property(lambda self: self.lib.entry("gl_ce_fwd"))
+    _ce_bwd = functools.cached_property(lambda self: self.lib.entry("gl_ce_bwd"))
+
+    def ce_forward(self, x, w, b, target, reduction, ignore_index, keep):
+        """(loss, what the backward takes with ``keep``) of x [M, K], w [N, K], b [N] or None (all of one dtype) and
+        target [M] (contiguous int64)."""
+        x, code, sx = _x_operand(x.resolve_neg())
+        w, _, sw = _x_operand(w.resolve_neg())
+        M, K = x.shape
+        F = w.shape[0]
+        dev = x.device
+        if b is not None:
+            b = b.resolve_neg().contiguous()
+        kept = torch.empty(4 + 5 * M, device=dev, dtype=torch.int32) if keep else None
+        if M == 0:
+            return torch.zeros(() if reduction != "none" else 0, device=dev), kept
+        loss = torch.empty(() if reduction != "none" else M, device=dev)
+        need = self._ce_bytes(M, F, K, code, x.data_ptr() % 16, sx, w.data_ptr() % 16, sw, N.GL_CE[reduction], keep)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        a = _CE(x.data_ptr(), sx, w.data_ptr(), sw, _ptr(b), target.data_ptr(), ignore_index, M, F, K, code,
+                N.GL_CE[reduction], loss.data_ptr(), _ptr(kept), ws.data_ptr(), need)
+        with _on(dev):
+            self._ce_fwd(a, _stream(dev))
+        return loss, kept
+
+    def ce_backward(self, dloss, x, w, b, target, reduction, ignore_index, kept, dx, dw, db, accumulate, piece_bytes=0):
+        """Gradients of ``ce_forward`` into dx [M, K] (x's dtype), dw [N, K] and db [N] (w's dtype, or fp32 and added
+        to with ``accumulate``); None for what is not needed."""
+        x, code, sx = _x_operand(x.resolve_neg())
+        w, _, sw = _x_operand(w.resolve_neg())
+        M, K = x.shape
+        F = w.shape[0]
+        dev = x.device
+        if b is not None:
+            b = b.resolve_neg().contiguous()
+        if M == 0:  # sums over no rows
+            for t in (dw, db):
+                if t is not None and not accumulate:
+                    t.zero_()
+            return
+        if dloss.dtype != torch.float32:
+            dloss = dloss.float()
+        need = self._ce_bwd_bytes(M, F, K, code, w.data_ptr() % 16, sw, dx is not None, dw is not None, db is not None,
+                                  piece_bytes)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        a = _CE_BWD(x.data_ptr(), sx, w.data_ptr(), sw, _ptr(b), target.data_ptr(), ignore_index, M, F, K, code,
+                    N.GL_CE[reduction], kept.data_ptr(), dloss.data_ptr(), dloss.stride(0) if dloss.dim() else 0, _ptr(dx),
+                    _ptr(dw), _ptr(db), N.GL_DTYPE_F32 if accumulate else code, accumulate, piece_bytes, ws.data_ptr(), need)
+        with _on(dev):
+            self._ce_bwd(a, _stream(dev))
+
+    def _ce_bytes_of(self, M, F, K, code, x16, sx, w16, sw, reduction, keep):
+        a = N.GlCeArgs(X=4096 + x16, sx=sx, W=4096 + w16, sw=sw, target=4096, M=M, N=F, K=K, dtype=code,
+                       reduction=reduction, loss=4096, kept=4096 * keep)
+        return self.lib.size_query("gl_ce_fwd_workspace", a)
+
+    def _ce_bwd_bytes_of(self, M, F, K, code, w16, sw, dx, dw, db, piece_bytes):
+        a = N.GlCeBwdArgs(X=4096, sx=K, W=4096 + w16, sw=sw, target=4096, M=M, N=F, K=K, dtype=code, kept=4096, dloss=4096,
+                          dX=4096 * dx, dW=4096 * dw, db=4096 * db, g_dtype=code, piece_bytes=piece_bytes)
+        return self.lib.size_query("gl_ce_bwd_workspace", a)
+
 
 def _norm_params(w, b):
     """Contiguous w and b and their dtype's code."""
@@ -579,6 +644,7 @@ def _norm_params(w, b):
 
 _DENSE_DTYPES = {torch.float32: N.GL_DTYPE_F32, torch.bfloat16: N.GL_DTYPE_BF16}
 _NORM, _NORM_BWD = N.packer(N.GlNormArgs), N.packer(N.GlNormBwdArgs)
+_CE, _CE_BWD = N.packer(N.GlCeArgs), N.packer(N.GlCeBwdArgs)
 _MOMENTS = {**_DENSE_DTYPES, torch.int8: N.GL_MOMENTS_INT8}
 adam_row = N.packer(N.GlAdamTensor)  # p, g, m, v, master, m_scale, v_scale, n, seed, bc1, bc2
 

@@ -52,6 +52,26 @@ struct DenseK {
   DenseEpi e;
 };
 
+// What a product's kernel does besides: nothing; take the number of its rows (of C, or where both operands
+// are RS of the reduction) from device memory; and the two products of the softmax cross entropy, logits = X W^T
+// of a piece of the classes, that leave a tile's softmax statistics or their gradient and no logits (gl_ce.hip).
+enum { DENSE_PLAIN, DENSE_ROWS, DENSE_CE_STATS, DENSE_CE_GRAD };
+struct DenseRowsK : DenseK {
+  const int* rows;           // or null: as the sizes say
+  // statistics
+  const long long* target;
+  const int* index;          // row of `target` of every row of X, or null: its own
+  float* target_logit;       // [M]; like all logits behind the product in units of log 2
+  float* stats;              // [M][tiles_n][2]: the tile's largest logit but the target's, and the sum of 2^(logit - it)
+  // gradient
+  const uv4* row_info;       // [M]: the largest logit; factor of 2^(logit - it); the target; the gradient at it
+  int first;                 // class of the product's first column
+  float* col_sums;           // [tiles_m * waves along m][N], or null
+  int pitch;                 // of C's rows; columns from N to there are zeros
+};
+template <int KIND> struct DenseArgs { typedef DenseRowsK type; };
+template <> struct DenseArgs<DENSE_PLAIN> { typedef DenseK type; };
+
 // ---- activations -----------------------------------------------------------------------------------
 // GELU from the normal distribution's upper tail: with a = |z| and Q(a) = 1 - Phi(a),
 //     gelu(z) = max(z, 0) - a Q(a)
@@ -462,8 +482,104 @@ __device__ __forceinline__ void copies_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <int ES, int MS, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC>
-__global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
+// Over the 64 / MS lanes that hold a row's sums.
+template <int MS, typename OP>
+__device__ __forceinline__ float over_row(float v, OP op) {
+  if constexpr (MS == 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  }
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+constexpr float LOG2E = 1.44269504f;
+// A bias in units of log 2.  The lowest finite one stays a number: logits of it and nothing else have a softmax.
+__device__ __forceinline__ float ce_bias(float b) {
+  constexpr float MOST = 3.402823466e38f;
+  return __builtin_fabsf(b) <= MOST ? __builtin_amdgcn_fmed3f(b * LOG2E, -MOST, MOST) : b;
+}
+__device__ __forceinline__ int n_pitch(const DenseRowsK& a) { return a.pitch; }
+__device__ __forceinline__ int n_pitch(const DenseK&) { return 0; }
+
+// DENSE_CE_STATS: every row's largest logit of the tile and the sum of 2^(logit - it), both without the target's, and the
+// target's where it is in the tile.  All from the sums' registers: a lane has MS columns of its row, the lanes of a row are joined by
+// two (or one) swaps, the waves of a row through LDS (BM rows of WN pairs, free behind the caller's barrier).
+// Columns behind N are -inf; a tile of nothing else has the largest logit -inf and the sum 0.  A NaN is left out of the
+// largest and makes the sum NaN, as +inf does.
+template <int MS, int BM, int BN, int WM, int WN, int TM, int TN>
+__device__ __forceinline__ void ce_stats(const DenseRowsK& a, long long M, int tm, int tn,
+                                         const typename Sums<MS>::type (&acc)[TM][TN], float (*lds)[2]) {
+  constexpr int G = MS * MS / 256;  // groups of four columns in a lane's sums of an instruction
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w / WN, wn = w % WN;
+  const int n0 = tn * BN + wn * 64, lane_col = 4 * (l / MS);
+  const long long m0 = (long long)tm * BM;
+  const bool inside = tn * BN + BN <= a.e.N;
+  float bias[TN][4 * G];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float b[4];
+      dense_bias(a.e, n0 + MS * j + 8 * g + lane_col, b);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) bias[j][4 * g + x] = ce_bias(b[x]);
+    }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int row = wm * TM * MS + i * MS + l % MS;
+    const long long m = m0 + row;
+    long long t = -1;
+    if (m < M) t = a.target[a.index ? a.index[m] : m] - n0;
+    const int at = t >= 0 && t < 64 ? (int)t - lane_col : -64;  // of this lane's columns
+    float v[TN][4 * G], top = -__builtin_inff(), picked = 0.f;
+    bool here = false;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int x = 0; x < 4 * G; ++x) {
+        const int col = MS * j + 8 * (x / 4) + x % 4;
+        v[j][x] = __builtin_fmaf(acc[i][j][x], LOG2E, bias[j][x]);
+        if (!inside && n0 + lane_col + col >= a.e.N) v[j][x] = -__builtin_inff();
+        if (at == col) {
+          picked = v[j][x];
+          here = true;
+          v[j][x] = -__builtin_inff();
+        }
+        top = __builtin_fmaxf(top, v[j][x]);
+      }
+    top = over_row<MS>(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+    const float ref = top == -__builtin_inff() ? 0.f : top;
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int x = 0; x < 4 * G; ++x) s += __builtin_amdgcn_exp2f(v[j][x] - ref);
+    s = over_row<MS>(s, [](float x, float y) { return x + y; });
+    if (here) a.target_logit[m] = picked;
+    if (l < MS) {
+      lds[wn * BM + row][0] = top;
+      lds[wn * BM + row][1] = s;
+    }
+  }
+  __syncthreads();
+  for (int row = threadIdx.x; row < BM; row += 64 * WM * WN) {
+    const long long m = m0 + row;
+    if (m >= M) return;
+    float top = lds[row][0];
+#pragma unroll
+    for (int k = 1; k < WN; ++k) top = __builtin_fmaxf(top, lds[k * BM + row][0]);
+    const float ref = top == -__builtin_inff() ? 0.f : top;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < WN; ++k) s = __builtin_fmaf(lds[k * BM + row][1], __builtin_amdgcn_exp2f(lds[k * BM + row][0] - ref), s);
+    float* to = a.stats + 2 * (m * a.tiles_n + tn);
+    to[0] = top;
+    to[1] = s;
+  }
+}
+
+template <int ES, int MS, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC, int KIND = DENSE_PLAIN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(typename DenseArgs<KIND>::type a) {
   constexpr int NW = WM * WN, TM = BM / WM / MS, TN = BN / WN / MS;  // fragments of a wave
   typedef Side<ES, BM, NW, PRC> SP;
   typedef Side<ES, BN, NW, QRC> SQ;
@@ -472,15 +588,36 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   int tm, tn, split;
   tile_of(blockIdx.x, gridDim.x, a.tiles_m, a.tiles_n, tm, tn, split);
   const int k0 = split * a.steps_per_split;
-  const int nk = min(a.steps - k0, a.steps_per_split);
   const long long m0 = (long long)tm * BM;
   const int n0 = tn * BN;
+  long long M = a.e.M, R = a.R;
+  int nk = min(a.steps - k0, a.steps_per_split);
+  if constexpr (KIND != DENSE_PLAIN) {
+    if (a.rows) {
+      const long long rows = *a.rows;
+      if constexpr (PRC) {
+        M = rows < M ? rows : M;
+        if (m0 >= M) {  // of the whole workgroup
+          if constexpr (KIND == DENSE_CE_GRAD) {
+            if (a.col_sums)
+              for (int i = threadIdx.x; i < WM * BN; i += 64 * WM * WN)
+                if (n0 + i % BN < a.e.N) a.col_sums[((long long)tm * WM + i / BN) * a.e.N + n0 + i % BN] = 0.f;
+          }
+          return;
+        }
+      } else {  // stages of zeros where a split has no rows
+        R = rows < R ? rows : R;
+        const int steps = (int)((R * ES + DENSE_BK - 1) / DENSE_BK);
+        nk = max(1, min(steps - k0, a.steps_per_split));
+      }
+    }
+  }
   const int w = threadIdx.x >> 6, wm = w / WN, wn = w % WN;
 
   SP sp;
   SQ sq;
-  sp.init(a.P, a.ldp, m0, a.e.M, a.R, k0);
-  sq.init(a.Q, a.ldq, n0, a.e.N, a.R, k0);
+  sp.init(a.P, a.ldp, m0, M, R, k0);
+  sq.init(a.Q, a.ldq, n0, a.e.N, R, k0);
   Reader<ES, MS, BM, PRC> rp;
   Reader<ES, MS, BN, QRC> rq;
   rp.init(wm * TM * MS);
@@ -591,7 +728,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   // are in registers four together, so types, kinds and edges are decided once for all of them.  (A row at a
   // time, with its loads and branches, took 33,000 clocks a tile, as long as 12 stages of products.)
   static_assert(TN * MS == 64 && TM * MS % 32 == 0 && NW * 32 * 68 * 4 <= LDS, "a wave's rows of 64 columns");
-  constexpr bool FORWARD = PRC && QRC;  // bias, activation, residual and what is kept; else sums as they are
+  constexpr bool FORWARD = PRC && QRC && KIND == DENSE_PLAIN;  // bias, activation, residual and what is kept; else sums as they are
   constexpr int ROWS = 4;               // of a lane at a time, 4 apart
   // The caches need not keep the large tile's results and what is added to them, but the operands of the tiles that
   // still run.  By tile, not by the outputs' size.  With it and without, us: 8192 x 8192 over 4096 with an fp32 residual
@@ -599,20 +736,35 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
   // x 4096 over 1024 no different (161 to 169), that forward alone 43.5 / 45.3.  What it loses: a next product that reads 32 MB of
   // results at once, 4096 x 1024 -> 4096 -> 1024 in a graph 80 / 75.  The smaller tiles go without: fp32 2048 x 4096
   // over 1024 takes 2% longer with it.
-  constexpr bool STREAM = BM * BN == 65536;
+  constexpr bool STREAM = BM * BN == 65536 && KIND != DENSE_CE_GRAD;
   copies_barrier<0>();
+  if constexpr (KIND == DENSE_CE_STATS) {
+    ce_stats<MS, BM, BN, WM, WN, TM, TN>(a, M, tm, tn, acc, reinterpret_cast<float(*)[2]>(smem));
+    return;
+  }
   const int l = threadIdx.x & 63;
+  uv4* info = reinterpret_cast<uv4*>(smem + NW * 32 * 68 * 4);  // DENSE_CE_GRAD: the tile's rows
+  if constexpr (KIND == DENSE_CE_GRAD) {
+    static_assert(NW * 32 * 68 * 4 + BM * 16 <= LDS, "the rows' place");
+    for (int r = threadIdx.x; r < BM; r += 64 * NW) info[r] = m0 + r < M ? a.row_info[m0 + r] : uv4{0u, 0u, 0u, 0u};
+    __syncthreads();
+  }
   float* own = reinterpret_cast<float*>(smem) + w * 32 * 68;
-  const bool split_up = a.part != nullptr;
-  const Added added = split_up ? Added{nullptr, 0, false} : dense_added(a.e);
+  const bool split_up = KIND != DENSE_CE_GRAD && a.part != nullptr;
+  const Added added = split_up || KIND == DENSE_CE_GRAD ? Added{nullptr, 0, false} : dense_added(a.e);
   char* C = split_up ? (char*)(a.part + (long long)split * a.e.M * a.e.N) : (char*)a.e.C;
   const bool c_bf = !split_up && a.e.c_bf;
   const long long c_step = (split_up ? a.e.N : a.e.sc) * (c_bf ? 2 : 4);
-  const bool inside = m0 + BM <= a.e.M && n0 + BN <= a.e.N;
+  const bool inside = m0 + BM <= M && n0 + BN <= a.e.N;
   const int n = n0 + wn * 64 + (l & 15) * 4, there = a.e.N - n;
   const long long mw = m0 + wm * TM * MS + (l >> 4);
   float bias[4];
-  if constexpr (FORWARD) dense_bias(a.e, n, bias);
+  if constexpr (FORWARD || KIND == DENSE_CE_GRAD) dense_bias(a.e, n, bias);
+  if constexpr (KIND == DENSE_CE_GRAD) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[j] = ce_bias(bias[j]);
+  }
+  float col[4] = {0.f, 0.f, 0.f, 0.f};  // DENSE_CE_GRAD: of this lane's columns
   uv4 r[ROWS];
   auto load_rows = [&](long long m) {
     const char* p = added.p + m * added.step + (long long)n * (added.bf ? 2 : 4);
@@ -635,7 +787,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
 #pragma unroll
       for (int x = 0; x < ROWS; ++x) {
         r[x] = uv4{0u, 0u, 0u, 0u};
-        if (m + 4 * x < a.e.M && there > 0) r[x] = load_added(p + 4 * x * added.step, added.bf, there);
+        if (m + 4 * x < M && there > 0) r[x] = load_added(p + 4 * x * added.step, added.bf, there);
       }
     }
   };
@@ -672,6 +824,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
       if constexpr (FORWARD) {
         if (!split_up) dense_forward<ROWS>(a.e, mi, 4, n, v, bias);
       }
+      if constexpr (KIND == DENSE_CE_GRAD) {
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x) {
+          const uv4 q = info[wm * TM * MS + i * 32 + y + 4 * x + (l >> 4)];
+          const float top = __uint_as_float(q[0]), f = __uint_as_float(q[1]);
+          const int t = (int)q[2] - a.first - n;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(v[x][j], LOG2E, bias[j]) - top);
+            v[x][j] = f == 0.f || j >= there ? 0.f : t == j ? __uint_as_float(q[3]) : f * p;
+            col[j] += v[x][j];
+          }
+        }
+      }
       if (added.p) {
         if (added.bf) {
 #pragma unroll
@@ -690,10 +856,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(DenseK a) {
 #pragma unroll
         for (int x = 0; x < ROWS; ++x) store4<STREAM>(c + 4 * x * c_step, false, 0, 4, v[x]);
       } else {
+        const int width = KIND == DENSE_CE_GRAD ? n_pitch(a) - n : there;
 #pragma unroll
         for (int x = 0; x < ROWS; ++x)
-          if (mi + 4 * x < a.e.M && there > 0) store4(c + 4 * x * c_step, c_bf, 0, there, v[x]);
+          if (mi + 4 * x < M && width > 0) store4(c + 4 * x * c_step, c_bf, 0, width, v[x]);
       }
+    }
+  }
+  if constexpr (KIND == DENSE_CE_GRAD) {
+    if (a.col_sums) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) col[j] = over_row<16>(col[j], [](float x, float y) { return x + y; });
+      if (l < 16 && there > 0) store4(a.col_sums, false, ((long long)tm * WM + wm) * a.e.N + n, there, col);
     }
   }
 }
@@ -706,18 +880,19 @@ enum { DENSE_NT = 0, DENSE_NN = 1, DENSE_TN = 2 };  // P, Q: RC RC; RC RS; RS RS
 enum { DENSE_256 = 0, DENSE_256X128 = 1, DENSE_128 = 2, DENSE_128_DEEP = 3, DENSE_64 = 4, DENSE_TILES = 5 };
 constexpr int DENSE_BM[DENSE_TILES] = {256, 256, 128, 128, 64}, DENSE_BN[DENSE_TILES] = {256, 128, 128, 128, 128};
 
-template <int ES, int MS, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC>
-int launch_dense_tile_as(const DenseK& a, int splits, hipStream_t s) {
+template <int ES, int MS, int BM, int BN, int WM, int WN, int NSP, int NSQ, bool PRC, bool QRC, int KIND = DENSE_PLAIN>
+int launch_dense_tile_as(const typename DenseArgs<KIND>::type& a, int splits, hipStream_t s) {
+  constexpr auto kernel = dense_tile_kernel<ES, MS, BM, BN, WM, WN, NSP, NSQ, PRC, QRC, KIND>;
   constexpr size_t lds = (NSP * BM + NSQ * BN) * DENSE_BK;
   // the kernel's LDS limit is raised once a device
   static std::atomic<unsigned long long> raised{0};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return GL_ERR_DEVICE;
   if (!(raised.load(std::memory_order_relaxed) >> dev & 1)) {
-    GL_TRY(set_lds_limit((const void*)dense_tile_kernel<ES, MS, BM, BN, WM, WN, NSP, NSQ, PRC, QRC>, lds));
+    GL_TRY(set_lds_limit((const void*)kernel, lds));
     raised.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  GL_LAUNCH(GL_KERNEL_DENSE, (dense_tile_kernel<ES, MS, BM, BN, WM, WN, NSP, NSQ, PRC, QRC>),
+  GL_LAUNCH(KIND == DENSE_CE_STATS ? GL_KERNEL_CE_STATS : KIND == DENSE_CE_GRAD ? GL_KERNEL_CE_GRAD : GL_KERNEL_DENSE, kernel,
             dim3((unsigned)(a.tiles_m * a.tiles_n * splits)), dim3(64 * WM * WN), lds, s, a);
   GL_CHECK_LAUNCH();
   return 0;
@@ -730,6 +905,44 @@ int launch_dense_tile_of(int form, const DenseK& a, int splits, hipStream_t s) {
 }
 int launch_dense_tile_bf16(int form, int tile, const DenseK& a, int splits, hipStream_t s);
 int launch_dense_tile_f32(int form, int tile, const DenseK& a, int splits, hipStream_t s);
+// the kinds but DENSE_PLAIN; form: NT for the two of the cross entropy, NN or TN with DENSE_ROWS
+template <int ES, int MS, int BM, int BN, int WM, int WN, int NSP, int NSQ>
+int launch_rows_tile_of(int kind, int form, const DenseRowsK& a, int splits, hipStream_t s) {
+  if (kind == DENSE_CE_STATS) return launch_dense_tile_as<ES, MS, BM, BN, WM, WN, NSP, NSQ, true, true, DENSE_CE_STATS>(a, splits, s);
+  if (kind == DENSE_CE_GRAD) return launch_dense_tile_as<ES, MS, BM, BN, WM, WN, NSP, NSQ, true, true, DENSE_CE_GRAD>(a, splits, s);
+  if (form == DENSE_NN) return launch_dense_tile_as<ES, MS, BM, BN, WM, WN, NSP, NSQ, true, false, DENSE_ROWS>(a, splits, s);
+  return launch_dense_tile_as<ES, MS, BM, BN, WM, WN, NSP, NSQ, false, false, DENSE_ROWS>(a, splits, s);
+}
+int launch_rows_tile_bf16(int kind, int form, int tile, const DenseRowsK& a, int splits, hipStream_t s);
+int launch_rows_tile_f32(int kind, int form, int tile, const DenseRowsK& a, int splits, hipStream_t s);
+
+// ---- plans (gl_dense.hip) ----------------------------------------------------------------------------
+constexpr int es_of(int dtype) { return dtype == GL_DTYPE_BF16 ? 2 : 4; }
+inline long long padded(long long n) { return round_up(n, 8); }  // row of a copied or computed operand
+
+struct Operand {
+  const void* p;
+  long long ld;  // elements
+  long long rows;
+  int cols;
+  bool rc;       // reduction along the row
+  bool copied;   // through workspace
+};
+Operand operand(const void* p, long long ld, long long rows, int cols, bool rc, int es);
+size_t copy_bytes(const Operand& o, int es);
+// copies those of the operands (null or not) that need it to their places; they then are the copies
+int launch_align(Operand* o0, void* dst0, Operand* o1, void* dst1, int es, hipStream_t s);
+struct Product {
+  double us;  // what the plan expects
+  int tile, splits, steps_per_split, steps, tiles_m, tiles_n;
+  size_t part_bytes;
+};
+Product plan_product(int dtype, long long M, int N, long long R, int most_splits = 32);
+// rows: DENSE_ROWS (null: DENSE_PLAIN)
+int run_product(int dtype, int form, const Operand& p, const Operand& q, long long R, const Product& pl, void* part,
+                const DenseEpi& e, hipStream_t s, const int* rows = nullptr);
+DenseEpi store_epi(void* C, long long sc, int c_dtype, long long M, int N, int op_dtype, int accumulate);
+int launch_db(const float* part, long long chunks, int N, void* db, int g_dtype, int accumulate, hipStream_t s);
 
 // few rows (gl_dense_few.hip): the forward of up to DENSE_FEW_ROWS rows that keeps nothing
 constexpr int DENSE_FEW_ROWS = 64;

@@ -5,9 +5,6 @@ namespace gl {
 
 namespace {
 
-constexpr int es_of(int dtype) { return dtype == GL_DTYPE_BF16 ? 2 : 4; }
-inline long long padded(long long n) { return round_up(n, 8); }  // row of a copied or computed operand
-
 // ---- rows at 16-byte addresses --------------------------------------------------------------------
 // The tile kernel loads 16 bytes at a time straight into LDS.  An operand whose rows do not start at
 // 16-byte addresses, or (reduction along the row) end inside 16 bytes, is copied to rows of padded(cols)
@@ -41,31 +38,24 @@ __global__ __launch_bounds__(256) void dense_align_kernel(AlignK a) {
   for (int j = 0; j < 8; ++j) d[j] = v[j];
 }
 
-struct Operand {
-  const void* p;
-  long long ld;  // elements
-  long long rows;
-  int cols;
-  bool rc;       // reduction along the row
-  bool copied;   // through workspace
-};
 // Whether the tile kernel takes the operand as it is.  Its 32-bit offsets span 256 rows.
 inline bool in_place(const Operand& o, int es) {
   const long long ldb = o.ld * es;
   return ((uintptr_t)o.p & 15) == 0 && (o.rows == 1 || ldb % 16 == 0) && (!o.rc || (long long)o.cols * es % 16 == 0) &&
          ldb * 256 < (1LL << 31);
 }
-inline Operand operand(const void* p, long long ld, long long rows, int cols, bool rc, int es) {
+}  // namespace
+
+Operand operand(const void* p, long long ld, long long rows, int cols, bool rc, int es) {
   Operand o{p, rows == 1 ? cols : ld, rows, cols, rc, false};
   if (!in_place(o, es)) o.copied = true;
   if (rows == 1) o.ld = padded(cols);  // never stepped along; keeps the buffer's size whole
   return o;
 }
-inline size_t copy_bytes(const Operand& o, int es) {
+size_t copy_bytes(const Operand& o, int es) {
   return o.copied ? (size_t)round_up(o.rows * padded(o.cols) * es, 256) : 0;
 }
 
-// copies those of the operands (null or not) that need it to their places; they then are the copies
 int launch_align(Operand* o0, void* dst0, Operand* o1, void* dst1, int es, hipStream_t s) {
   AlignK k{};
   int n = 0, cols = 0;
@@ -94,6 +84,8 @@ int launch_align(Operand* o0, void* dst0, Operand* o1, void* dst1, int es, hipSt
   return 0;
 }
 
+namespace {
+
 // ---- the sums of a split product --------------------------------------------------------------------
 // A lane holds 4 neighbouring columns and adds the splits in their order, then the epilogue.  Bound by the sums'
 // bytes: 2 x 2048 x 1024 fp32 in 5.7 us (4.4 TB/s).
@@ -120,11 +112,6 @@ __global__ __launch_bounds__(256) void dense_join_kernel(const float* __restrict
 }
 
 // ---- plan of a product --------------------------------------------------------------------------------
-struct Product {
-  double us;  // what the plan expects
-  int tile, splits, steps_per_split, steps, tiles_m, tiles_n;
-  size_t part_bytes;
-};
 // What a tile costs, measured on whole problems of 16 to 256 stages: workgroups of a CU, microseconds of a stage
 // with one of them on each CU and with all, and of a tile's start and end.
 struct TileCost {
@@ -136,9 +123,11 @@ constexpr TileCost COST_BF16[DENSE_TILES] = {
 constexpr TileCost COST_F32[DENSE_TILES] = {
     {0, 0, 0, 0}, {0, 0, 0, 0}, {2, 2.15, 4.25, 6}, {1, 1.96, 1.96, 6}, {2, 1.10, 2.20, 5}};
 
+}  // namespace
+
 // Tile and splits of the reduction: the least of rounds x (stages x cost + ends), no less than the operands' bytes
 // take, plus for a split product its partial sums written and read (4 TB/s) and the launch that joins them.
-Product plan_product(int dtype, long long M, int N, long long R) {
+Product plan_product(int dtype, long long M, int N, long long R, int most_splits) {
   constexpr int CUS = 256;
   constexpr long long MAX_BLOCKS = 1LL << 23;  // a launch has fewer than 2^32 threads
   const TileCost* cost = dtype == GL_DTYPE_BF16 ? COST_BF16 : COST_F32;
@@ -149,7 +138,7 @@ Product plan_product(int dtype, long long M, int N, long long R) {
   for (int t = 0; t < DENSE_TILES; ++t) {
     const long long tm = (M + DENSE_BM[t] - 1) / DENSE_BM[t], tn = (N + DENSE_BN[t] - 1) / DENSE_BN[t];
     if (!cost[t].per_cu) continue;
-    for (long long s = 1; s <= 32 && s <= steps; s = s < 4 ? s + 1 : s * 2) {
+    for (long long s = 1; s <= most_splits && s <= steps; s = s < 4 ? s + 1 : s * 2) {
       const long long per = (steps + s - 1) / s, n = tm * tn * s, slots = CUS * cost[t].per_cu;
       if ((steps + per - 1) / per != s || n >= MAX_BLOCKS) continue;
       const double stage = n <= CUS ? cost[t].alone : cost[t].full;
@@ -166,9 +155,9 @@ Product plan_product(int dtype, long long M, int N, long long R) {
 }
 
 int run_product(int dtype, int form, const Operand& p, const Operand& q, long long R, const Product& pl, void* part,
-                const DenseEpi& e, hipStream_t s) {
+                const DenseEpi& e, hipStream_t s, const int* rows) {
   const int es = es_of(dtype);
-  DenseK k{};
+  DenseRowsK k{};
   k.P = p.p;
   k.Q = q.p;
   k.ldp = p.ld * es;
@@ -180,8 +169,10 @@ int run_product(int dtype, int form, const Operand& p, const Operand& q, long lo
   k.steps_per_split = pl.steps_per_split;
   k.part = pl.splits > 1 ? (float*)part : nullptr;
   k.e = e;
-  GL_TRY(dtype == GL_DTYPE_BF16 ? launch_dense_tile_bf16(form, pl.tile, k, pl.splits, s)
-                                : launch_dense_tile_f32(form, pl.tile, k, pl.splits, s));
+  k.rows = rows;
+  const bool bf = dtype == GL_DTYPE_BF16;
+  if (rows) GL_TRY(bf ? launch_rows_tile_bf16(DENSE_ROWS, form, pl.tile, k, pl.splits, s) : launch_rows_tile_f32(DENSE_ROWS, form, pl.tile, k, pl.splits, s));
+  else GL_TRY(bf ? launch_dense_tile_bf16(form, pl.tile, k, pl.splits, s) : launch_dense_tile_f32(form, pl.tile, k, pl.splits, s));
   if (pl.splits > 1) {
     const dim3 grid((unsigned)((e.M + 3) / 4), (unsigned)ceil_div(e.N, 256));
     GL_LAUNCH(GL_KERNEL_DENSE_JOIN, dense_join_kernel, grid, dim3(256), 0, s, (const float*)part, pl.splits, e);
@@ -189,6 +180,8 @@ int run_product(int dtype, int form, const Operand& p, const Operand& q, long lo
   }
   return 0;
 }
+
+namespace {
 
 // ---- dz = dY act'(z) and the sums of its columns -------------------------------------------------------
 constexpr int DZ_COLS = 256;  // of a workgroup: 32 lanes of 8 columns by 8 rows at a time
@@ -435,6 +428,8 @@ int launch_dz(const GlDenseBwdArgs* a, void* dz, float* part, hipStream_t s) {
   return o ? launch_dz_of<false, true>(a, dz, part, s) : launch_dz_of<false, false>(a, dz, part, s);
 }
 
+}  // namespace
+
 DenseEpi store_epi(void* C, long long sc, int c_dtype, long long M, int N, int op_dtype, int accumulate) {
   DenseEpi e{};
   e.C = C;
@@ -449,7 +444,12 @@ DenseEpi store_epi(void* C, long long sc, int c_dtype, long long M, int N, int o
   return e;
 }
 
-}  // namespace
+int launch_db(const float* part, long long chunks, int N, void* db, int g_dtype, int accumulate, hipStream_t s) {
+  GL_LAUNCH(GL_KERNEL_DENSE_DB, dense_db_kernel, dim3((unsigned)ceil_div(N, 32)), dim3(1024), 0, s, part, chunks, N, db,
+            (int)(g_dtype == GL_DTYPE_BF16), accumulate);
+  GL_CHECK_LAUNCH();
+  return 0;
+}
 
 }  // namespace gl
 
@@ -514,11 +514,7 @@ extern "C" int gl_dense_bwd(const GlDenseBwdArgs* a, void* stream) {
   void* dz = p.own_dz ? ws : nullptr;
   float* db_part = a->db ? (float*)(ws + p.off_db) : nullptr;
   if (dz || db_part) GL_TRY(launch_dz(a, dz, db_part, s));
-  if (a->db) {
-    GL_LAUNCH(GL_KERNEL_DENSE_DB, dense_db_kernel, dim3((unsigned)ceil_div(a->N, 32)), dim3(1024), 0, s, (const float*)db_part,
-              p.chunks, a->N, a->db, (int)(a->g_dtype == GL_DTYPE_BF16), a->accumulate);
-    GL_CHECK_LAUNCH();
-  }
+  if (a->db) GL_TRY(launch_db(db_part, p.chunks, a->N, a->db, a->g_dtype, a->accumulate, s));
   if (dz) p.dz_nn.p = p.dz_tn.p = dz;
   GL_TRY(launch_align(a->dW && a->X ? &p.x : nullptr, ws + p.off_x, a->dX ? &p.w : nullptr, ws + p.off_w, es, s));
   if (a->dX) {

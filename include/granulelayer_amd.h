@@ -225,7 +225,8 @@ int gl_cover_select(const GlCoverArgs* a, void* stream);
  * order) so a binding can refuse a mismatched library.  Replaces sp_abi_version /
  * sp_struct_layout (sparse_pooling/kernels/cuda/abi.cu:17-62, checked in runtime.py:103-120).
  * which: 0 GlFwdArgs, 1 GlBwdArgs, 2 GlEdgeArgs, 3 GlAdamArgs, 4 GlCoverArgs, 5 GlPack8Args, 6 GlDenseArgs,
- * 7 GlDenseBwdArgs, 8 GlAdamTensor, 9 GlAdamManyArgs, 10 GlNormArgs, 11 GlNormBwdArgs.  Returns the number of values written
+ * 7 GlDenseBwdArgs, 8 GlAdamTensor, 9 GlAdamManyArgs, 10 GlNormArgs, 11 GlNormBwdArgs,
+ * 12 GlCeArgs, 13 GlCeBwdArgs.  Returns the number of values written
  * (or needed, when n is too small), negative on an unknown struct. */
 int gl_abi_version(void);
 int gl_struct_layout(int which, long long* out, int n);
@@ -455,6 +456,65 @@ typedef struct GlNormBwdArgs {
 int gl_norm_bwd_workspace(const GlNormBwdArgs* a, size_t* bytes);
 int gl_norm_bwd(const GlNormBwdArgs* a, void* stream);
 
+/* ---- softmax cross entropy of a dense head --------------------------------------------------------
+ *
+ *   z = X W^T + bias,   loss[m] = log(sum over n of exp z[m,n]) - z[m,target[m]]
+ *
+ * over N classes, without the logits in memory.  Rows whose target is ignore_index have the loss 0 and no gradient,
+ * whatever else they hold; another target outside [0, N) makes the row's loss and all gradients it reaches NaN.  The
+ * mean is over the rows that count, 0 of none.  Operands as of the dense projection. */
+enum { GL_CE_NONE = 0, GL_CE_MEAN = 1, GL_CE_SUM = 2 };
+#define GL_CE_KEPT_WORDS(M) (4 + 5 * (size_t)(M)) /* 32-bit words that the forward keeps for the backward */
+typedef struct GlCeArgs {
+  const void* X;          /* [M, K] of `dtype` */
+  int64_t sx;
+  const void* W;          /* [N, K] of `dtype` */
+  int64_t sw;
+  const void* bias;       /* [N] of `dtype`, or NULL */
+  const int64_t* target;  /* [M] */
+  int64_t ignore_index;
+  int64_t M;              /* up to 2^24 */
+  int32_t N, K;           /* up to GL_DENSE_MAX_FEATURES */
+  int32_t dtype;
+  int32_t reduction;      /* GL_CE_* */
+  float* loss;            /* out: [M] with GL_CE_NONE, else one */
+  int32_t* kept;          /* out: GL_CE_KEPT_WORDS(M) words, or NULL */
+  void* ws;               /* 256-byte aligned */
+  size_t ws_bytes;
+} GlCeArgs;
+int gl_ce_fwd_workspace(const GlCeArgs* a, size_t* bytes);
+int gl_ce_fwd(const GlCeArgs* a, void* stream);
+
+/* The backward, from the operands as they were and what the forward kept.  It goes through the classes in pieces
+ * whose gradients at the logits take up to piece_bytes of the workspace (0: 1 GiB; 256 classes at least).
+ * Gradients that are NULL are not computed. */
+typedef struct GlCeBwdArgs {
+  const void* X;
+  int64_t sx;
+  const void* W;
+  int64_t sw;
+  const void* bias;
+  const int64_t* target;
+  int64_t ignore_index;
+  int64_t M;
+  int32_t N, K;
+  int32_t dtype;
+  int32_t reduction;
+  const int32_t* kept;
+  const float* dloss;     /* [M] with GL_CE_NONE, else one */
+  int64_t sdl;            /* elements between the rows of dloss */
+  void* dX;               /* [M, K] of `dtype`, contiguous */
+  void* dW;               /* [N, K] of g_dtype, contiguous */
+  void* db;               /* [N] of g_dtype */
+  int32_t g_dtype;
+  int32_t accumulate;     /* dW and db (fp32) are added to */
+  size_t piece_bytes;
+  void* ws;               /* 256-byte aligned */
+  size_t ws_bytes;
+} GlCeBwdArgs;
+int gl_ce_bwd_workspace(const GlCeBwdArgs* a, size_t* bytes);
+int gl_ce_bwd(const GlCeBwdArgs* a, void* stream);
+
 /* Kernel ids reported by the trace below. */
 enum {
   GL_KERNEL_TILE_X = 1, GL_KERNEL_FWD = 2, GL_KERNEL_FWD_FINALIZE = 3, GL_KERNEL_C1T = 4, GL_KERNEL_BWD_W = 5,
@@ -472,7 +532,9 @@ enum {
   GL_KERNEL_DENSE_ALIGN = 25,                          /* operands copied to 16-byte rows */
   GL_KERNEL_ADAM_VALUES = 26,                          /* 8-bit moments to fp32 */
   GL_KERNEL_NORM = 27, GL_KERNEL_NORM_BWD = 28,        /* layer norm; dX and the workgroups' sums of dW, db */
-  GL_KERNEL_NORM_DW = 29                               /* their sum */
+  GL_KERNEL_NORM_DW = 29,                              /* their sum */
+  GL_KERNEL_CE_STATS = 30, GL_KERNEL_CE_GRAD = 31,     /* cross entropy: tiles' softmax statistics; dz of a piece */
+  GL_KERNEL_CE_GATHER = 32, GL_KERNEL_CE_ROWS = 33     /* its rows that count; what is done row by row */
 };
 
 /* Launch trace for benchmarks and tests (process-wide, not for concurrent callers): after
