@@ -531,22 +531,36 @@ __device__ __forceinline__ void ce_stats(const DenseRowsK& a, long long M, int t
     long long t = -1;
     if (m < M) t = a.target[a.index ? a.index[m] : m] - n0;
     const int at = t >= 0 && t < 64 ? (int)t - lane_col : -64;  // of this lane's columns
-    float v[TN][4 * G], top = -__builtin_inff(), picked = 0.f;
-    bool here = false;
+    float v[TN][4 * G], top = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int x = 0; x < 4 * G; ++x) {
-        const int col = MS * j + 8 * (x / 4) + x % 4;
-        v[j][x] = __builtin_fmaf(acc[i][j][x], LOG2E, bias[j][x]);
-        if (!inside && n0 + lane_col + col >= a.e.N) v[j][x] = -__builtin_inff();
-        if (at == col) {
-          picked = v[j][x];
-          here = true;
-          v[j][x] = -__builtin_inff();
-        }
-        top = __builtin_fmaxf(top, v[j][x]);
-      }
+      for (int x = 0; x < 4 * G; ++x) v[j][x] = __builtin_fmaf(acc[i][j][x], LOG2E, bias[j][x]);
+    if (!inside) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int x = 0; x < 4 * G; ++x)
+          if (n0 + lane_col + MS * j + 8 * (x / 4) + x % 4 >= a.e.N) v[j][x] = -__builtin_inff();
+    }
+    if (__builtin_amdgcn_ballot_w64(t >= 0 && t < 64)) {  // few waves have one of their rows' targets
+      float picked = 0.f;
+      bool here = false;
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int x = 0; x < 4 * G; ++x)
+          if (at == MS * j + 8 * (x / 4) + x % 4) {
+            picked = v[j][x];
+            here = true;
+            v[j][x] = -__builtin_inff();
+          }
+      if (here) a.target_logit[m] = picked;
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int x = 0; x < 4 * G; ++x) top = __builtin_fmaxf(top, v[j][x]);
     top = over_row<MS>(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
     const float ref = top == -__builtin_inff() ? 0.f : top;
     float s = 0.f;
@@ -555,7 +569,6 @@ __device__ __forceinline__ void ce_stats(const DenseRowsK& a, long long M, int t
 #pragma unroll
       for (int x = 0; x < 4 * G; ++x) s += __builtin_amdgcn_exp2f(v[j][x] - ref);
     s = over_row<MS>(s, [](float x, float y) { return x + y; });
-    if (here) a.target_logit[m] = picked;
     if (l < MS) {
       lds[wn * BM + row][0] = top;
       lds[wn * BM + row][1] = s;
@@ -585,32 +598,40 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(typename De
   typedef Side<ES, BN, NW, QRC> SQ;
   constexpr int LDS_Q = NSP * SP::BYTES, LDS = LDS_Q + NSQ * SQ::BYTES;  // P's stages, then Q's
   extern __shared__ __align__(1024) char smem[];
-  int tm, tn, split;
-  tile_of(blockIdx.x, gridDim.x, a.tiles_m, a.tiles_n, tm, tn, split);
-  const int k0 = split * a.steps_per_split;
-  const long long m0 = (long long)tm * BM;
-  const int n0 = tn * BN;
+  int tm, tn, split, tiles_m = a.tiles_m, blocks = gridDim.x;
   long long M = a.e.M, R = a.R;
-  int nk = min(a.steps - k0, a.steps_per_split);
   if constexpr (KIND != DENSE_PLAIN) {
     if (a.rows) {
       const long long rows = *a.rows;
       if constexpr (PRC) {
+        // The tiles that are there go to the first workgroups, as many to every XCD; the others end.
         M = rows < M ? rows : M;
-        if (m0 >= M) {  // of the whole workgroup
+        const int there = (int)((M + BM - 1) / BM);
+        blocks = blocks / tiles_m * there;
+        if ((int)blockIdx.x >= blocks) {
           if constexpr (KIND == DENSE_CE_GRAD) {
+            const int id = blockIdx.x - blocks, n0 = id % a.tiles_n * BN;
+            const long long first = (long long)(there + id / a.tiles_n) * WM;
             if (a.col_sums)
               for (int i = threadIdx.x; i < WM * BN; i += 64 * WM * WN)
-                if (n0 + i % BN < a.e.N) a.col_sums[((long long)tm * WM + i / BN) * a.e.N + n0 + i % BN] = 0.f;
+                if (n0 + i % BN < a.e.N) a.col_sums[(first + i / BN) * a.e.N + n0 + i % BN] = 0.f;
           }
           return;
         }
-      } else {  // stages of zeros where a split has no rows
+        tiles_m = there;
+      } else {
         R = rows < R ? rows : R;
-        const int steps = (int)((R * ES + DENSE_BK - 1) / DENSE_BK);
-        nk = max(1, min(steps - k0, a.steps_per_split));
       }
     }
+  }
+  tile_of(blockIdx.x, blocks, tiles_m, a.tiles_n, tm, tn, split);
+  const int k0 = split * a.steps_per_split;
+  const long long m0 = (long long)tm * BM;
+  const int n0 = tn * BN;
+  int nk = min(a.steps - k0, a.steps_per_split);
+  if constexpr (KIND != DENSE_PLAIN && !PRC) {  // a split without rows: a stage of zeros
+    const int steps = (int)((R * ES + DENSE_BK - 1) / DENSE_BK);
+    nk = max(1, min(steps - k0, a.steps_per_split));
   }
   const int w = threadIdx.x >> 6, wm = w / WN, wn = w % WN;
 
@@ -825,17 +846,40 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(typename De
         if (!split_up) dense_forward<ROWS>(a.e, mi, 4, n, v, bias);
       }
       if constexpr (KIND == DENSE_CE_GRAD) {
+        int t[ROWS];
+        float at_t[ROWS];
+        bool any = false;
 #pragma unroll
         for (int x = 0; x < ROWS; ++x) {
           const uv4 q = info[wm * TM * MS + i * 32 + y + 4 * x + (l >> 4)];
           const float top = __uint_as_float(q[0]), f = __uint_as_float(q[1]);
-          const int t = (int)q[2] - a.first - n;
+          t[x] = (int)q[2] - a.first - n;
+          at_t[x] = __uint_as_float(q[3]);
+          any |= (unsigned)t[x] < 4u || f == 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(v[x][j], LOG2E, bias[j]) - top);
-            v[x][j] = f == 0.f || j >= there ? 0.f : t == j ? __uint_as_float(q[3]) : f * p;
-            col[j] += v[x][j];
+          for (int j = 0; j < 4; ++j)
+            v[x][j] = f * __builtin_amdgcn_exp2f(__builtin_fmaf(v[x][j], LOG2E, bias[j]) - top);
+        }
+        // few waves have a target, or a row without a gradient
+        if (__builtin_amdgcn_ballot_w64(any)) {
+#pragma unroll
+          for (int x = 0; x < ROWS; ++x) {
+            const bool none = __uint_as_float(info[wm * TM * MS + i * 32 + y + 4 * x + (l >> 4)][1]) == 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[x][j] = none ? 0.f : t[x] == j ? at_t[x] : v[x][j];
           }
+        }
+        if (!inside) {
+#pragma unroll
+          for (int x = 0; x < ROWS; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[x][j] = j < there ? v[x][j] : 0.f;
+        }
+        if (a.col_sums) {
+#pragma unroll
+          for (int x = 0; x < ROWS; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) col[j] += v[x][j];
         }
       }
       if (added.p) {
