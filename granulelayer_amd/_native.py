@@ -110,14 +110,14 @@ class GlNormBwdArgs(ctypes.Structure):
 class GlCeArgs(ctypes.Structure):
     _fields_ = [("X", _P), ("sx", _I64), ("W", _P), ("sw", _I64), ("bias", _P), ("target", _P), ("ignore_index", _I64),
                 ("M", _I64), ("N", _I32), ("K", _I32), ("dtype", _I32), ("reduction", _I32), ("loss", _P), ("kept", _P),
-                ("ws", _P), ("ws_bytes", _SZ)]
+                ("piece_bytes", _SZ), ("exps", _P), ("ws", _P), ("ws_bytes", _SZ)]
 
 
 class GlCeBwdArgs(ctypes.Structure):
     _fields_ = [("X", _P), ("sx", _I64), ("W", _P), ("sw", _I64), ("bias", _P), ("target", _P), ("ignore_index", _I64),
                 ("M", _I64), ("N", _I32), ("K", _I32), ("dtype", _I32), ("reduction", _I32), ("kept", _P), ("dloss", _P),
                 ("sdl", _I64), ("dX", _P), ("dW", _P), ("db", _P), ("g_dtype", _I32), ("accumulate", _I32),
-                ("piece_bytes", _SZ), ("ws", _P), ("ws_bytes", _SZ)]
+                ("piece_bytes", _SZ), ("exps", _P), ("ws", _P), ("ws_bytes", _SZ)]
 
 
 # gl_struct_layout ids 0..13
@@ -131,7 +131,7 @@ EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_work
            "gl_sched_build", "gl_window_build_host", "gl_window_build", "gl_cover_select", "gl_trace_begin",
            "gl_trace_end", "gl_pack8", "gl_unpack8", "gl_dense_fwd_workspace", "gl_dense_fwd", "gl_dense_bwd_workspace",
            "gl_dense_bwd", "gl_adam_many", "gl_adam_values", "gl_norm_fwd", "gl_norm_bwd_workspace",
-           "gl_norm_bwd", "gl_ce_fwd_workspace", "gl_ce_fwd", "gl_ce_bwd_workspace", "gl_ce_bwd")
+           "gl_norm_bwd", "gl_ce_fwd_workspace", "gl_ce_exps_bytes", "gl_ce_fwd", "gl_ce_bwd_workspace", "gl_ce_bwd")
 KERNEL_NAMES = {1: "tile_x_kernel", 2: "fwd_kernel", 3: "fwd_finalize_kernel", 4: "c1t_kernel", 5: "bwd_w_kernel",
                 6: "dx_kernel", 7: "dx_reduce_kernel", 8: "adam_kernel", 9: "edges_build", 10: "fwd_kernel_win",
                 11: "bwd_w_kernel_win", 12: "max_events_dw_kernel", 13: "max_events_dx_kernel",
@@ -187,7 +187,7 @@ class Library:
         for name, st in (("gl_fwd_workspace", GlFwdArgs), ("gl_bwd_workspace", GlBwdArgs),
                          ("gl_dense_fwd_workspace", GlDenseArgs), ("gl_dense_bwd_workspace", GlDenseBwdArgs),
                          ("gl_norm_bwd_workspace", GlNormBwdArgs),
-                         ("gl_ce_fwd_workspace", GlCeArgs), ("gl_ce_bwd_workspace", GlCeBwdArgs)):
+                         ("gl_ce_fwd_workspace", GlCeArgs), ("gl_ce_exps_bytes", GlCeArgs), ("gl_ce_bwd_workspace", GlCeBwdArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), ctypes.POINTER(_SZ)]
         L.gl_trace_begin.restype = ctypes.c_int

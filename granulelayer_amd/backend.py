@@ -575,9 +575,9 @@ class HipBackend:
     _ce_fwd = functools.cached_property(lambda self: self.lib.entry("gl_ce_fwd"))
     _ce_bwd = functools.cached_property(lambda self: self.lib.entry("gl_ce_bwd"))
 
-    def ce_forward(self, x, w, b, target, reduction, ignore_index, keep):
-        """(loss, what the backward takes with ``keep``) of x [M, K], w [N, K], b [N] or None (all of one dtype) and
-        target [M] (contiguous int64)."""
+    def ce_forward(self, x, w, b, target, reduction, ignore_index, keep, piece_bytes=0):
+        """(loss, and with ``keep`` what the backward takes: five words a row, and the first piece's exponentials or
+        None) of x [M, K], w [N, K], b [N] or None (all of one dtype) and target [M] (contiguous int64)."""
         x, code, sx = _x_operand(x.resolve_neg())
         w, _, sw = _x_operand(w.resolve_neg())
         M, K = x.shape
@@ -587,19 +587,22 @@ class HipBackend:
             b = b.resolve_neg().contiguous()
         kept = torch.empty(4 + 5 * M, device=dev, dtype=torch.int32) if keep else None
         if M == 0:
-            return torch.zeros(() if reduction != "none" else 0, device=dev), kept
+            return torch.zeros(() if reduction != "none" else 0, device=dev), kept, None
         loss = torch.empty(() if reduction != "none" else M, device=dev)
-        need = self._ce_bytes(M, F, K, code, x.data_ptr() % 16, sx, w.data_ptr() % 16, sw, N.GL_CE[reduction], keep)
+        need, size = self._ce_bytes(M, F, K, code, x.data_ptr() % 16, sx, w.data_ptr() % 16, sw, N.GL_CE[reduction], keep,
+                                    piece_bytes)
         ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        exps = torch.empty(size, device=dev, dtype=torch.uint8) if keep and size else None
         a = _CE(x.data_ptr(), sx, w.data_ptr(), sw, _ptr(b), target.data_ptr(), ignore_index, M, F, K, code,
-                N.GL_CE[reduction], loss.data_ptr(), _ptr(kept), ws.data_ptr(), need)
+                N.GL_CE[reduction], loss.data_ptr(), _ptr(kept), piece_bytes, _ptr(exps), ws.data_ptr(), need)
         with _on(dev):
             self._ce_fwd(a, _stream(dev))
-        return loss, kept
+        return loss, kept, exps
 
-    def ce_backward(self, dloss, x, w, b, target, reduction, ignore_index, kept, dx, dw, db, accumulate, piece_bytes=0):
-        """Gradients of ``ce_forward`` into dx [M, K] (x's dtype), dw [N, K] and db [N] (w's dtype, or fp32 and added
-        to with ``accumulate``); None for what is not needed."""
+    def ce_backward(self, dloss, x, w, b, target, reduction, ignore_index, kept, dx, dw, db, accumulate, piece_bytes=0,
+                    exps=None):
+        """Gradients of ``ce_forward`` (of the same piece_bytes) into dx [M, K] (x's dtype), dw [N, K] and db [N] (w's
+        dtype, or fp32 and added to with ``accumulate``); None for what is not needed.  ``exps`` is used up."""
         x, code, sx = _x_operand(x.resolve_neg())
         w, _, sw = _x_operand(w.resolve_neg())
         M, K = x.shape
@@ -615,22 +618,24 @@ class HipBackend:
         if dloss.dtype != torch.float32:
             dloss = dloss.float()
         need = self._ce_bwd_bytes(M, F, K, code, w.data_ptr() % 16, sw, dx is not None, dw is not None, db is not None,
-                                  piece_bytes)
+                                  piece_bytes, exps is not None)
         ws = torch.empty(need, device=dev, dtype=torch.uint8)
         a = _CE_BWD(x.data_ptr(), sx, w.data_ptr(), sw, _ptr(b), target.data_ptr(), ignore_index, M, F, K, code,
                     N.GL_CE[reduction], kept.data_ptr(), dloss.data_ptr(), dloss.stride(0) if dloss.dim() else 0, _ptr(dx),
-                    _ptr(dw), _ptr(db), N.GL_DTYPE_F32 if accumulate else code, accumulate, piece_bytes, ws.data_ptr(), need)
+                    _ptr(dw), _ptr(db), N.GL_DTYPE_F32 if accumulate else code, accumulate, piece_bytes, _ptr(exps), ws.data_ptr(),
+                    need)
         with _on(dev):
             self._ce_bwd(a, _stream(dev))
 
-    def _ce_bytes_of(self, M, F, K, code, x16, sx, w16, sw, reduction, keep):
+    def _ce_bytes_of(self, M, F, K, code, x16, sx, w16, sw, reduction, keep, piece_bytes):
         a = N.GlCeArgs(X=4096 + x16, sx=sx, W=4096 + w16, sw=sw, target=4096, M=M, N=F, K=K, dtype=code,
-                       reduction=reduction, loss=4096, kept=4096 * keep)
-        return self.lib.size_query("gl_ce_fwd_workspace", a)
+                       reduction=reduction, loss=4096, kept=4096 * keep, piece_bytes=piece_bytes)
+        return self.lib.size_query("gl_ce_fwd_workspace", a), self.lib.size_query("gl_ce_exps_bytes", a)
 
-    def _ce_bwd_bytes_of(self, M, F, K, code, w16, sw, dx, dw, db, piece_bytes):
+    def _ce_bwd_bytes_of(self, M, F, K, code, w16, sw, dx, dw, db, piece_bytes, exps):
         a = N.GlCeBwdArgs(X=4096, sx=K, W=4096 + w16, sw=sw, target=4096, M=M, N=F, K=K, dtype=code, kept=4096, dloss=4096,
-                          dX=4096 * dx, dW=4096 * dw, db=4096 * db, g_dtype=code, piece_bytes=piece_bytes)
+                          dX=4096 * dx, dW=4096 * dw, db=4096 * db, g_dtype=code, piece_bytes=piece_bytes,
+                          exps=4096 * exps)
         return self.lib.size_query("gl_ce_bwd_workspace", a)
 
 

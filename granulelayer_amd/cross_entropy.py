@@ -3,7 +3,8 @@
 The other end of a model around the sparse layer: its last projection goes onto a large number of classes (a
 vocabulary), whose logits would be the largest tensor of the step.  The forward is one product whose tiles leave their
 softmax statistics instead of logits; the backward makes the logits again, a piece of the classes at a time, and
-keeps their gradient only until two more products have taken it.  Operands are those of ``dense_projection``, fp32 or
+keeps their gradient only until two more products have taken it.  The forward of a training step may fill the first
+piece's place already, with exponentials that the backward turns into the gradient: one piece's memory in all.  Operands are those of ``dense_projection``, fp32 or
 bf16 with products, sums and statistics in fp32, and gradients go to ``main_grad`` where the parameters have it (no
 counterpart in the reference).
 
@@ -52,11 +53,12 @@ def _check(x, weight, target, bias, reduction, workspace_budget):
 
 
 class DenseCrossEntropyFunction(torch.autograd.Function):
-    """x [M, K], target [M] -> the loss; keeps the operands and five words a row."""
+    """x [M, K], target [M] -> the loss; keeps the operands, five words a row, and the first piece's exponentials where
+    they are worth it, which the first backward turns into its gradient in place."""
 
     @staticmethod
     def forward(ctx, x, w, b, target, reduction, ignore_index, budget):
-        loss, kept = backend_for(x.device).ce_forward(x, w, b, target, reduction, ignore_index, True)
+        loss, kept, ctx.exps = backend_for(x.device).ce_forward(x, w, b, target, reduction, ignore_index, True, budget)
         ctx.save_for_backward(x, w, b, target, kept)
         ctx.reduction, ctx.ignore_index, ctx.budget = reduction, ignore_index, budget
         return loss
@@ -77,8 +79,9 @@ def _gradients(ctx, dloss):
     else:
         dw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if need_w else None
         db = torch.empty(b.shape, device=x.device, dtype=b.dtype) if need_b else None
+    exps, ctx.exps = ctx.exps, None  # used up: a second backward of a retained graph makes them again
     backend_for(x.device).ce_backward(dloss.resolve_neg(), x, w, b, target, ctx.reduction, ctx.ignore_index, kept, dx, dw, db,
-                                      use_main, ctx.budget)
+                                      use_main, ctx.budget, exps)
     return dx, None if use_main else dw, None if use_main else db, None, None, None, None
 
 

@@ -196,7 +196,7 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       typedef GlCeArgs S;
       long long t[] = {(long long)sizeof(S), OFF(S, X), OFF(S, sx), OFF(S, W), OFF(S, sw), OFF(S, bias), OFF(S, target),
                        OFF(S, ignore_index), OFF(S, M), OFF(S, N), OFF(S, K), OFF(S, dtype), OFF(S, reduction),
-                       OFF(S, loss), OFF(S, kept), OFF(S, ws), OFF(S, ws_bytes)};
+                       OFF(S, loss), OFF(S, kept), OFF(S, piece_bytes), OFF(S, exps), OFF(S, ws), OFF(S, ws_bytes)};
       for (long long x : t) v[c++] = x;
       break;
     }
@@ -205,7 +205,7 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       long long t[] = {(long long)sizeof(S), OFF(S, X), OFF(S, sx), OFF(S, W), OFF(S, sw), OFF(S, bias), OFF(S, target),
                        OFF(S, ignore_index), OFF(S, M), OFF(S, N), OFF(S, K), OFF(S, dtype), OFF(S, reduction),
                        OFF(S, kept), OFF(S, dloss), OFF(S, sdl), OFF(S, dX), OFF(S, dW), OFF(S, db), OFF(S, g_dtype),
-                       OFF(S, accumulate), OFF(S, piece_bytes), OFF(S, ws), OFF(S, ws_bytes)};
+                       OFF(S, accumulate), OFF(S, piece_bytes), OFF(S, exps), OFF(S, ws), OFF(S, ws_bytes)};
       for (long long x : t) v[c++] = x;
       break;
     }

@@ -8,6 +8,10 @@
 // operands' type (DENSE_CE_GRAD, with the sums of db from unrounded values), two more take it to dX, which is added up in
 // fp32 over the pieces, and to the piece's rows of dW.  8 M K N operations in all, 2 of them for what was not kept.
 //
+// The first piece's exponentials are kept where that takes less time than making them again: in the place of its
+// dz, so in memory that the backward takes anyway, over the largest of 64: of bf16 operands in 16 bits (exp_code: within 2^-11
+// of each, where rounding dz takes 2^-8), else as they are.  One pass then turns them into dz.
+//
 // Rows whose target is `ignore_index` count for nothing.  Of more than CE_ALL rows those that count are copied together first
 // (a row is read and written once, against N products with it), and the products take their number from device
 // memory: tiles and stages of rows that are not there end at once.  What ignored rows hold is never read then; of
@@ -26,6 +30,7 @@ namespace {
 // Rows above which ignored ones are left out of the products: no tile is smaller.
 constexpr int CE_ALL = 256;
 constexpr size_t CE_PIECE = 1ull << 30;  // bytes of dz of a piece, unless the caller says less
+constexpr long long CE_KEEP = 1024;      // bytes of a row of X from which exponentials are kept
 constexpr float LN2 = 0.693147181f;
 
 // what the forward keeps, in 32-bit words: rows that count, -, -, -; of every row that counts (in their order;
@@ -235,6 +240,64 @@ __global__ __launch_bounds__(256) void ce_info_kernel(const long long* __restric
   info[m] = uv4{__float_as_uint(k.top[m]), __float_as_uint(c == 0.f ? 0.f : c / k.sum[m]), (unsigned)t, __float_as_uint(c * expm1f(-k.loss[m]))};
 }
 
+// dz of the columns whose exponentials were kept, in their place, and the sums of 64 rows of every column.  32 lanes of 8
+// columns by 8 rows at a time, two rows of a lane in flight.
+constexpr int CE_DZ_ROWS = 64;
+template <bool BF>
+__global__ __launch_bounds__(256) void ce_dz_kernel(void* exps, const float* __restrict__ tops, int N, long long M, const int* count,
+                                                    const uv4* __restrict__ info, int first, float* __restrict__ part) {
+  __shared__ float sums[8][256];
+  const int ct = threadIdx.x & 31, rt = threadIdx.x >> 5, n = blockIdx.y * 256 + ct * 8;
+  const long long pitch = (N + 7) & ~7, groups = (N + 63) >> 6;
+  if (count && *count < M) M = *count;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (n < pitch) {
+#pragma unroll 1
+    for (int i = 0; i < CE_DZ_ROWS; i += 16) {
+      float e[2][8], f[2];
+      uv4 q[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const long long m = (long long)blockIdx.x * CE_DZ_ROWS + i + 8 * x + rt;
+        if (m >= M) continue;
+        q[x] = info[m];
+        f[x] = tops[m * groups + (n >> 6)];
+        if constexpr (BF) {
+          const uv4 h = *reinterpret_cast<const uv4*>((const char*)exps + 2 * (m * pitch + n));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[x][j] = exp_value(j & 1 ? h[j >> 1] >> 16 : h[j >> 1] & 0xffffu);
+        } else {
+          load8<false>(exps, m * pitch + n, 8, e[x]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const long long m = (long long)blockIdx.x * CE_DZ_ROWS + i + 8 * x + rt;
+        if (m >= M) continue;
+        const float c = __uint_as_float(q[x][1]);
+        const int t = (int)q[x][2] - first - n;
+        f[x] = c * __builtin_amdgcn_exp2f(f[x] - __uint_as_float(q[x][0]));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[x][j] = c == 0.f || n + j >= N ? 0.f : t == j ? __uint_as_float(q[x][3]) : f[x] * e[x][j];
+          s[j] += e[x][j];
+        }
+        store8<BF>(exps, m * pitch + n, 8, e[x]);
+      }
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sums[rt][ct * 8 + j] = s[j];
+  __syncthreads();
+  const int col = blockIdx.y * 256 + threadIdx.x;
+  if (col >= N) return;
+  float t = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) t += sums[r][threadIdx.x];
+  part[(long long)blockIdx.x * N + col] = t;
+}
+
 // dX by row from the sums by rows that count (rank null: by row); rows that do not: zeros.  8 neighbours a thread.
 template <bool FBF, bool TBF>
 __global__ __launch_bounds__(256) void ce_scatter_kernel(const void* __restrict__ from, const int* __restrict__ rank, long long M,
@@ -272,6 +335,22 @@ struct Layout {
     return p;
   }
 };
+
+// Classes of a piece: pieces of one size, in columns of the widest tiles, whose dz fits the budget.
+long long piece_of(long long M, int N, int dtype, size_t budget) {
+  const long long most = (long long)((budget ? budget : CE_PIECE) / ((size_t)M * es_of(dtype)));
+  if (most >= N) return N;
+  const long long pieces = (N + (most > 256 ? most : 256) - 1) / (most > 256 ? most : 256);
+  return round_up((N + pieces - 1) / pieces, 256);
+}
+// Classes whose exponentials are kept: the first piece, unless the product that makes them again is short.
+int kept_classes(long long M, int N, int K, int dtype, size_t budget) {
+  return (long long)K * es_of(dtype) >= CE_KEEP ? (int)piece_of(M, N, dtype, budget) : 0;
+}
+size_t exps_at_tops(long long M, int cols, int dtype) { return (size_t)round_up(M * padded(cols) * es_of(dtype), 256); }
+size_t exps_bytes(long long M, int cols, int dtype) {
+  return cols ? exps_at_tops(M, cols, dtype) + (size_t)round_up(M * ((cols + 63) / 64) * 4, 256) : 0;
+}
 
 struct CeFwd {
   bool all;
@@ -325,6 +404,7 @@ struct CeBwd {
   long long piece, pieces;  // classes of a piece
   Operand w;
   bool direct;              // dX's product writes dX itself
+  int kept;                 // classes whose exponentials were kept: the first piece, or none
   size_t x_at, w_at, info, dz, dx, part, cols, bytes;
 };
 // the three products of the classes [n0, n0 + n)
@@ -345,11 +425,7 @@ int plan_ce_bwd(const GlCeBwdArgs* a, CeBwd* out) {
   CeBwd p{};
   const int es = es_of(a->dtype);
   p.all = a->M <= CE_ALL;
-  // pieces of one size, in columns of the widest tiles
-  const size_t budget = a->piece_bytes ? a->piece_bytes : CE_PIECE;
-  const long long most = (long long)(budget / ((size_t)a->M * es));
-  const long long pieces = most >= a->N ? 1 : (a->N + (most > 256 ? most : 256) - 1) / (most > 256 ? most : 256);
-  p.piece = pieces == 1 ? a->N : round_up((a->N + pieces - 1) / pieces, 256);
+  p.piece = piece_of(a->M, a->N, a->dtype, a->piece_bytes);
   p.pieces = (a->N + p.piece - 1) / p.piece;
   p.w = operand(a->W, a->sw, a->N, a->K, true, es);
   p.direct = p.all && p.pieces == 1;
@@ -363,11 +439,16 @@ int plan_ce_bwd(const GlCeBwdArgs* a, CeBwd* out) {
     part = part > q.pw.part_bytes ? part : q.pw.part_bytes;
     cols = cols > c ? cols : c;
   }
+  p.kept = a->exps ? kept_classes(a->M, a->N, a->K, a->dtype, a->piece_bytes) : 0;
+  if (p.kept) {
+    const size_t c = (size_t)((a->M + CE_DZ_ROWS - 1) / CE_DZ_ROWS) * p.kept * 4;
+    cols = cols > c ? cols : c;
+  }
   Layout l;
   p.x_at = l.take((size_t)a->M * padded(a->K) * es);
   p.w_at = l.take(copy_bytes(p.w, es));
   p.info = l.take((size_t)a->M * 16);
-  p.dz = l.take((size_t)a->M * padded(p.piece) * es);
+  p.dz = l.take(p.kept && p.pieces == 1 ? 0 : (size_t)a->M * padded(p.piece) * es);
   p.dx = l.take(a->dX && !p.direct ? (size_t)a->M * a->K * (p.pieces > 1 ? 4 : es) : 0);
   p.part = l.take(part);
   p.cols = l.take(a->db ? cols : 0);
@@ -383,14 +464,17 @@ int check_bwd(const GlCeBwdArgs* a) {
   if (a->accumulate && a->g_dtype != GL_DTYPE_F32) return GL_ERR_ARG;
   if (a->M == 0) return 0;
   if (!a->kept || !a->dloss || ((uintptr_t)a->kept & 3) || ((uintptr_t)a->dloss & 3) || a->sdl < 0) return GL_ERR_ARG;
-  if (!on_element(a->dX, a->dtype) || !on_element(a->dW, a->g_dtype) || !on_element(a->db, a->g_dtype)) return GL_ERR_ARG;
+  if (!on_element(a->dX, a->dtype) || !on_element(a->dW, a->g_dtype) || !on_element(a->db, a->g_dtype) ||
+      ((uintptr_t)a->exps & 255))
+    return GL_ERR_ARG;
   return 0;
 }
 int check_fwd(const GlCeArgs* a) {
   if (!a) return GL_ERR_ARG;
   GL_TRY(check(a->X, a->sx, a->W, a->sw, a->bias, a->target, a->M, a->N, a->K, a->dtype, a->reduction));
   if (a->M == 0) return 0;
-  if (!a->loss || ((uintptr_t)a->loss & 3) || ((uintptr_t)a->kept & 3)) return GL_ERR_ARG;
+  if (!a->loss || ((uintptr_t)a->loss & 3) || ((uintptr_t)a->kept & 3) || ((uintptr_t)a->exps & 255) || (a->exps && !a->kept))
+    return GL_ERR_ARG;
   return 0;
 }
 
@@ -408,6 +492,13 @@ extern "C" int gl_ce_fwd_workspace(const GlCeArgs* a, size_t* bytes) {
   const CeFwd p = plan_ce(a);
   if (p.pr.splits == 0) return GL_ERR_UNSUPPORTED;
   *bytes = p.bytes;
+  return 0;
+}
+
+extern "C" int gl_ce_exps_bytes(const GlCeArgs* a, size_t* bytes) {
+  GL_TRY(check_fwd(a));
+  if (!bytes) return GL_ERR_ARG;
+  *bytes = a->M == 0 ? 0 : exps_bytes(a->M, kept_classes(a->M, a->N, a->K, a->dtype, a->piece_bytes), a->dtype);
   return 0;
 }
 
@@ -441,6 +532,10 @@ extern "C" int gl_ce_fwd(const GlCeArgs* a, void* stream) {
   d.index = p.all ? nullptr : k.index;
   d.target_logit = (float*)(ws + p.logit);
   d.stats = (float*)(ws + p.stats);
+  if (a->exps && (d.exps_cols = kept_classes(a->M, a->N, a->K, a->dtype, a->piece_bytes)) > 0) {
+    d.exps = a->exps;
+    d.exps_top = (float*)((char*)a->exps + exps_at_tops(a->M, d.exps_cols, a->dtype));
+  }
   GL_TRY(launch_rows(a->dtype, DENSE_CE_STATS, p.pr, d, s));
   JoinK j{d.stats, d.target_logit, target, a->M, a->ignore_index, p.pr.tiles_n, a->N, a->reduction, k, a->loss};
   if (p.all) {
@@ -494,19 +589,29 @@ extern "C" int gl_ce_bwd(const GlCeBwdArgs* a, void* stream) {
     Operand w = p.w;
     w.p = (const char*)w.p + n0 * w.ld * es;
     w.rows = n;
-    DenseEpi e = store_epi(ws + p.dz, pitch, a->dtype, a->M, (int)n, a->dtype, 0);
-    e.bias = a->bias ? (const char*)a->bias + n0 * es : nullptr;
-    DenseRowsK d = rows_product(a->dtype, x_rows, w, q.logits, e);
-    d.rows = count;
-    d.row_info = info;
-    d.first = (int)n0;
-    d.col_sums = a->db ? cols : nullptr;
-    d.pitch = (int)pitch;
-    GL_TRY(launch_rows(a->dtype, DENSE_CE_GRAD, q.logits, d, s));
-    const Operand dz{ws + p.dz, pitch, a->M, (int)n, true, true};
-    if (a->db)
-      GL_TRY(launch_db(cols, (long long)q.logits.tiles_m * waves_m(a->dtype, q.logits.tile), (int)n,
-                       (char*)a->db + n0 * es_of(a->g_dtype), a->g_dtype, a->accumulate, s));
+    void* at = i == 0 && p.kept ? a->exps : ws + p.dz;
+    long long chunks;
+    if (i == 0 && p.kept) {
+      const dim3 grid((unsigned)((a->M + CE_DZ_ROWS - 1) / CE_DZ_ROWS), (unsigned)ceil_div(n, 256));
+      const float* tops = (const float*)((char*)a->exps + exps_at_tops(a->M, p.kept, a->dtype));
+      if (es == 2) GL_LAUNCH(GL_KERNEL_CE_GRAD, ce_dz_kernel<true>, grid, dim3(256), 0, s, at, tops, (int)n, (long long)a->M, count, (const uv4*)info, 0, a->db ? cols : (float*)nullptr);
+      else GL_LAUNCH(GL_KERNEL_CE_GRAD, ce_dz_kernel<false>, grid, dim3(256), 0, s, at, tops, (int)n, (long long)a->M, count, (const uv4*)info, 0, a->db ? cols : (float*)nullptr);
+      GL_CHECK_LAUNCH();
+      chunks = grid.x;
+    } else {
+      DenseEpi e = store_epi(at, pitch, a->dtype, a->M, (int)n, a->dtype, 0);
+      e.bias = a->bias ? (const char*)a->bias + n0 * es : nullptr;
+      DenseRowsK d = rows_product(a->dtype, x_rows, w, q.logits, e);
+      d.rows = count;
+      d.row_info = info;
+      d.first = (int)n0;
+      d.col_sums = a->db ? cols : nullptr;
+      d.pitch = (int)pitch;
+      GL_TRY(launch_rows(a->dtype, DENSE_CE_GRAD, q.logits, d, s));
+      chunks = (long long)q.logits.tiles_m * waves_m(a->dtype, q.logits.tile);
+    }
+    const Operand dz{at, pitch, a->M, (int)n, true, true};
+    if (a->db) GL_TRY(launch_db(cols, chunks, (int)n, (char*)a->db + n0 * es_of(a->g_dtype), a->g_dtype, a->accumulate, s));
     if (a->dX) {
       const int to = p.pieces > 1 ? GL_DTYPE_F32 : a->dtype;
       GL_TRY(run_product(a->dtype, DENSE_NN, dz, w, n, q.px, ws + p.part,

@@ -63,6 +63,9 @@ struct DenseRowsK : DenseK {
   const int* index;          // row of `target` of every row of X, or null: its own
   float* target_logit;       // [M]; like all logits behind the product in units of log 2
   float* stats;              // [M][tiles_n][2]: the tile's largest logit but the target's, and the sum of 2^(logit - it)
+  void* exps;                // 2^(logit - the largest of its row's 64 columns) of the columns below exps_cols (16 bits of bf16
+  float* exps_top;           // operands: exp_code; else fp32; rows of padded(exps_cols), zeros behind the last and at the target), and
+  int exps_cols;             // these largest [M][ceil(exps_cols / 64)]; or null
   // gradient
   const uv4* row_info;       // [M]: the largest logit; factor of 2^(logit - it); the target; the gradient at it
   int first;                 // class of the product's first column
@@ -501,12 +504,20 @@ __device__ __forceinline__ float ce_bias(float b) {
 __device__ __forceinline__ int n_pitch(const DenseRowsK& a) { return a.pitch; }
 __device__ __forceinline__ int n_pitch(const DenseK&) { return 0; }
 
+// An exponential, between 0 and 1, in 16 bits: of an fp32 number's the lower 6 of the exponent and the upper 10 of the
+// mantissa, to the nearest.  Within 2^-11 of itself from 1 down to 2^-62 (fp16 is so down to 2^-14 and has nothing below 2^-25,
+// and a class that is no target has its whole gradient from such), 0 from 0.  Of a NaN any code: its row's factor is NaN.
+__device__ __forceinline__ unsigned exp_code(float e) {
+  return __builtin_elementwise_sub_sat((__float_as_uint(e) + 0x1000u) >> 13, 0x10000u) & 0xffffu;
+}
+__device__ __forceinline__ float exp_value(unsigned c) { return __uint_as_float((c << 13) + 0x20000000u) - 0x1p-63f; }
+
 // DENSE_CE_STATS: every row's largest logit of the tile and the sum of 2^(logit - it), both without the target's, and the
 // target's where it is in the tile.  All from the sums' registers: a lane has MS columns of its row, the lanes of a row are joined by
 // two (or one) swaps, the waves of a row through LDS (BM rows of WN pairs, free behind the caller's barrier).
 // Columns behind N are -inf; a tile of nothing else has the largest logit -inf and the sum 0.  A NaN is left out of the
 // largest and makes the sum NaN, as +inf does.
-template <int MS, int BM, int BN, int WM, int WN, int TM, int TN>
+template <int ES, int MS, int BM, int BN, int WM, int WN, int TM, int TN>
 __device__ __forceinline__ void ce_stats(const DenseRowsK& a, long long M, int tm, int tn,
                                          const typename Sums<MS>::type (&acc)[TM][TN], float (*lds)[2]) {
   constexpr int G = MS * MS / 256;  // groups of four columns in a lane's sums of an instruction
@@ -567,7 +578,25 @@ __device__ __forceinline__ void ce_stats(const DenseRowsK& a, long long M, int t
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int x = 0; x < 4 * G; ++x) s += __builtin_amdgcn_exp2f(v[j][x] - ref);
+      for (int x = 0; x < 4 * G; ++x) s += v[j][x] = __builtin_amdgcn_exp2f(v[j][x] - ref);
+    if (n0 < a.exps_cols && m < M) {  // a lane's four neighbours at a time
+      const int pitch = (a.exps_cols + 7) & ~7;
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const int n = n0 + MS * j + 8 * g + lane_col;
+          if (n >= pitch) continue;
+          const float* q = &v[j][4 * g];
+          if constexpr (ES == 2) {
+            const uv2 c = {exp_code(q[0]) | exp_code(q[1]) << 16, exp_code(q[2]) | exp_code(q[3]) << 16};
+            *reinterpret_cast<uv2*>((char*)a.exps + 2 * (m * pitch + n)) = c;
+          } else {
+            *reinterpret_cast<f32x4*>((char*)a.exps + 4 * (m * pitch + n)) = f32x4{q[0], q[1], q[2], q[3]};
+          }
+        }
+      if (l < MS) a.exps_top[m * ((a.exps_cols + 63) >> 6) + (n0 >> 6)] = top;
+    }
     s = over_row<MS>(s, [](float x, float y) { return x + y; });
     if (l < MS) {
       lds[wn * BM + row][0] = top;
@@ -760,7 +789,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(typename De
   constexpr bool STREAM = BM * BN == 65536 && KIND != DENSE_CE_GRAD;
   copies_barrier<0>();
   if constexpr (KIND == DENSE_CE_STATS) {
-    ce_stats<MS, BM, BN, WM, WN, TM, TN>(a, M, tm, tn, acc, reinterpret_cast<float(*)[2]>(smem));
+    ce_stats<ES, MS, BM, BN, WM, WN, TM, TN>(a, M, tm, tn, acc, reinterpret_cast<float(*)[2]>(smem));
     return;
   }
   const int l = threadIdx.x & 63;

@@ -479,10 +479,16 @@ typedef struct GlCeArgs {
   int32_t reduction;      /* GL_CE_* */
   float* loss;            /* out: [M] with GL_CE_NONE, else one */
   int32_t* kept;          /* out: GL_CE_KEPT_WORDS(M) words, or NULL */
+  size_t piece_bytes;     /* as of the backward that `exps` is for */
+  void* exps;             /* out: gl_ce_exps_bytes() bytes, 256-byte aligned, or NULL (then the backward makes the first
+                             piece's logits again, as the others') */
   void* ws;               /* 256-byte aligned */
   size_t ws_bytes;
 } GlCeArgs;
 int gl_ce_fwd_workspace(const GlCeArgs* a, size_t* bytes);
+/* The first piece's exponentials, for the backward: no more than a piece's gradients at the logits and 1/32 of
+ * them; 0 where they are not worth keeping. */
+int gl_ce_exps_bytes(const GlCeArgs* a, size_t* bytes);
 int gl_ce_fwd(const GlCeArgs* a, void* stream);
 
 /* The backward, from the operands as they were and what the forward kept.  It goes through the classes in pieces
@@ -509,6 +515,7 @@ typedef struct GlCeBwdArgs {
   int32_t g_dtype;
   int32_t accumulate;     /* dW and db (fp32) are added to */
   size_t piece_bytes;
+  void* exps;             /* what the forward kept with this piece_bytes, or NULL; the call uses it up */
   void* ws;               /* 256-byte aligned */
   size_t ws_bytes;
 } GlCeBwdArgs;

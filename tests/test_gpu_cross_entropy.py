@@ -52,7 +52,11 @@ def definition(t, reduction, g):
     c = {"none": lambda: g.double(), "sum": lambda: g.double(), "mean": lambda: g.double() / n}[reduction]().expand(M)
     c = torch.where(on, c, 0.0)[:, None]
     p = torch.exp(z - lse[:, None])
-    d_p = p * (d_z + d_lse[:, None] + 4 * E * (z.abs() + lse.abs()[:, None]) + 3 * E)
+    # an exponential below the least normal number, 2^-126, is 0
+    d_p = p * (d_z + d_lse[:, None] + 4 * E * (z.abs() + lse.abs()[:, None]) + 3 * E) + 2.0 ** -126
+    if x.shape[1] >= 512 and t["x"].dtype == BF:
+        # exponentials are kept in 16 bits: 10 of them the mantissa's, 6 the exponent's, down to 2^-63 of the largest of 64
+        d_p = d_p + 2.0 ** -11 * p + 2.0 ** -62 * p.amax(1, keepdim=True)
     dz = c * p.scatter_add(1, at, -torch.ones_like(at, dtype=torch.float64))
     d_dz = c.abs() * d_p + 3 * E * dz.abs()
     d_dzr = d_dz + HALF[t["x"].dtype] * (dz.abs() + d_dz)
@@ -126,11 +130,12 @@ def test_every_tile(dtype, M, K, N):
     compare(inputs(M, K, N, dtype, ignored=0.1), "mean")
 
 
+@pytest.mark.parametrize("K", [130, 520])
 @pytest.mark.parametrize("dtype", [BF, F])
 @pytest.mark.parametrize("M", [40, 700])
-def test_pieces(dtype, M):
+def test_pieces(K, dtype, M):
     """1001 classes in pieces of 256 and of 512 and whole."""
-    t = inputs(M, 130, 1001, dtype)
+    t = inputs(M, K, 1001, dtype)
     es = 2 if dtype == BF else 4
     whole = compare(t, "mean")
     for columns in (1, 300, 512, 1001):
@@ -139,11 +144,12 @@ def test_pieces(dtype, M):
         assert torch.equal(got["loss"], whole["loss"])
 
 
+@pytest.mark.parametrize("K", [64, 520])
 @pytest.mark.parametrize("dtype", [BF, F])
 @pytest.mark.parametrize("M", [1, 256, 257, 5000])
 @pytest.mark.parametrize("kept", ["none", "first", "last", "one in the middle"])
-def test_ignored_rows(dtype, M, kept):
-    t = inputs(M, 64, 300, dtype, ignored=0.0)
+def test_ignored_rows(K, dtype, M, kept):
+    t = inputs(M, K, 300, dtype, ignored=0.0)
     on = {"none": [], "first": [0], "last": [M - 1], "one in the middle": [M // 2]}[kept]
     target = torch.full_like(t["target"], IGNORED)
     target[on] = t["target"][on]
@@ -158,10 +164,11 @@ def test_ignored_rows(dtype, M, kept):
     assert not each[off].any()
 
 
+@pytest.mark.parametrize("K", [200, 520])
 @pytest.mark.parametrize("dtype", [BF, F])
 @pytest.mark.parametrize("M", [100, 900])
-def test_what_ignored_rows_hold_does_not_matter(dtype, M):
-    t = inputs(M, 200, 500, dtype, ignored=0.4)
+def test_what_ignored_rows_hold_does_not_matter(K, dtype, M):
+    t = inputs(M, K, 500, dtype, ignored=0.4)
     off = t["target"] == IGNORED
     clean = run(t, "mean")[1]
     for value in (float("nan"), float("inf"), torch.finfo(dtype).max):
@@ -173,10 +180,11 @@ def test_what_ignored_rows_hold_does_not_matter(dtype, M):
         assert not got["dx"][off].any()
 
 
+@pytest.mark.parametrize("K", [72, 520])
 @pytest.mark.parametrize("M", [60, 600])
-def test_classes_that_take_no_part(M):
+def test_classes_that_take_no_part(K, M):
     """A bias of -inf: a padded vocabulary, whole tiles of it among them."""
-    t = inputs(M, 72, 700, F, ignored=0.2)
+    t = inputs(M, K, 700, F, ignored=0.2)
     t["b"][300:] = float("-inf")
     t["target"] = torch.where(t["target"] == IGNORED, IGNORED, t["target"] % 300)
     got = run(t, "mean")[1]
@@ -195,10 +203,11 @@ def test_classes_that_take_no_part(M):
     assert torch.allclose(got["db"], 1.7 * (1 / 700 - share), rtol=1e-5, atol=1e-7)
 
 
+@pytest.mark.parametrize("K", [48, 520])
 @pytest.mark.parametrize("M", [60, 600])
 @pytest.mark.parametrize("bad", [-1, 300, 2 ** 40, -2 ** 63])
-def test_targets_that_are_no_class(M, bad):
-    t = inputs(M, 48, 300, BF, ignored=0.2)
+def test_targets_that_are_no_class(K, M, bad):
+    t = inputs(M, K, 300, BF, ignored=0.2)
     row = int((t["target"] != IGNORED).nonzero()[1])
     clean = run(t, "none")[1]
     t["target"][row] = bad
@@ -209,8 +218,9 @@ def test_targets_that_are_no_class(M, bad):
     assert torch.isnan(dense_cross_entropy(t["x"], t["w"], t["target"], t["b"]))
 
 
-def test_rows_that_are_no_numbers():
-    t = inputs(600, 48, 300, F, ignored=0.0)
+@pytest.mark.parametrize("K", [48, 520])
+def test_rows_that_are_no_numbers(K):
+    t = inputs(600, K, 300, F, ignored=0.0)
     clean = run(t, "none")[1]
     t["x"][7, 3], t["x"][500, 0] = float("nan"), float("inf")
     got = run(t, "none")[1]
@@ -221,9 +231,10 @@ def test_rows_that_are_no_numbers():
     assert torch.equal(got["loss"][good], clean["loss"][good]) and torch.equal(got["dx"][good], clean["dx"][good])
 
 
-def test_large_logits():
+@pytest.mark.parametrize("dtype,K", [(F, 64), (F, 520), (BF, 520)])
+def test_large_logits(dtype, K):
     """Logits of several hundreds: exponentials that overflow without the largest taken off."""
-    t = inputs(500, 64, 900, F, scale=200.0)
+    t = inputs(500, K, 900, dtype, scale=200.0)
     got = run(t, "none")
     want = definition(t, "none", got[0])
     for name, v in got[1].items():
@@ -260,9 +271,10 @@ def test_strides_views_and_types(dtype, M):
     assert torch.equal(dense_cross_entropy(neg, t["w"], t["target"], t["b"]), dense_cross_entropy(t["x"], t["w"], t["target"], t["b"]))
 
 
+@pytest.mark.parametrize("K", [64, 520])
 @pytest.mark.parametrize("M", [100, 500])
-def test_gradients_asked_for_alone_and_upstream_strides(M):
-    t = inputs(M, 64, 222, BF)
+def test_gradients_asked_for_alone_and_upstream_strides(K, M):
+    t = inputs(M, K, 222, BF)
     for names in ("x", "w", "b", "xw", "xb", "wb"):
         leaves = {k: t[k].detach().requires_grad_(k in names) for k in "xwb"}
         loss = dense_cross_entropy(leaves["x"], leaves["w"], t["target"], leaves["b"], "none")
@@ -317,9 +329,10 @@ def test_main_grad_is_added_to(M):
     assert not lay.weight.main_grad.any()
 
 
+@pytest.mark.parametrize("K", [96, 520])
 @pytest.mark.parametrize("M", [100, 700])
-def test_a_captured_training_pass_and_another_stream(M):
-    t = inputs(M, 96, 1000, BF)
+def test_a_captured_training_pass_and_another_stream(K, M):
+    t = inputs(M, K, 1000, BF)
     leaves = [t[k].detach().requires_grad_(True) for k in "xwb"]
     target = t["target"].clone()
 
@@ -348,6 +361,23 @@ def test_a_captured_training_pass_and_another_stream(M):
         got = [o.clone() for o in out]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(passes(), got))
+
+
+def test_a_second_backward_and_one_without_the_first():
+    """The kept exponentials serve one backward; another of the same graph makes them again."""
+    t = inputs(700, 520, 900, BF)
+    leaves = [t[k].detach().requires_grad_(True) for k in "xwb"]
+    want = definition(t, "mean", torch.ones((), device=DEV))
+    loss = dense_cross_entropy(leaves[0], leaves[1], t["target"], leaves[2])
+    for last in (False, False, True):
+        for v, name in zip(torch.autograd.grad(loss, leaves, retain_graph=not last), ("dx", "dw", "db")):
+            check(v, want, name)
+    dense_cross_entropy(leaves[0], leaves[1], t["target"], leaves[2])  # its graph goes without a backward
+    from torch.utils.checkpoint import checkpoint
+
+    loss = checkpoint(dense_cross_entropy, leaves[0], leaves[1], t["target"], leaves[2], use_reentrant=False)
+    for v, name in zip(torch.autograd.grad(loss, leaves), ("dx", "dw", "db")):
+        check(v, want, name)
 
 
 def test_operands_may_not_change_before_the_backward():
