@@ -226,15 +226,18 @@ __global__ __launch_bounds__(1024) void ce_join_all_kernel(JoinK a) {
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------
-// What a row's logits need to become dz.  A target that is no class makes the row's dz NaN.
+// What a row's logits need to become dz, without the factor that all rows share (alpha: the mean's 1 / count and the
+// upstream gradient, which the products' epilogues apply).  With it, the targets' dz, all near -alpha, would be rounded to bf16
+// alike: up to 2^-9 of dX and dW as a whole.  A target that is no class makes the row's dz NaN.
 __global__ __launch_bounds__(256) void ce_info_kernel(const long long* __restrict__ target, long long M, long long ignored, int N,
                                                       int reduction, Kept k, bool all, const float* __restrict__ g, long long sg,
-                                                      uv4* __restrict__ info) {
+                                                      uv4* __restrict__ info, float* __restrict__ alpha) {
   const long long m = (long long)blockIdx.x * 256 + threadIdx.x;
   const int n = *k.count;
+  if (m == 0) *alpha = reduction == GL_CE_NONE ? 1.f : reduction == GL_CE_SUM ? *g : n > 0 ? *g / (float)n : 0.f;
   if (m >= (all ? M : n)) return;
   const long long row = all ? m : k.index[m], t = target[row];
-  float c = reduction == GL_CE_NONE ? g[row * sg] : reduction == GL_CE_MEAN ? *g / (float)n : *g;
+  float c = reduction == GL_CE_NONE ? g[row * sg] : 1.f;
   if (t < 0 || t >= N) c = __builtin_nanf("");
   if (t == ignored) c = 0.f;
   info[m] = uv4{__float_as_uint(k.top[m]), __float_as_uint(c == 0.f ? 0.f : c / k.sum[m]), (unsigned)t, __float_as_uint(c * expm1f(-k.loss[m]))};
@@ -405,17 +408,34 @@ struct CeBwd {
   Operand w;
   bool direct;              // dX's product writes dX itself
   int kept;                 // classes whose exponentials were kept: the first piece, or none
-  size_t x_at, w_at, info, dz, dx, part, cols, bytes;
+  size_t x_at, w_at, info, alpha, dz, dx, part, cols, bytes;
 };
-// the three products of the classes [n0, n0 + n)
+// the products of the classes [n0, n0 + n); dW's rows behind `head` go through one of their own
 struct Piece {
-  Product logits, px, pw;
+  Product logits, px, pw, pw_tail;
+  long long head;
 };
 Piece plan_piece(const GlCeBwdArgs* a, long long n) {
   Piece p{};
+  p.head = n;
   p.logits = plan_product(a->dtype, a->M, (int)n, a->K, 1);
   if (a->dX) p.px = plan_product(a->dtype, a->M, a->K, n);
-  if (a->dW) p.pw = plan_product(a->dtype, n, a->K, a->M);
+  if (a->dW) {
+    p.pw = plan_product(a->dtype, n, a->K, a->M);
+    // Tiles come in rounds of one a CU, and a last round of few takes as long as a full one.  The rows of whole rounds and
+    // the rest as two products, where that is expected to take less: 50000 x 1024 over 4096, 784 tiles of 256 x 256 in 3.06
+    // rounds, 429 us; as two 388.
+    const long long per_row = (a->K + DENSE_BN[DENSE_256] - 1) / DENSE_BN[DENSE_256];
+    const long long tiles = (n + 255) / 256 * per_row, head = tiles / 256 * 256 / per_row * 256;
+    if (p.pw.splits && head > 0 && head < n) {
+      const Product h = plan_product(a->dtype, head, a->K, a->M), t = plan_product(a->dtype, n - head, a->K, a->M);
+      if (h.splits && t.splits && h.us + t.us < p.pw.us) {
+        p.pw = h;
+        p.pw_tail = t;
+        p.head = head;
+      }
+    }
+  }
   return p;
 }
 bool planned(const GlCeBwdArgs* a, const Piece& p) {
@@ -437,6 +457,7 @@ int plan_ce_bwd(const GlCeBwdArgs* a, CeBwd* out) {
     const size_t c = (size_t)q.logits.tiles_m * waves_m(a->dtype, q.logits.tile) * n * 4;
     part = part > q.px.part_bytes ? part : q.px.part_bytes;
     part = part > q.pw.part_bytes ? part : q.pw.part_bytes;
+    part = part > q.pw_tail.part_bytes ? part : q.pw_tail.part_bytes;
     cols = cols > c ? cols : c;
   }
   p.kept = a->exps ? kept_classes(a->M, a->N, a->K, a->dtype, a->piece_bytes) : 0;
@@ -448,6 +469,7 @@ int plan_ce_bwd(const GlCeBwdArgs* a, CeBwd* out) {
   p.x_at = l.take((size_t)a->M * padded(a->K) * es);
   p.w_at = l.take(copy_bytes(p.w, es));
   p.info = l.take((size_t)a->M * 16);
+  p.alpha = l.take(4);
   p.dz = l.take(p.kept && p.pieces == 1 ? 0 : (size_t)a->M * padded(p.piece) * es);
   p.dx = l.take(a->dX && !p.direct ? (size_t)a->M * a->K * (p.pieces > 1 ? 4 : es) : 0);
   p.part = l.take(part);
@@ -575,9 +597,10 @@ extern "C" int gl_ce_bwd(const GlCeBwdArgs* a, void* stream) {
   const Kept k = kept_of(const_cast<int32_t*>(a->kept), a->M);
   uv4* info = (uv4*)(ws + p.info);
   GL_LAUNCH(GL_KERNEL_CE_ROWS, ce_info_kernel, dim3((unsigned)((a->M + 255) / 256)), dim3(256), 0, s, (const long long*)a->target,
-            (long long)a->M, (long long)a->ignore_index, a->N, a->reduction, k, p.all, a->dloss, (long long)a->sdl, info);
+            (long long)a->M, (long long)a->ignore_index, a->N, a->reduction, k, p.all, a->dloss, (long long)a->sdl, info, (float*)(ws + p.alpha));
   GL_CHECK_LAUNCH();
   const int* count = p.all ? nullptr : k.count;
+  const float* alpha = a->reduction == GL_CE_NONE ? nullptr : (const float*)(ws + p.alpha);
   GL_TRY(launch_gather(a->X, a->sx, a->M, a->K, es, k.count, p.all ? nullptr : k.index, p.all ? info : nullptr, ws + p.x_at, s));
   GL_TRY(launch_align(nullptr, nullptr, &p.w, ws + p.w_at, es, s));
   const Operand x_rows{ws + p.x_at, padded(a->K), a->M, a->K, true, true};
@@ -611,16 +634,20 @@ extern "C" int gl_ce_bwd(const GlCeBwdArgs* a, void* stream) {
       chunks = (long long)q.logits.tiles_m * waves_m(a->dtype, q.logits.tile);
     }
     const Operand dz{at, pitch, a->M, (int)n, true, true};
-    if (a->db) GL_TRY(launch_db(cols, chunks, (int)n, (char*)a->db + n0 * es_of(a->g_dtype), a->g_dtype, a->accumulate, s));
+    if (a->db) GL_TRY(launch_db(cols, chunks, (int)n, (char*)a->db + n0 * es_of(a->g_dtype), a->g_dtype, a->accumulate, s, alpha));
     if (a->dX) {
       const int to = p.pieces > 1 ? GL_DTYPE_F32 : a->dtype;
       GL_TRY(run_product(a->dtype, DENSE_NN, dz, w, n, q.px, ws + p.part,
-                         store_epi(p.direct ? a->dX : ws + p.dx, a->K, to, a->M, a->K, a->dtype, i > 0), s, count));
+                         store_epi(p.direct ? a->dX : ws + p.dx, a->K, to, a->M, a->K, a->dtype, i > 0), s, count, alpha));
     }
-    if (a->dW)
-      GL_TRY(run_product(a->dtype, DENSE_TN, dz, x_rows, a->M, q.pw, ws + p.part,
-                         store_epi((char*)a->dW + n0 * a->K * es_of(a->g_dtype), a->K, a->g_dtype, n, a->K, a->dtype,
-                                   a->accumulate), s, count));
+    for (long long from = 0, rows = q.head; a->dW && rows > 0; from += rows, rows = from < n ? n - from : 0) {
+      Operand dz_t = dz;
+      dz_t.p = (const char*)at + from * es;
+      dz_t.cols = (int)rows;
+      GL_TRY(run_product(a->dtype, DENSE_TN, dz_t, x_rows, a->M, from ? q.pw_tail : q.pw, ws + p.part,
+                         store_epi((char*)a->dW + (n0 + from) * a->K * es_of(a->g_dtype), a->K, a->g_dtype, rows, a->K, a->dtype,
+                                   a->accumulate), s, count, alpha));
+    }
   }
   if (a->dX && !p.direct) {
     const dim3 grid((unsigned)((a->M + 3) / 4), (unsigned)ceil_div(a->K, 512));

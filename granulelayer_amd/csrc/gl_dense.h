@@ -53,11 +53,12 @@ struct DenseK {
 };
 
 // What a product's kernel does besides: nothing; take the number of its rows (of C, or where both operands
-// are RS of the reduction) from device memory; and the two products of the softmax cross entropy, logits = X W^T
+// are RS of the reduction) and a factor from device memory; and the two products of the softmax cross entropy, logits = X W^T
 // of a piece of the classes, that leave a tile's softmax statistics or their gradient and no logits (gl_ce.hip).
 enum { DENSE_PLAIN, DENSE_ROWS, DENSE_CE_STATS, DENSE_CE_GRAD };
 struct DenseRowsK : DenseK {
   const int* rows;           // or null: as the sizes say
+  const float* alpha;        // DENSE_ROWS: factor of the product, or null: 1
   // statistics
   const long long* target;
   const int* index;          // row of `target` of every row of X, or null: its own
@@ -814,6 +815,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(typename De
 #pragma unroll
     for (int j = 0; j < 4; ++j) bias[j] = ce_bias(bias[j]);
   }
+  float alpha = 1.f;
+  if constexpr (KIND == DENSE_ROWS) alpha = a.alpha && !split_up ? *a.alpha : 1.f;
   float col[4] = {0.f, 0.f, 0.f, 0.f};  // DENSE_CE_GRAD: of this lane's columns
   uv4 r[ROWS];
   auto load_rows = [&](long long m) {
@@ -873,6 +876,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void dense_tile_kernel(typename De
       }
       if constexpr (FORWARD) {
         if (!split_up) dense_forward<ROWS>(a.e, mi, 4, n, v, bias);
+      }
+      if constexpr (KIND == DENSE_ROWS) {
+#pragma unroll
+        for (int x = 0; x < ROWS; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[x][j] *= alpha;
       }
       if constexpr (KIND == DENSE_CE_GRAD) {
         int t[ROWS];
@@ -1011,11 +1020,12 @@ struct Product {
   size_t part_bytes;
 };
 Product plan_product(int dtype, long long M, int N, long long R, int most_splits = 32);
-// rows: DENSE_ROWS (null: DENSE_PLAIN)
+// rows, alpha: DENSE_ROWS (both null: DENSE_PLAIN)
 int run_product(int dtype, int form, const Operand& p, const Operand& q, long long R, const Product& pl, void* part,
-                const DenseEpi& e, hipStream_t s, const int* rows = nullptr);
+                const DenseEpi& e, hipStream_t s, const int* rows = nullptr, const float* alpha = nullptr);
 DenseEpi store_epi(void* C, long long sc, int c_dtype, long long M, int N, int op_dtype, int accumulate);
-int launch_db(const float* part, long long chunks, int N, void* db, int g_dtype, int accumulate, hipStream_t s);
+int launch_db(const float* part, long long chunks, int N, void* db, int g_dtype, int accumulate, hipStream_t s,
+              const float* alpha = nullptr);
 
 // few rows (gl_dense_few.hip): the forward of up to DENSE_FEW_ROWS rows that keeps nothing
 constexpr int DENSE_FEW_ROWS = 64;

@@ -89,7 +89,8 @@ namespace {
 // ---- the sums of a split product --------------------------------------------------------------------
 // A lane holds 4 neighbouring columns and adds the splits in their order, then the epilogue.  Bound by the sums'
 // bytes: 2 x 2048 x 1024 fp32 in 5.7 us (4.4 TB/s).
-__global__ __launch_bounds__(256) void dense_join_kernel(const float* __restrict__ part, int splits, DenseEpi e) {
+__global__ __launch_bounds__(256) void dense_join_kernel(const float* __restrict__ part, int splits, DenseEpi e,
+                                                         const float* __restrict__ alpha) {
   const long long m = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int l = threadIdx.x & 63, n = blockIdx.y * 256 + l * 4, there = m < e.M ? e.N - n : 0;
   float v[1][4] = {{0.f, 0.f, 0.f, 0.f}}, b[4];
@@ -105,6 +106,10 @@ __global__ __launch_bounds__(256) void dense_join_kernel(const float* __restrict
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[0][j] += t[j];
     }
+  }
+  if (alpha) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[0][j] *= *alpha;
   }
   dense_forward<1>(e, m, 1, n, v, b);
   if (added.p) add_added(v[0], r, added.bf);
@@ -155,7 +160,7 @@ Product plan_product(int dtype, long long M, int N, long long R, int most_splits
 }
 
 int run_product(int dtype, int form, const Operand& p, const Operand& q, long long R, const Product& pl, void* part,
-                const DenseEpi& e, hipStream_t s, const int* rows) {
+                const DenseEpi& e, hipStream_t s, const int* rows, const float* alpha) {
   const int es = es_of(dtype);
   DenseRowsK k{};
   k.P = p.p;
@@ -170,12 +175,13 @@ int run_product(int dtype, int form, const Operand& p, const Operand& q, long lo
   k.part = pl.splits > 1 ? (float*)part : nullptr;
   k.e = e;
   k.rows = rows;
+  k.alpha = alpha;
   const bool bf = dtype == GL_DTYPE_BF16;
-  if (rows) GL_TRY(bf ? launch_rows_tile_bf16(DENSE_ROWS, form, pl.tile, k, pl.splits, s) : launch_rows_tile_f32(DENSE_ROWS, form, pl.tile, k, pl.splits, s));
+  if (rows || alpha) GL_TRY(bf ? launch_rows_tile_bf16(DENSE_ROWS, form, pl.tile, k, pl.splits, s) : launch_rows_tile_f32(DENSE_ROWS, form, pl.tile, k, pl.splits, s));
   else GL_TRY(bf ? launch_dense_tile_bf16(form, pl.tile, k, pl.splits, s) : launch_dense_tile_f32(form, pl.tile, k, pl.splits, s));
   if (pl.splits > 1) {
     const dim3 grid((unsigned)((e.M + 3) / 4), (unsigned)ceil_div(e.N, 256));
-    GL_LAUNCH(GL_KERNEL_DENSE_JOIN, dense_join_kernel, grid, dim3(256), 0, s, (const float*)part, pl.splits, e);
+    GL_LAUNCH(GL_KERNEL_DENSE_JOIN, dense_join_kernel, grid, dim3(256), 0, s, (const float*)part, pl.splits, e, alpha);
     GL_CHECK_LAUNCH();
   }
   return 0;
@@ -266,7 +272,8 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const void* __restrict__ 
 // db from the sums of `chunks` row blocks: 32 columns a workgroup, 32 rows of lanes, then LDS.  256 x 4096 sums: 6 us,
 // the latency of 8 dependent loads.
 __global__ __launch_bounds__(1024) void dense_db_kernel(const float* __restrict__ part, long long chunks, int N,
-                                                        void* __restrict__ db, int g_bf, int accumulate) {
+                                                        void* __restrict__ db, int g_bf, int accumulate,
+                                                        const float* __restrict__ alpha) {
   __shared__ float sums[32][33];
   const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
   float s = 0.f;
@@ -278,6 +285,7 @@ __global__ __launch_bounds__(1024) void dense_db_kernel(const float* __restrict_
   float t = 0.f;
 #pragma unroll
   for (int i = 0; i < 32; ++i) t += sums[i][c];
+  if (alpha) t *= *alpha;
   if (g_bf) ((unsigned short*)db)[n] = to_bf16(t);
   else ((float*)db)[n] = accumulate ? ((float*)db)[n] + t : t;
 }
@@ -444,9 +452,10 @@ DenseEpi store_epi(void* C, long long sc, int c_dtype, long long M, int N, int o
   return e;
 }
 
-int launch_db(const float* part, long long chunks, int N, void* db, int g_dtype, int accumulate, hipStream_t s) {
+int launch_db(const float* part, long long chunks, int N, void* db, int g_dtype, int accumulate, hipStream_t s,
+              const float* alpha) {
   GL_LAUNCH(GL_KERNEL_DENSE_DB, dense_db_kernel, dim3((unsigned)ceil_div(N, 32)), dim3(1024), 0, s, part, chunks, N, db,
-            (int)(g_dtype == GL_DTYPE_BF16), accumulate);
+            (int)(g_dtype == GL_DTYPE_BF16), accumulate, alpha);
   GL_CHECK_LAUNCH();
   return 0;
 }

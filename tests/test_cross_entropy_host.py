@@ -84,7 +84,7 @@ def test_workspace_follows_the_budget():
         return out.value
 
     M, V = 8192, 131072
-    rest = M * 4096 * 2 + M * 16 + M * 4096 * 4  # x, the rows, dx in fp32 over the pieces
+    rest = M * 4096 * 2 + M * 16 + 256 + M * 4096 * 4  # x, the rows, their factor, dx in fp32 over the pieces
     for budget in (64 << 20, 256 << 20, 1 << 30):
         assert budget * 0.9 < need(M, V, budget) - rest <= budget + 256 * M * 2
     assert need(M, V, 0) == need(M, V, 1 << 30)
