@@ -58,7 +58,8 @@ class GlEdgeArgs(ctypes.Structure):
 class GlAdamArgs(ctypes.Structure):
     _fields_ = [("p", _P), ("g", _P), ("m", _P), ("v", _P), ("n", _I64), ("moments_dtype", _I32), ("lr", _F),
                 ("beta1", _F), ("beta2", _F), ("eps", _F), ("weight_decay", _F), ("bc1", _F), ("bc2", _F),
-                ("p_dtype", _I32), ("stochastic", _I32), ("master", _P), ("seed", ctypes.c_uint64)]
+                ("p_dtype", _I32), ("stochastic", _I32), ("master", _P), ("seed", ctypes.c_uint64), ("tensors", _P),
+                ("count", _I32), ("g_dtype", _I32), ("keep_g", _I32), ("beta1_64", _D), ("beta2_64", _D)]
 
 
 class GlCoverArgs(ctypes.Structure):
@@ -90,12 +91,6 @@ class GlAdamTensor(ctypes.Structure):
                 ("n", _I64), ("seed", ctypes.c_uint64), ("bc1", _F), ("bc2", _F)]
 
 
-class GlAdamManyArgs(ctypes.Structure):
-    _fields_ = [("t", _P), ("count", _I32), ("p_dtype", _I32), ("g_dtype", _I32), ("moments_dtype", _I32),
-                ("stochastic", _I32), ("clear", _I32), ("lr", _D), ("beta1", _D), ("beta2", _D), ("eps", _D),
-                ("weight_decay", _D)]
-
-
 class GlNormArgs(ctypes.Structure):
     _fields_ = [("X", _P), ("sx", _I64), ("weight", _P), ("bias", _P), ("Y", _P), ("sy", _I64), ("stats", _P), ("M", _I64),
                 ("D", _I32), ("x_dtype", _I32), ("w_dtype", _I32), ("y_dtype", _I32), ("eps", _F)]
@@ -120,9 +115,9 @@ class GlCeBwdArgs(ctypes.Structure):
                 ("piece_bytes", _SZ), ("exps", _P), ("ws", _P), ("ws_bytes", _SZ)]
 
 
-# gl_struct_layout ids 0..13
+# gl_struct_layout ids 0..12
 STRUCTS = (GlFwdArgs, GlBwdArgs, GlEdgeArgs, GlAdamArgs, GlCoverArgs, GlPack8Args, GlDenseArgs, GlDenseBwdArgs,
-           GlAdamTensor, GlAdamManyArgs, GlNormArgs, GlNormBwdArgs, GlCeArgs, GlCeBwdArgs)
+           GlAdamTensor, GlNormArgs, GlNormBwdArgs, GlCeArgs, GlCeBwdArgs)
 # every symbol include/granulelayer_amd.h declares
 EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_workspace", "gl_fwd", "gl_fwd_static",
            "gl_fwd_mask_bytes",
@@ -130,7 +125,7 @@ EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_work
            "gl_edges_build", "gl_bwd_workspace", "gl_bwd", "gl_adam", "gl_sched_size", "gl_sched_build_host",
            "gl_sched_build", "gl_window_build_host", "gl_window_build", "gl_cover_select", "gl_trace_begin",
            "gl_trace_end", "gl_pack8", "gl_unpack8", "gl_dense_fwd_workspace", "gl_dense_fwd", "gl_dense_bwd_workspace",
-           "gl_dense_bwd", "gl_adam_many", "gl_adam_values", "gl_norm_fwd", "gl_norm_bwd_workspace",
+           "gl_dense_bwd", "gl_adam_values", "gl_norm_fwd", "gl_norm_bwd_workspace",
            "gl_norm_bwd", "gl_ce_fwd_workspace", "gl_ce_exps_bytes", "gl_ce_fwd", "gl_ce_bwd_workspace", "gl_ce_bwd")
 KERNEL_NAMES = {1: "tile_x_kernel", 2: "fwd_kernel", 3: "fwd_finalize_kernel", 4: "c1t_kernel", 5: "bwd_w_kernel",
                 6: "dx_kernel", 7: "dx_reduce_kernel", 8: "adam_kernel", 9: "edges_build", 10: "fwd_kernel_win",
@@ -179,7 +174,7 @@ class Library:
         for name, st in (("gl_fwd", GlFwdArgs), ("gl_fwd_static", GlFwdArgs), ("gl_bwd", GlBwdArgs),
                          ("gl_edges_build", GlEdgeArgs), ("gl_adam", GlAdamArgs), ("gl_cover_select", GlCoverArgs), ("gl_pack8", GlPack8Args), ("gl_unpack8", GlPack8Args),
                          ("gl_dense_fwd", GlDenseArgs), ("gl_dense_bwd", GlDenseBwdArgs),
-                         ("gl_adam_many", GlAdamManyArgs), ("gl_adam_values", GlAdamManyArgs),
+                         ("gl_adam_values", GlAdamArgs),
                          ("gl_norm_fwd", GlNormArgs), ("gl_norm_bwd", GlNormBwdArgs),
                          ("gl_ce_fwd", GlCeArgs), ("gl_ce_bwd", GlCeBwdArgs)):
             f = getattr(L, name)

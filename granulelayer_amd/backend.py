@@ -414,17 +414,18 @@ class HipBackend:
         """In-place fused AdamW over the tensors of ``rows`` (``adam_row``); all of one dtype of parameters, gradients
         and moments (int8: codes), all with a master or none."""
         t = b"".join(rows)
-        a = N.GlAdamManyArgs(ctypes.cast(t, ctypes.c_void_p), len(rows), _DENSE_DTYPES[p_dtype], _DENSE_DTYPES[g_dtype], _MOMENTS[m_dtype],
-                             int(stochastic), int(clear), lr, beta1, beta2, eps, weight_decay)
+        a = N.GlAdamArgs(0, 0, 0, 0, 0, _MOMENTS[m_dtype], lr, beta1, beta2, eps, weight_decay, 0.0, 0.0, _DENSE_DTYPES[p_dtype],
+                         int(stochastic), 0, 0, ctypes.cast(t, ctypes.c_void_p), len(rows), _DENSE_DTYPES[g_dtype], int(not clear),
+                         beta1, beta2)
         with _on(device):
-            self.lib.call("gl_adam_many", ctypes.byref(a), _stream(device))
+            self.lib.call("gl_adam", ctypes.byref(a), ctypes.c_void_p(_stream(device)))
 
     def adam_values(self, device, rows):
         """The fp32 values of 8-bit moments: ``rows`` as for ``adam_many``, with m's values going to g and v's to p."""
         t = b"".join(rows)
-        a = N.GlAdamManyArgs(ctypes.cast(t, ctypes.c_void_p), len(rows), 0, 0, N.GL_MOMENTS_INT8)
+        a = N.GlAdamArgs(moments_dtype=N.GL_MOMENTS_INT8, tensors=ctypes.cast(t, ctypes.c_void_p), count=len(rows))
         with _on(device):
-            self.lib.call("gl_adam_values", ctypes.byref(a), _stream(device))
+            self.lib.call("gl_adam_values", ctypes.byref(a), ctypes.c_void_p(_stream(device)))
 
     # ------------------------------------------------------------------ activations in 8 bits
     def pack8(self, x):

@@ -125,7 +125,8 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       long long t[] = {(long long)sizeof(S), OFF(S, p), OFF(S, g), OFF(S, m), OFF(S, v), OFF(S, n),
                        OFF(S, moments_dtype), OFF(S, lr), OFF(S, beta1), OFF(S, beta2), OFF(S, eps),
                        OFF(S, weight_decay), OFF(S, bc1), OFF(S, bc2), OFF(S, p_dtype), OFF(S, stochastic),
-                       OFF(S, master), OFF(S, seed)};
+                       OFF(S, master), OFF(S, seed), OFF(S, tensors), OFF(S, count), OFF(S, g_dtype),
+                       OFF(S, keep_g), OFF(S, beta1_64), OFF(S, beta2_64)};
       for (long long x : t) v[c++] = x;
       break;
     }
@@ -170,21 +171,13 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       break;
     }
     case 9: {
-      typedef GlAdamManyArgs S;
-      long long t[] = {(long long)sizeof(S), OFF(S, t), OFF(S, count), OFF(S, p_dtype), OFF(S, g_dtype),
-                       OFF(S, moments_dtype), OFF(S, stochastic), OFF(S, clear), OFF(S, lr), OFF(S, beta1), OFF(S, beta2),
-                       OFF(S, eps), OFF(S, weight_decay)};
-      for (long long x : t) v[c++] = x;
-      break;
-    }
-    case 10: {
       typedef GlNormArgs S;
       long long t[] = {(long long)sizeof(S), OFF(S, X), OFF(S, sx), OFF(S, weight), OFF(S, bias), OFF(S, Y), OFF(S, sy),
                        OFF(S, stats), OFF(S, M), OFF(S, D), OFF(S, x_dtype), OFF(S, w_dtype), OFF(S, y_dtype), OFF(S, eps)};
       for (long long x : t) v[c++] = x;
       break;
     }
-    case 11: {
+    case 10: {
       typedef GlNormBwdArgs S;
       long long t[] = {(long long)sizeof(S), OFF(S, dY), OFF(S, sdy), OFF(S, X), OFF(S, sx), OFF(S, weight), OFF(S, stats),
                        OFF(S, dX), OFF(S, dweight), OFF(S, dbias), OFF(S, M), OFF(S, D), OFF(S, x_dtype), OFF(S, w_dtype),
@@ -192,7 +185,7 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       for (long long x : t) v[c++] = x;
       break;
     }
-    case 12: {
+    case 11: {
       typedef GlCeArgs S;
       long long t[] = {(long long)sizeof(S), OFF(S, X), OFF(S, sx), OFF(S, W), OFF(S, sw), OFF(S, bias), OFF(S, target),
                        OFF(S, ignore_index), OFF(S, M), OFF(S, N), OFF(S, K), OFF(S, dtype), OFF(S, reduction),
@@ -200,7 +193,7 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
       for (long long x : t) v[c++] = x;
       break;
     }
-    case 13: {
+    case 12: {
       typedef GlCeBwdArgs S;
       long long t[] = {(long long)sizeof(S), OFF(S, X), OFF(S, sx), OFF(S, W), OFF(S, sw), OFF(S, bias), OFF(S, target),
                        OFF(S, ignore_index), OFF(S, M), OFF(S, N), OFF(S, K), OFF(S, dtype), OFF(S, reduction),

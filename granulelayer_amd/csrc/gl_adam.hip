@@ -27,7 +27,7 @@ struct AdamK {
 };
 
 // The tensors of a launch travel as kernel arguments: nothing to copy to the device, nothing to keep alive.
-constexpr int ADAM_TENSORS = 40;      // of a launch: 3.7 of the 4 KB that arguments may take
+constexpr int ADAM_TENSORS = 38;      // of a launch: in the 4 KB that arguments may take
 constexpr int ADAM_BLOCK = 256;       // elements that share a scale
 constexpr int ADAM_CHUNK = 1024;      // elements of a workgroup: a vector of 4 a thread
 struct AdamTensorK {
@@ -39,6 +39,7 @@ struct AdamTensorK {
   float* m_scale;
   float* v_scale;
   long long n;
+  long long first;                     // of the tensor's elements
   unsigned long long seed;
   float bc1, bc2;
 };
@@ -321,7 +322,7 @@ __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensor
   if constexpr (PM == PM_BF16_SR) {
     unsigned o[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = round_stochastic(p[j], t.seed, block + i + j);
+    for (int j = 0; j < 4; ++j) o[j] = round_stochastic(p[j], t.seed, t.first + block + i + j);
     adam_store(O, i, n, o[0] | o[1] << 16, o[2] | o[3] << 16);
   } else if constexpr (PM != PM_F32) {
     adam_store(O, i, n, to_bf16x2(p[0], p[1]), to_bf16x2(p[2], p[3]));
@@ -370,38 +371,47 @@ void launch_adam_of(int pm, bool gbf, dim3 grid, hipStream_t s, const AdamTable&
   else launch_adam_as<MOM, PM_BF16_SR>(gbf, grid, s, a);
 }
 
-// one launch for every ADAM_TENSORS tensors; `values`: their moments' values instead of a step
-int launch_adam(const GlAdamManyArgs* a, bool values, hipStream_t s) {
+// one launch for every ADAM_TENSORS of the tensors; `values`: their moments' values instead of a step
+int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, bool values, hipStream_t s) {
   AdamTable k{};
-  k.lr = (float)a->lr;
-  k.b1 = (float)a->beta1;
-  k.b2 = (float)a->beta2;
-  k.eps = (float)a->eps;
-  k.wd = (float)a->weight_decay;
-  k.clear = a->clear;
-  k.b1d = a->beta1;
-  k.a1d = 1.0 - a->beta1;
-  k.b2d = a->beta2;
-  k.a2d = 1.0 - a->beta2;
+  k.lr = a->lr;
+  k.b1 = a->beta1;
+  k.b2 = a->beta2;
+  k.eps = a->eps;
+  k.wd = a->weight_decay;
+  k.clear = !a->keep_g;
+  k.b1d = a->beta1_64;
+  k.a1d = 1.0 - a->beta1_64;
+  k.b2d = a->beta2_64;
+  k.a2d = 1.0 - a->beta2_64;
   constexpr long long MAX_GROUPS = 1LL << 23;  // of a launch: fewer than 2^32 threads
+  constexpr long long MOST = MAX_GROUPS * ADAM_CHUNK;  // elements of a launch; a longer tensor takes several
   int next = 0;
-  while (next < a->count) {
+  long long done = 0;  // of the next tensor
+  while (next < count) {
     long long groups = 0;
     k.count = 0;
-    while (next < a->count && k.count < ADAM_TENSORS) {
-      const GlAdamTensor& t = a->t[next];
-      const long long need = (t.n + ADAM_CHUNK - 1) / ADAM_CHUNK;
-      if (groups + need > MAX_GROUPS) break;  // (a tensor has at most MAX_GROUPS: check_adam)
-      ++next;
-      if (need == 0) continue;
-      k.first[k.count] = (unsigned)groups;
-      AdamTensorK& d = k.t[k.count++];
-      d = AdamTensorK{t.p, t.g, t.m, t.v, t.master, t.m_scale, t.v_scale, (long long)t.n, (unsigned long long)t.seed, t.bc1, t.bc2};
-      if (a->moments_dtype == GL_MOMENTS_INT8) {  // as that update takes them
-        d.bc1 = (float)(a->lr / t.bc1);
-        d.bc2 = (float)(1.0 / __builtin_sqrt((double)t.bc2));
+    while (next < count && k.count < ADAM_TENSORS && groups < MAX_GROUPS) {
+      const GlAdamTensor& t = tensors[next];
+      const long long left = t.n - done, room = (MAX_GROUPS - groups) * ADAM_CHUNK, n = left < room ? left : room;
+      if (n > 0) {
+        AdamTensorK& d = k.t[k.count];
+        k.first[k.count++] = (unsigned)groups;
+        const auto at = [&](void* p, int bytes) { return (void*)((char*)p + done * bytes); };
+        const int pe = values || a->p_dtype == GL_DTYPE_F32 ? 4 : 2, ge = values || a->g_dtype == GL_DTYPE_F32 ? 4 : 2;
+        const bool i8 = a->moments_dtype == GL_MOMENTS_INT8;
+        const int me = i8 ? 1 : a->moments_dtype == GL_DTYPE_F32 ? 4 : 2;
+        d = AdamTensorK{at(t.p, pe), at(t.g, ge), at(t.m, me), at(t.v, me), t.master ? t.master + done : nullptr,
+                        i8 ? t.m_scale + done / ADAM_BLOCK : nullptr, i8 ? t.v_scale + done / ADAM_BLOCK : nullptr, n, done,
+                        (unsigned long long)t.seed, t.bc1, t.bc2};
+        if (i8) {  // as that update takes them
+          d.bc1 = (float)((double)a->lr / t.bc1);
+          d.bc2 = (float)(1.0 / __builtin_sqrt((double)t.bc2));
+        }
+        groups += (n + ADAM_CHUNK - 1) / ADAM_CHUNK;
       }
-      groups += need;
+      done = n < left ? done + n : 0;
+      next += n >= left;
     }
     if (groups == 0) continue;
     k.first[k.count] = (unsigned)groups;
@@ -409,8 +419,7 @@ int launch_adam(const GlAdamManyArgs* a, bool values, hipStream_t s) {
     if (values) {
       GL_LAUNCH(GL_KERNEL_ADAM_VALUES, adam_values_kernel, grid, dim3(256), 0, s, k);
     } else {
-      const AdamTensorK& t = k.t[0];
-      const int pm = a->p_dtype == GL_DTYPE_F32 ? PM_F32 : (t.master ? PM_BF16_MASTER : (a->stochastic ? PM_BF16_SR : PM_BF16_RNE));
+      const int pm = a->p_dtype == GL_DTYPE_F32 ? PM_F32 : (k.t[0].master ? PM_BF16_MASTER : (a->stochastic ? PM_BF16_SR : PM_BF16_RNE));
       const bool gbf = a->g_dtype == GL_DTYPE_BF16;
       if (a->moments_dtype == GL_DTYPE_F32) launch_adam_of<GL_DTYPE_F32>(pm, gbf, grid, s, k);
       else if (a->moments_dtype == GL_DTYPE_BF16) launch_adam_of<GL_DTYPE_BF16>(pm, gbf, grid, s, k);
@@ -421,8 +430,8 @@ int launch_adam(const GlAdamManyArgs* a, bool values, hipStream_t s) {
   return 0;
 }
 
-int check_adam(const GlAdamManyArgs* a, bool values) {
-  if (!a || a->count < 0 || (a->count > 0 && !a->t)) return GL_ERR_ARG;
+int check_tensors(const GlAdamArgs* a, bool values) {
+  if (a->count < 0 || !a->tensors) return GL_ERR_ARG;
   if (a->moments_dtype != GL_DTYPE_F32 && a->moments_dtype != GL_DTYPE_BF16 && a->moments_dtype != GL_MOMENTS_INT8)
     return GL_ERR_UNSUPPORTED;
   const bool i8 = a->moments_dtype == GL_MOMENTS_INT8;
@@ -430,19 +439,22 @@ int check_adam(const GlAdamManyArgs* a, bool values) {
   if (!values) {
     if ((a->p_dtype != GL_DTYPE_F32 && a->p_dtype != GL_DTYPE_BF16) || (a->g_dtype != GL_DTYPE_F32 && a->g_dtype != GL_DTYPE_BF16))
       return GL_ERR_UNSUPPORTED;
-    if (a->clear && a->g_dtype != GL_DTYPE_F32) return GL_ERR_ARG;
     if (a->p_dtype == GL_DTYPE_F32 && a->stochastic) return GL_ERR_ARG;  // fp32 parameters round nothing
   }
   const uintptr_t pe = values || a->p_dtype == GL_DTYPE_F32 ? 3 : 1, ge = values || a->g_dtype == GL_DTYPE_F32 ? 3 : 1;
   const uintptr_t me = i8 ? 0 : (a->moments_dtype == GL_DTYPE_F32 ? 3 : 1);
-  const bool master = a->count > 0 && a->t[0].master;
+  int master = -1;  // not known yet
   for (int i = 0; i < a->count; ++i) {
-    const GlAdamTensor& t = a->t[i];
+    const GlAdamTensor& t = a->tensors[i];
     if (t.n < 0) return GL_ERR_ARG;
     if (t.n == 0) continue;
     if (t.n > GL_ADAM_MAX_ELEMENTS) return GL_ERR_UNSUPPORTED;
     if (!t.p || !t.g || !t.m || !t.v || (i8 && (!t.m_scale || !t.v_scale))) return GL_ERR_ARG;
-    if (!values && ((t.master != nullptr) != master || (master && a->p_dtype == GL_DTYPE_F32))) return GL_ERR_ARG;
+    if (!values) {
+      if (master >= 0 && (t.master != nullptr) != (master == 1)) return GL_ERR_ARG;
+      master = t.master != nullptr;
+      if (t.master && a->p_dtype == GL_DTYPE_F32) return GL_ERR_ARG;
+    }
     if (((uintptr_t)t.p & pe) || ((uintptr_t)t.g & ge) || (((uintptr_t)t.m | (uintptr_t)t.v) & me) ||
         (((uintptr_t)t.master | (uintptr_t)t.m_scale | (uintptr_t)t.v_scale) & 3))
       return GL_ERR_ARG;
@@ -454,31 +466,33 @@ int check_adam(const GlAdamManyArgs* a, bool values) {
 
 using namespace gl;
 
-extern "C" int gl_adam_many(const GlAdamManyArgs* a, void* stream) {
-  GL_TRY(check_adam(a, false));
-  return launch_adam(a, false, (hipStream_t)stream);
-}
-
-extern "C" int gl_adam_values(const GlAdamManyArgs* a, void* stream) {
-  GL_TRY(check_adam(a, true));
-  return launch_adam(a, true, (hipStream_t)stream);
+extern "C" int gl_adam_values(const GlAdamArgs* a, void* stream) {
+  if (!a) return GL_ERR_ARG;
+  GL_TRY(check_tensors(a, true));
+  return launch_adam(a, a->tensors, a->count, true, (hipStream_t)stream);
 }
 
 extern "C" int gl_adam(const GlAdamArgs* a, void* stream) {
-  if (!a || a->n < 0) return GL_ERR_ARG;
+  if (!a) return GL_ERR_ARG;
+  if (a->tensors) {
+    GL_TRY(check_tensors(a, false));
+    return launch_adam(a, a->tensors, a->count, false, (hipStream_t)stream);
+  }
+  if (a->n < 0) return GL_ERR_ARG;
   if (a->n == 0) return 0;
   if (!a->p || !a->g || !a->m || !a->v) return GL_ERR_ARG;
   if (a->moments_dtype != GL_DTYPE_F32 && a->moments_dtype != GL_DTYPE_BF16) return GL_ERR_UNSUPPORTED;
   if (a->p_dtype != GL_DTYPE_F32 && a->p_dtype != GL_DTYPE_BF16) return GL_ERR_UNSUPPORTED;
   if (a->p_dtype == GL_DTYPE_F32 && (a->master || a->stochastic)) return GL_ERR_ARG;  // fp32 parameters round nothing
   const bool f32p = a->p_dtype == GL_DTYPE_F32;
-  // this entry point's tensors are at whole vectors: 16-byte fp32 streams, 8-byte bf16 streams
+  // one tensor is at whole vectors: 16-byte fp32 streams, 8-byte bf16 streams
   const uintptr_t a16 = (uintptr_t)a->g | (f32p ? (uintptr_t)a->p : 0) | (uintptr_t)a->master;
   const uintptr_t a8 = f32p ? 0 : (uintptr_t)a->p;
   const uintptr_t alm = (uintptr_t)a->m | (uintptr_t)a->v;
   if ((a16 & 15) || (a8 & 7) || (alm & (a->moments_dtype == GL_DTYPE_F32 ? 15 : 7))) return GL_ERR_ARG;
   const GlAdamTensor t{a->p, a->g, a->m, a->v, a->master, nullptr, nullptr, a->n, a->seed, a->bc1, a->bc2};
-  const GlAdamManyArgs k{&t, 1, a->p_dtype, GL_DTYPE_F32, a->moments_dtype, a->master ? 0 : a->stochastic, 1,
-                         a->lr, a->beta1, a->beta2, a->eps, a->weight_decay};
-  return gl_adam_many(&k, stream);
+  GlAdamArgs k = *a;
+  k.g_dtype = GL_DTYPE_F32;
+  k.keep_g = 0;
+  return launch_adam(&k, &t, 1, false, (hipStream_t)stream);
 }

@@ -2,7 +2,7 @@
 
 Reads the fp32 ``main_grad`` buffers written by the fused backward (zeroed in the same streaming pass) or
 ``.grad`` in its own type, and updates the tensors of a parameter group together: a launch of the HIP kernel
-takes 40 of them (gl_adam_many).
+takes 38 of them (gl_adam).
 Semantics are dense AdamW for every element (optim.py:1-15): m = b1 m + (1-b1) g,
 v = b2 v + (1-b2) g^2, p = p (1 - lr wd) - lr (m / bc1) / (sqrt(v / bc2) + eps), bc_i = 1 - b_i^t.
 
@@ -141,14 +141,18 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            self._step_group(group)
+            params = group["params"]
+            while len(params) > len(set(map(id, params))):  # one that is there twice makes two steps, not two at once
+                self._step_tensors(group, list({id(p): p for p in params}.values()))
+                params = [p for i, p in enumerate(params) if any(p is q for q in params[:i])]
+            self._step_tensors(group, params)
         return loss
 
-    def _step_group(self, group):
+    def _step_tensors(self, group, params):
         b1, b2 = group["betas"]
         f32, bf16 = torch.float32, torch.bfloat16
         todo = []
-        for p in group["params"]:  # everything is checked before anything changes
+        for p in params:  # everything is checked before anything changes
             g = getattr(p, "main_grad", None)
             main = g is not None
             if not main:

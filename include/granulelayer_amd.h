@@ -176,13 +176,14 @@ typedef struct GlEdgeArgs {
  * (sparse_pooling/optim.py:26-64, 116-123) for fp32 parameters (HAS_MASTER = STOCH = False):
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  upd = (m/bc1) / (sqrt(v/bc2) + eps)
  *   p = p (1 - lr wd) - lr upd;  g = 0 (fused zero_grad) */
+typedef struct GlAdamTensor GlAdamTensor;
 typedef struct GlAdamArgs {
   void* p;                /* parameters, fp32 or bf16 (p_dtype) */
   float* g;               /* fp32 gradient (main_grad), zeroed */
   void* m;                /* fp32 or bf16 (moments_dtype) */
   void* v;
   int64_t n;
-  int32_t moments_dtype;  /* GL_DTYPE_F32 | GL_DTYPE_BF16 */
+  int32_t moments_dtype;  /* GL_DTYPE_F32 | GL_DTYPE_BF16; of `tensors` GL_MOMENTS_INT8 too */
   float lr, beta1, beta2, eps, weight_decay, bc1, bc2;
   int32_t p_dtype;        /* GL_DTYPE_F32 | GL_DTYPE_BF16 */
   int32_t stochastic;     /* bf16 p without master: 1 = stochastic rounding (optim.py:59-62), 0 = nearest even */
@@ -190,7 +191,34 @@ typedef struct GlAdamArgs {
                              optim.py:54-56), or NULL */
   uint64_t seed;          /* stochastic rounding: element i adds the low 16 bits of Triton's
                              tl.randint(seed, i) (Philox-4x32-10) below the bf16 cut, then truncates */
+  const GlAdamTensor* tensors; /* in host memory: the step runs over these, in place of p, g, m, v, n, bc1, bc2, master
+                             and seed; NULL: over one */
+  int32_t count;          /* of them */
+  int32_t g_dtype;        /* their gradients: GL_DTYPE_F32 | GL_DTYPE_BF16 */
+  int32_t keep_g;         /* 1: which are not zeroed (as bf16 ones never are) */
+  double beta1_64, beta2_64; /* for GL_MOMENTS_INT8, in place of beta1, beta2 */
 } GlAdamArgs;
+
+/* One of many tensors (no counterpart in the reference, which launches a kernel a tensor).  A launch takes 38 of them,
+ * which travel as its arguments, so nothing is copied to the device and the array may go when the call returns.  No address
+ * needs more than its element's alignment.  Moments of GL_MOMENTS_INT8 are codes of one byte, m's signed, with two fp32
+ * scales for every 256 neighbouring elements (the last block of a tensor may be shorter):
+ *   m = m_scale c |c|,  m_scale = max |m| / 127^2;   v = (v_scale c^2)^2,  v_scale = sqrt(max v) / 255^2
+ * with the maxima rounded to fp32, c the nearest by its root, 1 at least where v > 0. */
+#define GL_MOMENTS_INT8 2
+#define GL_ADAM_MAX_ELEMENTS (1LL << 35) /* of a tensor */
+struct GlAdamTensor {
+  void* p;                /* [n] of p_dtype */
+  void* g;                /* [n] of g_dtype */
+  void* m;                /* [n] of moments_dtype */
+  void* v;
+  float* master;          /* as GlAdamArgs.master: all tensors of a call, or none */
+  float* m_scale;         /* [ceil(n / 256)] of 8-bit moments */
+  float* v_scale;
+  int64_t n;
+  uint64_t seed;          /* as GlAdamArgs.seed */
+  float bc1, bc2;
+};
 
 /* Cover-TopK support selection of an envelope (one-time preprocessing of CoverTopK16Layer).
  * Replaces local_supports.feature_importance / topk_select / cover_repair
@@ -225,8 +253,8 @@ int gl_cover_select(const GlCoverArgs* a, void* stream);
  * order) so a binding can refuse a mismatched library.  Replaces sp_abi_version /
  * sp_struct_layout (sparse_pooling/kernels/cuda/abi.cu:17-62, checked in runtime.py:103-120).
  * which: 0 GlFwdArgs, 1 GlBwdArgs, 2 GlEdgeArgs, 3 GlAdamArgs, 4 GlCoverArgs, 5 GlPack8Args, 6 GlDenseArgs,
- * 7 GlDenseBwdArgs, 8 GlAdamTensor, 9 GlAdamManyArgs, 10 GlNormArgs, 11 GlNormBwdArgs,
- * 12 GlCeArgs, 13 GlCeBwdArgs.  Returns the number of values written
+ * 7 GlDenseBwdArgs, 8 GlAdamTensor, 9 GlNormArgs, 10 GlNormBwdArgs, 11 GlCeArgs,
+ * 12 GlCeBwdArgs.  Returns the number of values written
  * (or needed, when n is too small), negative on an unknown struct. */
 int gl_abi_version(void);
 int gl_struct_layout(int which, long long* out, int n);
@@ -267,38 +295,8 @@ int gl_bwd(const GlBwdArgs* a, void* stream);
 /* Fused AdamW (in place). */
 int gl_adam(const GlAdamArgs* a, void* stream);
 
-/* The same step over many tensors: a launch takes 40 of them, which travel as its arguments, so nothing is
- * copied to the device and `t` may go when the call returns.  No address needs more than its element's
- * alignment.  Moments of GL_MOMENTS_INT8 are codes of one byte, m's signed, with two fp32 scales for every
- * 256 neighbouring elements (the last block of a tensor may be shorter):
- *   m = m_scale c |c|,  m_scale = max |m| / 127^2;   v = (v_scale c^2)^2,  v_scale = sqrt(max v) / 255^2
- * with the maxima rounded to fp32, c the nearest by its root, 1 at least where v > 0. */
-#define GL_MOMENTS_INT8 2
-#define GL_ADAM_MAX_ELEMENTS (1LL << 35) /* of a tensor */
-typedef struct GlAdamTensor {
-  void* p;                /* [n] of p_dtype */
-  void* g;                /* [n] of g_dtype */
-  void* m;                /* [n] of moments_dtype */
-  void* v;
-  float* master;          /* as GlAdamArgs.master: all tensors of a call, or none */
-  float* m_scale;         /* [ceil(n / 256)] of 8-bit moments */
-  float* v_scale;
-  int64_t n;
-  uint64_t seed;          /* as GlAdamArgs.seed */
-  float bc1, bc2;
-} GlAdamTensor;
-typedef struct GlAdamManyArgs {
-  const GlAdamTensor* t;  /* in host memory */
-  int32_t count;
-  int32_t p_dtype, g_dtype; /* GL_DTYPE_F32 | GL_DTYPE_BF16 */
-  int32_t moments_dtype;  /* GL_DTYPE_F32 | GL_DTYPE_BF16 | GL_MOMENTS_INT8 */
-  int32_t stochastic;     /* as GlAdamArgs.stochastic */
-  int32_t clear;          /* 1: fp32 gradients are zeroed */
-  double lr, beta1, beta2, eps, weight_decay;
-} GlAdamManyArgs;
-int gl_adam_many(const GlAdamManyArgs* a, void* stream);
-/* The fp32 values that 8-bit moments stand for: m's into g, v's into p (both [n] fp32). */
-int gl_adam_values(const GlAdamManyArgs* a, void* stream);
+/* The fp32 values that the 8-bit moments of `tensors` stand for: m's into g, v's into p (both [n] fp32). */
+int gl_adam_values(const GlAdamArgs* a, void* stream);
 
 /* Gather schedule of the forward and dW kernels (K = 8 only), built on the HOST once per index
  * tensor from host copies of idx [G*S, 8] and counts [G] (rec_shift 0); upload the result and pass it as

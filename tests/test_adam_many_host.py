@@ -60,21 +60,23 @@ def test_states_that_do_not_fit():
 def test_the_c_entry_points_refuse():
     lib = N.library()
 
-    def call(name="gl_adam_many", tensors=None, **kw):
+    def call(name="gl_adam", tensors=None, **kw):
         t = tensors if tensors is not None else [dict(p=16, g=16, m=16, v=16, m_scale=16, v_scale=16, n=5)]
         arr = (N.GlAdamTensor * max(1, len(t)))(*[N.GlAdamTensor(**x) for x in t])
-        a = N.GlAdamManyArgs(t=ctypes.addressof(arr), **{"count": len(t), **kw})
+        a = N.GlAdamArgs(tensors=ctypes.addressof(arr), **{"count": len(t), **kw})
         return getattr(lib.lib, name)(ctypes.byref(a), None)
 
     ok = dict(p=16, g=16, m=16, v=16, m_scale=16, v_scale=16, n=5)
     i8 = N.GL_MOMENTS_INT8
-    assert lib.lib.gl_adam_many(None, None) == -1
+    assert lib.lib.gl_adam(None, None) == -1 and lib.lib.gl_adam_values(None, None) == -1
+    empty = N.GlAdamArgs(moments_dtype=N.GL_MOMENTS_INT8)
+    assert lib.lib.gl_adam_values(ctypes.byref(empty), None) == -1  # of tensors only
     assert call(count=-1) == -1
     assert call(tensors=[]) == 0 and call(tensors=[dict(n=0)]) == 0  # nothing to do
     assert call(tensors=[dict(ok, n=-1)]) == -1
     assert call(tensors=[dict(ok, n=(1 << 35) + 1)]) == -2
     assert call(p_dtype=2) == -2 and call(g_dtype=2) == -2 and call(moments_dtype=3) == -2
-    assert call(g_dtype=1, clear=1) == -1 and call(stochastic=1) == -1
+    assert call(stochastic=1) == -1
     for key in ("p", "g", "m", "v"):
         assert call(tensors=[dict(ok, **{key: 0})]) == -1
         assert call(tensors=[dict(ok, **{key: 17})]) == -1  # off its element

@@ -96,6 +96,25 @@ def test_gradients_of_both_kinds_and_none():
     assert torch.equal(p[3].detach(), torch.ones_like(p[3])) and p[3] not in opt.state
 
 
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate")
+def test_a_parameter_that_is_there_twice():
+    """Two steps of it one after the other: the second has no gradient left (p.grad), or a zeroed one (main_grad)."""
+    for main in (False, True):
+        p, q = (torch.nn.Parameter(torch.ones(3000, device=DEV)) for _ in range(2))
+        opt = FusedAdamW([p, q, p], moments="fp32", lr=0.5, betas=(0.5, 0.5))
+        for t in (p, q):
+            if main:
+                t.main_grad = torch.ones(3000, device=DEV)
+            else:
+                t.grad = torch.ones(3000, device=DEV)
+        opt.step()
+        assert opt.state[p]["step"] == (2 if main else 1) and opt.state[q]["step"] == 1
+        # m = 1/2 then 1/4, v the same; corrected by 1 - 1/2 and 1 - 1/4: steps of 1/2 and of 1/2 (1/3) / sqrt(1/3)
+        want = 0.5 - (0.5 * 3 ** -0.5 if main else 0.0)
+        np.testing.assert_allclose(p.detach().cpu(), want, rtol=0, atol=2 ** -20)
+        np.testing.assert_allclose(q.detach().cpu(), 0.5, rtol=0, atol=2 ** -20)
+
+
 # ---- 8-bit moments ----------------------------------------------------------------------------------------
 def _values(cm, sm, cv, sv, n):
     of = np.arange(n) // 256

@@ -197,7 +197,7 @@ def test_classes_that_take_no_part(K, M):
     assert not got["dw"][300:].any() and not got["db"][300:].any()
     t["b"].fill_(torch.finfo(F).min)  # the type's lowest everywhere: a shift of all logits, no mask
     got = run(t, "mean")[1]
-    assert abs(float(got["loss"]) - math.log(700)) < 1e-5 and all(torch.isfinite(v).all() for v in got.values())
+    assert abs(float(got["loss"].detach()) - math.log(700)) < 1e-5 and all(torch.isfinite(v).all() for v in got.values())
     # x w is lost against it: every class has 1 / 700, so db is 1.7 / 700 - 1.7 times the class' share of the targets
     share = torch.bincount(t["target"][t["target"] != IGNORED], minlength=700) / int((t["target"] != IGNORED).sum())
     assert torch.allclose(got["db"], 1.7 * (1 / 700 - share), rtol=1e-5, atol=1e-7)
@@ -229,6 +229,28 @@ def test_rows_that_are_no_numbers(K):
     good[bad] = False
     assert torch.isnan(got["loss"][bad]).all() and torch.isnan(got["dx"][bad]).all()
     assert torch.equal(got["loss"][good], clean["loss"][good]) and torch.equal(got["dx"][good], clean["dx"][good])
+
+
+@pytest.mark.parametrize("M", [100, 700])
+def test_a_class_as_the_ignored_index(M):
+    t = inputs(M, 520, 300, BF, ignored=0.0)
+    t["target"][::3] = 7
+    other = dict(t, target=torch.where(t["target"] == 7, IGNORED, t["target"]))
+    want = run(other, "mean")[1]
+    leaves = [t[k].detach().requires_grad_(True) for k in "xwb"]
+    loss = dense_cross_entropy(*leaves[:2], t["target"], leaves[2], ignore_index=7)
+    assert torch.equal(loss, want["loss"])
+    for k, v in zip("xwb", torch.autograd.grad(loss, leaves, torch.tensor(1.7, device=DEV))):
+        assert torch.equal(v, want["d" + k])
+
+
+def test_a_graph_of_the_backward_is_refused_where_it_is_used():
+    t = inputs(300, 32, 64, F)
+    x = t["x"].detach().requires_grad_(True)
+    dx, = torch.autograd.grad(dense_cross_entropy(x, t["w"], t["target"], t["b"]), x, create_graph=True)
+    check(dx, definition(t, "mean", torch.ones((), device=DEV)), "dx")
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
 
 
 @pytest.mark.parametrize("dtype,K", [(F, 64), (F, 520), (BF, 520)])

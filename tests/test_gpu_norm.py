@@ -170,6 +170,15 @@ def test_rows_that_are_no_numbers_or_constant():
     assert torch.equal(layer_norm(const, w, b), b.expand(3, 600))  # sums of 600 sevens are whole: the mean is 7
 
 
+def test_a_graph_of_the_backward_is_refused_where_it_is_used():
+    x, w, b, dy = make(9, 300, F, F, F, seed=9)
+    xs = x.detach().requires_grad_(True)
+    dx, = torch.autograd.grad(layer_norm(xs, w, b), xs, dy, create_graph=True)
+    check(dx, definition(x, w, b, dy, 1e-5), "dx")
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
 def test_main_grad_is_added_to():
     lay = LayerNorm(300, device=DEV, out_dtype=BF)
     x, _, _, dy = make(40, 300, F, F, BF, seed=7)
