@@ -29,7 +29,8 @@ struct AdamK {
 // The tensors of a launch travel as kernel arguments: nothing to copy to the device, nothing to keep alive.
 constexpr int ADAM_TENSORS = 38;      // of a launch: in the 4 KB that arguments may take
 constexpr int ADAM_BLOCK = 256;       // elements that share a scale
-constexpr int ADAM_CHUNK = 1024;      // elements of a workgroup: a vector of 4 a thread
+// elements of a workgroup: a vector of 4 a thread, or two with 8-bit moments
+constexpr int adam_chunk(int moments) { return moments == GL_MOMENTS_INT8 ? 2048 : 1024; }
 struct AdamTensorK {
   void* p;
   void* g;
@@ -160,17 +161,15 @@ __device__ __forceinline__ unsigned round_stochastic(float p, unsigned long long
 }
 
 // ---- 8-bit moments -----------------------------------------------------------------------------------
-// the largest of 64 lanes, integer order (of values >= 0: the values' order, infinities and NaN above every number)
-__device__ __forceinline__ unsigned wave_umax(unsigned v) {
-  auto up = [](unsigned a, unsigned b) { return a > b ? a : b; };
+// the largest of the 32 lanes of half a wave, integer order (of values >= 0: the values' order, infinities and NaN above every number)
+__device__ __forceinline__ unsigned half_umax(unsigned v) {
+  auto up = [](unsigned a, unsigned b) { return umax(a, b); };
   v = up(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));   // lane ^ 1
   v = up(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));   // lane ^ 2
   v = up(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));  // row_ror:4
   v = up(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // row_ror:8
   const auto p16 = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = up(p16[0], p16[1]);
-  const auto p32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return up(p32[0], p32[1]);
+  return up(p16[0], p16[1]);
 }
 // 1 / x of a positive normal fp32 x to 2^-45, and sqrt(x) to about 2^-51: estimates of 2^-23 and one or two steps of Newton's
 __device__ __forceinline__ double reciprocal(float x) {
@@ -236,112 +235,150 @@ __device__ __forceinline__ int adam_tensor(const AdamTable& a) {
 }
 
 // MOM: GL_DTYPE_F32, GL_DTYPE_BF16 or GL_MOMENTS_INT8; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
-// thread one vector of each stream; with 8-bit moments a wave's vectors are a block.
-// WHOLE: all of the wave's 256 elements are there (no lane's ends are looked at).
+// thread a vector of each stream, or two with 8-bit moments: a block is half a wave's then, and what is done for a block (its
+// maxima and scales) is done for two at once.  150M bf16 parameters and gradients: 319 us (4.7 TB/s,
+// bound by instructions: 330 a wave before, 246 us at the memory's rate), 352 with a block a wave.
+// WHOLE: all of the wave's elements are there (no lane's ends are looked at).
+constexpr int adam_vectors(int mom) { return mom == GL_MOMENTS_INT8 ? 2 : 1; }
 template <int MOM, int PM, bool GBF, bool WHOLE>
-__device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensorK& t, long long block) {
+__device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensorK& t, long long base) {
   constexpr bool I8 = MOM == GL_MOMENTS_INT8, BM = MOM == GL_DTYPE_BF16;
+  constexpr int V = adam_vectors(MOM);
   const AdamK c{a.lr, a.b1, a.b2, a.eps, a.wd, t.bc1, t.bc2};
   constexpr int PB = PM == PM_BF16_RNE || PM == PM_BF16_SR ? 2 : 4, MB = I8 ? 1 : (BM ? 2 : 4);
-  const unsigned i = 4 * (threadIdx.x & 63);
-  const int n = WHOLE || t.n - block - i > 4 ? 4 : (t.n - block < i ? 0 : (int)(t.n - block - i));
-  float p[4], g[4], m[4], v[4];
-  char* P = (PM == PM_BF16_MASTER ? (char*)t.master : (char*)t.p) + block * PB;
-  char* G = (char*)t.g + block * (GBF ? 2 : 4);
-  char* M = (char*)t.m + block * MB;
-  char* V = (char*)t.v + block * MB;
-  adam_load<PB == 2>(P, i, n, p);
-  adam_load<GBF>(G, i, n, g);
+  const unsigned lane = threadIdx.x & 63;
+  unsigned i[V];
+  int n[V];
+#pragma unroll
+  for (int x = 0; x < V; ++x) {
+    i[x] = I8 ? (lane >> 5) * ADAM_BLOCK + x * (ADAM_BLOCK / 2) + 4 * (lane & 31) : 4 * lane;
+    const long long left = t.n - base - i[x];
+    n[x] = WHOLE || left > 4 ? 4 : (left < 0 ? 0 : (int)left);
+  }
+  float p[V][4], g[V][4], m[V][4], v[V][4];
+  char* P = (PM == PM_BF16_MASTER ? (char*)t.master : (char*)t.p) + base * PB;
+  char* G = (char*)t.g + base * (GBF ? 2 : 4);
+  char* M = (char*)t.m + base * MB;
+  char* U = (char*)t.v + base * MB;
+#pragma unroll
+  for (int x = 0; x < V; ++x) {
+    adam_load<PB == 2>(P, i[x], n[x], p[x]);
+    adam_load<GBF>(G, i[x], n[x], g[x]);
+  }
   if constexpr (I8) {
-    const unsigned cm = adam_load_codes(M, i, n), cv = adam_load_codes(V, i, n);
-    const double sm = (double)t.m_scale[block / ADAM_BLOCK], sv = (double)t.v_scale[block / ADAM_BLOCK];
+    unsigned cm[V], cv[V];
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+      cm[x] = adam_load_codes(M, i[x], n[x]);
+      cv[x] = adam_load_codes(U, i[x], n[x]);
+    }
+    const bool here = WHOLE || i[0] - 4 * (lane & 31) < t.n - base;  // this half's block
+    const unsigned half = lane >> 5;
+    float* scale_of_m = t.m_scale + base / ADAM_BLOCK;
+    float* scale_of_v = t.v_scale + base / ADAM_BLOCK;
+    const double sm = here ? (double)scale_of_m[half] : 0.0, sv = here ? (double)scale_of_v[half] : 0.0;
     // (behind the end: 0, and NaN in a block that is NaN anyway)
-    double dm[4], dv[4];
+    double dm[V][4], dv[V][4];
     unsigned tm = 0, tv = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double gj = (double)g[j];
-      dm[j] = __builtin_fma(a.b1d, value_m(cm, j, sm), a.a1d * gj);
-      dv[j] = __builtin_fma(a.b2d, value_v(cv, j, sv), a.a2d * (gj * gj));
-      m[j] = (float)dm[j];
-      v[j] = (float)dv[j];
-      tm = umax(tm, abs_bits(m[j]));
-      tv = umax(tv, __float_as_uint(v[j]));  // of v >= 0; a NaN is above every number with either sign
-    }
-    const float fs = scale_m(wave_umax(tm)), fr = scale_v(wave_umax(tv));
-    const bool live_m = fs > 0.f, live_v = fr > 0.f;  // of the whole wave
-    const double im = reciprocal(live_m ? fs : 1.f), ir = reciprocal(live_v ? fr : 1.f);
-    const float imf = (float)im, irf = (float)ir;
-    unsigned om[4], ov[4];
-    float near = 0.f, rv[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      om[j] = code_of(__builtin_copysignf(__builtin_amdgcn_sqrtf(__builtin_fabsf(m[j]) * imf), m[j]), near);
-      rv[j] = __builtin_amdgcn_sqrtf(v[j] * irf * irf);
-      ov[j] = code_of(__builtin_fmaxf(__builtin_amdgcn_sqrtf(rv[j]), dv[j] > 0.0 ? 0.75f : 0.f), near);
-    }
-    if (__builtin_amdgcn_ballot_w64(near > 0.5f - CODE_NEAR)) {
+    for (int x = 0; x < V; ++x)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const unsigned q = live_m ? code_m(__builtin_fabs(dm[j]) * im) : 0u, u = live_v ? code_v(dv[j] * ir * ir) : 0u;
-        om[j] = dm[j] < 0.0 ? 0u - q : q;
-        ov[j] = u == 0 && dv[j] > 0.0 ? 1u : u;
+        const double gj = (double)g[x][j];
+        dm[x][j] = __builtin_fma(a.b1d, value_m(cm[x], j, sm), a.a1d * gj);
+        dv[x][j] = __builtin_fma(a.b2d, value_v(cv[x], j, sv), a.a2d * (gj * gj));
+        m[x][j] = (float)dm[x][j];
+        v[x][j] = (float)dv[x][j];
+        tm = umax(tm, abs_bits(m[x][j]));
+        tv = umax(tv, __float_as_uint(v[x][j]));  // of v >= 0; a NaN is above every number with either sign
       }
+    const float fs = scale_m(half_umax(tm)), fr = scale_v(half_umax(tv));
+    const bool live_m = fs > 0.f, live_v = fr > 0.f;
+    const double im = reciprocal(live_m ? fs : 1.f), ir = reciprocal(live_v ? fr : 1.f);
+    const float imf = (float)im, irf = (float)ir;
+    unsigned om[V][4], ov[V][4];
+    float near = 0.f, rv[V][4];
+#pragma unroll
+    for (int x = 0; x < V; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        om[x][j] = code_of(__builtin_copysignf(__builtin_amdgcn_sqrtf(__builtin_fabsf(m[x][j]) * imf), m[x][j]), near);
+        rv[x][j] = __builtin_amdgcn_sqrtf(v[x][j] * irf * irf);
+        ov[x][j] = code_of(__builtin_fmaxf(__builtin_amdgcn_sqrtf(rv[x][j]), dv[x][j] > 0.0 ? 0.75f : 0.f), near);
+      }
+    if (__builtin_amdgcn_ballot_w64(near > 0.5f - CODE_NEAR)) {
+#pragma unroll
+      for (int x = 0; x < V; ++x)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned q = live_m ? code_m(__builtin_fabs(dm[x][j]) * im) : 0u, u = live_v ? code_v(dv[x][j] * ir * ir) : 0u;
+          om[x][j] = dm[x][j] < 0.0 ? 0u - q : q;
+          ov[x][j] = u == 0 && dv[x][j] > 0.0 ? 1u : u;
+        }
     }
-    adam_store_codes(M, i, n, live_m ? low_bytes(om) : 0u);
-    adam_store_codes(V, i, n, live_v ? low_bytes(ov) : 0u);
-    if (i == 0) {
-      t.m_scale[block / ADAM_BLOCK] = fs;
-      t.v_scale[block / ADAM_BLOCK] = fr;
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+      adam_store_codes(M, i[x], n[x], live_m ? low_bytes(om[x]) : 0u);
+      adam_store_codes(U, i[x], n[x], live_v ? low_bytes(ov[x]) : 0u);
+    }
+    if ((lane & 31) == 0 && here) {
+      scale_of_m[half] = fs;
+      scale_of_v[half] = fr;
     }
     // the update by the root that v's code has and an estimated quotient, within a few last places; bc1 and bc2 come as
     // lr / bc1 and 1 / sqrt(bc2)
     const float up = (live_v ? fr : 1.f) * c.bc2, keep = 1.f - c.lr * c.wd;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      p[j] = __builtin_fmaf(-(m[j] * c.bc1), __builtin_amdgcn_rcpf(__builtin_fmaf(rv[j], up, c.eps)), p[j] * keep);
-  } else {
-    adam_load<BM>(M, i, n, m);
-    adam_load<BM>(V, i, n, v);
+    for (int x = 0; x < V; ++x)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) adam_elem(c, p[j], g[j], m[j], v[j]);
+      for (int j = 0; j < 4; ++j)
+        p[x][j] = __builtin_fmaf(-(m[x][j] * c.bc1), __builtin_amdgcn_rcpf(__builtin_fmaf(rv[x][j], up, c.eps)), p[x][j] * keep);
+  } else {
+    adam_load<BM>(M, i[0], n[0], m[0]);
+    adam_load<BM>(U, i[0], n[0], v[0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) adam_elem(c, p[0][j], g[0][j], m[0][j], v[0][j]);
     if constexpr (BM) {
-      adam_store((unsigned short*)M, i, n, to_bf16x2(m[0], m[1]), to_bf16x2(m[2], m[3]));
-      adam_store((unsigned short*)V, i, n, to_bf16x2(v[0], v[1]), to_bf16x2(v[2], v[3]));
+      adam_store((unsigned short*)M, i[0], n[0], to_bf16x2(m[0][0], m[0][1]), to_bf16x2(m[0][2], m[0][3]));
+      adam_store((unsigned short*)U, i[0], n[0], to_bf16x2(v[0][0], v[0][1]), to_bf16x2(v[0][2], v[0][3]));
     } else {
-      adam_store((float*)M, i, n, m);
-      adam_store((float*)V, i, n, v);
+      adam_store((float*)M, i[0], n[0], m[0]);
+      adam_store((float*)U, i[0], n[0], v[0]);
     }
   }
-  if constexpr (!GBF) {
-    const float none[4] = {0.f, 0.f, 0.f, 0.f};
-    if (a.clear) adam_store((float*)G, i, n, none);
-  }
-  if constexpr (PM == PM_F32 || PM == PM_BF16_MASTER) adam_store((float*)P, i, n, p);
-  unsigned short* O = (unsigned short*)t.p + block;
-  if constexpr (PM == PM_BF16_SR) {
-    unsigned o[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = round_stochastic(p[j], t.seed, t.first + block + i + j);
-    adam_store(O, i, n, o[0] | o[1] << 16, o[2] | o[3] << 16);
-  } else if constexpr (PM != PM_F32) {
-    adam_store(O, i, n, to_bf16x2(p[0], p[1]), to_bf16x2(p[2], p[3]));
+  for (int x = 0; x < V; ++x) {
+    if constexpr (!GBF) {
+      const float none[4] = {0.f, 0.f, 0.f, 0.f};
+      if (a.clear) adam_store((float*)G, i[x], n[x], none);
+    }
+    if constexpr (PM == PM_F32 || PM == PM_BF16_MASTER) adam_store((float*)P, i[x], n[x], p[x]);
+    unsigned short* O = (unsigned short*)t.p + base;
+    if constexpr (PM == PM_BF16_SR) {
+      unsigned o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = round_stochastic(p[x][j], t.seed, t.first + base + i[x] + j);
+      adam_store(O, i[x], n[x], o[0] | o[1] << 16, o[2] | o[3] << 16);
+    } else if constexpr (PM != PM_F32) {
+      adam_store(O, i[x], n[x], to_bf16x2(p[x][0], p[x][1]), to_bf16x2(p[x][2], p[x][3]));
+    }
   }
 }
 template <int MOM, int PM, bool GBF>
 __global__ void __launch_bounds__(256) adam_kernel(AdamTable a) {
+  constexpr int WAVE = 256 * adam_vectors(MOM);  // elements of a wave
   const int ti = adam_tensor(a);
   const AdamTensorK& t = a.t[ti];
-  const long long block = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + wave_uniform(threadIdx.x >> 6) * 256;
-  if (block + 256 <= t.n) adam_vector<MOM, PM, GBF, true>(a, t, block);
-  else if (block < t.n) adam_vector<MOM, PM, GBF, false>(a, t, block);
+  const long long base = (long long)(blockIdx.x - a.first[ti]) * (4 * WAVE) + wave_uniform(threadIdx.x >> 6) * WAVE;
+  if (base + WAVE <= t.n) adam_vector<MOM, PM, GBF, true>(a, t, base);
+  else if (base < t.n) adam_vector<MOM, PM, GBF, false>(a, t, base);
 }
 
-// The fp32 values of 8-bit moments (into g: m's, into p: v's).
-__global__ void __launch_bounds__(256) adam_values_kernel(AdamTable a) {
+// The fp32 values of 8-bit moments (into g: m's, into p: v's), a vector a thread.  150M: 243 us, 6.2 TB/s.
+__global__ void __launch_bounds__(512) adam_values_kernel(AdamTable a) {
   const int ti = adam_tensor(a);
   const AdamTensorK& t = a.t[ti];
-  const long long block = (long long)(blockIdx.x - a.first[ti]) * ADAM_CHUNK + wave_uniform(threadIdx.x >> 6) * 256;
+  const long long block = (long long)(blockIdx.x - a.first[ti]) * adam_chunk(GL_MOMENTS_INT8) + wave_uniform(threadIdx.x >> 6) * ADAM_BLOCK;
   const unsigned i = 4 * (threadIdx.x & 63);
   const long long left = t.n - block - i;
   if (left <= 0) return;
@@ -385,15 +422,15 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
   k.b2d = a->beta2_64;
   k.a2d = 1.0 - a->beta2_64;
   constexpr long long MAX_GROUPS = 1LL << 23;  // of a launch: fewer than 2^32 threads
-  constexpr long long MOST = MAX_GROUPS * ADAM_CHUNK;  // elements of a launch; a longer tensor takes several
+  const int chunk = adam_chunk(a->moments_dtype);
   int next = 0;
-  long long done = 0;  // of the next tensor
+  long long done = 0;  // of the next tensor, which takes several launches where it has more chunks than one takes
   while (next < count) {
     long long groups = 0;
     k.count = 0;
     while (next < count && k.count < ADAM_TENSORS && groups < MAX_GROUPS) {
       const GlAdamTensor& t = tensors[next];
-      const long long left = t.n - done, room = (MAX_GROUPS - groups) * ADAM_CHUNK, n = left < room ? left : room;
+      const long long left = t.n - done, room = (MAX_GROUPS - groups) * chunk, n = left < room ? left : room;
       if (n > 0) {
         AdamTensorK& d = k.t[k.count];
         k.first[k.count++] = (unsigned)groups;
@@ -408,7 +445,7 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
           d.bc1 = (float)((double)a->lr / t.bc1);
           d.bc2 = (float)(1.0 / __builtin_sqrt((double)t.bc2));
         }
-        groups += (n + ADAM_CHUNK - 1) / ADAM_CHUNK;
+        groups += (n + chunk - 1) / chunk;
       }
       done = n < left ? done + n : 0;
       next += n >= left;
@@ -417,7 +454,7 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
     k.first[k.count] = (unsigned)groups;
     const dim3 grid((unsigned)groups);
     if (values) {
-      GL_LAUNCH(GL_KERNEL_ADAM_VALUES, adam_values_kernel, grid, dim3(256), 0, s, k);
+      GL_LAUNCH(GL_KERNEL_ADAM_VALUES, adam_values_kernel, grid, dim3(512), 0, s, k);
     } else {
       const int pm = a->p_dtype == GL_DTYPE_F32 ? PM_F32 : (k.t[0].master ? PM_BF16_MASTER : (a->stochastic ? PM_BF16_SR : PM_BF16_RNE));
       const bool gbf = a->g_dtype == GL_DTYPE_BF16;
