@@ -126,7 +126,7 @@ EXPORTS = ("gl_abi_version", "gl_struct_layout", "gl_error_string", "gl_fwd_work
            "gl_sched_build", "gl_window_build_host", "gl_window_build", "gl_cover_select", "gl_trace_begin",
            "gl_trace_end", "gl_pack8", "gl_unpack8", "gl_dense_fwd_workspace", "gl_dense_fwd", "gl_dense_bwd_workspace",
            "gl_dense_bwd", "gl_adam_values", "gl_norm_fwd", "gl_norm_bwd_workspace",
-           "gl_norm_bwd", "gl_ce_fwd_workspace", "gl_ce_exps_bytes", "gl_ce_fwd", "gl_ce_bwd_workspace", "gl_ce_bwd")
+           "gl_norm_bwd", "gl_ce_fwd_workspace", "gl_ce_exps_bytes", "gl_ce_fwd", "gl_ce_bwd_workspace", "gl_ce_bwd", "gl_capture_id")
 KERNEL_NAMES = {1: "tile_x_kernel", 2: "fwd_kernel", 3: "fwd_finalize_kernel", 4: "c1t_kernel", 5: "bwd_w_kernel",
                 6: "dx_kernel", 7: "dx_reduce_kernel", 8: "adam_kernel", 9: "edges_build", 10: "fwd_kernel_win",
                 11: "bwd_w_kernel_win", 12: "max_events_dw_kernel", 13: "max_events_dx_kernel",
@@ -185,6 +185,8 @@ class Library:
                          ("gl_ce_fwd_workspace", GlCeArgs), ("gl_ce_exps_bytes", GlCeArgs), ("gl_ce_bwd_workspace", GlCeBwdArgs)):
             f = getattr(L, name)
             f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(st), ctypes.POINTER(_SZ)]
+        L.gl_capture_id.restype = ctypes.c_int
+        L.gl_capture_id.argtypes = [_P, ctypes.POINTER(ctypes.c_uint64)]
         L.gl_trace_begin.restype = ctypes.c_int
         L.gl_trace_begin.argtypes = [ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(_I32), ctypes.c_int]
         L.gl_trace_end.restype = ctypes.c_int

@@ -576,6 +576,15 @@ class HipBackend:
     _ce_fwd = functools.cached_property(lambda self: self.lib.entry("gl_ce_fwd"))
     _ce_bwd = functools.cached_property(lambda self: self.lib.entry("gl_ce_bwd"))
 
+    def capture_id(self, dev) -> int:
+        """The number of the graph that the device's current stream is being captured into; 0: none."""
+        with _on(dev):
+            if not torch.cuda.is_current_stream_capturing():
+                return 0
+            v = ctypes.c_uint64()
+            self.lib.call("gl_capture_id", _stream(dev), ctypes.byref(v))
+            return v.value
+
     def ce_forward(self, x, w, b, target, reduction, ignore_index, keep, piece_bytes=0):
         """(loss, and with ``keep`` what the backward takes: five words a row, and the first piece's exponentials or
         None) of x [M, K], w [N, K], b [N] or None (all of one dtype) and target [M] (contiguous int64)."""

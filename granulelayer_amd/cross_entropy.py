@@ -58,7 +58,9 @@ class DenseCrossEntropyFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, target, reduction, ignore_index, budget):
-        loss, kept, ctx.exps = backend_for(x.device).ce_forward(x, w, b, target, reduction, ignore_index, True, budget)
+        be = backend_for(x.device)
+        loss, kept, ctx.exps = be.ce_forward(x, w, b, target, reduction, ignore_index, True, budget)
+        ctx.capture = be.capture_id(x.device) if ctx.exps is not None else 0
         ctx.save_for_backward(x, w, b, target, kept)
         ctx.reduction, ctx.ignore_index, ctx.budget = reduction, ignore_index, budget
         return loss
@@ -79,9 +81,14 @@ def _gradients(ctx, dloss):
     else:
         dw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if need_w else None
         db = torch.empty(b.shape, device=x.device, dtype=b.dtype) if need_b else None
-    exps, ctx.exps = ctx.exps, None  # used up: a second backward of a retained graph makes them again
-    backend_for(x.device).ce_backward(dloss.resolve_neg(), x, w, b, target, ctx.reduction, ctx.ignore_index, kept, dx, dw, db,
-                                      use_main, ctx.budget, exps)
+    be = backend_for(x.device)
+    # Used up: a second backward of a retained graph makes them again, and so does one that a captured graph may replay
+    # without its forward.
+    exps, ctx.exps = ctx.exps, None
+    if exps is not None and be.capture_id(x.device) != ctx.capture:
+        exps = None
+    be.ce_backward(dloss.resolve_neg(), x, w, b, target, ctx.reduction, ctx.ignore_index, kept, dx, dw, db, use_main,
+                   ctx.budget, exps)
     return dx, None if use_main else dw, None if use_main else db, None, None, None, None
 
 

@@ -65,6 +65,17 @@ using namespace gl;
 
 extern "C" int gl_abi_version(void) { return GL_ABI_VERSION; }
 
+extern "C" int gl_capture_id(void* stream, uint64_t* id) {
+  if (!id) return GL_ERR_ARG;
+  *id = 0;
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  unsigned long long v = 0;
+  const hipError_t e = hipStreamGetCaptureInfo((hipStream_t)stream, &st, &v);
+  if (e != hipSuccess) return (int)e;
+  if (st == hipStreamCaptureStatusActive) *id = v;
+  return 0;
+}
+
 extern "C" int gl_trace_begin(void** events, int32_t* kernel_ids, int n_pairs) {
   if (!events || !kernel_ids || n_pairs < 1) return GL_ERR_ARG;
   std::lock_guard<std::mutex> lk(g_trace_mu);

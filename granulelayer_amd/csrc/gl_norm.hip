@@ -8,6 +8,10 @@
 // subtracted before squares are summed (two reductions a row).  Workgroups take rows in turn and keep what belongs to
 // the features in registers meanwhile: w and b, and of the backward the sums of dw and db, which a second kernel adds
 // over the workgroups in a fixed order.  Sums are fp32; results are rounded once.
+//
+// 32768 x 8192 bf16: forward 207 us (5.2 TB/s), backward 270 (6.0) + 5; 8192 x 4096 fp32 with bf16 results: 38 (5.3),
+// 69 (4.8) + 4; 16384 x 1024 bf16: 13.5 (5.0), 25 (4.0); a copy of 4 GB reaches 4.97.  Rows that do not begin on 16 bytes are
+// slower (32768 x 2100 bf16 backward 142 us, x 2560 89): their vectors cross the lines of the caches.
 #include "gl_internal.h"
 #include "gl_pack8.h"
 
@@ -136,7 +140,7 @@ __device__ __forceinline__ void row_totals(float& a, float& b, float (*red)[2], 
 // A row is a wave's (WAVE: four rows a workgroup) or a workgroup's, with V vectors a thread.  The next turn's row is
 // loaded before this one's sums, so a workgroup always has a row on its way.
 template <bool WAVE, int V, bool XBF, bool YBF, bool STREAM>
-__global__ __launch_bounds__(WAVE ? 256 : V == 1 ? 1024 : 512) void norm_fwd_kernel(NormK a) {
+__global__ __launch_bounds__(WAVE || V == 1 ? 256 : 512) void norm_fwd_kernel(NormK a) {
   __shared__ float red[2][16][2];
   constexpr int ROWS = WAVE ? 4 : 1;
   const int T = WAVE ? 64 : blockDim.x, t = WAVE ? threadIdx.x & 63 : threadIdx.x;
@@ -435,21 +439,26 @@ __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__
 // ---- plans -----------------------------------------------------------------------------------------------------
 constexpr int CUS = 256;
 constexpr int NORM_MOST = 16384;  // features that the registers of a workgroup hold
-// bytes of x and y past which they go around the caches: 32768 x 8192 bf16 backward 268 us, 300 without; of 67 MB
-// (16384 x 1024) a forward that does takes 16 us, 13.5 without
+// Bytes of x and y past which they go around the caches: 32768 x 8192 bf16 forward 207 us, 217 without, backward 268 and
+// 294.  Of fewer what comes next finds them there; the pass itself is as fast (8192 x 4096 bf16 25.9 us around them, 27.1
+// through; 16384 x 1024 15.0 and 13.4).
 constexpr long long NORM_STREAM = 256LL << 20;
 inline long long least(long long a, long long b) { return a < b ? a : b; }
 
 // Forward: vectors of a thread (rows of up to 1024 features are a wave's), threads, and workgroups: as many as run at
-// once, no more than rows.
-inline int fwd_vectors(int D) { return D <= 512 ? 1 : D <= 1024 ? 2 : D <= 4096 ? 1 : D <= 8192 ? 2 : 4; }
+// once, no more than rows.  One vector and two, bf16: 16384 x 1024 by a workgroup 15.7 us, by a wave 13.5 (8192 x 640
+// 10.0 and 9.0); 32768 x 2560 77.0 and 69.5, 2100 99.7 and 79.0, 16384 x 4000 56.0 and
+// 58.5; 32768 x 8192 203.5 and 206.5.  (Four: 16384 features in 512 threads.)
+inline int fwd_vectors(int D) { return D <= 512 ? 1 : D <= 1024 ? 2 : D <= 2048 ? 1 : D <= 8192 ? 2 : 4; }
 inline int fwd_threads(int D) { return D <= 1024 ? 256 : 64 * ceil_div(D, 512 * fwd_vectors(D)); }
 inline int fwd_groups(long long M, int D) {
   if (D > NORM_MOST) return (int)least(M, 2 * CUS);
   return (int)least(D <= 1024 ? (M + 3) / 4 : M, 2048 / fwd_threads(D) * CUS);
 }
 // Backward: threads of a row (up to 512 features are a wave's), its teams (fewer where rows are: every CU has some),
-// and workgroups, one a CU, or two where half a CU's threads are enough for one.
+// and workgroups, one a CU, or two where half a CU's threads are enough for one (8192 x 5000: 63 us, 116 with one).
+// Teams against workgroups of one each, as many threads a CU: 16384 x 1024 25.4 us and 39.4, 8192 x 640 15.8 and 26.5,
+// 32768 x 2560 89 and 92.
 inline int bwd_threads(int D) { return D > 8192 ? 1024 : 64 * ceil_div(D, 512); }
 inline int bwd_teams(long long M, int D) { return (int)least(1024 / bwd_threads(D), (M + CUS - 1) / CUS); }
 inline int bwd_groups(long long M, int D) {
@@ -482,7 +491,7 @@ int launch_norm_rows(const NormK& k, hipStream_t s) {
   } else {
     if (k.D <= 512) return launch_fwd_as<true, 1, XBF, YBF, STREAM>(k, s);
     if (k.D <= 1024) return launch_fwd_as<true, 2, XBF, YBF, STREAM>(k, s);
-    if (k.D <= 4096) return launch_fwd_as<false, 1, XBF, YBF, STREAM>(k, s);
+    if (k.D <= 2048) return launch_fwd_as<false, 1, XBF, YBF, STREAM>(k, s);
     if (k.D <= 8192) return launch_fwd_as<false, 2, XBF, YBF, STREAM>(k, s);
     return launch_fwd_as<false, 4, XBF, YBF, STREAM>(k, s);
   }

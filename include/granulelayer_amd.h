@@ -259,6 +259,9 @@ int gl_cover_select(const GlCoverArgs* a, void* stream);
 int gl_abi_version(void);
 int gl_struct_layout(int which, long long* out, int n);
 const char* gl_error_string(int code);
+/* The number of the graph that `stream` is being captured into, 0 when into none: for a backward that uses up what its
+ * forward kept, which it may only where one replay runs both. */
+int gl_capture_id(void* stream, uint64_t* id);
 
 /* Forward.  gl_fwd_workspace writes the workspace size for these arguments to *bytes. */
 int gl_fwd_workspace(const GlFwdArgs* a, size_t* bytes);

@@ -106,7 +106,7 @@ def compare(t, reduction, budget=None):
     return got
 
 
-SHAPES = [(1, 16, 2), (1, 1, 1), (3, 7, 5), (16, 64, 130), (64, 1024, 1000), (1, 130, 5000), (256, 100, 257), (257, 100, 300),
+SHAPES = [(1, 16, 2), (1, 1, 1), (3, 7, 5), (16, 64, 130), (64, 1024, 1000), (1, 130, 5000), (128, 100, 257), (129, 100, 300), (256, 100, 257), (257, 100, 300),
           (300, 128, 2049), (777, 1001, 555), (1000, 72, 4097), (2, 8192, 33), (600, 33, 1), (4100, 40, 9)]
 
 
@@ -402,6 +402,45 @@ def test_a_second_backward_and_one_without_the_first():
         check(v, want, name)
 
 
+def test_a_captured_backward_without_its_forward():
+    """A graph of the backward alone is replayed as often as one likes; one forward serves all of them."""
+    t = inputs(700, 520, 900, BF)
+    leaves = [t[k].detach().requires_grad_(True) for k in "xwb"]
+    want = definition(t, "mean", torch.ones((), device=DEV))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = dense_cross_entropy(leaves[0], leaves[1], t["target"], leaves[2])
+        torch.autograd.grad(loss, leaves)
+        loss = dense_cross_entropy(leaves[0], leaves[1], t["target"], leaves[2])
+        one = torch.ones((), device=DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = torch.autograd.grad(loss, leaves, one, retain_graph=True)
+    for _ in range(3):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for v, name in zip(out, ("dx", "dw", "db")):
+            check(v, want, name)
+
+
+def test_a_capture_has_a_number():
+    from granulelayer_amd.backend import backend_for
+
+    be, dev, x = backend_for(torch.device(DEV)), torch.device(DEV), torch.zeros(4, device=DEV)
+    seen = [be.capture_id(dev)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g in graphs:
+        with torch.cuda.graph(g):
+            x.add_(1)
+            seen += [be.capture_id(dev), be.capture_id(dev)]
+    seen.append(be.capture_id(dev))
+    assert seen[0] == seen[5] == 0 and seen[1] == seen[2] != 0 and seen[3] == seen[4] != 0 and seen[1] != seen[3]
+
+
 def test_operands_may_not_change_before_the_backward():
     t = inputs(300, 32, 64, BF)
     for name in ("x", "w", "b", "target"):
@@ -433,9 +472,41 @@ def test_past_32_bits():
     for budget in (None, 16 << 30):
         xs, ws = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
         loss = dense_cross_entropy(xs, ws, target, None, "sum", IGNORED, budget)
-        assert abs(float(loss) / (M * 15 * math.log(2)) - 1) < 1e-6
+        assert abs(float(loss.detach()) / (M * 15 * math.log(2)) - 1) < 1e-6
         dx, dw = torch.autograd.grad(loss, (xs, ws))
         # sum over the classes of w[:, 1] dz: (N - 1) / N - (N - 1) / N; dz of the target rounded to bf16 is -1
         assert not dx[:, 0].any() and float(dx[:, 1].abs().max()) <= 2.0 ** -8
         assert float(dw[1, 0]) == float(torch.tensor(M / N).bfloat16()) and float(dw[N - 1, 0]) == float(torch.tensor((M - 1) / N - 1).bfloat16())
         assert not dw[:, 1:].any()
+
+
+def test_kept_exponentials_past_32_bits():
+    """70000 rows of 32768 classes, whose exponentials are 4.6 GB: every logit is 0 but that of each row's own class, 1."""
+    M, K, N = 70_000, 512, 32768
+    x = torch.zeros(M, K, device=DEV, dtype=BF)
+    rows = torch.arange(M, device=DEV)
+    x[rows, rows % K] = 1.0
+    w = torch.zeros(N, K, device=DEV, dtype=BF)
+    own = torch.arange(K, device=DEV)
+    w[64 * own, own] = 1.0  # row m's own class is 64 (m % K)
+    target = (64 * (rows % K) + 1) % N  # its neighbour
+    target[-1] = N - 1
+    xs, ws = x.requires_grad_(True), w.requires_grad_(True)
+    loss = dense_cross_entropy(xs, ws, target, None, "none", IGNORED, 16 << 30)
+    Z = N - 1 + math.e
+    assert float((loss.detach() - math.log(Z)).abs().max()) < 1e-5
+    dx, dw = torch.autograd.grad(loss, (xs, ws), torch.ones(M, device=DEV))
+    # dx[m, c] = dz[m, 64 c]: e / Z at the row's own, 1 / Z elsewhere, rounded to bf16 as dz and as dx (2^-7 for both)
+    for m in (0, 1, 32_767, 32_768, 65_536, M - 1):
+        want = torch.full((K,), 1 / Z, device=DEV)
+        want[m % K] = math.e / Z
+        assert float((dx[m].float() / want - 1).abs().max()) <= 2.0 ** -7 + 1e-4
+    # dw[n, c] = sum over the rows whose own is c of dz[m, n]: of the neighbour of another's class, 1 / Z each
+    c = 5
+    count = len(range(c, M, K))
+    assert abs(float(dw[1, c]) / (count / Z) - 1) <= 2.0 ** -7 + 1e-4
+    assert abs(float(dw[64 * c, c]) / (count * math.e / Z) - 1) <= 2.0 ** -7 + 1e-4
+    assert abs(float(dw[64 * c + 1, c]) / (count * (1 / Z - 1)) - 1) <= 2.0 ** -7 + 1e-4
+    # rows the last of all: (M - 1) % K's column holds its target's -1
+    last = (M - 1) % K
+    assert abs(float(dw[N - 1, last]) / (len(range(last, M, K)) / Z - 1) - 1) <= 2.0 ** -7 + 1e-4
