@@ -74,13 +74,13 @@ class DenseCrossEntropyFunction(torch.autograd.Function):
 def _gradients(ctx, dloss):
     x, w, b, target, kept = ctx.saved_tensors
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
     mg_w, mg_b, use_main = _main_grads(w, b, need_w, need_b)
     if use_main:
         dw, db = mg_w, mg_b
     else:
-        dw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if need_w else None
-        db = torch.empty(b.shape, device=x.device, dtype=b.dtype) if need_b else None
+        dw = torch.empty_like(w, memory_format=torch.contiguous_format) if need_w else None
+        db = torch.empty_like(b, memory_format=torch.contiguous_format) if need_b else None
     be = backend_for(x.device)
     # Used up: a second backward of a retained graph makes them again, and so does one that a captured graph may replay
     # without its forward.

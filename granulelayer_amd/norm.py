@@ -62,13 +62,13 @@ def _gradients(ctx, dy):
     x, w, stats = ctx.saved_tensors
     b = ctx.bias
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
     mg_w, mg_b, use_main = _main_grads(w, b, need_w, need_b)
     if use_main:
         dw, db = mg_w, mg_b
     else:
-        dw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if need_w else None
-        db = torch.empty(b.shape, device=x.device, dtype=b.dtype) if need_b else None
+        dw = torch.empty_like(w, memory_format=torch.contiguous_format) if need_w else None
+        db = torch.empty_like(b, device=x.device, memory_format=torch.contiguous_format) if need_b else None
     backend_for(x.device).norm_backward(dy.resolve_neg(), x, w, stats, dx, dw, db, use_main)
     return dx, None if use_main else dw, None if use_main else db, None, None
 
