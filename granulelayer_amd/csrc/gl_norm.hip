@@ -9,9 +9,9 @@
 // the features in registers meanwhile: w and b, and of the backward the sums of dw and db, which a second kernel adds
 // over the workgroups in a fixed order.  Sums are fp32; results are rounded once.
 //
-// 32768 x 8192 bf16: forward 207 us (5.2 TB/s), backward 270 (6.0) + 5; 8192 x 4096 fp32 with bf16 results: 38 (5.3),
-// 69 (4.8) + 4; 16384 x 1024 bf16: 13.5 (5.0), 25 (4.0); a copy of 4 GB reaches 4.97.  Rows that do not begin on 16 bytes are
-// slower (32768 x 2100 bf16 backward 142 us, x 2560 89): their vectors cross the lines of the caches.
+// 32768 x 8192 bf16: forward 191 us (5.6 TB/s), backward 269 (6.0) + 5; 8192 x 4096 fp32 with bf16 results: 39 (5.2),
+// 69 (4.8) + 4; 16384 x 1024 bf16: 13.4 (5.0), 26 (3.9); a copy of 4 GB reaches 4.97.  Rows that do not begin on 16 bytes:
+// 32768 x 2101 bf16 69 (4.0), 107 (3.9), where 2096 takes 63 and 93.
 #include "gl_internal.h"
 #include "gl_pack8.h"
 
@@ -111,6 +111,32 @@ __device__ __forceinline__ void store_eight(void* p, long long i, int n, const f
   }
 }
 
+// A thread's eight features from the c-th on: the row's last eight where it would end before them, of which those from `lo`
+// on are its own (rows of fewer: `hi` of them; threads behind the row: none).  So every load is a vector: a wave that
+// gathered a row's end by elements would wait for them at once, and with them for the row that is on its way.
+struct Place {
+  int c, lo, hi;
+};
+__device__ __forceinline__ Place place_of(int c, int D) {
+  const int last = D > 8 ? D - 8 : 0;
+  return Place{c < last ? c : last, c <= last ? 0 : c - last < 8 ? c - last : 8, D < 8 ? D : 8};
+}
+__device__ __forceinline__ bool own(const Place& p, int j) { return j >= p.lo && j < p.hi; }
+// stores a place's own features
+template <bool BF, bool STREAM>
+__device__ __forceinline__ void store_own(void* to, long long row, const Place& p, const float (&v)[8]) {
+  if (p.lo == 0) {
+    store_eight<BF, STREAM>(to, row + p.c, p.hi, v);
+  } else {
+#pragma unroll
+    for (int j = 1; j < 8; ++j)
+      if (own(p, j)) {
+        if constexpr (BF) ((unsigned short*)to)[row + p.c + j] = to_bf16(v[j]);
+        else ((float*)to)[row + p.c + j] = v[j];
+      }
+  }
+}
+
 // Totals over the threads of a row, the same bits in all of them: a wave's, or (WAVE false) those of up to 16 waves, of
 // which this is number `wave`, through `red`, 16 pairs that are 0 where there is no wave.
 template <bool WAVE>
@@ -148,22 +174,20 @@ __global__ __launch_bounds__(WAVE || V == 1 ? 256 : 512) void norm_fwd_kernel(No
     if (threadIdx.x < 64) (&red[0][0][0])[threadIdx.x] = 0.f;
     __syncthreads();
   }
+  Place at[V];
   float w[V][8], b[V][8];
 #pragma unroll
   for (int y = 0; y < V; ++y) {
-    const int c = (y * T + t) * 8;
-    norm_params(a.w, a.w_bf, c, a.D - c, 1.f, w[y]);
-    norm_params(a.b, a.w_bf, c, a.D - c, 0.f, b[y]);
+    at[y] = place_of((y * T + t) * 8, a.D);
+    norm_params(a.w, a.w_bf, at[y].c, at[y].hi, 1.f, w[y]);
+    norm_params(a.b, a.w_bf, at[y].c, at[y].hi, 0.f, b[y]);
   }
   const long long step = (long long)gridDim.x * ROWS;
   long long m = (long long)blockIdx.x * ROWS + (WAVE ? threadIdx.x >> 6 : 0);
   Eight<XBF> next[V];
   auto fetch = [&](long long row) {
 #pragma unroll
-    for (int y = 0; y < V; ++y) {
-      const int c = (y * T + t) * 8;
-      next[y] = load_eight<XBF, STREAM>(a.X, row * a.sx + c, a.D - c);
-    }
+    for (int y = 0; y < V; ++y) next[y] = load_eight<XBF, STREAM>(a.X, row * a.sx + at[y].c, at[y].hi);
   };
   if (m < a.M) fetch(m);
   for (; m < a.M; m += step) {
@@ -171,28 +195,28 @@ __global__ __launch_bounds__(WAVE || V == 1 ? 256 : 512) void norm_fwd_kernel(No
 #pragma unroll
     for (int y = 0; y < V; ++y)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += x[y][j] = value<XBF>(next[y], j);
+      for (int j = 0; j < 8; ++j) {
+        x[y][j] = value<XBF>(next[y], j);
+        if (own(at[y], j)) s += x[y][j];
+      }
     if (m + step < a.M) fetch(m + step);
     row_totals<WAVE>(s, none, red[0], t >> 6);
     const float mean = s / (float)a.D;  // (by 1 / D a constant row's would be off its value)
     s = 0.f;
 #pragma unroll
-    for (int y = 0; y < V; ++y) {
-      const int left = a.D - (y * T + t) * 8;
+    for (int y = 0; y < V; ++y)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[y][j] -= mean;
-        if (left >= 8 || j < left) s = __builtin_fmaf(x[y][j], x[y][j], s);
+        if (own(at[y], j)) s = __builtin_fmaf(x[y][j], x[y][j], s);
       }
-    }
     row_totals<WAVE>(s, none, red[1], t >> 6);
     const float r = 1.f / __builtin_sqrtf(s / (float)a.D + a.eps);
 #pragma unroll
     for (int y = 0; y < V; ++y) {
-      const int c = (y * T + t) * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[y][j] = __builtin_fmaf(x[y][j] * r, w[y][j], b[y][j]);
-      store_eight<YBF, STREAM>(a.Y, m * a.sy + c, a.D - c, x[y]);
+      store_own<YBF, STREAM>(a.Y, m * a.sy, at[y], x[y]);
     }
     if (a.stats && t == 0) {
       a.stats[2 * m] = mean;
@@ -215,11 +239,12 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormK a, int T, int team
     for (int i = threadIdx.x; i < MOST * 64; i += blockDim.x) (&red[0][0][0][0])[i] = 0.f;
     __syncthreads();
   }
+  Place at[V];
   float w[V][8], dw[V][8], db[V][8];
 #pragma unroll
   for (int y = 0; y < V; ++y) {
-    const int c = (y * T + t) * 8;
-    norm_params(a.w, a.w_bf, c, a.D - c, 1.f, w[y]);
+    at[y] = place_of((y * T + t) * 8, a.D);
+    norm_params(a.w, a.w_bf, at[y].c, at[y].hi, 1.f, w[y]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[y][j] = db[y][j] = 0.f;
   }
@@ -232,9 +257,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormK a, int T, int team
     if (row >= a.M) return;
 #pragma unroll
     for (int y = 0; y < V; ++y) {
-      const int c = (y * T + t) * 8;
-      nx[y] = load_eight<XBF, STREAM>(a.X, row * a.sx + c, a.D - c);
-      ng[y] = load_eight<YBF, STREAM>(a.dY, row * a.sdy + c, a.D - c);
+      nx[y] = load_eight<XBF, STREAM>(a.X, row * a.sx + at[y].c, at[y].hi);
+      ng[y] = load_eight<YBF, STREAM>(a.dY, row * a.sdy + at[y].c, at[y].hi);
     }
     next_mean = a.stats[2 * row];
     next_r = a.stats[2 * row + 1];
@@ -256,8 +280,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormK a, int T, int team
 #pragma unroll
       for (int y = 0; y < V; ++y)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {  // (behind the row g is 0)
-          const float h = (value<XBF>(x[y], j) - mean) * r, d = value<YBF>(g[y], j), e = d * w[y][j];
+        for (int j = 0; j < 8; ++j) {
+          const float h = (value<XBF>(x[y], j) - mean) * r, d = own(at[y], j) ? value<YBF>(g[y], j) : 0.f, e = d * w[y][j];
           dw[y][j] = __builtin_fmaf(d, h, dw[y][j]);
           db[y][j] += d;
           s0 += e;
@@ -273,14 +297,13 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormK a, int T, int team
     if (m < a.M) {
 #pragma unroll
       for (int y = 0; y < V; ++y) {
-        const int c = (y * T + t) * 8;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float h = (value<XBF>(x[y], j) - mean) * r;
           v[j] = r * (value<YBF>(g[y], j) * w[y][j] - s0 - h * s1);
         }
-        store_eight<XBF, STREAM>(a.Y, m * a.D + c, a.D - c, v);
+        store_own<XBF, STREAM>(a.Y, m * a.D, at[y], v);
       }
     }
   }
@@ -290,7 +313,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormK a, int T, int team
     if (V == 1 && teams > 1) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sums[threadIdx.x * 8 + j] = v[0][j];  // (teams are T threads apart)
+      for (int j = 0; j < 8; ++j)
+        if (own(at[0], j)) sums[team * 8 * T + at[0].c + j] = v[0][j];
       __syncthreads();
       for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
         float s = sums[c];
@@ -299,10 +323,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormK a, int T, int team
       }
     } else {
 #pragma unroll
-      for (int y = 0; y < V; ++y) {
-        const int c = (y * T + t) * 8;
-        store8<false>(to, c, a.D - c, v[y]);
-      }
+      for (int y = 0; y < V; ++y) store_own<false, false>(to, 0, at[y], v[y]);
     }
   };
   write(dw, part);
@@ -439,16 +460,16 @@ __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__
 // ---- plans -----------------------------------------------------------------------------------------------------
 constexpr int CUS = 256;
 constexpr int NORM_MOST = 16384;  // features that the registers of a workgroup hold
-// Bytes of x and y past which they go around the caches: 32768 x 8192 bf16 forward 207 us, 217 without, backward 268 and
-// 294.  Of fewer what comes next finds them there; the pass itself is as fast (8192 x 4096 bf16 25.9 us around them, 27.1
-// through; 16384 x 1024 15.0 and 13.4).
+// Bytes of x and y past which they go around the caches: 32768 x 8192 bf16 forward 191 us, 201 through them, backward 269
+// and 293.  Of fewer, what comes next finds them there, and the pass itself gains less (16384 x 4096 bf16, 268 MB, 50.0 and
+// 52.9 us) or loses (16384 x 1024 14.6 and 13.4).
 constexpr long long NORM_STREAM = 256LL << 20;
 inline long long least(long long a, long long b) { return a < b ? a : b; }
 
 // Forward: vectors of a thread (rows of up to 1024 features are a wave's), threads, and workgroups: as many as run at
-// once, no more than rows.  One vector and two, bf16: 16384 x 1024 by a workgroup 15.7 us, by a wave 13.5 (8192 x 640
-// 10.0 and 9.0); 32768 x 2560 77.0 and 69.5, 2100 99.7 and 79.0, 16384 x 4000 56.0 and
-// 58.5; 32768 x 8192 203.5 and 206.5.  (Four: 16384 features in 512 threads.)
+// once, no more than rows.  bf16: 16384 x 768 a workgroup a row 14.7 us, a wave 12.1 (8192 x 640 9.2 and 8.4; 16384 x 1024 15.0
+// and 13.4); one vector and two: 16384 x 1500 23.3 and 25.9, 2048 27.7 and 28.9, 32768 x 2100 73.3 and 62.5, 2560 77.3 and
+// 64.7, 16384 x 4000 54.9 and 54.4.  (Four: 16384 features in 512 threads.)
 inline int fwd_vectors(int D) { return D <= 512 ? 1 : D <= 1024 ? 2 : D <= 2048 ? 1 : D <= 8192 ? 2 : 4; }
 inline int fwd_threads(int D) { return D <= 1024 ? 256 : 64 * ceil_div(D, 512 * fwd_vectors(D)); }
 inline int fwd_groups(long long M, int D) {
@@ -456,9 +477,9 @@ inline int fwd_groups(long long M, int D) {
   return (int)least(D <= 1024 ? (M + 3) / 4 : M, 2048 / fwd_threads(D) * CUS);
 }
 // Backward: threads of a row (up to 512 features are a wave's), its teams (fewer where rows are: every CU has some),
-// and workgroups, one a CU, or two where half a CU's threads are enough for one (8192 x 5000: 63 us, 116 with one).
-// Teams against workgroups of one each, as many threads a CU: 16384 x 1024 25.4 us and 39.4, 8192 x 640 15.8 and 26.5,
-// 32768 x 2560 89 and 92.
+// and workgroups, one a CU, or two where half a CU's threads are enough for one (8192 x 5000 bf16: 56 us, 64 with one).
+// Teams against workgroups of one each, as many threads a CU: 16384 x 1024 26 us and 39, 8192 x 640 15.9 and 25.8,
+// 32768 x 2560 91 and 93.
 inline int bwd_threads(int D) { return D > 8192 ? 1024 : 64 * ceil_div(D, 512); }
 inline int bwd_teams(long long M, int D) { return (int)least(1024 / bwd_threads(D), (M + CUS - 1) / CUS); }
 inline int bwd_groups(long long M, int D) {
