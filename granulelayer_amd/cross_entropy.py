@@ -104,7 +104,7 @@ def dense_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Ten
     type; target [...] int64 or int32.  ``reduction``: "none" (a loss a row), "sum", or "mean" over the rows that
     count.  Rows with ``ignore_index`` have the loss 0 and no gradient, whatever x holds there; a mean of no rows is 0.
     Any other target that is no class makes the loss NaN.  A class whose bias is -inf takes no part.  The backward's
-    pieces of gradients at the logits take up to ``workspace_budget`` bytes (1 GiB by default; of 256 classes at
+    pieces of gradients at the logits take up to ``workspace_budget`` bytes (4 GiB by default; of 256 classes at
     least), and it takes the operands as they were: none of them may change before it."""
     _check(x, weight, target, bias, reduction, workspace_budget)
     N, K = weight.shape

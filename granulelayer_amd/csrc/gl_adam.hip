@@ -13,8 +13,8 @@
 // with the codes nearest in their root: a value is off by 1 / c of itself, 0.8% of m and 0.4% of sqrt(v) next to the
 // maximum, more towards zero, and sqrt(v) reaches down to 1.5e-5 of the largest.  Codes of v are 1 at least where v > 0: a
 // sqrt(v) rounded to nothing would leave m / eps.  The update itself takes the moments before they are put into 8 bits.
-// A value next to a border between two codes must not depend on how its sums are rounded, so moments and
-// codes are computed in 64 bits, which this chip does as fast as unpacked 32.  A block with an infinity or a NaN in m or v has
+// A value next to a border between two codes must not depend on how its sums are rounded, so moments are computed in
+// 64 bits, which this chip does as fast as unpacked 32, and so are the codes where fp32 cannot tell.  A block with an infinity or a NaN in m or v has
 // the scale NaN; one whose largest |m| is below 2^-100 (v: 2^-126) the scale 0.
 #include "gl_common.h"
 #include "gl_internal.h"
@@ -236,8 +236,8 @@ __device__ __forceinline__ int adam_tensor(const AdamTable& a) {
 
 // MOM: GL_DTYPE_F32, GL_DTYPE_BF16 or GL_MOMENTS_INT8; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
 // thread a vector of each stream, or two with 8-bit moments: a block is half a wave's then, and what is done for a block (its
-// maxima and scales) is done for two at once.  150M bf16 parameters and gradients: 319 us (4.7 TB/s,
-// bound by instructions: 330 a wave before, 246 us at the memory's rate), 352 with a block a wave.
+// maxima and scales) is done for two at once.  150M bf16 parameters and gradients: 319 us (4.7 TB/s; bound by instructions,
+// 246 us at the rate of the fp32 stream), 352 with a block a wave.  400M fp32 in all types: 2.2 ms (5.7 TB/s).
 // WHOLE: all of the wave's elements are there (no lane's ends are looked at).
 constexpr int adam_vectors(int mom) { return mom == GL_MOMENTS_INT8 ? 2 : 1; }
 template <int MOM, int PM, bool GBF, bool WHOLE>

@@ -31,7 +31,9 @@ namespace {
 // workgroup's work.  1024 features and 32768 classes, all rows and those that count: the forward alone of 64 rows 29 and
 // 40 us, of 128 41 and 42, of 192 56 and 46; with the backward of 128 rows 120 and 135, of 192 150 and 144.
 constexpr int CE_ALL = 128;
-constexpr size_t CE_PIECE = 1ull << 30;  // bytes of dz of a piece, unless the caller says less
+// Bytes of dz of a piece, unless the caller says otherwise: 1/72 of the card's memory.  16384 x 4096 over 131072 classes bf16, in
+// pieces of 1, 2 and 4 GiB (that is whole): 47.1, 45.2 and 40.9 ms.
+constexpr size_t CE_PIECE = 4ull << 30;
 // Features from which exponentials are kept: the product that makes them again reads and multiplies that many, keeping them
 // does not depend on it.  A training pass of 4096 rows, kept and not: bf16 and 50000 classes, 384 features 876 and 859 us,
 // 512 935 and 952, 1024 1389 and 1581; fp32 and 16384 classes, 64 features 570 and 580, 512 1729 and 2133.
@@ -475,7 +477,7 @@ int plan_ce_bwd(const GlCeBwdArgs* a, CeBwd* out) {
   p.w_at = l.take(copy_bytes(p.w, es));
   p.info = l.take((size_t)a->M * 16);
   p.alpha = l.take(4);
-  p.dz = l.take(p.kept && p.pieces == 1 ? 0 : (size_t)a->M * padded(p.piece) * es);
+  p.dz = l.take(p.kept ? 0 : (size_t)a->M * padded(p.piece) * es);  // (later pieces' too take the first one's place)
   p.dx = l.take(a->dX && !p.direct ? (size_t)a->M * a->K * (p.pieces > 1 ? 4 : es) : 0);
   p.part = l.take(part);
   p.cols = l.take(a->db ? cols : 0);
@@ -617,7 +619,7 @@ extern "C" int gl_ce_bwd(const GlCeBwdArgs* a, void* stream) {
     Operand w = p.w;
     w.p = (const char*)w.p + n0 * w.ld * es;
     w.rows = n;
-    void* at = i == 0 && p.kept ? a->exps : ws + p.dz;
+    void* at = p.kept ? a->exps : ws + p.dz;
     long long chunks;
     if (i == 0 && p.kept) {
       const dim3 grid((unsigned)((a->M + CE_DZ_ROWS - 1) / CE_DZ_ROWS), (unsigned)ceil_div(n, 256));
