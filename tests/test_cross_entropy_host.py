@@ -77,9 +77,9 @@ def test_workspace_follows_the_budget():
     lib = N.library()
     out = ctypes.c_size_t()
 
-    def need(M, classes, budget, dtype=1, K=4096):
+    def need(M, classes, budget, dtype=1, K=4096, exps=0):
         a = N.GlCeBwdArgs(X=4096, sx=K, W=4096, sw=K, target=4096, M=M, N=classes, K=K, dtype=dtype, reduction=1, kept=4096,
-                          dloss=4096, dX=4096, dW=4096, g_dtype=dtype, piece_bytes=budget)
+                          dloss=4096, dX=4096, dW=4096, g_dtype=dtype, piece_bytes=budget, exps=exps)
         assert lib.lib.gl_ce_bwd_workspace(ctypes.byref(a), ctypes.byref(out)) == 0
         return out.value
 
@@ -87,5 +87,7 @@ def test_workspace_follows_the_budget():
     rest = M * 4096 * 2 + M * 16 + 256 + M * 4096 * 4  # x, the rows, their factor, dx in fp32 over the pieces
     for budget in (64 << 20, 256 << 20, 1 << 30):
         assert budget * 0.9 < need(M, V, budget) - rest <= budget + 256 * M * 2
-    assert need(M, V, 0) == need(M, V, 1 << 30)
+    assert need(M, V, 0) == need(M, V, 4 << 30) and need(2 * M, 2 * V, 0) == need(2 * M, 2 * V, 4 << 30) > need(2 * M, 2 * V, 1 << 30)
+    # pieces' gradients at the logits have the place of the kept exponentials
+    assert need(M, V, 1 << 30, exps=4096) - rest <= 64 << 20
     assert need(M, V, 1) - rest <= 256 * M * 2 + (64 << 20)  # 256 classes at least (and their products' partial sums)
