@@ -21,6 +21,8 @@ in the optimizer state (``master_weights=True``; the update runs on it and the p
 nearest-even rounding), stochastic rounding (the default without masters: noise from Triton's
 ``tl.randint(seed, element)`` below the bf16 cut, the seed counting tensors as the reference's
 ``_seed`` does), or nearest-even rounding (``stochastic_rounding=False``).
+
+A step captured into a graph replays the learning rate, the bias corrections and the seeds that it was captured with.
 """
 from __future__ import annotations
 
@@ -33,6 +35,29 @@ from .backend import adam_row as _ROW, backend_for
 _MOMENTS = {"bf16": torch.bfloat16, "fp32": torch.float32, "int8": torch.int8}
 _TYPES = (torch.float32, torch.bfloat16)
 _BLOCK = 256  # elements of a tensor that share the scales of 8-bit moments
+
+
+_NONE = (0, 0, 0)
+
+
+def _addresses(of):
+    """Of a state's tensors (m, v, master, m_scale, v_scale): those of the last three."""
+    if of[2] is None and of[3] is None:
+        return _NONE
+    return tuple(0 if t is None else t.data_ptr() for t in of[2:])
+
+
+def _apart(todo):
+    """Of tensors to step: those that have no memory in common, and the parameters of the others."""
+    now, later, places = [], [], set()
+    for t in todo:
+        p, _, _, main, at, g_at = t
+        if p.numel() and (at in places or main and g_at in places):
+            later.append(p)
+            continue
+        places.update((at, g_at) if main else (at,))
+        now.append(t)
+    return now, later
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -111,7 +136,7 @@ class FusedAdamW(torch.optim.Optimizer):
         mdt = self._check_state(p, st)
         backend = backend_for(p.device)
         of = (st["m"], st["v"], st.get("master"), st.get("m_scale"), st.get("v_scale"))
-        rest = tuple(0 if t is None else t.data_ptr() for t in of[2:])
+        rest = _addresses(of)
         kind = (backend, p.device, p.dtype, mdt, of[2] is not None)
         kind = self._kinds.setdefault(kind, kind)
         known = (of, of[0].data_ptr(), of[1].data_ptr(), rest, p.numel(), p.dtype, p.get_device(), kind)
@@ -142,16 +167,16 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             params = group["params"]
-            while len(params) > len(set(map(id, params))):  # one that is there twice makes two steps, not two at once
-                self._step_tensors(group, list({id(p): p for p in params}.values()))
-                params = [p for i, p in enumerate(params) if any(p is q for q in params[:i])]
-            self._step_tensors(group, params)
+            while params:
+                params = self._step_tensors(group, params)
         return loss
 
     def _step_tensors(self, group, params):
+        """A step of the parameters; returns those that come after it: of parameters in one place (one that is there
+        twice, two over the same storage), or with one main_grad, all but the first, whose steps are not at once."""
         b1, b2 = group["betas"]
         f32, bf16 = torch.float32, torch.bfloat16
-        todo = []
+        todo, places = [], []
         for p in params:  # everything is checked before anything changes
             g = getattr(p, "main_grad", None)
             main = g is not None
@@ -165,10 +190,17 @@ class FusedAdamW(torch.optim.Optimizer):
                     or g.numel() != p.numel() or g.get_device() != p.get_device()):
                 g = self._gradient(p, g, main)
                 gdt = g.dtype
-            todo.append((p, g, gdt, main))
+            at, g_at = p.data_ptr(), g.data_ptr()
+            places.append(at)
+            if main:
+                places.append(g_at)
+            todo.append((p, g, gdt, main, at, g_at))
+        later = []
+        if len(set(places)) < len(places):
+            todo, later = _apart(todo)
         calls, states, corrections = {}, [], {}
         state, known_of, seed, last = self.state, self._known, self._seed, (None, None, None)
-        for p, g, gdt, main in todo:
+        for p, g, gdt, main, at, g_at in todo:
             st = state[p]
             known = known_of.get(id(p))
             known = None if known is None else known[1]
@@ -176,7 +208,7 @@ class FusedAdamW(torch.optim.Optimizer):
                     or st.get("master") is not known[0][2] or st.get("m_scale") is not known[0][3]
                     or st.get("v_scale") is not known[0][4] or known[0][0].data_ptr() != known[1]
                     or known[0][1].data_ptr() != known[2] or p.numel() != known[4] or p.dtype is not known[5]
-                    or p.get_device() != known[6]):
+                    or p.get_device() != known[6] or known[3] is not _NONE and known[3] != _addresses(known[0])):
                 known = self._known_state(p, st)
             _, m, v, rest, n, _, _, kind = known
             t = st["step"] + 1
@@ -185,7 +217,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 c = corrections[t] = (1 - b1 ** t, 1 - b2 ** t)
             seed += 1
             states.append(st)
-            row = _ROW(p.data_ptr(), g.data_ptr(), m, v, *rest, n, seed & 0xffffffffffffffff, *c)
+            row = _ROW(at, g_at, m, v, *rest, n, seed & 0xffffffffffffffff, *c)
             if kind is not last[0] or gdt is not last[1] or main is not last[2]:
                 last = (kind, gdt, main)
                 rows = calls.setdefault(last, [])
@@ -196,9 +228,10 @@ class FusedAdamW(torch.optim.Optimizer):
                               stochastic=self.stochastic_rounding and pdt is bf16 and not has_master, clear=main)
         for st in states:
             st["step"] += 1
-        for p, _, _, main in todo:
+        for p, _, _, main, _, _ in todo:
             if not main:
                 p.grad = None
+        return later
 
     @torch.no_grad()
     def moment_values(self) -> List[Tuple[torch.Tensor, torch.Tensor]]:

@@ -116,6 +116,46 @@ def test_a_parameter_that_is_there_twice():
 
 
 # ---- 8-bit moments ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shared", ["storage", "main_grad"])
+def test_parameters_that_share_memory_step_one_after_the_other(shared):
+    n = 300_000
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    data = torch.randn(2, n, device=DEV, generator=gen)
+    grads = torch.randn(2, n, device=DEV, generator=gen)
+
+    def make(together):
+        a, b = data.clone()
+        ps = [torch.nn.Parameter(a), torch.nn.Parameter(a if shared == "storage" else b)]
+        gs = grads.clone()
+        for p, g in zip(ps, (gs[0], gs[0] if shared == "main_grad" else gs[1])):
+            p.main_grad = g
+        groups = [dict(params=ps)] if together else [dict(params=[p]) for p in ps]
+        return ps, FusedAdamW(groups, lr=1e-2, moments="fp32", weight_decay=0.1)
+
+    (got, one), (want, two) = make(True), make(False)
+    for opt in (one, two):
+        for _ in range(3):
+            opt.step()
+    for p, q in zip(got, want):
+        assert torch.equal(p, q) and not p.main_grad.any()
+        assert torch.equal(one.state[p]["m"], two.state[q]["m"]) and one.state[p]["step"] == 3
+
+
+def test_a_state_whose_memory_moved():
+    """A state's tensor that has other memory under it is read and written there."""
+    p, q = (torch.nn.Parameter(torch.full((1000,), 0.5, device=DEV, dtype=torch.bfloat16)) for _ in range(2))
+    opts = [FusedAdamW([t], lr=1e-2, moments="int8", master_weights=True) for t in (p, q)]
+    for k in range(4):
+        for t, opt in zip((p, q), opts):
+            t.grad = torch.full_like(t, 0.25 + k)
+            opt.step()
+        st = opts[1].state[q]
+        for key in ("master", "m_scale", "v_scale", "m", "v"):
+            st[key].data = st[key].data.clone()
+    a, b = opts[0].state[p], opts[1].state[q]
+    assert torch.equal(p, q) and all(torch.equal(a[k], b[k]) for k in ("master", "m_scale", "v_scale", "m", "v"))
+
+
 def _values(cm, sm, cv, sv, n):
     of = np.arange(n) // 256
     m = cm.astype(np.float64) * np.abs(cm.astype(np.float64)) * sm.astype(np.float64)[of]
