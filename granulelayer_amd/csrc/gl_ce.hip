@@ -235,16 +235,19 @@ __global__ __launch_bounds__(1024) void ce_join_all_kernel(JoinK a) {
 // ---- backward ------------------------------------------------------------------------------------------------
 // What a row's logits need to become dz, without the factor that all rows share (alpha: the mean's 1 / count and the
 // upstream gradient, which the products' epilogues apply).  With it, the targets' dz, all near -alpha, would be rounded to bf16
-// alike: up to 2^-9 of dX and dW as a whole.  A target that is no class makes the row's dz NaN.
+// alike: up to 2^-9 of dX and dW as a whole.  (One that is no number stays with its rows: the others' gradients are 0.)  A target
+// that is no class makes the row's dz NaN.
 __global__ __launch_bounds__(256) void ce_info_kernel(const long long* __restrict__ target, long long M, long long ignored, int N,
                                                       int reduction, Kept k, bool all, const float* __restrict__ g, long long sg,
                                                       uv4* __restrict__ info, float* __restrict__ alpha) {
   const long long m = (long long)blockIdx.x * 256 + threadIdx.x;
   const int n = *k.count;
-  if (m == 0) *alpha = reduction == GL_CE_NONE ? 1.f : reduction == GL_CE_SUM ? *g : n > 0 ? *g / (float)n : 0.f;
+  const float shared = reduction == GL_CE_NONE ? 1.f : reduction == GL_CE_SUM ? *g : n > 0 ? *g / (float)n : 0.f;
+  const bool number = __builtin_fabsf(shared) < __builtin_inff();
+  if (m == 0) *alpha = number ? shared : 1.f;
   if (m >= (all ? M : n)) return;
   const long long row = all ? m : k.index[m], t = target[row];
-  float c = reduction == GL_CE_NONE ? g[row * sg] : 1.f;
+  float c = reduction == GL_CE_NONE ? g[row * sg] : number ? 1.f : shared;
   if (t < 0 || t >= N) c = __builtin_nanf("");
   if (t == ignored) c = 0.f;
   info[m] = uv4{__float_as_uint(k.top[m]), __float_as_uint(c == 0.f ? 0.f : c / k.sum[m]), (unsigned)t, __float_as_uint(c * expm1f(-k.loss[m]))};

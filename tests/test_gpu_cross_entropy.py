@@ -402,6 +402,24 @@ def test_a_second_backward_and_one_without_the_first():
         check(v, want, name)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("K", [64, 520])
+@pytest.mark.parametrize("M", [100, 700])
+@pytest.mark.parametrize("upstream", [float("inf"), float("nan")])
+def test_an_upstream_gradient_that_is_no_number(upstream, M, K, reduction):
+    """It reaches the rows that count and no others."""
+    t = inputs(M, K, 300, BF)
+    off = t["target"] == IGNORED
+    for target in (t["target"], torch.full_like(t["target"], IGNORED)):
+        leaves = [t[k].detach().requires_grad_(True) for k in "xwb"]
+        loss = dense_cross_entropy(leaves[0], leaves[1], target, leaves[2], reduction)
+        dx, dw, db = torch.autograd.grad(loss, leaves, torch.full((), upstream, device=DEV))
+        if target is t["target"]:
+            assert not dx[off].any() and not dx[~off].isfinite().all(1).any() and not dw.isfinite().all() and not db.isfinite().all()
+        else:
+            assert not dx.any() and not dw.any() and not db.any()
+
+
 def test_a_captured_backward_without_its_forward():
     """A graph of the backward alone is replayed as often as one likes; one forward serves all of them."""
     t = inputs(700, 520, 900, BF)
