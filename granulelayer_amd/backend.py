@@ -71,6 +71,14 @@ def _x_operand(x: torch.Tensor):
     return x, code, x.stride(0)
 
 
+def _rows(x: torch.Tensor):
+    """``_x_operand`` of a matrix of one of these types, in less time."""
+    sx, unit = x.stride()
+    if unit != 1 or sx < x.shape[1] or x.is_neg():
+        return _x_operand(x.resolve_neg())
+    return x, _DENSE_DTYPES[x.dtype], sx
+
+
 def _params(w: torch.Tensor, b: torch.Tensor):
     """(W, bias, dtype code) as the kernels read them: fp32 or bf16 (widened in the kernels), both
     of one dtype (a bf16 / fp32 mix is widened to fp32, exactly), contiguous, W 4-byte aligned."""
@@ -533,14 +541,15 @@ class HipBackend:
     _norm_bwd = functools.cached_property(lambda self: self.lib.entry("gl_norm_bwd"))
 
     def norm_forward(self, x, w, b, eps, out_dtype, keep):
-        """(y [M, D] of ``out_dtype``, what the backward takes: [M, 2] fp32 with ``keep``) of x [M, D], w and b [D]
+        """(y [M, D] of ``out_dtype``, what the backward takes: two fp32 numbers a row with ``keep``) of x [M, D], w and b [D]
         of one dtype or None."""
-        x, code, sx = _x_operand(x.resolve_neg())
+        x, code, sx = _rows(x)
         M, D = x.shape
         dev = x.device
         w, b, wcode = _norm_params(w, b)
-        y = torch.empty((M, D), device=dev, dtype=out_dtype)
-        stats = torch.empty((M, 2), device=dev) if keep else None
+        # (each form of an allocation is the one that takes the least time on the host)
+        y = torch.empty_like(x, dtype=out_dtype) if sx == D else torch.empty((M, D), device=dev, dtype=out_dtype)
+        stats = x.new_empty(2 * M, dtype=torch.float32) if keep else None
         a = _NORM(x.data_ptr(), sx, _ptr(w), _ptr(b), y.data_ptr(), D, _ptr(stats), M, D, code, wcode,
                   _DENSE_DTYPES[out_dtype], eps)
         with _on(dev):
@@ -550,8 +559,8 @@ class HipBackend:
     def norm_backward(self, dy, x, w, stats, dx, dw, db, accumulate):
         """Gradients of ``norm_forward`` into dx [M, D] (x's dtype), dw and db [D] (one dtype, or fp32 and added to
         with ``accumulate``); None for what is not needed."""
-        dy, ycode, sdy = _x_operand(dy)
-        x, code, sx = _x_operand(x.resolve_neg())
+        dy, ycode, sdy = _rows(dy)
+        x, code, sx = _rows(x)
         M, D = x.shape
         dev = x.device
         w, _, wcode = _norm_params(w, None)
@@ -578,9 +587,9 @@ class HipBackend:
 
     def capture_id(self, dev) -> int:
         """The number of the graph that the device's current stream is being captured into; 0: none."""
+        if dev.index == torch._C._cuda_getDevice() and not torch.cuda.is_current_stream_capturing():
+            return 0
         with _on(dev):
-            if not torch.cuda.is_current_stream_capturing():
-                return 0
             v = ctypes.c_uint64()
             self.lib.call("gl_capture_id", _stream(dev), ctypes.byref(v))
             return v.value
@@ -588,8 +597,8 @@ class HipBackend:
     def ce_forward(self, x, w, b, target, reduction, ignore_index, keep, piece_bytes=0):
         """(loss, and with ``keep`` what the backward takes: five words a row, and the first piece's exponentials or
         None) of x [M, K], w [N, K], b [N] or None (all of one dtype) and target [M] (contiguous int64)."""
-        x, code, sx = _x_operand(x.resolve_neg())
-        w, _, sw = _x_operand(w.resolve_neg())
+        x, code, sx = _rows(x)
+        w, _, sw = _rows(w)
         M, K = x.shape
         F = w.shape[0]
         dev = x.device
@@ -613,8 +622,8 @@ class HipBackend:
                     exps=None):
         """Gradients of ``ce_forward`` (of the same piece_bytes) into dx [M, K] (x's dtype), dw [N, K] and db [N] (w's
         dtype, or fp32 and added to with ``accumulate``); None for what is not needed.  ``exps`` is used up."""
-        x, code, sx = _x_operand(x.resolve_neg())
-        w, _, sw = _x_operand(w.resolve_neg())
+        x, code, sx = _rows(x)
+        w, _, sw = _rows(w)
         M, K = x.shape
         F = w.shape[0]
         dev = x.device
@@ -651,8 +660,10 @@ class HipBackend:
 
 def _norm_params(w, b):
     """Contiguous w and b and their dtype's code."""
-    w = None if w is None else w.resolve_neg().contiguous()
-    b = None if b is None else b.resolve_neg().contiguous()
+    if w is not None and (w.is_neg() or not w.is_contiguous()):
+        w = w.resolve_neg().contiguous()
+    if b is not None and (b.is_neg() or not b.is_contiguous()):
+        b = b.resolve_neg().contiguous()
     t = b if w is None else w
     return w, b, 0 if t is None else _DENSE_DTYPES[t.dtype]
 

@@ -69,7 +69,7 @@ def _gradients(ctx, dy):
     else:
         dw = torch.empty_like(w, memory_format=torch.contiguous_format) if need_w else None
         db = torch.empty_like(b, device=x.device, memory_format=torch.contiguous_format) if need_b else None
-    backend_for(x.device).norm_backward(dy.resolve_neg(), x, w, stats, dx, dw, db, use_main)
+    backend_for(x.device).norm_backward(dy, x, w, stats, dx, dw, db, use_main)
     return dx, None if use_main else dw, None if use_main else db, None, None
 
 
