@@ -192,7 +192,7 @@ __device__ __forceinline__ float scale_v(unsigned top) {
   if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
   return top < 0x00800000u ? 0.f : (float)(root(__uint_as_float(top)) * (1.0 / 65025.0));
 }
-// Codes.  In fp32, where a root is within 6e-5 of its own: adding 1.5 x 2^23 rounds it to a whole number, which is left in
+// Codes.  In fp32, where a root is within 8e-5 of its own: adding 1.5 x 2^23 rounds it to a whole number, which is left in
 // the low byte in two's complement, and `near` gathers how far roots are from whole numbers.  Where one is within
 // CODE_NEAR of a border between two codes (a wave in nine) all of the wave's are decided in 64 bits instead: of floor(x + 1/2),
 // x the root, an estimate decides all but which side of i + 1/2 x is on, and (i + 1/2)^2, exact in 64 bits, decides that.
@@ -215,15 +215,14 @@ __device__ __forceinline__ unsigned code_v(double y) {
 __device__ __forceinline__ unsigned low_bytes(const unsigned (&c)[4]) {
   return __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u) | __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
 }
-// values of codes
-__device__ __forceinline__ double value_m(unsigned codes, int j, double s) {
+// c |c| of code j of m, c^4 of v: m and v over the scale and over its square
+__device__ __forceinline__ double square_m(unsigned codes, int j) {
   const int c = (int)(codes << (24 - 8 * j)) >> 24;
-  return (double)(c * __builtin_abs(c)) * s;
+  return (double)(c * __builtin_abs(c));
 }
-__device__ __forceinline__ double value_v(unsigned codes, int j, double r) {
-  const unsigned c = (codes >> (8 * j)) & 255u;
-  const double t = (double)(c * c) * r;
-  return t * t;
+__device__ __forceinline__ double fourth_v(unsigned codes, int j) {
+  const unsigned c = (codes >> (8 * j)) & 255u, s = c * c;
+  return (double)(s * s);  // up to 255^4 < 2^32
 }
 
 // the tensor of this workgroup
@@ -236,8 +235,8 @@ __device__ __forceinline__ int adam_tensor(const AdamTable& a) {
 
 // MOM: GL_DTYPE_F32, GL_DTYPE_BF16 or GL_MOMENTS_INT8; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
 // thread a vector of each stream, or two with 8-bit moments: a block is half a wave's then, and what is done for a block (its
-// maxima and scales) is done for two at once.  150M bf16 parameters and gradients: 319 us (4.7 TB/s; bound by instructions,
-// 246 us at the rate of the fp32 stream), 352 with a block a wave.  400M fp32 in all types: 2.2 ms (5.7 TB/s).
+// maxima and scales) is done for two at once.  150M bf16 parameters and gradients: 305 us (4.9 TB/s; bound by instructions,
+// 246 us at the rate of the fp32 stream), 352 with a block a wave (319 then).  400M fp32 in all types: 2.2 ms (5.7 TB/s).
 // WHOLE: all of the wave's elements are there (no lane's ends are looked at).
 constexpr int adam_vectors(int mom) { return mom == GL_MOMENTS_INT8 ? 2 : 1; }
 template <int MOM, int PM, bool GBF, bool WHOLE>
@@ -277,6 +276,7 @@ __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensor
     float* scale_of_m = t.m_scale + base / ADAM_BLOCK;
     float* scale_of_v = t.v_scale + base / ADAM_BLOCK;
     const double sm = here ? (double)scale_of_m[half] : 0.0, sv = here ? (double)scale_of_v[half] : 0.0;
+    const double bm = a.b1d * sm, bv = a.b2d * (sv * sv);
     // (behind the end: 0, and NaN in a block that is NaN anyway)
     double dm[V][4], dv[V][4];
     unsigned tm = 0, tv = 0;
@@ -285,8 +285,8 @@ __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensor
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const double gj = (double)g[x][j];
-        dm[x][j] = __builtin_fma(a.b1d, value_m(cm[x], j, sm), a.a1d * gj);
-        dv[x][j] = __builtin_fma(a.b2d, value_v(cv[x], j, sv), a.a2d * (gj * gj));
+        dm[x][j] = __builtin_fma(square_m(cm[x], j), bm, a.a1d * gj);
+        dv[x][j] = __builtin_fma(fourth_v(cv[x], j), bv, a.a2d * (gj * gj));
         m[x][j] = (float)dm[x][j];
         v[x][j] = (float)dv[x][j];
         tm = umax(tm, abs_bits(m[x][j]));
@@ -294,24 +294,24 @@ __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensor
       }
     const float fs = scale_m(half_umax(tm)), fr = scale_v(half_umax(tv));
     const bool live_m = fs > 0.f, live_v = fr > 0.f;
-    const double im = reciprocal(live_m ? fs : 1.f), ir = reciprocal(live_v ? fr : 1.f);
-    const float imf = (float)im, irf = (float)ir;
+    const float im = __builtin_amdgcn_rcpf(live_m ? fs : 1.f), ir = __builtin_amdgcn_rcpf(live_v ? fr : 1.f);
     unsigned om[V][4], ov[V][4];
     float near = 0.f, rv[V][4];
 #pragma unroll
     for (int x = 0; x < V; ++x)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        om[x][j] = code_of(__builtin_copysignf(__builtin_amdgcn_sqrtf(__builtin_fabsf(m[x][j]) * imf), m[x][j]), near);
-        rv[x][j] = __builtin_amdgcn_sqrtf(v[x][j] * irf * irf);
+        om[x][j] = code_of(__builtin_copysignf(__builtin_amdgcn_sqrtf(__builtin_fabsf(m[x][j]) * im), m[x][j]), near);
+        rv[x][j] = __builtin_amdgcn_sqrtf(v[x][j] * ir * ir);
         ov[x][j] = code_of(__builtin_fmaxf(__builtin_amdgcn_sqrtf(rv[x][j]), dv[x][j] > 0.0 ? 0.75f : 0.f), near);
       }
     if (__builtin_amdgcn_ballot_w64(near > 0.5f - CODE_NEAR)) {
+      const double dim = reciprocal(live_m ? fs : 1.f), dir = reciprocal(live_v ? fr : 1.f);
 #pragma unroll
       for (int x = 0; x < V; ++x)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const unsigned q = live_m ? code_m(__builtin_fabs(dm[x][j]) * im) : 0u, u = live_v ? code_v(dv[x][j] * ir * ir) : 0u;
+          const unsigned q = live_m ? code_m(__builtin_fabs(dm[x][j]) * dim) : 0u, u = live_v ? code_v(dv[x][j] * dir * dir) : 0u;
           om[x][j] = dm[x][j] < 0.0 ? 0u - q : q;
           ov[x][j] = u == 0 && dv[x][j] > 0.0 ? 1u : u;
         }
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(256) adam_kernel(AdamTable a) {
   else if (base < t.n) adam_vector<MOM, PM, GBF, false>(a, t, base);
 }
 
-// The fp32 values of 8-bit moments (into g: m's, into p: v's), a vector a thread.  150M: 243 us, 6.2 TB/s.
+// The fp32 values of 8-bit moments (into g: m's, into p: v's), a vector a thread.  150M: 237 us, 6.3 TB/s.
 __global__ void __launch_bounds__(512) adam_values_kernel(AdamTable a) {
   const int ti = adam_tensor(a);
   const AdamTensorK& t = a.t[ti];
@@ -384,12 +384,12 @@ __global__ void __launch_bounds__(512) adam_values_kernel(AdamTable a) {
   if (left <= 0) return;
   const int n = left > 4 ? 4 : (int)left;
   const unsigned cm = adam_load_codes((char*)t.m + block, i, n), cv = adam_load_codes((char*)t.v + block, i, n);
-  const double sm = (double)t.m_scale[block / ADAM_BLOCK], sv = (double)t.v_scale[block / ADAM_BLOCK];
+  const double sm = (double)t.m_scale[block / ADAM_BLOCK], sv = (double)t.v_scale[block / ADAM_BLOCK], sv2 = sv * sv;
   float m[4], v[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    m[j] = (float)value_m(cm, j, sm);
-    v[j] = (float)value_v(cv, j, sv);
+    m[j] = (float)(square_m(cm, j) * sm);
+    v[j] = (float)(fourth_v(cv, j) * sv2);
   }
   adam_store((float*)t.g + block, i, n, m);
   adam_store((float*)t.p + block, i, n, v);
