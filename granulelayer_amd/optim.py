@@ -26,6 +26,7 @@ A step captured into a graph replays the learning rate, the bias corrections and
 """
 from __future__ import annotations
 
+from operator import le
 from typing import Iterable, List, Tuple
 
 import torch
@@ -47,17 +48,40 @@ def _addresses(of):
     return tuple(0 if t is None else t.data_ptr() for t in of[2:])
 
 
-def _apart(todo):
-    """Of tensors to step: those that have no memory in common, and the parameters of the others."""
-    now, later, places = [], [], set()
+def _disjoint(starts, ends) -> bool:
+    """Whether of ranges of bytes, given by their starts and their ends in any order, no two meet."""
+    starts, ends = sorted(starts), sorted(ends)
+    return all(map(le, ends, starts[1:]))
+
+
+def _in_turn(todo):
+    """Of tensors to step of which some meet in memory: lists of those that may step at once.  A tensor comes after all
+    earlier ones that write what it touches, or touch what it writes."""
+    kept, seen = [], set()
     for t in todo:
-        p, _, _, main, at, g_at = t
-        if p.numel() and (at in places or main and g_at in places):
-            later.append(p)
-            continue
-        places.update((at, g_at) if main else (at,))
-        now.append(t)
-    return now, later
+        if t[3] or id(t[0]) not in seen:  # (there twice: its first step uses up its .grad)
+            seen.add(id(t[0]))
+            kept.append((*t[:-1], todo[0][-1] + len(kept)))
+    spans = []
+    for k, (p, g, _, main, at, g_at, n, _, _) in enumerate(kept):
+        if n:
+            spans.append((at, at + n * p.element_size(), k, True))
+            spans.append((g_at, g_at + n * g.element_size(), k, main))
+    meets, writers, readers = [[] for _ in kept], [], []
+    for start, end, k, written in sorted(spans):
+        writers = [s for s in writers if s[0] > start]
+        readers = [s for s in readers if s[0] > start] if written else readers
+        for _, j in writers + readers if written else writers:
+            if j != k:
+                meets[max(j, k)].append(min(j, k))
+        (writers if written else readers).append((end, k))
+    turns, turn = [], []
+    for t, earlier in zip(kept, meets):
+        turn.append(1 + max((turn[j] for j in earlier), default=-1))
+        if turn[-1] == len(turns):
+            turns.append([])
+        turns[turn[-1]].append(t)
+    return turns
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -166,72 +190,75 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            params = group["params"]
-            while params:
-                params = self._step_tensors(group, params)
+            self._step_group(group)
         return loss
 
-    def _step_tensors(self, group, params):
-        """A step of the parameters; returns those that come after it: of parameters in one place (one that is there
-        twice, two over the same storage), or with one main_grad, all but the first, whose steps are not at once."""
-        b1, b2 = group["betas"]
+    def _step_group(self, group):
         f32, bf16 = torch.float32, torch.bfloat16
-        todo, places = [], []
-        for p in params:  # everything is checked before anything changes
+        todo, starts, ends, seed = [], [], [], self._seed
+        for p in group["params"]:  # everything is checked before anything changes
             g = getattr(p, "main_grad", None)
             main = g is not None
             if not main:
                 g = p.grad
                 if g is None:
                     continue
-            gdt = g.dtype
+            pdt, gdt, n = p.dtype, g.dtype, p.numel()
             if (not (gdt is f32 or (gdt is bf16 and not main)) or not g.is_contiguous() or g.is_neg()
-                    or not p.is_contiguous() or not (p.dtype is f32 or p.dtype is bf16)
-                    or g.numel() != p.numel() or g.get_device() != p.get_device()):
+                    or not p.is_contiguous() or not (pdt is f32 or pdt is bf16)
+                    or g.numel() != n or g.get_device() != p.get_device()):
                 g = self._gradient(p, g, main)
                 gdt = g.dtype
             at, g_at = p.data_ptr(), g.data_ptr()
-            places.append(at)
-            if main:
-                places.append(g_at)
-            todo.append((p, g, gdt, main, at, g_at))
-        later = []
-        if len(set(places)) < len(places):
-            todo, later = _apart(todo)
+            if n:
+                starts += at, g_at
+                ends += at + n * (4 if pdt is f32 else 2), g_at + n * (4 if gdt is f32 else 2)
+            seed += 1
+            todo.append((p, g, gdt, main, at, g_at, n, pdt, seed))
+        turns = [todo] if _disjoint(starts, ends) else _in_turn(todo)
+        if len(turns) > 1:
+            for t in todo:
+                if self.state.get(t[0]):
+                    self._check_state(t[0], self.state[t[0]])
+        for turn in turns:
+            self._step_tensors(group, turn)
+
+    def _step_tensors(self, group, todo):
+        """A step of tensors of which none writes what another touches."""
+        b1, b2 = group["betas"]
+        bf16 = torch.bfloat16
         calls, states, corrections = {}, [], {}
-        state, known_of, seed, last = self.state, self._known, self._seed, (None, None, None)
-        for p, g, gdt, main, at, g_at in todo:
+        state, known_of, last = self.state, self._known, (None, None, None)
+        for p, g, gdt, main, at, g_at, n, pdt, seed in todo:
             st = state[p]
             known = known_of.get(id(p))
             known = None if known is None else known[1]
             if (known is None or not st or st["m"] is not known[0][0] or st["v"] is not known[0][1]
                     or st.get("master") is not known[0][2] or st.get("m_scale") is not known[0][3]
                     or st.get("v_scale") is not known[0][4] or known[0][0].data_ptr() != known[1]
-                    or known[0][1].data_ptr() != known[2] or p.numel() != known[4] or p.dtype is not known[5]
+                    or known[0][1].data_ptr() != known[2] or n != known[4] or pdt is not known[5]
                     or p.get_device() != known[6] or known[3] is not _NONE and known[3] != _addresses(known[0])):
                 known = self._known_state(p, st)
-            _, m, v, rest, n, _, _, kind = known
+            _, m, v, rest, _, _, _, kind = known
             t = st["step"] + 1
             c = corrections.get(t)
             if c is None:
                 c = corrections[t] = (1 - b1 ** t, 1 - b2 ** t)
-            seed += 1
             states.append(st)
             row = _ROW(at, g_at, m, v, *rest, n, seed & 0xffffffffffffffff, *c)
             if kind is not last[0] or gdt is not last[1] or main is not last[2]:
                 last = (kind, gdt, main)
                 rows = calls.setdefault(last, [])
             rows.append(row)
-        self._seed = seed
+        self._seed += len(todo)
         for ((backend, dev, pdt, mdt, has_master), gdt, main), rows in calls.items():
             backend.adam_many(dev, rows, pdt, gdt, mdt, group["lr"], b1, b2, group["eps"], group["weight_decay"],
                               stochastic=self.stochastic_rounding and pdt is bf16 and not has_master, clear=main)
         for st in states:
             st["step"] += 1
-        for p, _, _, main, _, _ in todo:
+        for p, _, _, main, *_ in todo:
             if not main:
                 p.grad = None
-        return later
 
     @torch.no_grad()
     def moment_values(self) -> List[Tuple[torch.Tensor, torch.Tensor]]:
