@@ -107,8 +107,18 @@ class FusedAdamW(torch.optim.Optimizer):
         return n
 
     def load_state_dict(self, state_dict):
-        """As torch's, but every tensor of the state keeps its own type (torch's casts it to the parameter's)."""
-        super().load_state_dict(state_dict)
+        """As torch's, but every tensor of the state keeps its own type (torch's casts it to the parameter's).  Hooks see
+        and change what they do with any optimizer: what the last pre-hook leaves is loaded, and post-hooks come last."""
+        seen = []
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, given: seen.append(given)),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_tensors(seen[-1]), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_tensors(self, state_dict):
         self._known.clear()
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
