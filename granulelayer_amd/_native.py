@@ -14,7 +14,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libgranulelayer_amd.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 GL_ACT = {"identity": 0, "relu": 1, "gelu": 2}
 GL_POOL = {"mean": 0, "sum": 1, "max": 2, "topk_mean": 3, "logmeanexp": 4, "power_mean": 5, "softmax_weighted": 6}
@@ -59,7 +59,8 @@ class GlAdamArgs(ctypes.Structure):
     _fields_ = [("p", _P), ("g", _P), ("m", _P), ("v", _P), ("n", _I64), ("moments_dtype", _I32), ("lr", _F),
                 ("beta1", _F), ("beta2", _F), ("eps", _F), ("weight_decay", _F), ("bc1", _F), ("bc2", _F),
                 ("p_dtype", _I32), ("stochastic", _I32), ("master", _P), ("seed", ctypes.c_uint64), ("tensors", _P),
-                ("count", _I32), ("g_dtype", _I32), ("keep_g", _I32), ("beta1_64", _D), ("beta2_64", _D)]
+                ("count", _I32), ("g_dtype", _I32), ("keep_g", _I32), ("beta1_64", _D), ("beta2_64", _D),
+                ("nearest_codes", _I32)]
 
 
 class GlCoverArgs(ctypes.Structure):

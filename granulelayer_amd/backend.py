@@ -418,13 +418,13 @@ class HipBackend:
             self.lib.call("gl_adam", ctypes.byref(a), ctypes.c_void_p(_stream(p.device)))
 
     def adam_many(self, device, rows, p_dtype, g_dtype, m_dtype, lr, beta1, beta2, eps, weight_decay, stochastic=False,
-                  clear=False):
+                  clear=False, nearest_codes=False):
         """In-place fused AdamW over the tensors of ``rows`` (``adam_row``); all of one dtype of parameters, gradients
-        and moments (int8: codes), all with a master or none."""
+        and moments (int8: codes, drawn or the nearest), all with a master or none."""
         t = b"".join(rows)
         a = N.GlAdamArgs(0, 0, 0, 0, 0, _MOMENTS[m_dtype], lr, beta1, beta2, eps, weight_decay, 0.0, 0.0, _DENSE_DTYPES[p_dtype],
                          int(stochastic), 0, 0, ctypes.cast(t, ctypes.c_void_p), len(rows), _DENSE_DTYPES[g_dtype], int(not clear),
-                         beta1, beta2)
+                         beta1, beta2, int(nearest_codes))
         with _on(device):
             self.lib.call("gl_adam", ctypes.byref(a), ctypes.c_void_p(_stream(device)))
 

@@ -137,7 +137,7 @@ extern "C" int gl_struct_layout(int which, long long* out, int n) {
                        OFF(S, moments_dtype), OFF(S, lr), OFF(S, beta1), OFF(S, beta2), OFF(S, eps),
                        OFF(S, weight_decay), OFF(S, bc1), OFF(S, bc2), OFF(S, p_dtype), OFF(S, stochastic),
                        OFF(S, master), OFF(S, seed), OFF(S, tensors), OFF(S, count), OFF(S, g_dtype),
-                       OFF(S, keep_g), OFF(S, beta1_64), OFF(S, beta2_64)};
+                       OFF(S, keep_g), OFF(S, beta1_64), OFF(S, beta2_64), OFF(S, nearest_codes)};
       for (long long x : t) v[c++] = x;
       break;
     }

@@ -10,11 +10,16 @@
 // fp32 scales,
 //     m = s c |c|      c from -127 to 127    s = max |m| / 127^2
 //     v = (r c^2)^2    c from 0 to 255       r = sqrt(max v) / 255^2
-// with the codes nearest in their root: a value is off by 1 / c of itself, 0.8% of m and 0.4% of sqrt(v) next to the
-// maximum, more towards zero, and sqrt(v) reaches down to 1.5e-5 of the largest.  Codes of v are 1 at least where v > 0: a
-// sqrt(v) rounded to nothing would leave m / eps.  The update itself takes the moments before they are put into 8 bits.
-// A value next to a border between two codes must not depend on how its sums are rounded, so moments are computed in
-// 64 bits, which this chip does as fast as unpacked 32, and so are the codes where fp32 cannot tell.  A block with an infinity or a NaN in m or v has
+// Two neighbouring codes are 2 / c of m and 4 / c of v apart, 1.6% each next to the maximum, and sqrt(v) reaches down to
+// 1.5e-5 of the largest.  A step takes a share 1 - b2 off v, 0.1%, so codes are not the nearest, which would stay where they
+// are while the value decays: a value goes to one of its two neighbours, drawn so that it is kept on average, and the kept v
+// is the unrounded one's on average after any number of steps, apart from it by about sqrt(2 / c) of itself (simulated over 7,000
+// steps: sqrt(v) off by 4% at c = 200, 20% at 25; nearest codes 1.37 and 17 times too large there).  Codes of v are 1 at
+// least where v > 0: a sqrt(v) rounded to nothing would leave m / eps.  The update itself takes the moments before they are
+// put into 8 bits.
+// Nearest codes (in their root) are there for callers that want no noise.  A value next to a border between two of them must not
+// depend on how its sums are rounded, so moments are computed in 64 bits, which this chip does as fast as unpacked 32, and so
+// are these codes where fp32 cannot tell.  A block with an infinity or a NaN in m or v has
 // the scale NaN; one whose largest |m| is below 2^-100 (v: 2^-126) the scale 0.
 #include "gl_common.h"
 #include "gl_internal.h"
@@ -29,8 +34,11 @@ struct AdamK {
 // The tensors of a launch travel as kernel arguments: nothing to copy to the device, nothing to keep alive.
 constexpr int ADAM_TENSORS = 38;      // of a launch: in the 4 KB that arguments may take
 constexpr int ADAM_BLOCK = 256;       // elements that share a scale
+// the kernels' kinds of moments: GL_DTYPE_F32, GL_DTYPE_BF16, GL_MOMENTS_INT8, and that with nearest codes
+constexpr int MOMENTS_INT8_NEAREST = 3;
+constexpr bool in_8bit(int moments) { return moments == GL_MOMENTS_INT8 || moments == MOMENTS_INT8_NEAREST; }
 // elements of a workgroup: a vector of 4 a thread, or two with 8-bit moments
-constexpr int adam_chunk(int moments) { return moments == GL_MOMENTS_INT8 ? 2048 : 1024; }
+constexpr int adam_chunk(int moments) { return in_8bit(moments) ? 2048 : 1024; }
 struct AdamTensorK {
   void* p;
   void* g;
@@ -135,24 +143,23 @@ __device__ __forceinline__ void adam_store_codes(void* p, unsigned i, int n, uns
 // stochastic rounding (optim.py:59-62).
 enum { PM_F32 = 0, PM_BF16_RNE = 1, PM_BF16_MASTER = 2, PM_BF16_SR = 3 };
 
-// Triton's tl.randint(seed, offset) (triton/language/random.py, 3.6): Philox-4x32-10 (Salmon et
-// al., SC'11) of the counter (offset low, offset high, 0, 0) under the key (seed low, seed high),
-// first output word.
-__device__ __forceinline__ unsigned philox_randint(unsigned long long seed, unsigned long long off) {
-  unsigned c0 = (unsigned)off, c1 = (unsigned)(off >> 32), c2 = 0u, c3 = 0u;
-  unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+// Philox-4x32 (Salmon et al., SC'11) of the counter c under the key (k0, k1)
+template <int ROUNDS>
+__device__ __forceinline__ uv4 philox(uv4 c, unsigned k0, unsigned k1) {
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const unsigned h0 = __umulhi(0xD2511F53u, c0), l0 = 0xD2511F53u * c0;
-    const unsigned h1 = __umulhi(0xCD9E8D57u, c2), l1 = 0xCD9E8D57u * c2;
-    c0 = h1 ^ c1 ^ k0;
-    c2 = h0 ^ c3 ^ k1;
-    c1 = l1;
-    c3 = l0;
+  for (int r = 0; r < ROUNDS; ++r) {
+    const unsigned h0 = __umulhi(0xD2511F53u, c[0]), l0 = 0xD2511F53u * c[0];
+    const unsigned h1 = __umulhi(0xCD9E8D57u, c[2]), l1 = 0xCD9E8D57u * c[2];
+    c = uv4{h1 ^ c[1] ^ k0, l1, h0 ^ c[3] ^ k1, l0};
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return c0;
+  return c;
+}
+// Triton's tl.randint(seed, offset) (triton/language/random.py, 3.6): the first word of Philox-4x32-10 of the counter
+// (offset low, offset high, 0, 0) under the key (seed low, seed high).
+__device__ __forceinline__ unsigned philox_randint(unsigned long long seed, unsigned long long off) {
+  return philox<10>(uv4{(unsigned)off, (unsigned)(off >> 32), 0u, 0u}, (unsigned)seed, (unsigned)(seed >> 32))[0];
 }
 
 // the bf16 parameter of element i from its fp32 update p
@@ -212,6 +219,33 @@ __device__ __forceinline__ unsigned code_v(double y) {
   const double h2 = (double)(h * h);
   return (unsigned)i + (y >= h2 * h2 ? 1u : 0u);
 }
+// Noise of the codes of four neighbours, 16 bits for each m and 16 above them for each v.  It is a hash of what the step has in
+// hand: the elements' place, their parameters and new moments, and the step's corrections; nothing is kept for it, and a
+// replayed graph, whose arguments are those of its capture, draws anew from the moments.  Seven rounds are the fewest that pass
+// Philox's authors' tests.
+__device__ __forceinline__ uv4 code_noise(unsigned long long vec, const float (&p)[4], const float (&m)[4], const float (&v)[4],
+                                          float k0, float k1) {
+  auto hash = [](const float (&x)[4]) {
+    unsigned h = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h = h * 0x9E3779B1u + __float_as_uint(x[j]);
+    return h;
+  };
+  return philox<7>(uv4{(unsigned)vec, (unsigned)(vec >> 32) ^ hash(p), hash(m), hash(v)}, __float_as_uint(k0), __float_as_uint(k1));
+}
+// Codes of |m| and v over the scale (over its square): the lower neighbour or, with the probability that keeps the value on
+// average, the upper one; `noise` is one of 2^16 equal shares.  (Where fp32 puts a quotient next to a code on its other side, the
+// code is still the neighbour that is taken nearly always.)
+__device__ __forceinline__ unsigned drawn_m(float q, unsigned noise) {
+  const float i = __builtin_fminf(__builtin_floorf(__builtin_amdgcn_sqrtf(q)), 126.f);
+  const float u = __builtin_fmaf((float)noise, 0x1p-16f, 0x1p-17f);
+  return (unsigned)i + (__builtin_fmaf(-i, i, q) > u * (2.f * i + 1.f) ? 1u : 0u);
+}
+__device__ __forceinline__ unsigned drawn_v(float q, unsigned noise) {
+  const float i = __builtin_fminf(__builtin_floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(q))), 254.f), i2 = i * i;
+  const float u = __builtin_fmaf((float)noise, 0x1p-16f, 0x1p-17f), t = 2.f * i + 1.f;
+  return (unsigned)i + (__builtin_fmaf(-i2, i2, q) > u * (t * (2.f * i2 + t)) ? 1u : 0u);  // t (2 i^2 + t) = (i + 1)^4 - i^4
+}
 __device__ __forceinline__ unsigned low_bytes(const unsigned (&c)[4]) {
   return __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u) | __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
 }
@@ -233,15 +267,15 @@ __device__ __forceinline__ int adam_tensor(const AdamTable& a) {
   return t;
 }
 
-// MOM: GL_DTYPE_F32, GL_DTYPE_BF16 or GL_MOMENTS_INT8; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
+// MOM: the kind of moments; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
 // thread a vector of each stream, or two with 8-bit moments: a block is half a wave's then, and what is done for a block (its
 // maxima and scales) is done for two at once.  150M bf16 parameters and gradients: 305 us (4.9 TB/s; bound by instructions,
 // 246 us at the rate of the fp32 stream), 352 with a block a wave (319 then).  400M fp32 in all types: 2.2 ms (5.7 TB/s).
 // WHOLE: all of the wave's elements are there (no lane's ends are looked at).
-constexpr int adam_vectors(int mom) { return mom == GL_MOMENTS_INT8 ? 2 : 1; }
+constexpr int adam_vectors(int mom) { return in_8bit(mom) ? 2 : 1; }
 template <int MOM, int PM, bool GBF, bool WHOLE>
 __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensorK& t, long long base) {
-  constexpr bool I8 = MOM == GL_MOMENTS_INT8, BM = MOM == GL_DTYPE_BF16;
+  constexpr bool I8 = in_8bit(MOM), BM = MOM == GL_DTYPE_BF16;
   constexpr int V = adam_vectors(MOM);
   const AdamK c{a.lr, a.b1, a.b2, a.eps, a.wd, t.bc1, t.bc2};
   constexpr int PB = PM == PM_BF16_RNE || PM == PM_BF16_SR ? 2 : 4, MB = I8 ? 1 : (BM ? 2 : 4);
@@ -296,25 +330,44 @@ __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensor
     const bool live_m = fs > 0.f, live_v = fr > 0.f;
     const float im = __builtin_amdgcn_rcpf(live_m ? fs : 1.f), ir = __builtin_amdgcn_rcpf(live_v ? fr : 1.f);
     unsigned om[V][4], ov[V][4];
-    float near = 0.f, rv[V][4];
+    float rv[V][4];  // sqrt(v) over its scale
 #pragma unroll
     for (int x = 0; x < V; ++x)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        om[x][j] = code_of(__builtin_copysignf(__builtin_amdgcn_sqrtf(__builtin_fabsf(m[x][j]) * im), m[x][j]), near);
-        rv[x][j] = __builtin_amdgcn_sqrtf(v[x][j] * ir * ir);
-        ov[x][j] = code_of(__builtin_fmaxf(__builtin_amdgcn_sqrtf(rv[x][j]), dv[x][j] > 0.0 ? 0.75f : 0.f), near);
+      for (int j = 0; j < 4; ++j) rv[x][j] = __builtin_amdgcn_sqrtf(v[x][j] * ir * ir);
+    if constexpr (MOM == GL_MOMENTS_INT8) {
+      const double dim = reciprocal(live_m ? fs : 1.f), dir = reciprocal(live_v ? fr : 1.f), dir2 = dir * dir;
+#pragma unroll
+      for (int x = 0; x < V; ++x) {
+        const uv4 noise = code_noise((unsigned long long)(t.first + base + i[x]) >> 2, p[x], m[x], v[x], c.bc1, c.bc2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned q = drawn_m((float)(__builtin_fabs(dm[x][j]) * dim), noise[j] & 0xffffu);
+          const unsigned u = drawn_v((float)(dv[x][j] * dir2), noise[j] >> 16);
+          om[x][j] = dm[x][j] < 0.0 ? 0u - q : q;
+          ov[x][j] = u == 0 && dv[x][j] > 0.0 ? 1u : u;
+        }
       }
-    if (__builtin_amdgcn_ballot_w64(near > 0.5f - CODE_NEAR)) {
-      const double dim = reciprocal(live_m ? fs : 1.f), dir = reciprocal(live_v ? fr : 1.f);
+    } else {
+      float near = 0.f;
 #pragma unroll
       for (int x = 0; x < V; ++x)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const unsigned q = live_m ? code_m(__builtin_fabs(dm[x][j]) * dim) : 0u, u = live_v ? code_v(dv[x][j] * dir * dir) : 0u;
-          om[x][j] = dm[x][j] < 0.0 ? 0u - q : q;
-          ov[x][j] = u == 0 && dv[x][j] > 0.0 ? 1u : u;
+          om[x][j] = code_of(__builtin_copysignf(__builtin_amdgcn_sqrtf(__builtin_fabsf(m[x][j]) * im), m[x][j]), near);
+          ov[x][j] = code_of(__builtin_fmaxf(__builtin_amdgcn_sqrtf(rv[x][j]), dv[x][j] > 0.0 ? 0.75f : 0.f), near);
         }
+      if (__builtin_amdgcn_ballot_w64(near > 0.5f - CODE_NEAR)) {
+        const double dim = reciprocal(live_m ? fs : 1.f), dir = reciprocal(live_v ? fr : 1.f);
+#pragma unroll
+        for (int x = 0; x < V; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const unsigned q = live_m ? code_m(__builtin_fabs(dm[x][j]) * dim) : 0u, u = live_v ? code_v(dv[x][j] * dir * dir) : 0u;
+            om[x][j] = dm[x][j] < 0.0 ? 0u - q : q;
+            ov[x][j] = u == 0 && dv[x][j] > 0.0 ? 1u : u;
+          }
+      }
     }
 #pragma unroll
     for (int x = 0; x < V; ++x) {
@@ -422,6 +475,7 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
   k.b2d = a->beta2_64;
   k.a2d = 1.0 - a->beta2_64;
   constexpr long long MAX_GROUPS = 1LL << 23;  // of a launch: fewer than 2^32 threads
+  const bool i8 = a->moments_dtype == GL_MOMENTS_INT8;
   const int chunk = adam_chunk(a->moments_dtype);
   int next = 0;
   long long done = 0;  // of the next tensor, which takes several launches where it has more chunks than one takes
@@ -436,7 +490,6 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
         k.first[k.count++] = (unsigned)groups;
         const auto at = [&](void* p, int bytes) { return (void*)((char*)p + done * bytes); };
         const int pe = values || a->p_dtype == GL_DTYPE_F32 ? 4 : 2, ge = values || a->g_dtype == GL_DTYPE_F32 ? 4 : 2;
-        const bool i8 = a->moments_dtype == GL_MOMENTS_INT8;
         const int me = i8 ? 1 : a->moments_dtype == GL_DTYPE_F32 ? 4 : 2;
         d = AdamTensorK{at(t.p, pe), at(t.g, ge), at(t.m, me), at(t.v, me), t.master ? t.master + done : nullptr,
                         i8 ? t.m_scale + done / ADAM_BLOCK : nullptr, i8 ? t.v_scale + done / ADAM_BLOCK : nullptr, n, done,
@@ -460,6 +513,7 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
       const bool gbf = a->g_dtype == GL_DTYPE_BF16;
       if (a->moments_dtype == GL_DTYPE_F32) launch_adam_of<GL_DTYPE_F32>(pm, gbf, grid, s, k);
       else if (a->moments_dtype == GL_DTYPE_BF16) launch_adam_of<GL_DTYPE_BF16>(pm, gbf, grid, s, k);
+      else if (a->nearest_codes) launch_adam_of<MOMENTS_INT8_NEAREST>(pm, gbf, grid, s, k);
       else launch_adam_of<GL_MOMENTS_INT8>(pm, gbf, grid, s, k);
     }
     GL_CHECK_LAUNCH();

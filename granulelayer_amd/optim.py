@@ -12,8 +12,12 @@ counterpart in the reference): blocks of 256 neighbouring elements of a tensor s
     m = s c |c|       c from -127 to 127    s = max |m| / 127^2
     v = (r c^2)^2     c from 0 to 255       r = sqrt(max v) / 255^2
 
-with c the nearest by its root and 1 at least where v > 0.  A step takes the new moments before they are put
-into 8 bits; a block with an infinity or a NaN in its moments is NaN from then on.  The state of a parameter has codes
+with c one of a value's two neighbours, drawn so that it is kept on average, and 1 at least where v > 0: a step takes
+1 - b2 off v, less than codes are apart, so the nearest one would stay where it is.  The draw is a hash of the element's place,
+parameter, moments and step: equal runs are equal.  ``stochastic_rounding=False`` takes the nearest all the same: sqrt(v) is
+then 1.1 of itself after 2,000 steps of like gradients and b2 = 0.999, and many times too large a few thousand steps after
+gradients got small.  A step takes the new moments before they are put into 8 bits; a block with an infinity or a NaN
+in its moments is NaN from then on.  The state of a parameter has codes
 ``m`` (int8) and ``v`` (uint8) and scales ``m_scale`` and ``v_scale``; ``moment_values`` gives what they stand for.
 
 Parameters are fp32, or bf16 with the reference's three variants (optim.py:5-9, 52-62): an fp32 master copy
@@ -263,7 +267,8 @@ class FusedAdamW(torch.optim.Optimizer):
         self._seed += len(todo)
         for ((backend, dev, pdt, mdt, has_master), gdt, main), rows in calls.items():
             backend.adam_many(dev, rows, pdt, gdt, mdt, group["lr"], b1, b2, group["eps"], group["weight_decay"],
-                              stochastic=self.stochastic_rounding and pdt is bf16 and not has_master, clear=main)
+                              stochastic=self.stochastic_rounding and pdt is bf16 and not has_master, clear=main,
+                              nearest_codes=not self.stochastic_rounding)
         for st in states:
             st["step"] += 1
         for p, _, _, main, *_ in todo:

@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define GL_ABI_VERSION 15
+#define GL_ABI_VERSION 16
 
 enum {
   GL_OK = 0,
@@ -197,6 +197,7 @@ typedef struct GlAdamArgs {
   int32_t g_dtype;        /* their gradients: GL_DTYPE_F32 | GL_DTYPE_BF16 */
   int32_t keep_g;         /* 1: which are not zeroed (as bf16 ones never are) */
   double beta1_64, beta2_64; /* for GL_MOMENTS_INT8, in place of beta1, beta2 */
+  int32_t nearest_codes;  /* for GL_MOMENTS_INT8: 1 = the nearest codes, 0 = drawn */
 } GlAdamArgs;
 
 /* One of many tensors (no counterpart in the reference, which launches a kernel a tensor).  A launch takes 38 of them,
@@ -204,7 +205,9 @@ typedef struct GlAdamArgs {
  * needs more than its element's alignment.  Moments of GL_MOMENTS_INT8 are codes of one byte, m's signed, with two fp32
  * scales for every 256 neighbouring elements (the last block of a tensor may be shorter):
  *   m = m_scale c |c|,  m_scale = max |m| / 127^2;   v = (v_scale c^2)^2,  v_scale = sqrt(max v) / 255^2
- * with the maxima rounded to fp32, c the nearest by its root, 1 at least where v > 0. */
+ * with the maxima rounded to fp32, and c one of the value's two neighbours, drawn so that it is kept on average, 1 at least where
+ * v > 0.  The draw is a hash of the element's place in the tensor, parameters, moments and corrections: equal calls give equal codes.
+ * With GlAdamArgs.nearest_codes it is the nearest by its root; a moment that a step changes by less than half a code then stays. */
 #define GL_MOMENTS_INT8 2
 #define GL_ADAM_MAX_ELEMENTS (1LL << 35) /* of a tensor */
 struct GlAdamTensor {
