@@ -32,6 +32,7 @@ from __future__ import annotations
 
 from operator import le
 from typing import Iterable, List, Tuple
+from weakref import ref
 
 import torch
 
@@ -42,14 +43,16 @@ _TYPES = (torch.float32, torch.bfloat16)
 _BLOCK = 256  # elements of a tensor that share the scales of 8-bit moments
 
 
-_NONE = (0, 0, 0)
+_EXTRA = ("master", "m_scale", "v_scale")  # what the state of some kinds has beside m and v
 
 
-def _addresses(of):
-    """Of a state's tensors (m, v, master, m_scale, v_scale): those of the last three."""
-    if of[2] is None and of[3] is None:
-        return _NONE
-    return tuple(0 if t is None else t.data_ptr() for t in of[2:])
+def _as_known(st, refs, at) -> bool:
+    """Whether a state's further tensors are those of the references, and where they were."""
+    for key, ref, a in zip(_EXTRA, refs, at):
+        t = st.get(key)
+        if (t is not None) if ref is None else (t is None or t is not ref() or t.data_ptr() != a):
+            return False
+    return True
 
 
 def _disjoint(starts, ends) -> bool:
@@ -167,18 +170,20 @@ class FusedAdamW(torch.optim.Optimizer):
         return m.dtype
 
     def _known_state(self, p, st):
-        """What a step needs of a parameter's state, checked: held for the next step, which looks whether the tensors
-        are still these and where they were."""
+        """What a step needs of a parameter's state, checked: addresses for the next step, which looks whether the tensors
+        are still these and where they were (nothing is kept alive for that)."""
         if not st:
             st.update(self._new_state(p))
         mdt = self._check_state(p, st)
         backend = backend_for(p.device)
-        of = (st["m"], st["v"], st.get("master"), st.get("m_scale"), st.get("v_scale"))
-        rest = _addresses(of)
-        kind = (backend, p.device, p.dtype, mdt, of[2] is not None)
+        extra = [st.get(key) for key in _EXTRA]
+        kind = (backend, p.device, p.dtype, mdt, extra[0] is not None)
         kind = self._kinds.setdefault(kind, kind)
-        known = (of, of[0].data_ptr(), of[1].data_ptr(), rest, p.numel(), p.dtype, p.get_device(), kind)
-        self._known[id(p)] = (p, known)  # (p is held, so that its id is its own)
+        known = (ref(p), ref(st["m"]), ref(st["v"]), st["m"].data_ptr(), st["v"].data_ptr(),
+                 tuple(0 if t is None else t.data_ptr() for t in extra),
+                 tuple(None if t is None else ref(t) for t in extra) if any(t is not None for t in extra) else None,
+                 p.numel(), p.dtype, p.get_device(), kind)
+        self._known[id(p)] = known
         return known
 
     @staticmethod
@@ -246,20 +251,21 @@ class FusedAdamW(torch.optim.Optimizer):
         for p, g, gdt, main, at, g_at, n, pdt, seed in todo:
             st = state[p]
             known = known_of.get(id(p))
-            known = None if known is None else known[1]
-            if (known is None or not st or st["m"] is not known[0][0] or st["v"] is not known[0][1]
-                    or st.get("master") is not known[0][2] or st.get("m_scale") is not known[0][3]
-                    or st.get("v_scale") is not known[0][4] or known[0][0].data_ptr() != known[1]
-                    or known[0][1].data_ptr() != known[2] or n != known[4] or pdt is not known[5]
-                    or p.get_device() != known[6] or known[3] is not _NONE and known[3] != _addresses(known[0])):
+            if known is None or known[0]() is not p or not st:
                 known = self._known_state(p, st)
-            _, m, v, rest, _, _, _, kind = known
+            _, m_ref, v_ref, m_at, v_at, rest, extra, size, dtype, device, kind = known
+            m, v = st["m"], st["v"]
+            if (m_ref() is not m or v_ref() is not v or m.data_ptr() != m_at or v.data_ptr() != v_at
+                    or n != size or pdt is not dtype or p.get_device() != device
+                    or (("master" in st or "m_scale" in st or "v_scale" in st) if extra is None
+                        else not _as_known(st, extra, rest))):
+                _, _, _, m_at, v_at, rest, _, _, _, _, kind = self._known_state(p, st)
             t = st["step"] + 1
             c = corrections.get(t)
             if c is None:
                 c = corrections[t] = (1 - b1 ** t, 1 - b2 ** t)
             states.append(st)
-            row = _ROW(at, g_at, m, v, *rest, n, seed & 0xffffffffffffffff, *c)
+            row = _ROW(at, g_at, m_at, v_at, *rest, n, seed & 0xffffffffffffffff, *c)
             if kind is not last[0] or gdt is not last[1] or main is not last[2]:
                 last = (kind, gdt, main)
                 rows = calls.setdefault(last, [])
