@@ -164,7 +164,7 @@ struct JoinK {
   float* loss;  // by row, or the result
 };
 // A row's statistics and loss, by a wave: every lane joins its tiles, then the lanes.  The loss is NaN where the target is no
-// class.
+// class, or a logit is +inf (infinity less infinity).
 struct Row {
   float top, sum, loss;
 };
@@ -178,8 +178,10 @@ __device__ __forceinline__ Row join_row(const JoinK& a, long long m, long long t
   }
   const float up = wave_max(top), ref = up == -__builtin_inff() ? 0.f : up;
   s = wave_add(s * __builtin_amdgcn_exp2f(top - ref));
-  if (t < 0 || t >= a.N) return Row{up, s, __builtin_nanf("")};
+  const float nan = __builtin_nanf("");
+  if (t < 0 || t >= a.N) return Row{up, s, nan};
   const float z = a.target_logit[m], q = s * __builtin_amdgcn_exp2f(up - z);
+  if (z == __builtin_inff()) return Row{z, nan, nan};  // (the others' sum has seen every +inf but the target's)
   const Row r = z >= up ? Row{z, 1.f + q, 0.f} : Row{up, s + __builtin_amdgcn_exp2f(z - up), 0.f};
   return Row{r.top, r.sum, q > 1e6f ? (up - z + log2f(r.sum)) * LN2 : log1pf(q)};
 }
