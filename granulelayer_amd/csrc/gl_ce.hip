@@ -362,7 +362,8 @@ long long piece_of(long long M, int N, int dtype, size_t budget) {
   const long long most = (long long)((budget ? budget : CE_PIECE) / ((size_t)M * es_of(dtype)));
   if (most >= N) return N;
   const long long pieces = (N + (most > 256 ? most : 256) - 1) / (most > 256 ? most : 256);
-  return round_up((N + pieces - 1) / pieces, 256);
+  const long long even = round_up((N + pieces - 1) / pieces, 256);
+  return even < N ? even : N;
 }
 // Classes whose exponentials are kept: the first piece, unless the product that makes them again is short.
 int kept_classes(long long M, int N, int K, int dtype, size_t budget) {

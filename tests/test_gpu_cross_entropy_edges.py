@@ -1,10 +1,10 @@
-"""Cross entropy of a dense head on the GPU: logits that overflow."""
+"""Cross entropy of a dense head on the GPU: logits that overflow, budgets below the least piece."""
 import pytest
 import torch
 
 from conftest import gpu_available
 
-from test_gpu_cross_entropy import inputs, run
+from test_gpu_cross_entropy import compare, inputs, run
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a ROCm GPU")]
 DEV = "cuda"
@@ -54,3 +54,17 @@ def test_the_only_class(M):
         t["b"][0] = b
         got = run(t, "none")[1]
         assert torch.isnan(got["loss"]).all() and torch.isnan(got["dx"]).all()
+
+
+@pytest.mark.parametrize("K", [48, 520])
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("M", [100, 700])
+@pytest.mark.parametrize("N", [5, 100, 255, 256, 300])
+def test_a_budget_of_less_than_the_least_piece(N, M, dtype, K):
+    """Fewer classes than a piece has at least, and a budget of fewer still."""
+    t = inputs(M, K, N, dtype)
+    whole = compare(t, "mean")
+    for budget in (1, M * (N // 2)):
+        got = compare(t, "mean", budget=budget)
+        if N <= 256:  # the same single piece
+            assert all(torch.equal(got[k], whole[k]) for k in whole)
