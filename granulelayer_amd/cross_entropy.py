@@ -105,7 +105,8 @@ def dense_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Ten
     count.  Rows with ``ignore_index`` have the loss 0 and no gradient, whatever x holds there; a mean of no rows is 0.
     Any other target that is no class makes the loss NaN.  A class whose bias is -inf takes no part.  The backward's
     pieces of gradients at the logits take up to ``workspace_budget`` bytes (4 GiB by default; of 256 classes at
-    least), from the forward on where that keeps exponentials for it (from 512 bfloat16 or 64 float32 features on).  It
+    least), from the forward on where that keeps exponentials for it (from 512 bfloat16 or 64 float32 features on; with 4 bytes
+    for every 64 of them).  It
     takes the operands as they were: none of them may change before it."""
     _check(x, weight, target, bias, reduction, workspace_budget)
     N, K = weight.shape

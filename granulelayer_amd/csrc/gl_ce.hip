@@ -357,11 +357,11 @@ struct Layout {
   }
 };
 
-// Classes of a piece: pieces of one size, in columns of the widest tiles, whose dz fits the budget.
+// Classes of a piece: pieces of one size, in columns of the widest tiles, whose dz fits the budget (256 at least).
 long long piece_of(long long M, int N, int dtype, size_t budget) {
-  const long long most = (long long)((budget ? budget : CE_PIECE) / ((size_t)M * es_of(dtype)));
-  if (most >= N) return N;
-  const long long pieces = (N + (most > 256 ? most : 256) - 1) / (most > 256 ? most : 256);
+  const long long fit = (long long)((budget ? budget : CE_PIECE) / ((size_t)M * es_of(dtype)));
+  if (fit >= padded(N)) return N;
+  const long long most = fit < 256 ? 256 : fit / 256 * 256, pieces = (N + most - 1) / most;
   const long long even = round_up((N + pieces - 1) / pieces, 256);
   return even < N ? even : N;
 }

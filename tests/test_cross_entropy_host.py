@@ -91,3 +91,31 @@ def test_workspace_follows_the_budget():
     # pieces' gradients at the logits have the place of the kept exponentials
     assert need(M, V, 1 << 30, exps=4096) - rest <= 64 << 20
     assert need(M, V, 1) - rest <= 256 * M * 2 + (64 << 20)  # 256 classes at least (and their products' partial sums)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_pieces_stay_within_the_budget(dtype):
+    """A piece's place, given as that of the exponentials kept for it: rows of whole 8 columns, and 4 bytes of every 64."""
+    lib = N.library()
+    out = ctypes.c_size_t()
+    es = 4 >> dtype
+
+    def place(M, classes, budget):
+        a = N.GlCeArgs(X=4096, sx=1024, W=4096, sw=1024, target=4096, M=M, N=classes, K=1024, dtype=dtype, reduction=1,
+                       loss=4096, kept=4096, piece_bytes=budget)
+        assert lib.lib.gl_ce_exps_bytes(ctypes.byref(a), ctypes.byref(out)) == 0
+        return out.value
+
+    def bytes_of(M, columns):
+        up = lambda n: -(-n // 256) * 256  # noqa: E731
+        return up(M * (-(-columns // 8) * 8) * es) + up(M * -(-columns // 64) * 4)
+
+    for M, classes in ((4096, 50000), (777, 12553), (1, 300), (129, 257), (6_000_000, 50000)):
+        for columns in (1, 100, 255, 256, 257, 300, 511, 513, 1000, 12552, 12553, 12559, 12560, 30000, 49999, 50000):
+            got = place(M, classes, M * es * columns)
+            assert got <= max(bytes_of(M, columns // 8 * 8), bytes_of(M, 256)), (M, classes, columns)
+            if columns >= -(-classes // 8) * 8:
+                assert got == bytes_of(M, classes)
+        for budget in (0, 1 << 20, (1 << 30) + 12345):
+            most = (budget or 4 << 30) // (M * es)
+            assert place(M, classes, budget) <= max(bytes_of(M, most // 8 * 8), bytes_of(M, 256))
