@@ -417,8 +417,9 @@ __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensor
     }
   }
 }
+constexpr int STEP_THREADS = 256;
 template <int MOM, int PM, bool GBF>
-__global__ void __launch_bounds__(256) adam_kernel(AdamTable a) {
+__global__ void __launch_bounds__(STEP_THREADS) adam_kernel(AdamTable a) {
   constexpr int WAVE = 256 * adam_vectors(MOM);  // elements of a wave
   const int ti = adam_tensor(a);
   const AdamTensorK& t = a.t[ti];
@@ -428,7 +429,8 @@ __global__ void __launch_bounds__(256) adam_kernel(AdamTable a) {
 }
 
 // The fp32 values of 8-bit moments (into g: m's, into p: v's), a vector a thread.  150M: 237 us, 6.3 TB/s.
-__global__ void __launch_bounds__(512) adam_values_kernel(AdamTable a) {
+constexpr int VALUES_THREADS = 512;
+__global__ void __launch_bounds__(VALUES_THREADS) adam_values_kernel(AdamTable a) {
   const int ti = adam_tensor(a);
   const AdamTensorK& t = a.t[ti];
   const long long block = (long long)(blockIdx.x - a.first[ti]) * adam_chunk(GL_MOMENTS_INT8) + wave_uniform(threadIdx.x >> 6) * ADAM_BLOCK;
@@ -450,8 +452,8 @@ __global__ void __launch_bounds__(512) adam_values_kernel(AdamTable a) {
 
 template <int MOM, int PM>
 void launch_adam_as(bool gbf, dim3 grid, hipStream_t s, const AdamTable& a) {
-  if (gbf) GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<MOM, PM, true>), grid, dim3(256), 0, s, a);
-  else GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<MOM, PM, false>), grid, dim3(256), 0, s, a);
+  if (gbf) GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<MOM, PM, true>), grid, dim3(STEP_THREADS), 0, s, a);
+  else GL_LAUNCH(GL_KERNEL_ADAM, (adam_kernel<MOM, PM, false>), grid, dim3(STEP_THREADS), 0, s, a);
 }
 template <int MOM>
 void launch_adam_of(int pm, bool gbf, dim3 grid, hipStream_t s, const AdamTable& a) {
@@ -474,7 +476,8 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
   k.a1d = 1.0 - a->beta1_64;
   k.b2d = a->beta2_64;
   k.a2d = 1.0 - a->beta2_64;
-  constexpr long long MAX_GROUPS = 1LL << 23;  // of a launch: fewer than 2^32 threads
+  // workgroups of a launch: 2^31 threads, of the 2^32 - 1 that one may have
+  const long long most = (1LL << 31) / (values ? VALUES_THREADS : STEP_THREADS);
   const bool i8 = a->moments_dtype == GL_MOMENTS_INT8;
   const int chunk = adam_chunk(a->moments_dtype);
   int next = 0;
@@ -482,9 +485,9 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
   while (next < count) {
     long long groups = 0;
     k.count = 0;
-    while (next < count && k.count < ADAM_TENSORS && groups < MAX_GROUPS) {
+    while (next < count && k.count < ADAM_TENSORS && groups < most) {
       const GlAdamTensor& t = tensors[next];
-      const long long left = t.n - done, room = (MAX_GROUPS - groups) * chunk, n = left < room ? left : room;
+      const long long left = t.n - done, room = (most - groups) * chunk, n = left < room ? left : room;
       if (n > 0) {
         AdamTensorK& d = k.t[k.count];
         k.first[k.count++] = (unsigned)groups;
@@ -507,7 +510,7 @@ int launch_adam(const GlAdamArgs* a, const GlAdamTensor* tensors, int count, boo
     k.first[k.count] = (unsigned)groups;
     const dim3 grid((unsigned)groups);
     if (values) {
-      GL_LAUNCH(GL_KERNEL_ADAM_VALUES, adam_values_kernel, grid, dim3(512), 0, s, k);
+      GL_LAUNCH(GL_KERNEL_ADAM_VALUES, adam_values_kernel, grid, dim3(VALUES_THREADS), 0, s, k);
     } else {
       const int pm = a->p_dtype == GL_DTYPE_F32 ? PM_F32 : (k.t[0].master ? PM_BF16_MASTER : (a->stochastic ? PM_BF16_SR : PM_BF16_RNE));
       const bool gbf = a->g_dtype == GL_DTYPE_BF16;

@@ -9,6 +9,7 @@ import torch
 from conftest import gpu_available
 
 from granulelayer_amd import FusedAdamW
+from granulelayer_amd.backend import HipBackend, adam_row
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a ROCm GPU")]
 DEV = "cuda"
@@ -177,3 +178,24 @@ def test_like_gradients_keep_their_moments():
     v32, _, v8, ways = _follow([(torch.ones(n, device=DEV), 3000, False)], n)
     assert abs(float(v8.mean() / v32.mean()) - 1) < 0.0226
     assert float((ways[1] - ways[0]).norm() / ways[0].norm()) < 0.2
+
+
+def test_values_of_more_elements_than_a_launch_takes():
+    """2^34 elements, 2^32 threads in all: 32 rows of one tensor's codes, most of them into one place (each writes the same)."""
+    n = 1 << 29
+    codes = torch.arange(256, device=DEV, dtype=torch.int32)
+    m, v = codes.to(torch.int8).repeat(n // 256), codes.to(torch.uint8).repeat(n // 256)
+    scales = [torch.rand(n // 256, device=DEV) + 0.5 for _ in range(2)]
+    places = {i: [torch.zeros(n, device=DEV) for _ in range(2)] for i in (0, 15, 16, 31)}
+    rows = [adam_row(places.get(i, places[0])[1].data_ptr(), places.get(i, places[0])[0].data_ptr(), m.data_ptr(), v.data_ptr(), 0,
+                     scales[0].data_ptr(), scales[1].data_ptr(), n, 0, 1.0, 1.0) for i in range(32)]
+    HipBackend.get().adam_values(m.device, rows)
+    torch.cuda.synchronize()
+    for k in (0, 1, n // 512, n // 256 - 1):
+        part = slice(256 * k, 256 * k + 256)
+        cm, cv = m[part].double(), v[part].double()
+        wm, wv = (cm * cm.abs() * scales[0][k].double()).float(), (cv * cv * scales[1][k].double()).square().float()
+        for pm, pv in places.values():
+            assert torch.equal(pm[part], wm) and torch.equal(pv[part], wv)
+    for pm, pv in places.values():
+        assert torch.equal(pm, places[0][0]) and torch.equal(pv, places[0][1])
