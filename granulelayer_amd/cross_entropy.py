@@ -54,14 +54,17 @@ def _check(x, weight, target, bias, reduction, workspace_budget):
 
 class DenseCrossEntropyFunction(torch.autograd.Function):
     """x [M, K], target [M] -> the loss; keeps the operands, five words a row, and the first piece's exponentials where
-    they are worth it, which the first backward turns into its gradient in place."""
+    they are worth it, which the first backward turns into its gradient in place.  All of them are saved tensors: activation
+    checkpointing and hooks on saved tensors have them."""
 
     @staticmethod
     def forward(ctx, x, w, b, target, reduction, ignore_index, budget):
         be = backend_for(x.device)
-        loss, kept, ctx.exps = be.ce_forward(x, w, b, target, reduction, ignore_index, True, budget)
-        ctx.capture = be.capture_id(x.device) if ctx.exps is not None else 0
-        ctx.save_for_backward(x, w, b, target, kept)
+        loss, kept, exps = be.ce_forward(x, w, b, target, reduction, ignore_index, True, budget)
+        ctx.capture = be.capture_id(x.device) if exps is not None else 0
+        ctx.place = 0 if exps is None else exps.data_ptr()
+        ctx.used_up = False
+        ctx.save_for_backward(x, w, b, target, kept, exps)
         ctx.reduction, ctx.ignore_index, ctx.budget = reduction, ignore_index, budget
         return loss
 
@@ -72,7 +75,7 @@ class DenseCrossEntropyFunction(torch.autograd.Function):
 
 
 def _gradients(ctx, dloss):
-    x, w, b, target, kept = ctx.saved_tensors
+    x, w, b, target, kept, exps = ctx.saved_tensors
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
     mg_w, mg_b, use_main = _main_grads(w, b, need_w, need_b)
@@ -83,12 +86,15 @@ def _gradients(ctx, dloss):
         db = torch.empty_like(b, memory_format=torch.contiguous_format) if need_b else None
     be = backend_for(x.device)
     # Used up: a second backward of a retained graph makes them again, and so does one that a captured graph may replay
-    # without its forward.
-    exps, ctx.exps = ctx.exps, None
-    if exps is not None and be.capture_id(x.device) != ctx.capture:
+    # without its forward.  (A hook may have brought them to any address.)
+    used_up, ctx.used_up = ctx.used_up, True
+    own = exps if not used_up and exps is not None and exps.data_ptr() == ctx.place else None
+    if exps is not None and (used_up or be.capture_id(x.device) != ctx.capture or exps.data_ptr() % 256):
         exps = None
     be.ce_backward(dloss.resolve_neg(), x, w, b, target, ctx.reduction, ctx.ignore_index, kept, dx, dw, db, use_main,
                    ctx.budget, exps)
+    if own is not None and own.untyped_storage().nbytes() == own.numel():
+        own.untyped_storage().resize_(0)  # a retained graph need not hold what nothing reads again
     return dx, None if use_main else dw, None if use_main else db, None, None, None, None
 
 
