@@ -20,7 +20,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from .backend import backend_for
-from .dense import _main_grads
+from .dense import _main_grads, _through_function
 
 REDUCTIONS = ("none", "mean", "sum")
 
@@ -113,14 +113,14 @@ def dense_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Ten
     pieces of gradients at the logits take up to ``workspace_budget`` bytes (4 GiB by default; of 256 classes at
     least), from the forward on where that keeps exponentials for it (from 512 bfloat16 or 64 float32 features on; with 4 bytes
     for every 64 of them).  It
-    takes the operands as they were: none of them may change before it."""
+    takes the operands as they were: none of them may change before it.  Tangents of forward-mode differentiation are refused."""
     _check(x, weight, target, bias, reduction, workspace_budget)
     N, K = weight.shape
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     t = target.reshape(-1)
     t = (t if t.dtype == torch.int64 else t.long()).contiguous()
     budget = 0 if workspace_budget is None else workspace_budget
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if _through_function(x, weight, bias):
         loss = DenseCrossEntropyFunction.apply(x2, weight, bias, t, reduction, ignore_index, budget)
     else:
         loss = backend_for(x.device).ce_forward(x2, weight, bias, t, reduction, ignore_index, False)[0]

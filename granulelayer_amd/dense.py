@@ -21,6 +21,7 @@ from typing import Optional
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .activations8 import check_activation_checkpoint
@@ -55,6 +56,18 @@ def _check(x, weight, bias, residual, activation, activation_checkpoint):
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
         if t is not None and t.device != x.device:
             raise ValueError(f"{name} on {t.device} but x on {x.device}")
+
+
+def _through_function(*operands) -> bool:
+    """Whether a call goes through its autograd function: an operand needs its gradient, or may have a tangent of forward-mode
+    differentiation, which the function refuses."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _main_grads(w, b, need_w, need_b):
@@ -121,13 +134,13 @@ def dense_projection(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     x [..., K] and weight [N, K], both float32 or both bfloat16 (products and sums in fp32); bias [N] of
     their type; residual [..., N] float32 or bfloat16.  The result has x's type, or float32 with a
     float32 residual, and is rounded once.  Rows may be any stride apart.  The backward of bfloat16
-    operands rounds the gradient at the product to bfloat16 before the products for x and the weight."""
+    operands rounds the gradient at the product to bfloat16 before the products for x and the weight.  Tangents of
+    forward-mode differentiation are refused."""
     _check(x, weight, bias, residual, activation, activation_checkpoint)
     N, K = weight.shape
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(-1, N)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if _through_function(x, weight, bias, residual):
         y = DenseProjectionFunction.apply(x2, weight, bias, r2, activation, activation_checkpoint)
     else:
         y = backend_for(x.device).dense_forward(x2, weight, bias, r2, activation, "none")[0]

@@ -14,7 +14,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from .backend import backend_for
-from .dense import _main_grads
+from .dense import _main_grads, _through_function
 
 _DTYPES = (torch.float32, torch.bfloat16)
 
@@ -82,13 +82,13 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x [..., D] float32 or bfloat16, its rows any stride apart; weight and bias [D] of one of these types, or None.
     The result is of ``out_dtype`` (x's type by default).  A row with an infinity or a NaN is NaN, the others are
-    not touched by it; so are the gradients but for those of weight and bias, which sum over all rows."""
+    not touched by it; so are the gradients but for those of weight and bias, which sum over all rows.  Tangents of
+    forward-mode differentiation are refused."""
     out_dtype = x.dtype if out_dtype is None else out_dtype
     _check(x, weight, bias, eps, out_dtype)
     D = x.shape[-1]
     x2 = x if x.dim() == 2 else x.reshape(-1, D)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _through_function(x, weight, bias):
         y = LayerNormFunction.apply(x2, weight, bias, eps, out_dtype)
     else:
         y = backend_for(x.device).norm_forward(x2, weight, bias, eps, out_dtype, False)[0]
