@@ -1,12 +1,14 @@
-"""Softmax cross entropy of a dense head, without its logits: the loss of ``softmax(x W^T + b)`` against a class a row.
+"""Softmax cross entropy of a dense head, without a tensor of its logits: the loss of ``softmax(x W^T + b)`` against a class a row.
 
 The other end of a model around the sparse layer: its last projection goes onto a large number of classes (a
 vocabulary), whose logits would be the largest tensor of the step.  The forward is one product whose tiles leave their
 softmax statistics instead of logits; the backward makes the logits again, a piece of the classes at a time, and
-keeps their gradient only until two more products have taken it.  The forward of a training step may fill the first
-piece's place already, with exponentials that the backward turns into the gradient: one piece's memory in all.  Operands are those of ``dense_projection``, fp32 or
-bf16 with products, sums and statistics in fp32, and gradients go to ``main_grad`` where the parameters have it (no
-counterpart in the reference).
+keeps their gradient only until two more products have taken it.  The forward of a training step fills the first
+piece's place already where that saves time, with exponentials (of bf16 operands 2 bytes each, of fp32 ones 4) that the
+backward turns into the gradient: one piece's memory in all, held from the forward to the backward, for every loss that
+waits for its own.  ``workspace_budget`` bounds it; under activation checkpointing it is held in the backward alone.
+Operands are those of ``dense_projection``, fp32 or bf16 with products, sums and statistics in fp32, and gradients go to
+``main_grad`` where the parameters have it (no counterpart in the reference).
 
 With bf16 operands the gradient at the logits is rounded to bf16 before the products with the weight and with x, half a
 step, 2^-8, of each term at most; the bias' gradient sums it unrounded.
@@ -109,7 +111,8 @@ def dense_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Ten
     x [..., K] and weight [N, K], both float32 or both bfloat16 (their rows any stride apart); bias [N] of their
     type; target [...] int64 or int32.  ``reduction``: "none" (a loss a row), "sum", or "mean" over the rows that
     count.  Rows with ``ignore_index`` have the loss 0 and no gradient, whatever x holds there; a mean of no rows is 0.
-    Any other target that is no class makes the loss NaN.  A class whose bias is -inf takes no part.  The backward's
+    Any other target that is no class makes the loss NaN.  A class whose bias is -inf takes no part; logits past 2.3e38 in
+    size count as infinite.  The backward's
     pieces of gradients at the logits take up to ``workspace_budget`` bytes (4 GiB by default; of 256 classes at
     least), from the forward on where that keeps exponentials for it (from 512 bfloat16 or 64 float32 features on; with 4 bytes
     for every 64 of them).  It

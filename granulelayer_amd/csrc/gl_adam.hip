@@ -61,6 +61,8 @@ struct AdamTable {
 };
 static_assert(sizeof(AdamTable) <= 4096, "kernel arguments");
 
+// (1 - b1 and 1 - b2 of the fp32 betas, as the reference has them: 0.999 is off by 1.3e-8, 1 - 0.999 by 1.3e-5 of itself.  8-bit
+// moments take the betas in 64 bits.)
 __device__ __forceinline__ void adam_elem(const AdamK& c, float& p, float g, float& m, float& v) {
 #pragma clang fp contract(off)
   m = c.b1 * m + (1.0f - c.b1) * g;
@@ -269,8 +271,9 @@ __device__ __forceinline__ int adam_tensor(const AdamTable& a) {
 
 // MOM: the kind of moments; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
 // thread a vector of each stream, or two with 8-bit moments: a block is half a wave's then, and what is done for a block (its
-// maxima and scales) is done for two at once.  150M bf16 parameters and gradients: 305 us (4.9 TB/s; bound by instructions,
-// 246 us at the rate of the fp32 stream), 352 with a block a wave (319 then).  400M fp32 in all types: 2.2 ms (5.7 TB/s).
+// maxima and scales) is done for two at once.  150M bf16 parameters and gradients, nearest codes: 305 us (4.9 TB/s; bound by instructions,
+// 246 us at the rate of the fp32 stream), 352 with a block a wave (319 then); fp32 ones 393, drawn codes 432.  400M fp32 in all types:
+// 2.2 ms (5.7 TB/s).  Parameters rounded stochastically take a Philox-4x32-10 an element: bf16 moments 529 us, 345 rounded to nearest.
 // WHOLE: all of the wave's elements are there (no lane's ends are looked at).
 constexpr int adam_vectors(int mom) { return in_8bit(mom) ? 2 : 1; }
 template <int MOM, int PM, bool GBF, bool WHOLE>

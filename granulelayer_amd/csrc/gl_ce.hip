@@ -9,8 +9,8 @@
 // fp32 over the pieces, and to the piece's rows of dW.  8 M K N operations in all, 2 of them for what was not kept.
 //
 // The first piece's exponentials are kept where that takes less time than making them again: in the place of its
-// dz, so in memory that the backward takes anyway, over the largest of 64: of bf16 operands in 16 bits (exp_code: within 2^-11
-// of each, where rounding dz takes 2^-8), else as they are.  One pass then turns them into dz.
+// dz, so in memory that the backward takes anyway, but held from the forward on, over the largest of 64: of bf16 operands in 16 bits
+// (exp_code: within 2^-11 of each, and 2^-63, where rounding dz takes 2^-8), else as they are.  One pass then turns them into dz.
 //
 // Rows whose target is `ignore_index` count for nothing.  Of more than CE_ALL rows those that count are copied together first
 // (a row is read and written once, against N products with it), and the products take their number from device

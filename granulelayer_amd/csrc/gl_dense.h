@@ -506,8 +506,9 @@ __device__ __forceinline__ int n_pitch(const DenseRowsK& a) { return a.pitch; }
 __device__ __forceinline__ int n_pitch(const DenseK&) { return 0; }
 
 // An exponential, between 0 and 1, in 16 bits: of an fp32 number's the lower 6 of the exponent and the upper 10 of the
-// mantissa, to the nearest.  Within 2^-11 of itself from 1 down to 2^-62 (fp16 is so down to 2^-14 and has nothing below 2^-25,
-// and a class that is no target has its whole gradient from such), 0 from 0.  Of a NaN any code: its row's factor is NaN.
+// mantissa, to the nearest.  The value is off by up to 2^-11 of itself and by 2^-63 besides, which the code 0 stands for: 2^-11 relative
+// down to about 2^-48, 0 from 2^-63 (fp16 is so down to 2^-14 and has nothing below 2^-25, and a class that is no target has
+// its whole gradient from such), 0 from 0.  Of a NaN any code: its row's factor is NaN.
 __device__ __forceinline__ unsigned exp_code(float e) {
   return __builtin_elementwise_sub_sat((__float_as_uint(e) + 0x1000u) >> 13, 0x10000u) & 0xffffu;
 }

@@ -496,7 +496,8 @@ int gl_ce_exps_bytes(const GlCeArgs* a, size_t* bytes);
 int gl_ce_fwd(const GlCeArgs* a, void* stream);
 
 /* The backward, from the operands as they were and what the forward kept.  It goes through the classes in pieces
- * whose gradients at the logits take up to piece_bytes of the workspace, or of `exps` (0: 4 GiB; 256 classes at least).
+ * whose gradients at the logits take up to piece_bytes of the workspace, or of `exps` (0: 4 GiB; 256 classes at least; `exps` has 4
+ * bytes more for every 64 of them).
  * Gradients that are NULL are not computed. */
 typedef struct GlCeBwdArgs {
   const void* X;
