@@ -62,15 +62,15 @@ def _disjoint(starts, ends) -> bool:
 
 
 def _in_turn(todo):
-    """Of tensors to step of which some meet in memory: lists of those that may step at once.  A tensor comes after all
-    earlier ones that write what it touches, or touch what it writes."""
+    """Of tensors to step of which some meet in memory: lists of those that may step at once, with their numbers in the order
+    of all.  A tensor comes after all earlier ones that write what it touches, or touch what it writes."""
     kept, seen = [], set()
     for t in todo:
         if t[3] or id(t[0]) not in seen:  # (there twice: its first step uses up its .grad)
             seen.add(id(t[0]))
-            kept.append((*t[:-1], todo[0][-1] + len(kept)))
+            kept.append(t)
     spans = []
-    for k, (p, g, _, main, at, g_at, n, _, _) in enumerate(kept):
+    for k, (p, g, _, main, at, g_at, n, *_) in enumerate(kept):
         if n:
             spans.append((at, at + n * p.element_size(), k, True))
             spans.append((g_at, g_at + n * g.element_size(), k, main))
@@ -83,11 +83,12 @@ def _in_turn(todo):
                 meets[max(j, k)].append(min(j, k))
         (writers if written else readers).append((end, k))
     turns, turn = [], []
-    for t, earlier in zip(kept, meets):
+    for k, (t, earlier) in enumerate(zip(kept, meets)):
         turn.append(1 + max((turn[j] for j in earlier), default=-1))
         if turn[-1] == len(turns):
-            turns.append([])
-        turns[turn[-1]].append(t)
+            turns.append(([], []))
+        turns[turn[-1]][0].append(t)
+        turns[turn[-1]][1].append(k)
     return turns
 
 
@@ -179,7 +180,7 @@ class FusedAdamW(torch.optim.Optimizer):
         extra = [st.get(key) for key in _EXTRA]
         kind = (backend, p.device, p.dtype, mdt, extra[0] is not None)
         kind = self._kinds.setdefault(kind, kind)
-        known = (ref(p), ref(st["m"]), ref(st["v"]), st["m"].data_ptr(), st["v"].data_ptr(),
+        known = (ref(st["m"]), ref(st["v"]), st["m"].data_ptr(), st["v"].data_ptr(),
                  tuple(0 if t is None else t.data_ptr() for t in extra),
                  tuple(None if t is None else ref(t) for t in extra) if any(t is not None for t in extra) else None,
                  p.numel(), p.dtype, p.get_device(), kind)
@@ -214,7 +215,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _step_group(self, group):
         f32, bf16 = torch.float32, torch.bfloat16
-        todo, starts, ends, seed = [], [], [], self._seed
+        todo, starts, ends = [], [], []
         for p in group["params"]:  # everything is checked before anything changes
             g = getattr(p, "main_grad", None)
             main = g is not None
@@ -222,44 +223,43 @@ class FusedAdamW(torch.optim.Optimizer):
                 g = p.grad
                 if g is None:
                     continue
-            pdt, gdt, n = p.dtype, g.dtype, p.numel()
+            pdt, gdt, n, device = p.dtype, g.dtype, p.numel(), p.get_device()
             if (not (gdt is f32 or (gdt is bf16 and not main)) or not g.is_contiguous() or g.is_neg()
                     or not p.is_contiguous() or not (pdt is f32 or pdt is bf16)
-                    or g.numel() != n or g.get_device() != p.get_device()):
+                    or g.numel() != n or g.get_device() != device):
                 g = self._gradient(p, g, main)
                 gdt = g.dtype
             at, g_at = p.data_ptr(), g.data_ptr()
             if n:
                 starts += at, g_at
                 ends += at + n * (4 if pdt is f32 else 2), g_at + n * (4 if gdt is f32 else 2)
-            seed += 1
-            todo.append((p, g, gdt, main, at, g_at, n, pdt, seed))
-        turns = [todo] if _disjoint(starts, ends) else _in_turn(todo)
+            todo.append((p, g, gdt, main, at, g_at, n, pdt, device))
+        turns = [(todo, range(len(todo)))] if _disjoint(starts, ends) else _in_turn(todo)
         if len(turns) > 1:
             for t in todo:
                 if self.state.get(t[0]):
                     self._check_state(t[0], self.state[t[0]])
-        for turn in turns:
-            self._step_tensors(group, turn)
+        seed = self._seed + 1
+        for turn, numbers in turns:
+            self._step_tensors(group, turn, [seed + k for k in numbers])
 
-    def _step_tensors(self, group, todo):
+    def _step_tensors(self, group, todo, seeds):
         """A step of tensors of which none writes what another touches."""
         b1, b2 = group["betas"]
         bf16 = torch.bfloat16
         calls, states, corrections = {}, [], {}
         state, known_of, last = self.state, self._known, (None, None, None)
-        for p, g, gdt, main, at, g_at, n, pdt, seed in todo:
+        for (p, g, gdt, main, at, g_at, n, pdt, device), seed in zip(todo, seeds):
             st = state[p]
-            known = known_of.get(id(p))
-            if known is None or known[0]() is not p or not st:
+            known = known_of.get(id(p)) if st else None
+            if known is None:
                 known = self._known_state(p, st)
-            _, m_ref, v_ref, m_at, v_at, rest, extra, size, dtype, device, kind = known
+            m_ref, v_ref, m_at, v_at, rest, extra, size, dtype, on, kind = known
             m, v = st["m"], st["v"]
             if (m_ref() is not m or v_ref() is not v or m.data_ptr() != m_at or v.data_ptr() != v_at
-                    or n != size or pdt is not dtype or p.get_device() != device
-                    or (("master" in st or "m_scale" in st or "v_scale" in st) if extra is None
-                        else not _as_known(st, extra, rest))):
-                _, _, _, m_at, v_at, rest, _, _, _, _, kind = self._known_state(p, st)
+                    or n != size or pdt is not dtype or device != on
+                    or ("master" in st if extra is None else not _as_known(st, extra, rest))):
+                _, _, m_at, v_at, rest, *_, kind = self._known_state(p, st)
             t = st["step"] + 1
             c = corrections.get(t)
             if c is None:

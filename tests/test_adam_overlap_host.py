@@ -110,7 +110,7 @@ def test_turns_against_pairs_looked_at_one_by_one():
         for k in range(rng.randint(1, 9)):
             n, m = rng.choice([0, 1, 5, 20]), rng.random() < 0.5
             p, g = torch.empty(n, device="meta"), torch.empty(n, device="meta")
-            todo.append((p, g, torch.float32, m, rng.randint(0, 150), rng.randint(1000, 1100), n, p.dtype, k + 1))
+            todo.append((p, g, torch.float32, m, rng.randint(0, 150), rng.randint(1000, 1100), n, p.dtype, -1))
         spans = [[(t[4], t[4] + 4 * t[0].numel(), True), (t[5], t[5] + 4 * t[0].numel(), t[3])] if t[0].numel() else []
                  for t in todo]
 
@@ -118,8 +118,9 @@ def test_turns_against_pairs_looked_at_one_by_one():
             return any(x < f and e < y and (w or v) for x, y, w in spans[a] for e, f, v in spans[b])
 
         turns = optim._in_turn(todo)
-        of = {id(t[0]): i for i, turn in enumerate(turns) for t in turn}
-        assert sorted(t[-1] for turn in turns for t in turn) == list(range(1, len(todo) + 1))
+        of = {id(t[0]): i for i, (turn, _) in enumerate(turns) for t in turn}
+        assert all(todo[k] is t for turn, numbers in turns for t, k in zip(turn, numbers))
+        assert sorted(k for _, numbers in turns for k in numbers) == list(range(len(todo)))
         for b in range(len(todo)):
             earlier = [of[id(todo[a][0])] for a in range(b) if meet(a, b)]
             assert of[id(todo[b][0])] == 1 + max(earlier, default=-1)
