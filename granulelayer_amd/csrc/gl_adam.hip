@@ -222,18 +222,20 @@ __device__ __forceinline__ unsigned code_v(double y) {
   return (unsigned)i + (y >= h2 * h2 ? 1u : 0u);
 }
 // Noise of the codes of four neighbours, 16 bits for each m and 16 above them for each v.  It is a hash of what the step has in
-// hand: the elements' place, their parameters and new moments, and the step's corrections; nothing is kept for it, and a
-// replayed graph, whose arguments are those of its capture, draws anew from the moments.  Seven rounds are the fewest that pass
-// Philox's authors' tests.
+// hand: the elements' place, their parameters and new moments, and the step's corrections and seed; nothing is kept for it, and a
+// replayed graph, whose arguments are those of its capture, draws anew from the moments.  (Where gradients are the same in every step,
+// these stop changing in time, and then the corrections do: the seed must tell such steps apart.)  Seven rounds are the fewest
+// that pass Philox's authors' tests.
 __device__ __forceinline__ uv4 code_noise(unsigned long long vec, const float (&p)[4], const float (&m)[4], const float (&v)[4],
-                                          float k0, float k1) {
+                                          float k0, float k1, unsigned long long seed) {
   auto hash = [](const float (&x)[4]) {
     unsigned h = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) h = h * 0x9E3779B1u + __float_as_uint(x[j]);
     return h;
   };
-  return philox<7>(uv4{(unsigned)vec, (unsigned)(vec >> 32) ^ hash(p), hash(m), hash(v)}, __float_as_uint(k0), __float_as_uint(k1));
+  return philox<7>(uv4{(unsigned)vec, (unsigned)(vec >> 32) ^ hash(p), hash(m), hash(v)}, __float_as_uint(k0) ^ (unsigned)seed,
+                   __float_as_uint(k1) ^ (unsigned)(seed >> 32));
 }
 // Codes of |m| and v over the scale (over its square): the lower neighbour or, with the probability that keeps the value on
 // average, the upper one; `noise` is one of 2^16 equal shares.  (Where fp32 puts a quotient next to a code on its other side, the
@@ -342,7 +344,7 @@ __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensor
       const double dim = reciprocal(live_m ? fs : 1.f), dir = reciprocal(live_v ? fr : 1.f), dir2 = dir * dir;
 #pragma unroll
       for (int x = 0; x < V; ++x) {
-        const uv4 noise = code_noise((unsigned long long)(t.first + base + i[x]) >> 2, p[x], m[x], v[x], c.bc1, c.bc2);
+        const uv4 noise = code_noise((unsigned long long)(t.first + base + i[x]) >> 2, p[x], m[x], v[x], c.bc1, c.bc2, t.seed);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const unsigned q = drawn_m((float)(__builtin_fabs(dm[x][j]) * dim), noise[j] & 0xffffu);

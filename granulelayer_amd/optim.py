@@ -14,7 +14,7 @@ counterpart in the reference): blocks of 256 neighbouring elements of a tensor s
 
 with c one of a value's two neighbours, drawn so that it is kept on average, and 1 at least where v > 0: a step takes
 1 - b2 off v, less than codes are apart, so the nearest one would stay where it is.  The draw is a hash of the element's place,
-parameter, moments and step: equal runs are equal.  ``stochastic_rounding=False`` takes the nearest all the same: sqrt(v) is
+parameter, moments and step (and, as the rounding of bf16 parameters, of the seed): equal runs are equal.  ``stochastic_rounding=False`` takes the nearest all the same: sqrt(v) is
 then 1.1 of itself after 2,000 steps of like gradients and b2 = 0.999, and many times too large a few thousand steps after
 gradients got small.  A step takes the new moments before they are put into 8 bits; a block with an infinity or a NaN
 in its moments is NaN from then on.  The state of a parameter has codes
@@ -262,10 +262,12 @@ class FusedAdamW(torch.optim.Optimizer):
                 _, _, m_at, v_at, rest, *_, kind = self._known_state(p, st)
             t = st["step"] + 1
             c = corrections.get(t)
-            if c is None:
-                c = corrections[t] = (1 - b1 ** t, 1 - b2 ** t)
+            if c is None:  # the last: tells steps apart whose corrections are alike in fp32, for drawn codes
+                c = corrections[t] = (1 - b1 ** t, 1 - b2 ** t, 0 if b2 ** t * (1 - b2) >= 2.0 ** -24 else t)
             states.append(st)
-            row = _ROW(at, g_at, m_at, v_at, *rest, n, seed & 0xffffffffffffffff, *c)
+            if pdt is not bf16 or kind[4]:  # nothing of the parameter is rounded by noise
+                seed = c[2]
+            row = _ROW(at, g_at, m_at, v_at, *rest, n, seed & 0xffffffffffffffff, c[0], c[1])
             if kind is not last[0] or gdt is not last[1] or main is not last[2]:
                 last = (kind, gdt, main)
                 rows = calls.setdefault(last, [])

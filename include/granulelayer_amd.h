@@ -206,7 +206,8 @@ typedef struct GlAdamArgs {
  * scales for every 256 neighbouring elements (the last block of a tensor may be shorter):
  *   m = m_scale c |c|,  m_scale = max |m| / 127^2;   v = (v_scale c^2)^2,  v_scale = sqrt(max v) / 255^2
  * with the maxima rounded to fp32, and c one of the value's two neighbours, drawn so that it is kept on average, 1 at least where
- * v > 0.  The draw is a hash of the element's place in the tensor, parameters, moments and corrections: equal calls give equal codes.
+ * v > 0.  The draw is a hash of the element's place in the tensor, parameters, moments, corrections and seed: equal calls give equal
+ * codes, and steps whose corrections are alike need seeds of their own.
  * With GlAdamArgs.nearest_codes it is the nearest by its root; a moment that a step changes by less than half a code then stays. */
 #define GL_MOMENTS_INT8 2
 #define GL_ADAM_MAX_ELEMENTS (1LL << 35) /* of a tensor */
@@ -219,7 +220,7 @@ struct GlAdamTensor {
   float* m_scale;         /* [ceil(n / 256)] of 8-bit moments */
   float* v_scale;
   int64_t n;
-  uint64_t seed;          /* as GlAdamArgs.seed */
+  uint64_t seed;          /* as GlAdamArgs.seed; of drawn codes */
   float bc1, bc2;
 };
 

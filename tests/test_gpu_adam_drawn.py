@@ -123,11 +123,11 @@ def test_every_kind_of_parameter_draws(pdt, master):
     assert abs((up - share)[between].sum()) <= 5 * np.sqrt((share * (1 - share))[between].sum())
 
 
-def _follow(phases, n, lr=1e-3):
+def _follow(phases, n, lr=1e-3, b2=B2):
     """fp32 and 8-bit moments over the same gradients; phases: (scale of every element, steps, gradients of one sign)."""
     gen = torch.Generator(device=DEV).manual_seed(6)
     ps = [torch.nn.Parameter(torch.zeros(n, device=DEV)) for _ in range(2)]
-    opts = [FusedAdamW([p], moments=k, lr=lr, betas=(B1, B2)) for p, k in zip(ps, ("fp32", "int8"))]
+    opts = [FusedAdamW([p], moments=k, lr=lr, betas=(B1, b2)) for p, k in zip(ps, ("fp32", "int8"))]
     was = []
     for scale, steps, constant in phases:
         was = [p.detach().clone() for p in ps]
@@ -170,6 +170,18 @@ def test_moments_decay_beside_constant_gradients():
     assert abs(float(v8[stopped].mean() / v32[stopped].mean()) - 1) < 0.0226
     assert not m8[stopped].any()
     assert float((v8 / v32 - 1)[~stopped].abs().max()) < 2.0 ** -6  # each the largest of its block
+
+
+def test_moments_decay_beside_constant_gradients_after_the_corrections():
+    """b2 = 0.95: when gradients stop, 600 equal steps have made moments, scales and corrections constants.  A step moves v by 0.05 of
+    itself between codes 4 / c apart, and forgets as much: a variance of 0.05 (4 / c) / 0.1 = 2 / c of v^2, c = 5 after 300
+    steps: sqrt(0.4) / sqrt(4096) = 1%, five times; and 1 / c^4 where v may not fall below the code 1."""
+    n = 8192
+    one = torch.ones(n, device=DEV)
+    stopped = torch.arange(n, device=DEV) // 4 % 2 == 1  # all that a draw is made of
+    v32, m8, v8, _ = _follow([(one, 600, True), (torch.where(stopped, 0.0, one), 300, True)], n, b2=0.95)
+    assert abs(float(v8[stopped].mean() / v32[stopped].mean()) - 1) < 0.05 + 0.0016
+    assert not m8[stopped].any()
 
 
 def test_like_gradients_keep_their_moments():
