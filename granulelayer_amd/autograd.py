@@ -235,9 +235,14 @@ def _compute_operands(x, w, b, compute_dtype):
     return xc, wc.contiguous(), bc.contiguous()
 
 
-def _grad_buffers(w, b):
-    mg_w = getattr(w, "main_grad", None)
-    mg_b = getattr(b, "main_grad", None)
+def _owners(w, b):
+    """The tensors whose ``main_grad`` a backward looks for.  (What is saved may come back as other tensors, without their
+    attributes: activation checkpointing and hooks on saved tensors do that.)"""
+    return tuple(t if t.is_leaf or hasattr(t, "main_grad") else None for t in (w, b))
+
+
+def _grad_buffers(w, b, owners):
+    mg_w, mg_b = (getattr(t, "main_grad", None) for t in owners)
     if mg_w is not None and mg_b is not None:
         return mg_w, mg_b, True
     return (torch.zeros(w.shape, device=w.device, dtype=torch.float32),
@@ -357,6 +362,7 @@ class SparsePoolFunction(torch.autograd.Function):
         ctx.rt, ctx.policy, ctx.compute_dtype = rt, policy, compute_dtype
         ctx.saved_keys = list(saved.keys())
         ctx.save_for_backward(*_keep_input(ctx, rt, x, xc, rounded), w, b, *saved.values())
+        ctx.owners = _owners(w, b)
         rt.last_info["checkpoint_bytes"] = sum(t.numel() * t.element_size() for t in saved.values())
         return y
 
@@ -368,7 +374,7 @@ class SparsePoolFunction(torch.autograd.Function):
         rt: Level1Runtime = ctx.rt
         x, x_dtype = _kept_input(ctx, kept)
         xc, wc, bc = _compute_operands(x, w, b, ctx.compute_dtype)
-        dw_buf, db_buf, use_main = _grad_buffers(w, b)
+        dw_buf, db_buf, use_main = _grad_buffers(w, b, ctx.owners)
         dx = _level1_backward(rt, xc, wc, bc, dy, saved, ctx.policy, dw_buf, db_buf)
         gw = None if use_main else dw_buf.to(w.dtype)
         gb = None if use_main else db_buf.to(b.dtype)

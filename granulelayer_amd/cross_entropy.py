@@ -22,7 +22,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from .backend import backend_for
-from .dense import _main_grads, _through_function
+from .dense import _main_grads, _owner, _through_function
 
 REDUCTIONS = ("none", "mean", "sum")
 
@@ -67,6 +67,7 @@ class DenseCrossEntropyFunction(torch.autograd.Function):
         ctx.place = 0 if exps is None else exps.data_ptr()
         ctx.used_up = False
         ctx.save_for_backward(x, w, b, target, kept, exps)
+        ctx.owners = _owner(w), _owner(b)
         ctx.reduction, ctx.ignore_index, ctx.budget = reduction, ignore_index, budget
         return loss
 
@@ -80,7 +81,7 @@ def _gradients(ctx, dloss):
     x, w, b, target, kept, exps = ctx.saved_tensors
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-    mg_w, mg_b, use_main = _main_grads(w, b, need_w, need_b)
+    mg_w, mg_b, use_main = _main_grads(*ctx.owners, need_w, need_b)
     if use_main:
         dw, db = mg_w, mg_b
     else:

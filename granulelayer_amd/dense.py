@@ -70,6 +70,12 @@ def _through_function(*operands) -> bool:
     return False
 
 
+def _owner(t):
+    """The tensor whose ``main_grad`` a backward looks for, or None.  (What is saved may come back as another tensor, without
+    its attributes: activation checkpointing and hooks on saved tensors do that.)"""
+    return t if t is not None and t.requires_grad and (t.is_leaf or hasattr(t, "main_grad")) else None
+
+
 def _main_grads(w, b, need_w, need_b):
     """The fp32 ``main_grad`` buffers when every parameter that needs a gradient has one."""
     bufs = []
@@ -101,6 +107,7 @@ class DenseProjectionFunction(torch.autograd.Function):
         if need_w:
             xs = (None, *be.pack8(x)) if packed else (x, None, None)
         ctx.save_for_backward(*xs, w, None, z, z_exp)
+        ctx.weight = _owner(w)
         # a computed bias stands there by its shape and type alone
         ctx.bias = b if b is None or b.is_leaf or hasattr(b, "main_grad") else torch.empty_like(b, device="meta")
         ctx.activation, ctx.keep, ctx.x_shape, ctx.x_dtype = activation, keep, x.shape, x.dtype
@@ -117,7 +124,7 @@ class DenseProjectionFunction(torch.autograd.Function):
         dres = dy.to(ctx.res_dtype) if need_r else None
         if not (need_x or need_w or need_b):
             return None, None, None, dres, None, None
-        mg_w, mg_b, use_main = _main_grads(w, b, need_w, need_b)
+        mg_w, mg_b, use_main = _main_grads(ctx.weight, b, need_w, need_b)
         gtype = torch.float32 if use_main else w.dtype
         dx = torch.empty(ctx.x_shape, device=w.device, dtype=ctx.x_dtype) if need_x else None
         dw = mg_w if use_main else (torch.empty(w.shape, device=w.device, dtype=gtype) if need_w else None)

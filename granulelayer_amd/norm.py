@@ -14,7 +14,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from .backend import backend_for
-from .dense import _main_grads, _through_function
+from .dense import _main_grads, _owner, _through_function
 
 _DTYPES = (torch.float32, torch.bfloat16)
 
@@ -48,6 +48,7 @@ class LayerNormFunction(torch.autograd.Function):
     def forward(ctx, x, w, b, eps, out_dtype):
         y, stats = backend_for(x.device).norm_forward(x, w, b, eps, out_dtype, True)
         ctx.save_for_backward(x, w, stats)
+        ctx.weight = _owner(w)
         # a computed bias stands there by its shape and type alone
         ctx.bias = b if b is None or b.is_leaf or hasattr(b, "main_grad") else torch.empty_like(b, device="meta")
         return y
@@ -63,7 +64,7 @@ def _gradients(ctx, dy):
     b = ctx.bias
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-    mg_w, mg_b, use_main = _main_grads(w, b, need_w, need_b)
+    mg_w, mg_b, use_main = _main_grads(ctx.weight, b, need_w, need_b)
     if use_main:
         dw, db = mg_w, mg_b
     else:

@@ -21,7 +21,7 @@ from typing import Dict, List
 
 import torch
 
-from .autograd import (CHECKPOINT_BUDGET, Level1Runtime, _compute_operands, _grad_buffers, _ids_per_token,
+from .autograd import (CHECKPOINT_BUDGET, Level1Runtime, _compute_operands, _grad_buffers, _ids_per_token, _owners,
                        _keep_input, _kept_input, _level1_backward, _rounds_input, _saved_stats, act_torch, fit_policy)
 from .config import LevelSpec, PoolingConfig
 
@@ -124,6 +124,7 @@ class SemanticPoolFunction(torch.autograd.Function):
         ctx.saved_keys = list(saved.keys())
         ctx.n_t = len(tparams)
         ctx.save_for_backward(*_keep_input(ctx, rt, x, xc, rounded), w, b, *tparams, *saved.values())
+        ctx.owners = _owners(w, b)
         rt.last_info["checkpoint_bytes"] = sum(t.numel() * t.element_size() for t in saved.values())
         return y
 
@@ -154,7 +155,7 @@ class SemanticPoolFunction(torch.autograd.Function):
             grads = torch.autograd.grad(y, [Fv] + tp, dy, allow_unused=True)
         dF = grads[0].reshape(B, G * S)
         policy = ctx.policy if ctx.policy != "recompute_stats" else "minimal_stats"
-        dw_buf, db_buf, use_main = _grad_buffers(w, b)
+        dw_buf, db_buf, use_main = _grad_buffers(w, b, ctx.owners)
         dx = _level1_backward(rt, xc, wc, bc, dF, saved, policy, dw_buf, db_buf, rebuilt)
         gw = None if use_main else dw_buf.to(w.dtype)
         gb = None if use_main else db_buf.to(b.dtype)
