@@ -134,7 +134,8 @@ def dense_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Ten
 class DenseCrossEntropy(nn.Module):
     """``dense_cross_entropy`` with the head's parameters: weight [classes, input_dim] ~ N(0, 1 / input_dim) and, with
     ``bias``, zeros [classes], of ``dtype``.  The input is cast to the weight's type.  A weight shared with another
-    module (an embedding's table) is passed as ``weight``."""
+    module (an embedding's table) is passed as ``weight``; where it has ``main_grad``, the other module's gradient has to
+    go there too, as FusedAdamW reads nothing else then."""
 
     def __init__(self, input_dim: int, classes: int, bias: bool = False, dtype: torch.dtype = torch.bfloat16,
                  reduction: str = "mean", ignore_index: int = -100, workspace_budget: Optional[int] = None, device=None,

@@ -1,8 +1,8 @@
 """Fused AdamW for the layer parameters, mirroring sparse_pooling/optim.py (FusedAdamW).
 
-Reads the fp32 ``main_grad`` buffers written by the fused backward (zeroed in the same streaming pass) or
-``.grad`` in its own type, and updates the tensors of a parameter group together: a launch of the HIP kernel
-takes 38 of them (gl_adam).
+Reads the fp32 ``main_grad`` buffers written by the fused backward (zeroed in the same streaming pass) or, of parameters
+without one, ``.grad`` in its own type, and updates the tensors of a parameter group together: a launch of the HIP
+kernel takes 38 of them (gl_adam).
 Semantics are dense AdamW for every element (optim.py:1-15): m = b1 m + (1-b1) g,
 v = b2 v + (1-b2) g^2, p = p (1 - lr wd) - lr (m / bc1) / (sqrt(v / bc2) + eps), bc_i = 1 - b_i^t.
 
@@ -26,7 +26,8 @@ nearest-even rounding), stochastic rounding (the default without masters: noise 
 ``tl.randint(seed, element)`` below the bf16 cut, the seed counting tensors as the reference's
 ``_seed`` does), or nearest-even rounding (``stochastic_rounding=False``).
 
-A step captured into a graph replays the learning rate, the bias corrections and the seeds that it was captured with.
+A step captured into a graph replays the learning rate, the bias corrections and the seeds that it was captured with.  A
+first step makes the state, so it comes before the capture.
 """
 from __future__ import annotations
 
