@@ -1,4 +1,5 @@
-"""Softmax cross entropy of a dense head, without a tensor of its logits: the loss of ``softmax(x W^T + b)`` against a class a row.
+"""Softmax cross entropy of a dense head, without a tensor of its logits: the loss of ``softmax(x W^T + b)`` against a class a
+row.
 
 The other end of a model around the sparse layer: its last projection goes onto a large number of classes (a
 vocabulary), whose logits would be the largest tensor of the step.  The forward is one product whose tiles leave their
@@ -115,9 +116,9 @@ def dense_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Ten
     Any other target that is no class makes the loss NaN.  A class whose bias is -inf takes no part; logits past 2.3e38 in
     size count as infinite.  The backward's
     pieces of gradients at the logits take up to ``workspace_budget`` bytes (4 GiB by default; of 256 classes at
-    least), from the forward on where that keeps exponentials for it (from 512 bfloat16 or 64 float32 features on; with 4 bytes
-    for every 64 of them).  It
-    takes the operands as they were: none of them may change before it.  Tangents of forward-mode differentiation are refused."""
+    least), from the forward on where that keeps exponentials for it (from 512 bfloat16 or 64 float32 features on; with 4
+    bytes for every 64 of them).  It takes the operands as they were: none of them may change before it.  Tangents of
+    forward-mode differentiation are refused."""
     _check(x, weight, target, bias, reduction, workspace_budget)
     N, K = weight.shape
     x2 = x if x.dim() == 2 else x.reshape(-1, K)

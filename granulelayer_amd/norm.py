@@ -11,10 +11,11 @@ from typing import Optional
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .backend import backend_for
-from .dense import _main_grads, _owner, _through_function
+from .dense import _main_grads, _owner
 
 _DTYPES = (torch.float32, torch.bfloat16)
 
@@ -89,7 +90,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     _check(x, weight, bias, eps, out_dtype)
     D = x.shape[-1]
     x2 = x if x.dim() == 2 else x.reshape(-1, D)
-    if _through_function(x, weight, bias):
+    if (forward_ad._current_level >= 0  # an operand may have a tangent, which the function refuses
+            or torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                            or (bias is not None and bias.requires_grad))):
         y = LayerNormFunction.apply(x2, weight, bias, eps, out_dtype)
     else:
         y = backend_for(x.device).norm_forward(x2, weight, bias, eps, out_dtype, False)[0]

@@ -14,11 +14,12 @@ counterpart in the reference): blocks of 256 neighbouring elements of a tensor s
 
 with c one of a value's two neighbours, drawn so that it is kept on average, and 1 at least where v > 0: a step takes
 1 - b2 off v, less than codes are apart, so the nearest one would stay where it is.  The draw is a hash of the element's place,
-parameter, moments and step (and, as the rounding of bf16 parameters, of the seed): equal runs are equal.  ``stochastic_rounding=False`` takes the nearest all the same: sqrt(v) is
-then 1.1 of itself after 2,000 steps of like gradients and b2 = 0.999, and many times too large a few thousand steps after
-gradients got small.  A step takes the new moments before they are put into 8 bits; a block with an infinity or a NaN
-in its moments is NaN from then on.  The state of a parameter has codes
-``m`` (int8) and ``v`` (uint8) and scales ``m_scale`` and ``v_scale``; ``moment_values`` gives what they stand for.
+parameter, moments and step (and, as the rounding of bf16 parameters, of the seed): equal runs are equal.
+``stochastic_rounding=False`` takes the nearest all the same: sqrt(v) is then 1.1 of itself after 2,000 steps of like
+gradients and b2 = 0.999, and many times too large a few thousand steps after gradients got small.  A step takes the new
+moments before they are put into 8 bits; a block with an infinity or a NaN in its moments is NaN from then on.  The state of
+a parameter has codes ``m`` (int8) and ``v`` (uint8) and scales ``m_scale`` and ``v_scale``; ``moment_values`` gives what they
+stand for.
 
 Parameters are fp32, or bf16 with the reference's three variants (optim.py:5-9, 52-62): an fp32 master copy
 in the optimizer state (``master_weights=True``; the update runs on it and the parameter gets its
