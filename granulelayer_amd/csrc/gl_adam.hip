@@ -221,7 +221,8 @@ __device__ __forceinline__ unsigned code_v(double y) {
   const double h2 = (double)(h * h);
   return (unsigned)i + (y >= h2 * h2 ? 1u : 0u);
 }
-// Noise of the codes of four neighbours, 16 bits for each m and 16 above them for each v.  It is a hash of what the step has in
+// Noise of the codes of four neighbours, 14 bits for each m and 18 above them for each v, of which a step changes less: with
+// b2 = 0.9999 and c = 10, 1 / 4000 of the way to the next code.  It is a hash of what the step has in
 // hand: the elements' place, their parameters and new moments, and the step's corrections and seed; nothing is kept for it, and a
 // replayed graph, whose arguments are those of its capture, draws anew from the moments.  (Where gradients are the same in every step,
 // these stop changing in time, and then the corrections do: the seed must tell such steps apart.)  Seven rounds are the fewest
@@ -238,16 +239,16 @@ __device__ __forceinline__ uv4 code_noise(unsigned long long vec, const float (&
                    __float_as_uint(k1) ^ (unsigned)(seed >> 32));
 }
 // Codes of |m| and v over the scale (over its square): the lower neighbour or, with the probability that keeps the value on
-// average, the upper one; `noise` is one of 2^16 equal shares.  (Where fp32 puts a quotient next to a code on its other side, the
+// average, the upper one; `noise` is one of 2^14 (2^18) equal shares.  (Where fp32 puts a quotient next to a code on its other side, the
 // code is still the neighbour that is taken nearly always.)
 __device__ __forceinline__ unsigned drawn_m(float q, unsigned noise) {
   const float i = __builtin_fminf(__builtin_floorf(__builtin_amdgcn_sqrtf(q)), 126.f);
-  const float u = __builtin_fmaf((float)noise, 0x1p-16f, 0x1p-17f);
+  const float u = __builtin_fmaf((float)noise, 0x1p-14f, 0x1p-15f);
   return (unsigned)i + (__builtin_fmaf(-i, i, q) > u * (2.f * i + 1.f) ? 1u : 0u);
 }
 __device__ __forceinline__ unsigned drawn_v(float q, unsigned noise) {
   const float i = __builtin_fminf(__builtin_floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(q))), 254.f), i2 = i * i;
-  const float u = __builtin_fmaf((float)noise, 0x1p-16f, 0x1p-17f), t = 2.f * i + 1.f;
+  const float u = __builtin_fmaf((float)noise, 0x1p-18f, 0x1p-19f), t = 2.f * i + 1.f;
   return (unsigned)i + (__builtin_fmaf(-i2, i2, q) > u * (t * (2.f * i2 + t)) ? 1u : 0u);  // t (2 i^2 + t) = (i + 1)^4 - i^4
 }
 __device__ __forceinline__ unsigned low_bytes(const unsigned (&c)[4]) {
@@ -274,7 +275,7 @@ __device__ __forceinline__ int adam_tensor(const AdamTable& a) {
 // MOM: the kind of moments; GBF: bf16 gradients.  A workgroup takes a chunk of one tensor, a
 // thread a vector of each stream, or two with 8-bit moments: a block is half a wave's then, and what is done for a block (its
 // maxima and scales) is done for two at once.  150M bf16 parameters and gradients, nearest codes: 305 us (4.9 TB/s; bound by instructions,
-// 246 us at the rate of the fp32 stream), 352 with a block a wave (319 then); fp32 ones 393, drawn codes 432.  400M fp32 in all types:
+// 246 us at the rate of the fp32 stream), 352 with a block a wave (319 then); fp32 ones 393, drawn codes 445.  400M fp32 in all types:
 // 2.2 ms (5.7 TB/s).  Parameters rounded stochastically take a Philox-4x32-10 an element: bf16 moments 529 us, 345 rounded to nearest.
 // WHOLE: all of the wave's elements are there (no lane's ends are looked at).
 constexpr int adam_vectors(int mom) { return in_8bit(mom) ? 2 : 1; }
@@ -347,8 +348,8 @@ __device__ __forceinline__ void adam_vector(const AdamTable& a, const AdamTensor
         const uv4 noise = code_noise((unsigned long long)(t.first + base + i[x]) >> 2, p[x], m[x], v[x], c.bc1, c.bc2, t.seed);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const unsigned q = drawn_m((float)(__builtin_fabs(dm[x][j]) * dim), noise[j] & 0xffffu);
-          const unsigned u = drawn_v((float)(dv[x][j] * dir2), noise[j] >> 16);
+          const unsigned q = drawn_m((float)(__builtin_fabs(dm[x][j]) * dim), noise[j] & 0x3fffu);
+          const unsigned u = drawn_v((float)(dv[x][j] * dir2), noise[j] >> 14);
           om[x][j] = dm[x][j] < 0.0 ? 0u - q : q;
           ov[x][j] = u == 0 && dv[x][j] > 0.0 ? 1u : u;
         }

@@ -184,6 +184,19 @@ def test_moments_decay_beside_constant_gradients_after_the_corrections():
     assert not m8[stopped].any()
 
 
+def test_slow_second_moments_decay():
+    """b2 = 0.9999, gradients that fall to nearly nothing: a step takes 1 / 4000 of the way to the next code where c = 10.  Of v that the
+    steps leave alone but for the share 1 - b2, variances are 2 / c of v^2; codes of 20 and more after 20,000 steps (v is 0.135 of
+    what it was, 1e-4 of the others'): sqrt(0.1) / sqrt(4096) = 0.5%, five times; twice that for the block's scale, which moves."""
+    n = 8192
+    one = torch.ones(n, device=DEV)
+    small = torch.arange(n, device=DEV) // 4 % 2 == 1
+    first = torch.where(small, 0.03, one)
+    v32, _, v8, _ = _follow([(first, 3000, False), (torch.where(small, 1e-5, one), 20000, False)], n, b2=0.9999)
+    assert abs(float(v8[small].mean() / v32[small].mean()) - 1) < 0.05
+    assert abs(float(v8[~small].mean() / v32[~small].mean()) - 1) < 0.0226
+
+
 def test_like_gradients_keep_their_moments():
     """Codes of 60 and more for nearly all: sqrt(10 / 60) / sqrt(8192) = 0.45%, five times."""
     n = 8192
